@@ -207,6 +207,120 @@ typedef struct bolt3_silu_mul_args {
 } bolt3_silu_mul_args;
 int bolt3_silu_mul(const bolt3_silu_mul_args* a, void* stream);
 
+/* ---- 8-bit KV cache of a softmax anchor layer. No counterpart in the reference, whose caches are
+ * bf16 (vsa_lm/decode.py:88-106).
+ * Layout: data int8 [2][B][HKV][cap][HD] (keys, then values), scale fp32 [2][B][HKV][cap]. Row r of a
+ * head stands for data * scale with scale = max(max |x| / 127, 2^-40), data = x / scale rounded to the
+ * nearest integer (ties to even). A row that holds a NaN or an infinity gets that as its scale, so that
+ * it spoils what attends to it as it would in a bf16 cache. HD 64 or 128.
+ * Lengths. Sequence b holds s_b rows before the call: s_b = n, or n + *pos_dev - pos_ref with a device
+ * step position, or lens[b] where `lens` (device int32 [B]) is given; lens and pos_dev exclude each
+ * other. lens[b] = -1 marks an idle sequence. A length that is otherwise out of [0, cap - T] makes that
+ * sequence idle too and ORs 8 into `status`. */
+
+/* Writes T new tokens of every sequence: per-head RMSNorm of q and k (optional: q_norm_w, k_norm_w),
+ * rotate-half RoPE of q and k (optional: inv_freq) at position pos0 + (s_b - n) + t, q rounded once to
+ * q_out, k and v quantised into rows s_b .. s_b + T - 1 of the cache. All in fp32; the angle is
+ * fp32(position) * inv_freq rounded to fp32. Head h of token t of sequence b is the HD values at
+ * x + b * x_sb + t * x_st + h * HD (x = q, k, v; strides in elements, multiples of 8), so that column
+ * blocks of one fused projection can be given. q_out of an idle sequence is 0. H, HKV >= 1 (H need not
+ * be a multiple of HKV here); H + 2 HKV <= 4096; T <= 1048576. */
+typedef struct bolt3_kv8_append_args {
+  int B, T, H, HKV, HD;
+  const void* q; const void* k; const void* v;
+  int64_t q_sb, q_st, k_sb, k_st, v_sb, v_st;
+  const float* q_norm_w; const float* k_norm_w; float eps;
+  const float* inv_freq;
+  void* q_out;                         /* bf16 [B][T][H][HD] */
+  int8_t* data; float* scale; int64_t cap;
+  int64_t n; int64_t pos0;
+  const int32_t* lens;
+  int32_t* status;                     /* optional */
+  const int64_t* pos_dev; int64_t pos_ref; int64_t pos_span;
+} bolt3_kv8_append_args;
+int bolt3_kv8_append(const bolt3_kv8_append_args* a, void* stream);
+
+/* Rows r0_b .. r0_b + T - 1 of every sequence back as bf16 [2][B][HKV][T][HD] (r0_b = t0, or lens[b]);
+ * zeros for an idle sequence. B * HKV <= 32767. */
+typedef struct bolt3_kv8_read_args {
+  int B, HKV, HD;
+  int64_t T;
+  const int8_t* data; const float* scale; int64_t cap;
+  int64_t t0;
+  const int32_t* lens;
+  void* out;
+  int32_t* status;                     /* optional */
+} bolt3_kv8_read_args;
+int bolt3_kv8_read(const bolt3_kv8_read_args* a, void* stream);
+
+/* Softmax attention of the T newest tokens (already appended) over the cache: query t of sequence b sees
+ * rows 0 .. s_b + t. q: bf16, head h of token t of sequence b at q + b * q_sb + t * q_st + h * HD; y: bf16
+ * [B][T][H][HD], rounded once; 0 for an idle sequence. H a multiple of HKV, G = H / HKV <= 16.
+ * With `lens`, n is the longest length to expect (it sizes the split of the cache, nothing else).
+ * `workspace`: device memory of bolt3_kv8_attend_workspace(...) bytes, 16-byte aligned, used only
+ * within the call (0 bytes: none needed). */
+typedef struct bolt3_kv8_attend_args {
+  int B, T, H, HKV, HD;
+  const void* q; int64_t q_sb, q_st;
+  const int8_t* data; const float* scale; int64_t cap;
+  int64_t n;
+  const int32_t* lens;
+  void* y;
+  float sm_scale;
+  void* workspace; size_t workspace_bytes;
+  int32_t* status;                     /* optional; also OR-ed with 2 if a bounded wait expired */
+  const int64_t* pos_dev; int64_t pos_ref; int64_t pos_span;
+} bolt3_kv8_attend_args;
+int bolt3_kv8_attend(const bolt3_kv8_attend_args* a, void* stream);
+size_t bolt3_kv8_attend_workspace(int B, int T, int H, int HKV, int HD, int64_t n);
+
+/* ---- Beam search. No counterpart in the reference, which samples (vsa_lm/config/bolt3.py:321-333).
+ * One selection step of B groups of K beams over V tokens. Continuation (k, v) of a group scores
+ * scores[k] + log_softmax(logits[k])[v]; a finished beam has one continuation, eos_ids[0] at its own
+ * score, and its logits are not read. A NaN logit, or a NaN score, counts as -infinity. The K best continuations with a score above
+ * -infinity survive, equal ones by the lowest k * V + v; within a beam the order is the logits' (two
+ * different logits whose scores round to the same value keep their order).
+ * Slots: the best continuation of each parent takes its parent's slot, the others take the slots that
+ * are left in ascending order, best first. So a beam that lives on stays in place, and out_parent can be
+ * applied to the states in place. A slot without a continuation gets score -infinity, itself as parent,
+ * eos_ids[0] (0 if there is none) as token, and is finished.
+ * out_finished = finished, or the token is one of eos_ids. K <= 16, n_eos <= 8; V <= 524288; row r = b * K + k
+ * of the logits is V values at logits + r * row_stride elements (bf16, or fp32 with logits_fp32). */
+typedef struct bolt3_beam_select_args {
+  int B, K; int64_t V;
+  const void* logits; int64_t row_stride; int logits_fp32;
+  const float* scores; const uint8_t* finished;       /* [B][K]; finished may be NULL */
+  int64_t eos_ids[8]; int n_eos;
+  float* out_scores; int32_t* out_parent; int64_t* out_token; uint8_t* out_finished;   /* [B][K] */
+  void* workspace; size_t workspace_bytes;            /* bolt3_beam_select_workspace bytes, 16-byte aligned */
+} bolt3_beam_select_args;
+int bolt3_beam_select(const bolt3_beam_select_args* a, void* stream);
+size_t bolt3_beam_select_workspace(int B, int K, int64_t V);
+
+/* One state array whose beams are to be moved: for i < n_outer, beam x (of B * K) and r < n_row, the
+ * bytes [lo, hi) at base + i * outer_stride + x * beam_stride + r * row_stride, with lo = t0 * token_bytes,
+ * hi = t1 * token_bytes, or all row_bytes where token_bytes is 0. Base, strides and lengths are multiples
+ * of `unit`, 1, 4 or 16 bytes. */
+typedef struct bolt3_beam_item {
+  void* base;
+  int64_t outer_stride, beam_stride, row_stride;
+  int64_t row_bytes, token_bytes;
+  int32_t n_outer, n_row, unit, reserved;
+} bolt3_beam_item;
+
+/* Every listed state of beam j of group b becomes that of beam parent[b][j], in place, for any map
+ * (a thread reads all parents of its bytes before it writes). Beams that are their own parent cost
+ * nothing. Items must not overlap. `items` is a host array, read during the call. A parent out of
+ * [0, K) leaves its beam as it is and ORs 8 into `status`. K <= 16. */
+typedef struct bolt3_beam_reorder_args {
+  int B, K;
+  const int32_t* parent;               /* device [B][K] */
+  const bolt3_beam_item* items; int n_items;
+  int64_t t0, t1;
+  int32_t* status;                     /* optional */
+} bolt3_beam_reorder_args;
+int bolt3_beam_reorder(const bolt3_beam_reorder_args* a, void* stream);
+
 /* Bytes of snapshot workspace bolt3_prefill_fwd needs for n_chains chains of T tokens. */
 size_t bolt3_prefill_workspace_size(int n_chains, int64_t T, int HD);
 
@@ -252,8 +366,8 @@ int bolt3_prefill_fwd_noalloc(const bolt3_prefill_args* a, void* stream);
 int bolt3_abi_version(void);
 const char* bolt3_status_string(int status);
 /* sizeof of an argument struct (0 prep, 1 consolidate, 2 attend, 3 prefill, 4 anchor, 5 rmsnorm,
- * 6 silu_mul; 0 for others), so a
- * binding can check its own layout of the structs against the compiled one */
+ * 6 silu_mul, 8 kv8_append, 9 kv8_read, 10 kv8_attend, 11 beam_select, 12 beam_item, 13 beam_reorder;
+ * 0 for others), so a binding can check its own layout of the structs against the compiled one */
 size_t bolt3_args_size(int which);
 /* Host-only: reorder indices 0..n-1 of `vals` into the order CPU torch.topk(vals, k, largest)
  * returns (first k written to out_idx). Returns 0, or 1 if a bounds check fired. */

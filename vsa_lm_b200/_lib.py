@@ -22,7 +22,8 @@ STATUS = {0: "ok", 1: "invalid argument", 2: "unsupported shape", 3: "misaligned
 DEVICE_STATUS_BITS = {1: "a bounds check of the consolidation's tie-order emulation fired",
                       2: "a bounded wait in an attention kernel expired",
                       4: "a bounded wait in the consolidation scan expired",
-                      8: "a decode step's device position was outside the range its launch was built for"}
+                      8: "a decode step's device position (or a sequence length or beam parent on the device) was "
+                         "outside the range its launch was built for"}
 
 
 class PrepArgs(ctypes.Structure):
@@ -106,6 +107,80 @@ class SiluMulArgs(ctypes.Structure):
     _fields_ = [("gu", _P), ("y", _P), ("rows", _I64), ("I", _I64)]
 
 
+class Kv8AppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", _I), ("T", _I), ("H", _I), ("HKV", _I), ("HD", _I),
+        ("q", _P), ("k", _P), ("v", _P),
+        ("q_sb", _I64), ("q_st", _I64), ("k_sb", _I64), ("k_st", _I64), ("v_sb", _I64), ("v_st", _I64),
+        ("q_norm_w", _P), ("k_norm_w", _P), ("eps", _F),
+        ("inv_freq", _P),
+        ("q_out", _P),
+        ("data", _P), ("scale", _P), ("cap", _I64),
+        ("n", _I64), ("pos0", _I64),
+        ("lens", _P),
+        ("status", _P),
+        ("pos_dev", _P), ("pos_ref", _I64), ("pos_span", _I64),
+    ]
+
+
+class Kv8ReadArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", _I), ("HKV", _I), ("HD", _I),
+        ("T", _I64),
+        ("data", _P), ("scale", _P), ("cap", _I64),
+        ("t0", _I64),
+        ("lens", _P),
+        ("out", _P),
+        ("status", _P),
+    ]
+
+
+class Kv8AttendArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", _I), ("T", _I), ("H", _I), ("HKV", _I), ("HD", _I),
+        ("q", _P), ("q_sb", _I64), ("q_st", _I64),
+        ("data", _P), ("scale", _P), ("cap", _I64),
+        ("n", _I64),
+        ("lens", _P),
+        ("y", _P),
+        ("sm_scale", _F),
+        ("workspace", _P), ("workspace_bytes", _SZ),
+        ("status", _P),
+        ("pos_dev", _P), ("pos_ref", _I64), ("pos_span", _I64),
+    ]
+
+
+class BeamSelectArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", _I), ("K", _I), ("V", _I64),
+        ("logits", _P), ("row_stride", _I64), ("logits_fp32", _I),
+        ("scores", _P), ("finished", _P),
+        ("eos_ids", _I64 * 8), ("n_eos", _I),
+        ("out_scores", _P), ("out_parent", _P), ("out_token", _P), ("out_finished", _P),
+        ("workspace", _P), ("workspace_bytes", _SZ),
+    ]
+
+
+class BeamItem(ctypes.Structure):
+    _fields_ = [
+        ("base", _P),
+        ("outer_stride", _I64), ("beam_stride", _I64), ("row_stride", _I64),
+        ("row_bytes", _I64), ("token_bytes", _I64),
+        ("n_outer", ctypes.c_int32), ("n_row", ctypes.c_int32), ("unit", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class BeamReorderArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", _I), ("K", _I),
+        ("parent", _P),
+        ("items", ctypes.POINTER(BeamItem)), ("n_items", _I),
+        ("t0", _I64), ("t1", _I64),
+        ("status", _P),
+    ]
+
+
 class PrefillArgs(ctypes.Structure):
     _fields_ = [
         ("B", _I), ("T", _I), ("H", _I), ("HKV", _I), ("HD", _I),
@@ -130,6 +205,13 @@ SIGNATURES = {
     "bolt3_anchor_decode": ([ctypes.POINTER(AnchorArgs), _P], _I),
     "bolt3_rmsnorm": ([ctypes.POINTER(RMSNormArgs), _P], _I),
     "bolt3_silu_mul": ([ctypes.POINTER(SiluMulArgs), _P], _I),
+    "bolt3_kv8_append": ([ctypes.POINTER(Kv8AppendArgs), _P], _I),
+    "bolt3_kv8_read": ([ctypes.POINTER(Kv8ReadArgs), _P], _I),
+    "bolt3_kv8_attend": ([ctypes.POINTER(Kv8AttendArgs), _P], _I),
+    "bolt3_kv8_attend_workspace": ([_I, _I, _I, _I, _I, _I64], _SZ),
+    "bolt3_beam_select": ([ctypes.POINTER(BeamSelectArgs), _P], _I),
+    "bolt3_beam_select_workspace": ([_I, _I, _I64], _SZ),
+    "bolt3_beam_reorder": ([ctypes.POINTER(BeamReorderArgs), _P], _I),
     "bolt3_prefill_fwd": ([ctypes.POINTER(PrefillArgs), _P], _I),
     "bolt3_prefill_fwd_noalloc": ([ctypes.POINTER(PrefillArgs), _P], _I),
     "bolt3_prefill_workspace_size": ([_I, _I64, _I], _SZ),
@@ -138,6 +220,11 @@ SIGNATURES = {
     "bolt3_status_string": ([_I], ctypes.c_char_p),
     "bolt3_topk_order_host": ([_P, _I, _I, _I, _P], _I),
 }
+
+# number of each struct for bolt3_args_size
+ARG_STRUCTS = {0: PrepArgs, 1: ConsolidateArgs, 2: AttendArgs, 3: PrefillArgs, 4: AnchorArgs, 5: RMSNormArgs,
+               6: SiluMulArgs, 8: Kv8AppendArgs, 9: Kv8ReadArgs, 10: Kv8AttendArgs, 11: BeamSelectArgs, 12: BeamItem,
+               13: BeamReorderArgs}
 
 ABI_VERSION = 10   # BOLT3_ABI_VERSION in include/bolt3.h
 
@@ -167,8 +254,7 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
             fn.restype = rest
         if lib.bolt3_abi_version() != ABI_VERSION:
             raise RuntimeError("libbolt3.so ABI version mismatch; rebuild with `python -m vsa_lm_b200.build`")
-        for i, st in enumerate((PrepArgs, ConsolidateArgs, AttendArgs, PrefillArgs, AnchorArgs, RMSNormArgs,
-                                SiluMulArgs)):
+        for i, st in ARG_STRUCTS.items():
             if lib.bolt3_args_size(i) != ctypes.sizeof(st):
                 raise RuntimeError(f"{st.__name__} has {ctypes.sizeof(st)} bytes here but "
                                    f"{lib.bolt3_args_size(i)} in libbolt3.so: the bindings and the header differ")

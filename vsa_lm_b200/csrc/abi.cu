@@ -45,6 +45,12 @@ extern "C" size_t bolt3_args_size(int which) {
     case 4: return sizeof(bolt3_anchor_args);
     case 5: return sizeof(bolt3_rmsnorm_args);
     case 6: return sizeof(bolt3_silu_mul_args);
+    case 8: return sizeof(bolt3_kv8_append_args);
+    case 9: return sizeof(bolt3_kv8_read_args);
+    case 10: return sizeof(bolt3_kv8_attend_args);
+    case 11: return sizeof(bolt3_beam_select_args);
+    case 12: return sizeof(bolt3_beam_item);
+    case 13: return sizeof(bolt3_beam_reorder_args);
     default: return 0;
   }
 }

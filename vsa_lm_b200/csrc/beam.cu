@@ -1,0 +1,489 @@
+// Beam search on the device: the selection over beams and vocabulary, and the reordering of decode states.
+//
+// select. With lse_k = log sum_v e^x_kv, continuation (k, v) scores s_k + (x_kv - lse_k); the K best of a
+// group's K * V survive. Bound by HBM: the logits are read once. Within a beam the order is the logits',
+// so the pass that sums the exponentials also finds each chunk's K best logits:
+// - select_chunk_kernel: a block holds a chunk of 8192 logits of one row in registers. Maximum and sum of
+//   exponentials, then a threshold: the K-th largest of 16 half-warp maxima is no larger than the chunk's
+//   K-th largest logit, so the few logits at or above it contain the K best; they are ranked by counting.
+//   Chunks with many equal logits (more than the list holds) take K rounds of a block maximum instead.
+// - select_group_kernel: a block per group merges the chunks' sums and lists, scores, ranks and assigns slots.
+// reorder. Bound by HBM: the bytes of every beam that is not its own parent are read from the parent and
+// written. A thread holds its bytes of all parents of the group before it writes any, so the move is in
+// place for any map. Blocks cover the items' bytes flattened, so that many small arrays are one launch.
+#include "../../include/bolt3.h"
+#include "common.cuh"
+#include "trace.h"
+
+namespace {
+
+using namespace b3;
+
+constexpr int kMaxK = 16;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ------------------------------------------------------------------------------------------- select
+
+constexpr int kSelThreads = 256;
+constexpr int kPerThread = 32;
+constexpr int kChunk = kSelThreads * kPerThread;      // logits of a block
+constexpr int kListCap = 256;                         // candidates at or above the threshold
+constexpr int64_t kMaxV = 64 * kChunk;
+
+struct Cand {
+  float x;
+  int32_t v;
+};
+// a before b in the order of a row: larger logit, then lower index
+B3_DEV bool before(Cand a, Cand b) { return a.x > b.x || (a.x == b.x && a.v < b.v); }
+
+struct SelParams {
+  bolt3_beam_select_args a;
+  int n_chunks;
+  float2* sums;       // [B * K][n_chunks] (maximum, sum of e^(x - maximum))
+  Cand* cands;        // [B * K][n_chunks][K], best first, v = -1 where there are fewer
+};
+
+// the row has continuations of its own (its logits count)
+B3_DEV bool row_live(const bolt3_beam_select_args& a, int64_t r) {
+  return !(a.finished != nullptr && a.finished[r]) && a.scores[r] > neg_inf();
+}
+
+template <bool FP32>
+__global__ void __launch_bounds__(kSelThreads) select_chunk_kernel(const SelParams p) {
+  constexpr int EPL = FP32 ? 4 : 8;                   // logits of a 16-byte load
+  constexpr int NL = kPerThread / EPL;
+  __shared__ float s_max[16];
+  __shared__ float s_sum[8];
+  __shared__ int s_count;
+  __shared__ Cand s_list[kListCap];
+  const bolt3_beam_select_args& a = p.a;
+  const int64_t r = blockIdx.x;
+  const int chunk = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (!row_live(a, r)) return;
+  const int64_t lo = (int64_t)chunk * kChunk;
+  const int n = (int)min((int64_t)kChunk, a.V - lo);
+  const char* row = reinterpret_cast<const char*>(a.logits) + (r * a.row_stride + lo) * (FP32 ? 4 : 2);
+  const bool vec = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
+  float x[kPerThread];
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int e = (i * kSelThreads + tid) * EPL;
+    if (vec && e + EPL <= n) {
+      const uint4 w = __ldcs(reinterpret_cast<const uint4*>(row + (size_t)e * (FP32 ? 4 : 2)));
+      if constexpr (FP32) {
+        x[4 * i] = __uint_as_float(w.x); x[4 * i + 1] = __uint_as_float(w.y);
+        x[4 * i + 2] = __uint_as_float(w.z); x[4 * i + 3] = __uint_as_float(w.w);
+      } else {
+        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = unpack_bf16(ww[j]);
+          x[8 * i + 2 * j] = f.x;
+          x[8 * i + 2 * j + 1] = f.y;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < EPL; ++j)
+        x[EPL * i + j] = e + j >= n ? neg_inf()
+                         : FP32     ? reinterpret_cast<const float*>(row)[e + j]
+                                    : bf2f(reinterpret_cast<const bf16*>(row)[e + j]);
+    }
+  }
+  auto index = [&](int i) { return (int)lo + ((i / EPL) * kSelThreads + tid) * EPL + i % EPL; };
+  float m = neg_inf();
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) {
+    if (x[i] != x[i]) x[i] = neg_inf();
+    m = fmaxf(m, x[i]);
+  }
+  float g = m;                                        // maximum of the half-warp, then of the block
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+  if ((lane & 15) == 0) s_max[warp * 2 + (lane >> 4)] = g;
+  if (tid == 0) s_count = 0;
+  __syncthreads();
+  g = s_max[lane & 15];
+  // tau: the K-th largest of the 16 half-warps' maxima
+  int rank = 0;
+  float top = neg_inf();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float o = __shfl_sync(0xffffffffu, g, i);
+    rank += o > g || (o == g && i < (lane & 15));
+    top = fmaxf(top, o);
+  }
+  const unsigned who = __ballot_sync(0xffffffffu, rank == a.K - 1);
+  const float tau = __shfl_sync(0xffffffffu, g, __ffs(who) - 1);
+  float sum = 0.f;
+  if (top > neg_inf()) {
+    const float off = top * kLog2e;
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) sum += exp2f(fmaf(x[i], kLog2e, -off));
+  }
+  sum = warp_sum(sum);
+  if (lane == 0) s_sum[warp] = sum;
+  if (m >= tau && m > neg_inf()) {
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i)
+      if (x[i] >= tau && x[i] > neg_inf()) {
+        const int at = atomicAdd(&s_count, 1);        // the list's order does not matter: it is ranked below
+        if (at < kListCap) s_list[at] = Cand{x[i], index(i)};
+      }
+  }
+  __syncthreads();
+  const int count = s_count;
+  Cand* out = p.cands + (r * p.n_chunks + chunk) * a.K;
+  if (tid == 0) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t += s_sum[i];
+    p.sums[r * p.n_chunks + chunk] = make_float2(top, t);
+  }
+  if (count <= kListCap) {
+    if (tid < count) {
+      const Cand c = s_list[tid];
+      int better = 0;
+      for (int i = 0; i < count; ++i) better += before(s_list[i], c);
+      if (better < a.K) out[better] = c;
+    }
+    if (tid >= count && tid < a.K) out[tid] = Cand{neg_inf(), -1};
+    return;
+  }
+  // many equal logits: K rounds, each the best candidate after the last one
+  Cand last{__int_as_float(0x7f800000), -1};
+  for (int k = 0; k < a.K; ++k) {
+    Cand best{neg_inf(), 0x7fffffff};
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) {
+      const Cand c{x[i], index(i)};
+      if (c.x > neg_inf() && before(last, c) && before(c, best)) best = c;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const Cand c{__shfl_xor_sync(0xffffffffu, best.x, o), __shfl_xor_sync(0xffffffffu, best.v, o)};
+      if (before(c, best)) best = c;
+    }
+    __syncthreads();
+    if (lane == 0) s_list[warp] = best;
+    __syncthreads();
+    best = s_list[0];
+    for (int i = 1; i < kSelThreads / 32; ++i)
+      if (before(s_list[i], best)) best = s_list[i];
+    last = best;
+    if (tid == 0) out[k] = best;                       // more than kListCap are above -infinity: all K exist
+  }
+}
+
+// a block per group, a warp per beam for the merge of its chunks
+__global__ void __launch_bounds__(32 * kMaxK) select_group_kernel(const SelParams p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ float c_score[kMaxK * kMaxK];
+  __shared__ Cand c_cand[kMaxK * kMaxK];
+  __shared__ int s_pick[kMaxK];
+  __shared__ bool s_done[kMaxK];
+  const bolt3_beam_select_args& a = p.a;
+  const int K = a.K, tid = threadIdx.x, lane = tid & 31, k = tid >> 5;
+  const int64_t b = blockIdx.x, r = b * K + k;
+  const int per_row = p.n_chunks * K;
+  Cand* all = reinterpret_cast<Cand*>(smem) + (size_t)k * per_row;
+  const bool live = row_live(a, r);
+  const bool done = a.finished != nullptr && a.finished[r];
+  const float own = a.scores[r];
+  if (tid < kMaxK) s_pick[tid] = -1;
+  if (lane == 0) s_done[k] = done;       // the outputs may be the inputs: nothing of these is read later
+  if (live) {
+    for (int i = lane; i < per_row; i += 32) all[i] = p.cands[r * per_row + i];
+    float m = neg_inf();
+    for (int i = lane; i < p.n_chunks; i += 32) m = fmaxf(m, p.sums[r * p.n_chunks + i].x);
+    m = warp_max(m);
+    float s = 0.f;
+    for (int i = lane; i < p.n_chunks; i += 32) {
+      const float2 c = p.sums[r * p.n_chunks + i];
+      if (c.x > neg_inf()) s += c.y * exp2f((c.x - m) * kLog2e);
+    }
+    s = warp_sum(s);
+    const float lse = m + logf(s);
+    __syncwarp();
+    // each lane walks the sorted lists of two chunks (at most 64)
+    int at[2] = {0, 0};
+    for (int i = 0; i < K; ++i) {
+      Cand best{neg_inf(), 0x7fffffff};
+      int from = -1;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int c = lane + 32 * j;
+        if (c < p.n_chunks && at[j] < K) {
+          const Cand h = all[c * K + at[j]];
+          if (h.v >= 0 && before(h, best)) {
+            best = h;
+            from = j;
+          }
+        }
+      }
+      Cand win = best;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const Cand c{__shfl_xor_sync(0xffffffffu, win.x, o), __shfl_xor_sync(0xffffffffu, win.v, o)};
+        if (before(c, win)) win = c;
+      }
+      if (from >= 0 && best.v == win.v) at[from]++;
+      if (lane == 0) {
+        float sc = neg_inf();
+        if (win.v != 0x7fffffff) sc = own + (win.x - lse);
+        c_score[k * K + i] = sc != sc ? neg_inf() : sc;
+        c_cand[k * K + i] = win;
+      }
+    }
+  } else if (lane < K) {
+    const float sc = done && lane == 0 ? own : neg_inf();
+    c_score[k * K + lane] = sc != sc ? neg_inf() : sc;
+    c_cand[k * K + lane] = Cand{0.f, (int32_t)a.eos_ids[0]};
+  }
+  __syncthreads();
+  // rank of every candidate: score, then beam, then its place in the beam's list
+  for (int i = tid; i < K * K; i += blockDim.x) {
+    const float sc = c_score[i];
+    if (!(sc > neg_inf())) continue;
+    int better = 0;
+    for (int j = 0; j < K * K; ++j) better += c_score[j] > sc || (c_score[j] == sc && j < i);
+    if (better < K) s_pick[better] = i;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    unsigned taken = 0, later = 0;
+    int slot[kMaxK];
+    for (int i = 0; i < K; ++i) {
+      const int c = s_pick[i];
+      if (c < 0) continue;
+      const int par = c / K;
+      if (taken >> par & 1) {
+        later |= 1u << i;
+      } else {
+        taken |= 1u << par;
+        slot[i] = par;
+      }
+    }
+    for (int i = 0; i < K; ++i) {
+      if (!(later >> i & 1)) continue;
+      const int f = __ffs(~taken) - 1;
+      taken |= 1u << f;
+      slot[i] = f;
+    }
+    for (int j = 0; j < K; ++j) {
+      if (taken >> j & 1) continue;
+      a.out_scores[b * K + j] = neg_inf();
+      a.out_parent[b * K + j] = j;
+      a.out_token[b * K + j] = a.n_eos > 0 ? a.eos_ids[0] : 0;
+      a.out_finished[b * K + j] = 1;
+    }
+    for (int i = 0; i < K; ++i) {
+      const int c = s_pick[i];
+      if (c < 0) continue;
+      const int64_t o = b * K + slot[i], tok = c_cand[c].v;
+      bool fin = s_done[c / K];
+      for (int e = 0; e < a.n_eos; ++e) fin |= tok == a.eos_ids[e];
+      a.out_scores[o] = c_score[c];
+      a.out_parent[o] = c / K;
+      a.out_token[o] = tok;
+      a.out_finished[o] = fin;
+    }
+  }
+}
+
+size_t align16(size_t x) { return (x + 15) & ~(size_t)15; }
+
+// ------------------------------------------------------------------------------------------- reorder
+
+constexpr int kMoveThreads = 256;
+constexpr int kMaxItems = 128;
+
+struct MoveItem {
+  unsigned char* base;
+  int64_t outer_stride, beam_stride, row_stride;
+  int64_t lo;                         // first byte of a row
+  int64_t units;                      // n_row * units_per_row
+  uint32_t row_units;                 // units of a row
+  int32_t unit;
+  uint32_t first_block, blocks;       // of one (outer, group)
+};
+
+struct MoveParams {
+  const int32_t* parent;
+  int32_t* status;
+  int K, B, n_items;
+  MoveItem item[kMaxItems];
+};
+
+template <typename V, int KM, int U>
+B3_DEV void move_units(const MoveItem& it, unsigned char* group, uint32_t blk, int K, const int (&par)[KM], unsigned moved) {
+  const int64_t i0 = (int64_t)blk * (kMoveThreads * U) + threadIdx.x;
+  V v[KM][U];
+  int64_t off[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t i = i0 + u * kMoveThreads;
+    const int64_t r = i / it.row_units;
+    off[u] = i < it.units ? r * it.row_stride + it.lo + (i - r * it.row_units) * (int64_t)sizeof(V) : -1;
+  }
+#pragma unroll
+  for (int j = 0; j < KM; ++j)
+    if (moved >> j & 1) {
+      const unsigned char* src = group + par[j] * it.beam_stride;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (off[u] >= 0) v[j][u] = *reinterpret_cast<const V*>(src + off[u]);
+    }
+#pragma unroll
+  for (int j = 0; j < KM; ++j)
+    if (moved >> j & 1) {
+      unsigned char* dst = group + j * it.beam_stride;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (off[u] >= 0) *reinterpret_cast<V*>(dst + off[u]) = v[j][u];
+    }
+}
+
+template <int KM>
+constexpr int units_per_thread() { return KM <= 4 ? 4 : KM <= 8 ? 2 : 1; }
+
+template <int KM>
+__global__ void __launch_bounds__(kMoveThreads) reorder_kernel(const __grid_constant__ MoveParams p) {
+  constexpr int U = units_per_thread<KM>();
+  // the item of this block: the last one that starts at or before it
+  int lo = 0, hi = p.n_items - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (p.item[mid].first_block <= blockIdx.x) lo = mid;
+    else hi = mid - 1;
+  }
+  const MoveItem& it = p.item[lo];
+  const uint32_t local = blockIdx.x - it.first_block;
+  const uint32_t blk = local % it.blocks, og = local / it.blocks;
+  const int g = (int)(og % p.B), outer = (int)(og / p.B);
+  int par[KM];
+  unsigned moved = 0;
+#pragma unroll
+  for (int j = 0; j < KM; ++j) {
+    par[j] = j;
+    if (j < p.K) {
+      const int q = p.parent[(int64_t)g * p.K + j];
+      if (q < 0 || q >= p.K) {
+        if (threadIdx.x == 0 && p.status) atomicOr(p.status, 8);
+      } else if (q != j) {
+        par[j] = q;
+        moved |= 1u << j;
+      }
+    }
+  }
+  if (moved == 0) return;
+  unsigned char* group = it.base + outer * it.outer_stride + (int64_t)g * p.K * it.beam_stride;
+  if (it.unit == 16) move_units<uint4, KM, U>(it, group, blk, p.K, par, moved);
+  else if (it.unit == 4) move_units<uint32_t, KM, U>(it, group, blk, p.K, par, moved);
+  else move_units<unsigned char, KM, U>(it, group, blk, p.K, par, moved);
+}
+
+template <int KM>
+int launch_reorder(const MoveParams& p, uint32_t blocks, cudaStream_t s) {
+  reorder_kernel<KM><<<blocks, kMoveThreads, 0, s>>>(p);
+  return cudaGetLastError() == cudaSuccess ? BOLT3_OK : BOLT3_ERR_CUDA;
+}
+
+}  // namespace
+
+extern "C" size_t bolt3_beam_select_workspace(int B, int K, int64_t V) {
+  if (B <= 0 || K <= 0 || K > kMaxK || V <= 0 || V > kMaxV) return 0;
+  const size_t rows = (size_t)B * K, nc = (size_t)((V + kChunk - 1) / kChunk);
+  return align16(rows * nc * sizeof(float2)) + align16(rows * nc * K * sizeof(Cand));
+}
+
+extern "C" int bolt3_beam_select(const bolt3_beam_select_args* a, void* stream) {
+  const b3::TraceRange trace_range("bolt3_beam_select");
+  if (!a || !a->logits || !a->scores || !a->out_scores || !a->out_parent || !a->out_token || !a->out_finished)
+    return BOLT3_ERR_ARG;
+  if (a->n_eos < 0 || a->n_eos > 8) return BOLT3_ERR_ARG;
+  if (a->finished != nullptr && a->n_eos == 0) return BOLT3_ERR_ARG;   // a finished beam goes on with eos_ids[0]
+  if (a->B <= 0 || a->K <= 0 || a->K > kMaxK || a->V <= 0 || a->V > kMaxV || (int64_t)a->B * a->K > 0x7fffffff)
+    return BOLT3_ERR_SHAPE;
+  if (a->row_stride < a->V) return BOLT3_ERR_CAPACITY;
+  const uintptr_t el = a->logits_fp32 ? 3 : 1;
+  if (((uintptr_t)a->logits & el) || ((uintptr_t)a->workspace & 15)) return BOLT3_ERR_ALIGN;
+  if (!a->workspace || a->workspace_bytes < bolt3_beam_select_workspace(a->B, a->K, a->V)) return BOLT3_ERR_CAPACITY;
+  for (int i = 0; i < a->n_eos; ++i)
+    if (a->eos_ids[i] < 0 || a->eos_ids[i] >= a->V) return BOLT3_ERR_ARG;
+  SelParams p;
+  p.a = *a;
+  p.n_chunks = (int)((a->V + kChunk - 1) / kChunk);
+  const size_t rows = (size_t)a->B * a->K;
+  p.sums = reinterpret_cast<float2*>(a->workspace);
+  p.cands = reinterpret_cast<Cand*>(reinterpret_cast<char*>(a->workspace) + align16(rows * p.n_chunks * sizeof(float2)));
+  cudaStream_t s = (cudaStream_t)stream;
+  const dim3 grid((unsigned)rows, (unsigned)p.n_chunks);
+  if (a->logits_fp32) select_chunk_kernel<true><<<grid, kSelThreads, 0, s>>>(p);
+  else select_chunk_kernel<false><<<grid, kSelThreads, 0, s>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return BOLT3_ERR_CUDA;
+  const size_t smem = (size_t)a->K * p.n_chunks * a->K * sizeof(Cand);
+  if (smem > 40 * 1024 &&
+      cudaFuncSetAttribute(select_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return BOLT3_ERR_CUDA;
+  select_group_kernel<<<(unsigned)a->B, 32 * a->K, smem, s>>>(p);
+  return cudaGetLastError() == cudaSuccess ? BOLT3_OK : BOLT3_ERR_CUDA;
+}
+
+extern "C" int bolt3_beam_reorder(const bolt3_beam_reorder_args* a, void* stream) {
+  const b3::TraceRange trace_range("bolt3_beam_reorder");
+  if (!a || !a->parent || (a->n_items > 0 && !a->items) || a->n_items < 0) return BOLT3_ERR_ARG;
+  if (a->B <= 0 || a->K <= 0 || a->K > kMaxK) return BOLT3_ERR_SHAPE;
+  if (a->t0 < 0 || a->t1 < a->t0) return BOLT3_ERR_ARG;
+  for (int i = 0; i < a->n_items; ++i) {
+    const bolt3_beam_item& it = a->items[i];
+    if (!it.base || it.n_outer <= 0 || it.n_row <= 0 || it.row_bytes <= 0 || it.token_bytes < 0) return BOLT3_ERR_ARG;
+    if (it.unit != 1 && it.unit != 4 && it.unit != 16) return BOLT3_ERR_ARG;
+    if (it.token_bytes > 0 && a->t1 > it.row_bytes / it.token_bytes) return BOLT3_ERR_CAPACITY;
+    const int64_t m = it.outer_stride | it.beam_stride | it.row_stride | it.token_bytes |
+                      (it.token_bytes > 0 ? 0 : it.row_bytes) | (int64_t)(uintptr_t)it.base;
+    if (m & (it.unit - 1)) return BOLT3_ERR_ALIGN;
+  }
+  const int km = a->K <= 4 ? 4 : a->K <= 8 ? 8 : 16;
+  const int per_block = kMoveThreads * (km == 4 ? units_per_thread<4>() : km == 8 ? units_per_thread<8>() : units_per_thread<16>());
+  cudaStream_t s = (cudaStream_t)stream;
+  MoveParams p;
+  p.parent = a->parent;
+  p.status = a->status;
+  p.K = a->K;
+  p.B = a->B;
+  int i = 0;
+  while (i < a->n_items) {
+    uint64_t blocks = 0;
+    p.n_items = 0;
+    for (; i < a->n_items && p.n_items < kMaxItems; ++i) {
+      const bolt3_beam_item& it = a->items[i];
+      const int64_t lo = it.token_bytes > 0 ? a->t0 * it.token_bytes : 0;
+      const int64_t bytes = it.token_bytes > 0 ? (a->t1 - a->t0) * it.token_bytes : it.row_bytes;
+      if (bytes == 0) continue;
+      MoveItem m;
+      m.base = reinterpret_cast<unsigned char*>(it.base);
+      m.outer_stride = it.outer_stride; m.beam_stride = it.beam_stride; m.row_stride = it.row_stride;
+      m.lo = lo;
+      m.unit = it.unit;
+      if (bytes / it.unit > 0x7fffffff) return BOLT3_ERR_SHAPE;
+      m.row_units = (uint32_t)(bytes / it.unit);
+      m.units = (int64_t)m.row_units * it.n_row;
+      const uint64_t nb = (uint64_t)((m.units + per_block - 1) / per_block);
+      const uint64_t total = nb * (uint64_t)it.n_outer * (uint64_t)a->B;
+      if (nb > 0x7fffffff || total > 0x7fffffff) return BOLT3_ERR_SHAPE;
+      if (blocks + total > 0x7fffffff) break;            // the rest goes into another launch
+      m.blocks = (uint32_t)nb;
+      m.first_block = (uint32_t)blocks;
+      blocks += total;
+      p.item[p.n_items++] = m;
+    }
+    if (p.n_items == 0) continue;
+    const int rc = km == 4 ? launch_reorder<4>(p, (uint32_t)blocks, s)
+                 : km == 8 ? launch_reorder<8>(p, (uint32_t)blocks, s)
+                           : launch_reorder<16>(p, (uint32_t)blocks, s);
+    if (rc != BOLT3_OK) return rc;
+  }
+  return BOLT3_OK;
+}
