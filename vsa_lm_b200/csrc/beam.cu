@@ -49,10 +49,54 @@ B3_DEV bool row_live(const bolt3_beam_select_args& a, int64_t r) {
   return !(a.finished != nullptr && a.finished[r]) && a.scores[r] > neg_inf();
 }
 
+B3_DEV float ex2(float x) {      // 2^x, relative error 2^-22
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+// the larger of two bf16 pairs, a number before a NaN
+B3_DEV uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.bf16x2 %0, %1, %2;\n" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// A thread's logits as they were loaded: words of one fp32 or two bf16. `clean` replaces NaNs by -infinity.
+template <bool FP32>
+struct Logits {
+  static constexpr int EPL = FP32 ? 4 : 8;            // logits of a 16-byte load
+  static constexpr int NL = kPerThread / EPL;
+  static constexpr uint32_t kNone = FP32 ? 0xff800000u : 0xff80ff80u;   // -infinity in every place
+  uint32_t w[4 * NL];
+  B3_DEV void clean(float& m) {                       // m: the largest
+    if constexpr (FP32) {
+      m = neg_inf();
+#pragma unroll
+      for (int i = 0; i < 4 * NL; ++i) {
+        w[i] = __float_as_uint(fmaxf(__uint_as_float(w[i]), neg_inf()));
+        m = fmaxf(m, __uint_as_float(w[i]));
+      }
+    } else {
+      uint32_t mm = kNone;
+#pragma unroll
+      for (int i = 0; i < 4 * NL; ++i) {
+        w[i] = max_bf16x2(w[i], kNone);
+        mm = max_bf16x2(mm, w[i]);
+      }
+      const float2 f = unpack_bf16(mm);
+      m = fmaxf(f.x, f.y);
+    }
+  }
+  B3_DEV float x(int i) const {
+    if constexpr (FP32) return __uint_as_float(w[i]);
+    else return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  }
+};
+
 template <bool FP32>
 __global__ void __launch_bounds__(kSelThreads) select_chunk_kernel(const SelParams p) {
-  constexpr int EPL = FP32 ? 4 : 8;                   // logits of a 16-byte load
-  constexpr int NL = kPerThread / EPL;
+  using L = Logits<FP32>;
+  constexpr int EPL = L::EPL;
   __shared__ float s_max[16];
   __shared__ float s_sum[8];
   __shared__ int s_count;
@@ -60,44 +104,39 @@ __global__ void __launch_bounds__(kSelThreads) select_chunk_kernel(const SelPara
   const bolt3_beam_select_args& a = p.a;
   const int64_t r = blockIdx.x;
   const int chunk = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (!row_live(a, r)) return;
   const int64_t lo = (int64_t)chunk * kChunk;
   const int n = (int)min((int64_t)kChunk, a.V - lo);
   const char* row = reinterpret_cast<const char*>(a.logits) + (r * a.row_stride + lo) * (FP32 ? 4 : 2);
   const bool vec = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
-  float x[kPerThread];
+  grid_dep_launch();
+  grid_dep_wait();
+  if (!row_live(a, r)) return;
+  L l;
 #pragma unroll
-  for (int i = 0; i < NL; ++i) {
+  for (int i = 0; i < L::NL; ++i) {
     const int e = (i * kSelThreads + tid) * EPL;
+    uint4 q = make_uint4(L::kNone, L::kNone, L::kNone, L::kNone);
     if (vec && e + EPL <= n) {
-      const uint4 w = __ldcs(reinterpret_cast<const uint4*>(row + (size_t)e * (FP32 ? 4 : 2)));
-      if constexpr (FP32) {
-        x[4 * i] = __uint_as_float(w.x); x[4 * i + 1] = __uint_as_float(w.y);
-        x[4 * i + 2] = __uint_as_float(w.z); x[4 * i + 3] = __uint_as_float(w.w);
-      } else {
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = unpack_bf16(ww[j]);
-          x[8 * i + 2 * j] = f.x;
-          x[8 * i + 2 * j + 1] = f.y;
-        }
-      }
-    } else {
+      q = __ldcs(reinterpret_cast<const uint4*>(row + (size_t)e * (FP32 ? 4 : 2)));
+    } else if (e < n) {
+      uint32_t w[4] = {L::kNone, L::kNone, L::kNone, L::kNone};
 #pragma unroll
       for (int j = 0; j < EPL; ++j)
-        x[EPL * i + j] = e + j >= n ? neg_inf()
-                         : FP32     ? reinterpret_cast<const float*>(row)[e + j]
-                                    : bf2f(reinterpret_cast<const bf16*>(row)[e + j]);
+        if (e + j < n) {
+          if constexpr (FP32) {
+            w[j] = reinterpret_cast<const uint32_t*>(row)[e + j];
+          } else {
+            const uint32_t v = reinterpret_cast<const uint16_t*>(row)[e + j];
+            w[j / 2] = j & 1 ? (w[j / 2] & 0xffffu) | v << 16 : (w[j / 2] & 0xffff0000u) | v;
+          }
+        }
+      q = make_uint4(w[0], w[1], w[2], w[3]);
     }
+    l.w[4 * i] = q.x; l.w[4 * i + 1] = q.y; l.w[4 * i + 2] = q.z; l.w[4 * i + 3] = q.w;
   }
   auto index = [&](int i) { return (int)lo + ((i / EPL) * kSelThreads + tid) * EPL + i % EPL; };
-  float m = neg_inf();
-#pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
-    if (x[i] != x[i]) x[i] = neg_inf();
-    m = fmaxf(m, x[i]);
-  }
+  float m;
+  l.clean(m);
   float g = m;                                        // maximum of the half-warp, then of the block
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
@@ -110,26 +149,29 @@ __global__ void __launch_bounds__(kSelThreads) select_chunk_kernel(const SelPara
   float top = neg_inf();
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const float o = __shfl_sync(0xffffffffu, g, i);
+    const float o = s_max[i];
     rank += o > g || (o == g && i < (lane & 15));
     top = fmaxf(top, o);
   }
   const unsigned who = __ballot_sync(0xffffffffu, rank == a.K - 1);
   const float tau = __shfl_sync(0xffffffffu, g, __ffs(who) - 1);
-  float sum = 0.f;
+  float sum = 0.f, sum2 = 0.f;
   if (top > neg_inf()) {
     const float off = top * kLog2e;
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) sum += exp2f(fmaf(x[i], kLog2e, -off));
+    for (int i = 0; i < kPerThread; i += 2) {
+      sum += ex2(fmaf(l.x(i), kLog2e, -off));
+      sum2 += ex2(fmaf(l.x(i + 1), kLog2e, -off));
+    }
   }
-  sum = warp_sum(sum);
+  sum = warp_sum(sum + sum2);
   if (lane == 0) s_sum[warp] = sum;
   if (m >= tau && m > neg_inf()) {
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i)
-      if (x[i] >= tau && x[i] > neg_inf()) {
+      if (l.x(i) >= tau && l.x(i) > neg_inf()) {
         const int at = atomicAdd(&s_count, 1);        // the list's order does not matter: it is ranked below
-        if (at < kListCap) s_list[at] = Cand{x[i], index(i)};
+        if (at < kListCap) s_list[at] = Cand{l.x(i), index(i)};
       }
   }
   __syncthreads();
@@ -157,7 +199,7 @@ __global__ void __launch_bounds__(kSelThreads) select_chunk_kernel(const SelPara
     Cand best{neg_inf(), 0x7fffffff};
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
-      const Cand c{x[i], index(i)};
+      const Cand c{l.x(i), index(i)};
       if (c.x > neg_inf() && before(last, c) && before(c, best)) best = c;
     }
 #pragma unroll
@@ -180,7 +222,7 @@ __global__ void __launch_bounds__(kSelThreads) select_chunk_kernel(const SelPara
 __global__ void __launch_bounds__(32 * kMaxK) select_group_kernel(const SelParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float c_score[kMaxK * kMaxK];
-  __shared__ Cand c_cand[kMaxK * kMaxK];
+  __shared__ int32_t c_token[kMaxK * kMaxK];
   __shared__ int s_pick[kMaxK];
   __shared__ bool s_done[kMaxK];
   const bolt3_beam_select_args& a = p.a;
@@ -188,12 +230,13 @@ __global__ void __launch_bounds__(32 * kMaxK) select_group_kernel(const SelParam
   const int64_t b = blockIdx.x, r = b * K + k;
   const int per_row = p.n_chunks * K;
   Cand* all = reinterpret_cast<Cand*>(smem) + (size_t)k * per_row;
-  const bool live = row_live(a, r);
+  grid_dep_launch();
+  grid_dep_wait();
   const bool done = a.finished != nullptr && a.finished[r];
   const float own = a.scores[r];
   if (tid < kMaxK) s_pick[tid] = -1;
   if (lane == 0) s_done[k] = done;       // the outputs may be the inputs: nothing of these is read later
-  if (live) {
+  if (!done && own > neg_inf()) {
     for (int i = lane; i < per_row; i += 32) all[i] = p.cands[r * per_row + i];
     float m = neg_inf();
     for (int i = lane; i < p.n_chunks; i += 32) m = fmaxf(m, p.sums[r * p.n_chunks + i].x);
@@ -206,40 +249,39 @@ __global__ void __launch_bounds__(32 * kMaxK) select_group_kernel(const SelParam
     s = warp_sum(s);
     const float lse = m + logf(s);
     __syncwarp();
-    // each lane walks the sorted lists of two chunks (at most 64)
+    // each lane walks the sorted lists of two chunks (at most 64); the order is (logit, lowest index) as a pair of
+    // integers (x + 0 makes one of the two zeros)
     int at[2] = {0, 0};
     for (int i = 0; i < K; ++i) {
-      Cand best{neg_inf(), 0x7fffffff};
-      int from = -1;
+      uint32_t key[2] = {0, 0};
+      int32_t v[2] = {0x7fffffff, 0x7fffffff};
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int c = lane + 32 * j;
         if (c < p.n_chunks && at[j] < K) {
           const Cand h = all[c * K + at[j]];
-          if (h.v >= 0 && before(h, best)) {
-            best = h;
-            from = j;
+          if (h.v >= 0) {
+            key[j] = fkey(h.x + 0.f);
+            v[j] = h.v;
           }
         }
       }
-      Cand win = best;
+      const uint32_t top = __reduce_max_sync(0xffffffffu, max(key[0], key[1]));
+      const int32_t win = __reduce_min_sync(0xffffffffu, min(key[0] == top ? v[0] : 0x7fffffff, key[1] == top ? v[1] : 0x7fffffff));
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const Cand c{__shfl_xor_sync(0xffffffffu, win.x, o), __shfl_xor_sync(0xffffffffu, win.v, o)};
-        if (before(c, win)) win = c;
-      }
-      if (from >= 0 && best.v == win.v) at[from]++;
-      if (lane == 0) {
-        float sc = neg_inf();
-        if (win.v != 0x7fffffff) sc = own + (win.x - lse);
-        c_score[k * K + i] = sc != sc ? neg_inf() : sc;
-        c_cand[k * K + i] = win;
-      }
+      for (int j = 0; j < 2; ++j)
+        if (key[j] == top && v[j] == win && win != 0x7fffffff) {
+          const float sc = own + (all[(lane + 32 * j) * K + at[j]].x - lse);
+          c_score[k * K + i] = sc != sc ? neg_inf() : sc;
+          c_token[k * K + i] = win;
+          at[j]++;
+        }
+      if (win == 0x7fffffff && lane == 0) c_score[k * K + i] = neg_inf();
     }
   } else if (lane < K) {
     const float sc = done && lane == 0 ? own : neg_inf();
     c_score[k * K + lane] = sc != sc ? neg_inf() : sc;
-    c_cand[k * K + lane] = Cand{0.f, (int32_t)a.eos_ids[0]};
+    c_token[k * K + lane] = (int32_t)a.eos_ids[0];
   }
   __syncthreads();
   // rank of every candidate: score, then beam, then its place in the beam's list
@@ -251,44 +293,35 @@ __global__ void __launch_bounds__(32 * kMaxK) select_group_kernel(const SelParam
     if (better < K) s_pick[better] = i;
   }
   __syncthreads();
-  if (tid == 0) {
-    unsigned taken = 0, later = 0;
-    int slot[kMaxK];
-    for (int i = 0; i < K; ++i) {
-      const int c = s_pick[i];
-      if (c < 0) continue;
-      const int par = c / K;
-      if (taken >> par & 1) {
-        later |= 1u << i;
-      } else {
-        taken |= 1u << par;
-        slot[i] = par;
-      }
-    }
-    for (int i = 0; i < K; ++i) {
-      if (!(later >> i & 1)) continue;
-      const int f = __ffs(~taken) - 1;
-      taken |= 1u << f;
-      slot[i] = f;
-    }
-    for (int j = 0; j < K; ++j) {
-      if (taken >> j & 1) continue;
-      a.out_scores[b * K + j] = neg_inf();
-      a.out_parent[b * K + j] = j;
-      a.out_token[b * K + j] = a.n_eos > 0 ? a.eos_ids[0] : 0;
-      a.out_finished[b * K + j] = 1;
-    }
-    for (int i = 0; i < K; ++i) {
-      const int c = s_pick[i];
-      if (c < 0) continue;
-      const int64_t o = b * K + slot[i], tok = c_cand[c].v;
-      bool fin = s_done[c / K];
-      for (int e = 0; e < a.n_eos; ++e) fin |= tok == a.eos_ids[e];
-      a.out_scores[o] = c_score[c];
-      a.out_parent[o] = c / K;
-      a.out_token[o] = tok;
-      a.out_finished[o] = fin;
-    }
+  if (tid >= 32) return;
+  // lane i: the continuation of rank i. The first child of a parent takes the parent's slot, the others what is left
+  const int c = lane < K ? s_pick[lane] : -1;
+  const int par = c < 0 ? 32 + lane : c / K;
+  const unsigned same = __match_any_sync(0xffffffffu, par);
+  const bool first = c >= 0 && __ffs(same) - 1 == lane;
+  const unsigned held = __reduce_or_sync(0xffffffffu, first ? 1u << par : 0u);
+  const unsigned later = __ballot_sync(0xffffffffu, c >= 0 && !first);
+  int slot = par;
+  if (c >= 0 && !first) {
+    unsigned left = ~held;
+    for (int i = __popc(later & ((1u << lane) - 1)); i > 0; --i) left &= left - 1;
+    slot = __ffs(left) - 1;
+  }
+  const unsigned used = __reduce_or_sync(0xffffffffu, c >= 0 ? 1u << slot : 0u);
+  if (lane < K && !(used >> lane & 1)) {
+    a.out_scores[b * K + lane] = neg_inf();
+    a.out_parent[b * K + lane] = lane;
+    a.out_token[b * K + lane] = a.n_eos > 0 ? a.eos_ids[0] : 0;
+    a.out_finished[b * K + lane] = 1;
+  }
+  if (c >= 0) {
+    const int64_t o = b * K + slot, tok = c_token[c];
+    bool fin = s_done[par];
+    for (int e = 0; e < a.n_eos; ++e) fin |= tok == a.eos_ids[e];
+    a.out_scores[o] = c_score[c];
+    a.out_parent[o] = par;
+    a.out_token[o] = tok;
+    a.out_finished[o] = fin;
   }
 }
 
@@ -420,15 +453,15 @@ extern "C" int bolt3_beam_select(const bolt3_beam_select_args* a, void* stream) 
   p.cands = reinterpret_cast<Cand*>(reinterpret_cast<char*>(a->workspace) + align16(rows * p.n_chunks * sizeof(float2)));
   cudaStream_t s = (cudaStream_t)stream;
   const dim3 grid((unsigned)rows, (unsigned)p.n_chunks);
-  if (a->logits_fp32) select_chunk_kernel<true><<<grid, kSelThreads, 0, s>>>(p);
-  else select_chunk_kernel<false><<<grid, kSelThreads, 0, s>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return BOLT3_ERR_CUDA;
+  if (launch_overlapped(a->logits_fp32 ? select_chunk_kernel<true> : select_chunk_kernel<false>, grid, dim3(kSelThreads), 0,
+                        s, p) != cudaSuccess)
+    return BOLT3_ERR_CUDA;
   const size_t smem = (size_t)a->K * p.n_chunks * a->K * sizeof(Cand);
   if (smem > 40 * 1024 &&
       cudaFuncSetAttribute(select_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return BOLT3_ERR_CUDA;
-  select_group_kernel<<<(unsigned)a->B, 32 * a->K, smem, s>>>(p);
-  return cudaGetLastError() == cudaSuccess ? BOLT3_OK : BOLT3_ERR_CUDA;
+  return launch_overlapped(select_group_kernel, dim3((unsigned)a->B), dim3(32 * a->K), smem, s, p) == cudaSuccess
+             ? BOLT3_OK : BOLT3_ERR_CUDA;
 }
 
 extern "C" int bolt3_beam_reorder(const bolt3_beam_reorder_args* a, void* stream) {
