@@ -3,8 +3,7 @@
 // select. With lse_k = log sum_v e^x_kv, continuation (k, v) scores s_k + (x_kv - lse_k); the K best of a
 // group's K * V survive. Bound by HBM: the logits are read once. Within a beam the order is the logits',
 // so the pass that sums the exponentials also finds each chunk's K best logits:
-// - select_chunk_kernel: a block holds a chunk of 8192 logits of one row in registers. Maximum and sum of
-//   exponentials, then a threshold: the K-th largest of 16 half-warp maxima is no larger than the chunk's
+// - select_chunk_kernel: a block holds a chunk of one row in registers (8192 fp32 or 16384 bf16 logits). Maximum and sum of exponentials, then a threshold: the K-th largest of 16 half-warp maxima is no larger than the chunk's
 //   K-th largest logit, so the few logits at or above it contain the K best; they are ranked by counting.
 //   Chunks with many equal logits (more than the list holds) take K rounds of a block maximum instead.
 // - select_group_kernel: a block per group merges the chunks' sums and lists, scores, ranks and assigns slots.
@@ -25,10 +24,17 @@ constexpr float kLog2e = 1.4426950408889634f;
 // ------------------------------------------------------------------------------------------- select
 
 constexpr int kSelThreads = 256;
-constexpr int kPerThread = 32;
-constexpr int kChunk = kSelThreads * kPerThread;      // logits of a block
+constexpr int kMinChunk = 8192;                       // logits of a block: fp32; bf16 twice that
+template <bool FP32>
+constexpr int kPerThread = FP32 ? 32 : 64;
+template <bool FP32>
+constexpr int kChunk = kSelThreads * kPerThread<FP32>;
+constexpr int kSelBlocks = 5;                         // of an SM
 constexpr int kListCap = 256;                         // candidates at or above the threshold
-constexpr int64_t kMaxV = 64 * kChunk;
+constexpr int64_t kMaxV = 64 * kMinChunk;             // (with a slip a row may have 65 chunks)
+
+// the float of an fkey
+B3_DEV float unkey(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 struct Cand {
   float x;
@@ -54,6 +60,27 @@ B3_DEV float ex2(float x) {      // 2^x, relative error 2^-22
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
 }
+// two fp32 at a time
+B3_DEV uint64_t pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+B3_DEV float2 unpair(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+B3_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+B3_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 // the larger of two bf16 pairs, a number before a NaN
 B3_DEV uint32_t max_bf16x2(uint32_t a, uint32_t b) {
   uint32_t d;
@@ -61,127 +88,158 @@ B3_DEV uint32_t max_bf16x2(uint32_t a, uint32_t b) {
   return d;
 }
 
-// A thread's logits as they were loaded: words of one fp32 or two bf16. `clean` replaces NaNs by -infinity.
+// A thread's logits as they were loaded: words of one fp32 or two bf16
 template <bool FP32>
 struct Logits {
   static constexpr int EPL = FP32 ? 4 : 8;            // logits of a 16-byte load
-  static constexpr int NL = kPerThread / EPL;
+  static constexpr int NW = 32;
   static constexpr uint32_t kNone = FP32 ? 0xff800000u : 0xff80ff80u;   // -infinity in every place
-  uint32_t w[4 * NL];
-  B3_DEV void clean(float& m) {                       // m: the largest
+  uint32_t w[NW];
+  B3_DEV float largest() const {                      // NaNs left out
     if constexpr (FP32) {
-      m = neg_inf();
+      float m = neg_inf();
 #pragma unroll
-      for (int i = 0; i < 4 * NL; ++i) {
-        w[i] = __float_as_uint(fmaxf(__uint_as_float(w[i]), neg_inf()));
-        m = fmaxf(m, __uint_as_float(w[i]));
-      }
+      for (int i = 0; i < NW; ++i) m = fmaxf(m, __uint_as_float(w[i]));
+      return m;
     } else {
-      uint32_t mm = kNone;
+      uint32_t m = kNone;
 #pragma unroll
-      for (int i = 0; i < 4 * NL; ++i) {
-        w[i] = max_bf16x2(w[i], kNone);
-        mm = max_bf16x2(mm, w[i]);
-      }
-      const float2 f = unpack_bf16(mm);
-      m = fmaxf(f.x, f.y);
+      for (int i = 0; i < NW; ++i) m = max_bf16x2(m, w[i]);
+      const float2 f = unpack_bf16(m);
+      return fmaxf(f.x, f.y);
     }
   }
   B3_DEV float x(int i) const {
     if constexpr (FP32) return __uint_as_float(w[i]);
     else return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
   }
+  // of words 16 h .. 16 h + 15 (bf16) or all (fp32): a bit for every logit at or above t, a bf16 value where they are
+  B3_DEV uint32_t at_least(float t, int h) const {
+    uint32_t mask = 0;
+    if constexpr (FP32) {
+#pragma unroll
+      for (int i = 0; i < NW; ++i) mask |= __uint_as_float(w[i]) >= t ? 1u << i : 0u;
+    } else {
+      const __nv_bfloat162 tt = __float2bfloat162_rn(t);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        mask |= __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w[16 * h + i]), tt) & (0x10001u << i);
+    }
+    return mask;
+  }
+  static B3_DEV int of_bit(int bit, int h) { return FP32 ? bit : 32 * h + (bit & 15) * 2 + (bit >> 4); }
 };
 
 template <bool FP32>
-__global__ void __launch_bounds__(kSelThreads) select_chunk_kernel(const SelParams p) {
+__global__ void __launch_bounds__(kSelThreads, kSelBlocks) select_chunk_kernel(const __grid_constant__ SelParams p) {
   using L = Logits<FP32>;
-  constexpr int EPL = L::EPL;
-  __shared__ float s_max[16];
-  __shared__ float s_sum[8];
+  constexpr int EPL = L::EPL, kBytes = FP32 ? 4 : 2, kPer = kPerThread<FP32>;
+  __shared__ float s_max[16], s_sum[8];
   __shared__ int s_count;
   __shared__ Cand s_list[kListCap];
   const bolt3_beam_select_args& a = p.a;
-  const int64_t r = blockIdx.x;
-  const int chunk = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t lo = (int64_t)chunk * kChunk;
-  const int n = (int)min((int64_t)kChunk, a.V - lo);
-  const char* row = reinterpret_cast<const char*>(a.logits) + (r * a.row_stride + lo) * (FP32 ? 4 : 2);
-  const bool vec = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t r = blockIdx.x, item = r * p.n_chunks + blockIdx.y;
+  // Chunks are cut at 16-byte boundaries whatever the row's alignment: logit e of the chunk is logit lo + e of the row,
+  // lo < 0 where the row begins within the chunk's first 16 bytes
+  const char* row = reinterpret_cast<const char*>(a.logits) + r * a.row_stride * kBytes;
+  const int lo = (int)blockIdx.y * kChunk<FP32> - (int)(reinterpret_cast<uintptr_t>(row) & 15) / kBytes;
+  row += (int64_t)lo * kBytes;
+  const int from = max(0, -lo), n = min(kChunk<FP32>, (int)a.V - lo);   // logits of the chunk: [from, n)
   grid_dep_launch();
   grid_dep_wait();
   if (!row_live(a, r)) return;
+  auto bits = [&](int e) {
+    if constexpr (FP32) return reinterpret_cast<const uint32_t*>(row)[e];
+    else return (uint32_t) reinterpret_cast<const uint16_t*>(row)[e];
+  };
+  auto value = [&](int e) { return __uint_as_float(FP32 ? bits(e) : bits(e) << 16); };
+  auto place = [&](int i) { return ((i / EPL) * kSelThreads + tid) * EPL + i % EPL; };   // of a thread's logit i in the chunk
   L l;
 #pragma unroll
-  for (int i = 0; i < L::NL; ++i) {
+  for (int i = 0; i < L::NW / 4; ++i) {
     const int e = (i * kSelThreads + tid) * EPL;
     uint4 q = make_uint4(L::kNone, L::kNone, L::kNone, L::kNone);
-    if (vec && e + EPL <= n) {
-      q = __ldcs(reinterpret_cast<const uint4*>(row + (size_t)e * (FP32 ? 4 : 2)));
-    } else if (e < n) {
+    if (e >= from && e + EPL <= n) {
+      q = __ldcs(reinterpret_cast<const uint4*>(row + (int64_t)e * kBytes));
+    } else if (e + EPL > from && e < n) {             // the row's first or last 16 bytes
       uint32_t w[4] = {L::kNone, L::kNone, L::kNone, L::kNone};
 #pragma unroll
       for (int j = 0; j < EPL; ++j)
-        if (e + j < n) {
-          if constexpr (FP32) {
-            w[j] = reinterpret_cast<const uint32_t*>(row)[e + j];
-          } else {
-            const uint32_t v = reinterpret_cast<const uint16_t*>(row)[e + j];
-            w[j / 2] = j & 1 ? (w[j / 2] & 0xffffu) | v << 16 : (w[j / 2] & 0xffff0000u) | v;
-          }
+        if (e + j >= from && e + j < n) {
+          if constexpr (FP32) w[j] = bits(e + j);
+          else w[j / 2] = j & 1 ? (w[j / 2] & 0xffffu) | bits(e + j) << 16 : (w[j / 2] & 0xffff0000u) | bits(e + j);
         }
       q = make_uint4(w[0], w[1], w[2], w[3]);
     }
     l.w[4 * i] = q.x; l.w[4 * i + 1] = q.y; l.w[4 * i + 2] = q.z; l.w[4 * i + 3] = q.w;
   }
-  auto index = [&](int i) { return (int)lo + ((i / EPL) * kSelThreads + tid) * EPL + i % EPL; };
-  float m;
-  l.clean(m);
-  float g = m;                                        // maximum of the half-warp, then of the block
+  // every thread sums against its own maximum: nothing here waits for another warp
+  const float m = l.largest();
+  float sum = 0.f;
+  if (m > neg_inf()) {
+    const float off = m * kLog2e;
+    const uint64_t l2e = pair(kLog2e, kLog2e), minus = pair(-off, -off);
+    uint64_t s0 = 0, s1 = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; i += 4) {
+      const float2 u = unpair(fma2(pair(l.x(i), l.x(i + 1)), l2e, minus));
+      const float2 v = unpair(fma2(pair(l.x(i + 2), l.x(i + 3)), l2e, minus));
+      s0 = add2(s0, pair(ex2(u.x), ex2(u.y)));
+      s1 = add2(s1, pair(ex2(v.x), ex2(v.y)));
+    }
+    const float2 u = unpair(add2(s0, s1));
+    sum = u.x + u.y;
+    if (sum != sum) {                                 // NaNs among the logits count as -infinity
+      sum = 0.f;
+#pragma unroll 1
+      for (int i = 0; i < kPer; ++i)
+        if (place(i) >= from && place(i) < n) sum += ex2(fmaf(fmaxf(value(place(i)), neg_inf()), kLog2e, -off));
+    }
+  }
+  float g = m;                                        // maximum of the half-warp, of the warp
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
   if ((lane & 15) == 0) s_max[warp * 2 + (lane >> 4)] = g;
+  g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 16));
+  sum = warp_sum(m > neg_inf() ? sum * ex2((m - g) * kLog2e) : 0.f);
+  if (lane == 0) s_sum[warp] = sum;
   if (tid == 0) s_count = 0;
   __syncthreads();
-  g = s_max[lane & 15];
-  // tau: the K-th largest of the 16 half-warps' maxima
-  int rank = 0;
-  float top = neg_inf();
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float o = s_max[i];
-    rank += o > g || (o == g && i < (lane & 15));
-    top = fmaxf(top, o);
+  // tau: the K-th largest of the 16 half-warps' maxima (one of them leaves per round)
+  uint32_t key = lane < 16 ? fkey(s_max[lane]) : 0;
+  uint32_t best = __reduce_max_sync(0xffffffffu, key);
+  const float top = unkey(best);
+#pragma unroll 1
+  for (int i = 1; i < a.K; ++i) {
+    if (lane == __ffs(__ballot_sync(0xffffffffu, key == best)) - 1) key = 0;
+    best = __reduce_max_sync(0xffffffffu, key);
   }
-  const unsigned who = __ballot_sync(0xffffffffu, rank == a.K - 1);
-  const float tau = __shfl_sync(0xffffffffu, g, __ffs(who) - 1);
-  float sum = 0.f, sum2 = 0.f;
-  if (top > neg_inf()) {
-    const float off = top * kLog2e;
-#pragma unroll
-    for (int i = 0; i < kPerThread; i += 2) {
-      sum += ex2(fmaf(l.x(i), kLog2e, -off));
-      sum2 += ex2(fmaf(l.x(i + 1), kLog2e, -off));
-    }
-  }
-  sum = warp_sum(sum + sum2);
-  if (lane == 0) s_sum[warp] = sum;
+  const float tau = unkey(best);
   if (m >= tau && m > neg_inf()) {
+    // tau is one of the logits, or -infinity: then any logit above that counts
+    const float t = tau > neg_inf() ? tau : FP32 ? -3.4028235e38f : -3.3895314e38f;
+    uint32_t mask[2] = {l.at_least(t, 0), FP32 ? 0u : l.at_least(t, 1)};
+    const bool one = __popc(mask[0]) + __popc(mask[1]) == 1;         // then it is the largest
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i)
-      if (l.x(i) >= tau && l.x(i) > neg_inf()) {
+    for (int h = 0; h < 2; ++h)
+      for (; mask[h]; mask[h] &= mask[h] - 1) {
+        const int e = place(L::of_bit(__ffs(mask[h]) - 1, h));
         const int at = atomicAdd(&s_count, 1);        // the list's order does not matter: it is ranked below
-        if (at < kListCap) s_list[at] = Cand{l.x(i), index(i)};
+        if (at < kListCap) s_list[at] = Cand{one ? m : value(e), lo + e};
       }
   }
   __syncthreads();
   const int count = s_count;
-  Cand* out = p.cands + (r * p.n_chunks + chunk) * a.K;
+  Cand* out = p.cands + item * a.K;
   if (tid == 0) {
     float t = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t += s_sum[i];
-    p.sums[r * p.n_chunks + chunk] = make_float2(top, t);
+    for (int i = 0; i < 8; ++i) {
+      const float g = fmaxf(s_max[2 * i], s_max[2 * i + 1]);
+      if (g > neg_inf()) t = fmaf(s_sum[i], ex2((g - top) * kLog2e), t);
+    }
+    p.sums[item] = make_float2(top, t);
   }
   if (count <= kListCap) {
     if (tid < count) {
@@ -195,11 +253,13 @@ __global__ void __launch_bounds__(kSelThreads) select_chunk_kernel(const SelPara
   }
   // many equal logits: K rounds, each the best candidate after the last one
   Cand last{__int_as_float(0x7f800000), -1};
+#pragma unroll 1
   for (int k = 0; k < a.K; ++k) {
     Cand best{neg_inf(), 0x7fffffff};
-#pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
-      const Cand c{l.x(i), index(i)};
+#pragma unroll 1
+    for (int i = 0; i < kPer; ++i) {
+      if (place(i) < from || place(i) >= n) continue;
+      const Cand c{value(place(i)), lo + place(i)};
       if (c.x > neg_inf() && before(last, c) && before(c, best)) best = c;
     }
 #pragma unroll
@@ -214,12 +274,12 @@ __global__ void __launch_bounds__(kSelThreads) select_chunk_kernel(const SelPara
     for (int i = 1; i < kSelThreads / 32; ++i)
       if (before(s_list[i], best)) best = s_list[i];
     last = best;
-    if (tid == 0) out[k] = best;                       // more than kListCap are above -infinity: all K exist
+    if (tid == 0) out[k] = best;                      // more than kListCap are above -infinity: all K exist
   }
 }
 
 // a block per group, a warp per beam for the merge of its chunks
-__global__ void __launch_bounds__(32 * kMaxK) select_group_kernel(const SelParams p) {
+__global__ void __launch_bounds__(32 * kMaxK) select_group_kernel(const __grid_constant__ SelParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float c_score[kMaxK * kMaxK];
   __shared__ int32_t c_token[kMaxK * kMaxK];
@@ -249,14 +309,14 @@ __global__ void __launch_bounds__(32 * kMaxK) select_group_kernel(const SelParam
     s = warp_sum(s);
     const float lse = m + logf(s);
     __syncwarp();
-    // each lane walks the sorted lists of two chunks (at most 64); the order is (logit, lowest index) as a pair of
+    // each lane walks the sorted lists of three chunks (at most 65 in all); the order is (logit, lowest index) as a pair of
     // integers (x + 0 makes one of the two zeros)
-    int at[2] = {0, 0};
+    int at[3] = {0, 0, 0};
     for (int i = 0; i < K; ++i) {
-      uint32_t key[2] = {0, 0};
-      int32_t v[2] = {0x7fffffff, 0x7fffffff};
+      uint32_t key[3] = {0, 0, 0};
+      int32_t v[3] = {0x7fffffff, 0x7fffffff, 0x7fffffff};
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < 3; ++j) {
         const int c = lane + 32 * j;
         if (c < p.n_chunks && at[j] < K) {
           const Cand h = all[c * K + at[j]];
@@ -266,10 +326,11 @@ __global__ void __launch_bounds__(32 * kMaxK) select_group_kernel(const SelParam
           }
         }
       }
-      const uint32_t top = __reduce_max_sync(0xffffffffu, max(key[0], key[1]));
-      const int32_t win = __reduce_min_sync(0xffffffffu, min(key[0] == top ? v[0] : 0x7fffffff, key[1] == top ? v[1] : 0x7fffffff));
+      const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(key[0], key[1]), key[2]));
+      const int32_t win = __reduce_min_sync(0xffffffffu, min(min(key[0] == top ? v[0] : 0x7fffffff, key[1] == top ? v[1] : 0x7fffffff),
+                                                             key[2] == top ? v[2] : 0x7fffffff));
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 3; ++j)
         if (key[j] == top && v[j] == win && win != 0x7fffffff) {
           const float sc = own + (all[(lane + 32 * j) * K + at[j]].x - lse);
           c_score[k * K + i] = sc != sc ? neg_inf() : sc;
@@ -427,7 +488,7 @@ int launch_reorder(const MoveParams& p, uint32_t blocks, cudaStream_t s) {
 
 extern "C" size_t bolt3_beam_select_workspace(int B, int K, int64_t V) {
   if (B <= 0 || K <= 0 || K > kMaxK || V <= 0 || V > kMaxV) return 0;
-  const size_t rows = (size_t)B * K, nc = (size_t)((V + kChunk - 1) / kChunk);
+  const size_t rows = (size_t)B * K, nc = (size_t)((V + 3 + kMinChunk - 1) / kMinChunk);
   return align16(rows * nc * sizeof(float2)) + align16(rows * nc * K * sizeof(Cand));
 }
 
@@ -437,7 +498,7 @@ extern "C" int bolt3_beam_select(const bolt3_beam_select_args* a, void* stream) 
     return BOLT3_ERR_ARG;
   if (a->n_eos < 0 || a->n_eos > 8) return BOLT3_ERR_ARG;
   if (a->finished != nullptr && a->n_eos == 0) return BOLT3_ERR_ARG;   // a finished beam goes on with eos_ids[0]
-  if (a->B <= 0 || a->K <= 0 || a->K > kMaxK || a->V <= 0 || a->V > kMaxV || (int64_t)a->B * a->K > 0x7fffffff)
+  if (a->B <= 0 || a->K <= 0 || a->K > kMaxK || a->V <= 0 || a->V > kMaxV || (int64_t)a->B * a->K > 0x1ffffff)
     return BOLT3_ERR_SHAPE;
   if (a->row_stride < a->V) return BOLT3_ERR_CAPACITY;
   const uintptr_t el = a->logits_fp32 ? 3 : 1;
@@ -447,7 +508,9 @@ extern "C" int bolt3_beam_select(const bolt3_beam_select_args* a, void* stream) 
     if (a->eos_ids[i] < 0 || a->eos_ids[i] >= a->V) return BOLT3_ERR_ARG;
   SelParams p;
   p.a = *a;
-  p.n_chunks = (int)((a->V + kChunk - 1) / kChunk);
+  const int chunk = a->logits_fp32 ? kChunk<true> : kChunk<false>;
+  const int slip = a->logits_fp32 ? 3 : 7;            // logits by which a row may begin after a 16-byte boundary
+  p.n_chunks = (int)((a->V + slip + chunk - 1) / chunk);
   const size_t rows = (size_t)a->B * a->K;
   p.sums = reinterpret_cast<float2*>(a->workspace);
   p.cands = reinterpret_cast<Cand*>(reinterpret_cast<char*>(a->workspace) + align16(rows * p.n_chunks * sizeof(float2)));
