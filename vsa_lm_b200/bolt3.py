@@ -539,12 +539,15 @@ class Bolt3LayerState:
 class Bolt3Decoder:
     """Constant-memory decoder (reference: vsa_lm/config/bolt3.py:279-557) with native Bolt-3 layers.
 
-    Softmax anchor layers use a static KV cache and SDPA as in the reference (bolt3.py:426-445).
+    Softmax anchor layers use a static KV cache and SDPA as in the reference (bolt3.py:426-445), or, with
+    kv_cache="int8", an 8-bit cache with kernels of its own for prompts and single tokens.
     """
 
     def __init__(self, model, wrap_positions: bool = False, max_cache_pos: int = 65536, cuda_graphs: bool = True,
-                 **kwargs):
+                 kv_cache: str = "bf16", **kwargs):
         self.model = model.eval()
+        _check_kv_cache(kv_cache)
+        self.kv_cache = kv_cache          # the anchors' caches: "bf16" (as the reference) or "int8" (AnchorKV8)
         self.max_T = model.config["max_T"]
         self.max_cache_pos = max_cache_pos
         self.C = int(model.config.get("bolt3_C", 128))
@@ -553,19 +556,25 @@ class Bolt3Decoder:
         self.use_cuda_graphs = cuda_graphs
 
     @staticmethod
-    def state_bytes(model):
+    def state_bytes(model, kv_cache: str = "bf16"):
         """(bytes of fixed-size state per sequence, bytes per token of the anchor layers' KV caches),
         the same pair the reference reports (bolt3.py:290-300), counted from the buffers this
-        decoder actually keeps (Bolt3LayerState.bytes_per_sequence, AnchorKV's bf16 k and v)."""
+        decoder actually keeps (Bolt3LayerState.bytes_per_sequence, AnchorKV's bf16 k and v or AnchorKV8's
+        int8 with a scale per row)."""
+        _check_kv_cache(kv_cache)
         fixed = sum(Bolt3LayerState.bytes_per_sequence(b.vsa) for b in model.blocks if hasattr(b, "vsa"))
-        per_token = sum(2 * b.attn.HKV * b.attn.HD * 2 for b in model.blocks if not hasattr(b, "vsa"))
+        row = (lambda hd: hd + 4) if kv_cache == "int8" else (lambda hd: 2 * hd)
+        per_token = sum(2 * b.attn.HKV * row(b.attn.HD) for b in model.blocks if not hasattr(b, "vsa"))
         return fixed, per_token
 
     @staticmethod
-    def blank_state(model, batch_size: int, device, max_kv_len: int = 4096, state_dtype=torch.float32, **kwargs):
+    def blank_state(model, batch_size: int, device, max_kv_len: int = 4096, state_dtype=torch.float32,
+                    kv_cache: str = "bf16", **kwargs):
         """(states, kv_caches) for `batch_size` sequences (bolt3.py:302-319): per Bolt-3 layer an fp32
         M_res [B, HKV, HD, HD] in states and a Bolt3LayerState in kv_caches; per softmax anchor an
-        AnchorKV with room for max_kv_len tokens. M_res is always fp32 (the kernels update it in place)."""
+        AnchorKV (kv_cache "int8": an AnchorKV8) with room for max_kv_len tokens. M_res is always fp32 (the
+        kernels update it in place)."""
+        _check_kv_cache(kv_cache)
         states, kv_caches = [], []
         for blk in model.blocks:
             if hasattr(blk, "vsa"):
@@ -575,7 +584,8 @@ class Bolt3Decoder:
             else:
                 a = blk.attn
                 states.append(None)
-                kv_caches.append(AnchorKV(batch_size, a.HKV, max_kv_len, a.HD, device, dt=torch.bfloat16))
+                kv_caches.append(AnchorKV8(batch_size, a.HKV, max_kv_len, a.HD, device) if kv_cache == "int8" else
+                                 AnchorKV(batch_size, a.HKV, max_kv_len, a.HD, device, dt=torch.bfloat16))
         return states, kv_caches
 
     @staticmethod
@@ -898,6 +908,9 @@ class Bolt3Decoder:
         dev_pos (a step captured into a CUDA graph) the position comes from the device and the cache's
         host count is left to the caller."""
         b, t, _ = h.shape
+        if isinstance(cache, AnchorKV8):
+            y = cache.attention(ly, h, pos_start, dev_pos)
+            return Bolt3Decoder._anchor_out(ly, y, partial_fp32)
         q, k, v = ly.head_qkv(h)
         if t == 1 and h.is_cuda and q.dtype == torch.bfloat16 and cache.buf.dtype == torch.bfloat16:
             if dev_pos is None:
@@ -923,9 +936,14 @@ class Bolt3Decoder:
             y = F.scaled_dot_product_attention(q, keys.to(q.dtype), vals.to(q.dtype), attn_mask=mask,
                                                enable_gqa=ly.G > 1)
             y = y.transpose(1, 2).reshape(b, t, ly.H * ly.HD)
+        return Bolt3Decoder._anchor_out(ly, y, partial_fp32)
+
+    @staticmethod
+    def _anchor_out(ly, y: torch.Tensor, partial_fp32: bool) -> torch.Tensor:
+        """o_proj of an anchor's attention output [b, t, H * HD]."""
         if partial_fp32:
             w = ly.o_proj.weight
-            return torch.mm(y.reshape(b * t, -1).to(w.dtype), w.t(), out_dtype=torch.float32).view(b, t, -1)
+            return torch.mm(y.reshape(-1, y.shape[-1]).to(w.dtype), w.t(), out_dtype=torch.float32).view(*y.shape[:2], -1)
         return ly.o_proj(y)
 
     @torch.no_grad()
@@ -994,7 +1012,8 @@ class Bolt3Decoder:
     @torch.no_grad()
     def prefill(self, ids: torch.Tensor, max_kv_len: int = 4096):
         """Fresh state for ids [b, t] and the prompt run through it (bolt3.py:449-457)."""
-        states, kv = self.blank_state(self.model, ids.shape[0], ids.device, max_kv_len=max(max_kv_len, ids.shape[1] + 1024))
+        states, kv = self.blank_state(self.model, ids.shape[0], ids.device, max_kv_len=max(max_kv_len, ids.shape[1] + 1024),
+                                      kv_cache=self.kv_cache)
         h, _ = self._feed(ids, 0, states, kv)
         return h, states, kv
 
@@ -1051,6 +1070,13 @@ class Bolt3Decoder:
         if runner is not None:
             runner.close()
         return torch.cat(toks, dim=1), lengths
+
+    def beam_search(self, ids: torch.Tensor, beams: int, max_new_tokens: int, eos_ids=()):
+        """The `beams` best continuations of every row of ids [B, T] by total log probability (no counterpart
+        in the reference): (tokens [B, beams, n], scores [B, beams], lengths [B, beams]), best first."""
+        from .beam import beam_search
+
+        return beam_search(self, ids, beams, max_new_tokens, eos_ids)
 
     @torch.no_grad()
     def generate(self, prompt: torch.Tensor, max_new_tokens: int, temperature: float = 0.0, top_k: int = 40,
@@ -1119,6 +1145,23 @@ class Bolt3Decoder:
         return states
 
 
+def _check_kv_cache(kind: str) -> None:
+    if kind not in ("bf16", "int8"):
+        raise ValueError(f"kv_cache must be 'bf16' or 'int8', got {kind!r}")
+
+
+def _fp32_weight(norm: "LlamaRMSNorm", device) -> torch.Tensor:
+    """A norm's weight as a contiguous fp32 tensor on `device`, kept between calls (made again when the
+    parameter is replaced or changed in place)."""
+    t = norm.weight
+    key = (t.data_ptr(), t._version, t.dtype, str(torch.device(device)))
+    cached = getattr(norm, "_fp32_cache", None)
+    if cached is None or cached[0] != key:
+        cached = (key, t.detach().to(device=device, dtype=torch.float32).contiguous())
+        norm._fp32_cache = cached
+    return cached[1]
+
+
 def _fp32_inv_freq(rope: "LlamaRoPE", device) -> torch.Tensor:
     """The RoPE module's frequencies as a contiguous fp32 tensor on `device`, kept between calls (made
     again when the buffer is replaced or changed in place): a kernel argument, not a per-step copy."""
@@ -1174,6 +1217,93 @@ class AnchorKV:
         self.buf[1, :, :, self.n:self.n + L].copy_(v_new)
         self.n += L
         return self.buf[0, :, :, :self.n], self.buf[1, :, :, :self.n]
+
+    def tensors(self) -> list[torch.Tensor]:
+        """What holds the tokens: sequences in dimension 1, tokens in dimension 3."""
+        return [self.buf]
+
+    def repeated(self, times: int) -> "AnchorKV":
+        """A copy whose sequences are this cache's, each `times` times in a row."""
+        new = AnchorKV.__new__(AnchorKV)
+        new.buf, new.n = self.buf.repeat_interleave(times, dim=1), self.n
+        return new
+
+
+class AnchorKV8:
+    """8-bit KV cache of one softmax anchor layer: int8 `data` [2, B, HKV, capacity, HD] with an fp32
+    `scale` per row [2, B, HKV, capacity], 0.52 of AnchorKV's bytes at HD 128. Tokens enter through
+    attention() (norm, rotation, quantisation and the attention itself are kernels: csrc/kv8.cu,
+    csrc/kv8_attend.cu); `k` and `v` read the held tokens back as bf16 copies. GPU only. The capacity is
+    max_kv_len rounded up to a multiple of 256 tokens and doubles when an append does not fit."""
+
+    def __init__(self, B: int, HKV: int, Tmax: int, HD: int, dev):
+        cap = max(256, -(-int(Tmax) // 256) * 256)
+        self.data = torch.empty(2, B, HKV, cap, HD, device=dev, dtype=torch.int8)
+        self.scale = torch.empty(2, B, HKV, cap, device=dev, dtype=torch.float32)
+        self.n = 0
+
+    @property
+    def capacity(self) -> int:
+        return self.data.shape[3]
+
+    @property
+    def k(self) -> torch.Tensor:
+        return self.read()[0]
+
+    @property
+    def v(self) -> torch.Tensor:
+        return self.read()[1]
+
+    def read(self, t0: int = 0, t1: int | None = None) -> torch.Tensor:
+        """Tokens t0 .. t1 - 1 (all held ones by default) as bf16 [2, B, HKV, t1 - t0, HD]: keys, values."""
+        t1 = self.n if t1 is None else t1
+        if not 0 <= t0 <= t1 <= self.n:
+            raise ValueError(f"tokens [{t0}, {t1}) of a cache that holds {self.n}")
+        if t0 == t1:
+            return torch.empty(*self.data.shape[:3], 0, self.data.shape[4], dtype=torch.bfloat16, device=self.data.device)
+        return K.kv8_read(self.data, self.scale, t0, t1 - t0)
+
+    def tensors(self) -> list[torch.Tensor]:
+        """What holds the tokens: sequences in dimension 1, tokens in dimension 3."""
+        return [self.data, self.scale]
+
+    def reserve(self, L: int) -> None:
+        """Room for L more tokens: the capacity doubles (one copy of the held tokens) until they fit."""
+        if self.n + L > self.capacity:
+            cap = self.capacity
+            while cap < self.n + L:
+                cap *= 2
+            data = self.data.new_empty(*self.data.shape[:3], cap, self.data.shape[4])
+            scale = self.scale.new_empty(*self.scale.shape[:3], cap)
+            data[:, :, :, :self.n].copy_(self.data[:, :, :, :self.n])
+            scale[:, :, :, :self.n].copy_(self.scale[:, :, :, :self.n])
+            self.data, self.scale = data, scale
+
+    def repeated(self, times: int) -> "AnchorKV8":
+        """A copy whose sequences are this cache's, each `times` times in a row."""
+        new = AnchorKV8.__new__(AnchorKV8)
+        new.data, new.scale = (t.repeat_interleave(times, dim=1) for t in (self.data, self.scale))
+        new.n = self.n
+        return new
+
+    def attention(self, ly, h: torch.Tensor, pos_start: int, dev_pos: "K.DevicePosition | None" = None) -> torch.Tensor:
+        """An anchor layer's attention for t new tokens h [b, t, D]: q and k normed and rotated, k and v
+        appended, the causal attention over all held tokens; [b, t, H * HD] bf16. With dev_pos (a step
+        captured into a CUDA graph) the position comes from the device and the count is left to the caller."""
+        t = h.shape[1]
+        if dev_pos is None:
+            self.reserve(t)
+        q, k, v = ly.q_proj(h), ly.k_proj(h), ly.v_proj(h)
+        norm = ly.q_norm is not None
+        q = K.kv8_append(q=q, k=k, v=v, data=self.data, scale=self.scale, n=self.n, pos0=pos_start,
+                         inv_freq=_fp32_inv_freq(ly.rope, h.device),
+                         q_norm=_fp32_weight(ly.q_norm, h.device) if norm else None,
+                         k_norm=_fp32_weight(ly.k_norm, h.device) if norm else None,
+                         eps=ly.q_norm.eps if norm else 0.0, dev_pos=dev_pos)
+        y = K.kv8_attend(q=q, data=self.data, scale=self.scale, n=self.n, sm_scale=ly.HD ** -0.5, dev_pos=dev_pos)
+        if dev_pos is None:
+            self.n += t
+        return y
 
 
 class _ChunkGraph:
@@ -1260,11 +1390,11 @@ class DecodeGraph(_ChunkGraph):
 
     def __init__(self, dec: "Bolt3Decoder", states, kv_caches):
         bolt = [st for st in kv_caches if isinstance(st, Bolt3LayerState)]
-        anch = [c for c in kv_caches if isinstance(c, AnchorKV)]
-        ref = bolt[0].ring_kp if bolt else anch[0].buf
+        anch = [c for c in kv_caches if isinstance(c, (AnchorKV, AnchorKV8))]
+        ref = bolt[0].ring_kp if bolt else anch[0].tensors()[0]
         super().__init__(ref.device, dec.C)
         self.dec, self.states, self.kv = dec, states, kv_caches
-        self.B = bolt[0].B if bolt else anch[0].buf.shape[1]
+        self.B = bolt[0].B if bolt else ref.shape[1]
         self.tok = torch.zeros(self.B, 1, dtype=torch.long, device=self.device)
 
     def _phase(self) -> int:
