@@ -10,6 +10,8 @@ view or too few elements raise before anything is launched.
 from __future__ import annotations
 
 import ctypes
+import functools
+import math
 
 import torch
 
@@ -587,17 +589,38 @@ def new_bank(n_chains: int, HD: int, device, S: int = S_SLOTS, m_res: bool = Tru
 
 
 # ---- 8-bit KV cache of a softmax anchor (include/bolt3.h: bolt3_kv8_*)
+# These calls are made for single tokens too, where the kernel is shorter than the checks around it: the
+# checks look at a tensor's dtype, device and layout directly, and only a failing one goes through _need for
+# its message.
 
-def _heads(t: torch.Tensor, name: str, B: int, T: int, HD: int) -> tuple[int, int, int]:
+def _here() -> int:
+    return torch._C._cuda_getDevice()
+
+
+def _fits(t, dtype: torch.dtype, dev: int, name: str, numel: int) -> int:
+    """Address of `t`: a contiguous `dtype` tensor on device `dev` of at least `numel` elements."""
+    if type(t) is torch.Tensor and t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and t.numel() >= numel:
+        return t.data_ptr()
+    _need(t, dtype, name, numel)
+    return t.data_ptr()
+
+
+def _maybe(t, dtype: torch.dtype, dev: int, name: str, numel: int) -> int:
+    return 0 if t is None else _fits(t, dtype, dev, name, numel)
+
+
+def _status_ptr(status) -> int:
+    return 0 if status is None else _status(status)
+
+
+def _heads(t: torch.Tensor, name: str, B: int, T: int, HD: int, dev: int) -> tuple[int, int, int]:
     """(heads, sequence stride, token stride) of `t` = [B, T, heads * HD] or [B, T, heads, HD], a bf16
     CUDA tensor whose head rows are dense: a column block of a projection may be given as a view."""
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} must be a CUDA tensor (the 8-bit cache has no CPU implementation)")
-    if t.device.index != torch.cuda.current_device():
-        raise RuntimeError(f"{name} is on {t.device}, but the current device is cuda:{torch.cuda.current_device()}")
-    if t.dtype != torch.bfloat16:
+    if t.dtype is not torch.bfloat16 or t.get_device() != dev:
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} must be a CUDA tensor (the 8-bit cache has no CPU implementation)")
+        if t.get_device() != dev:
+            raise RuntimeError(f"{name} is on {t.device}, but the current device is cuda:{dev}")
         raise TypeError(f"{name} must be torch.bfloat16, got {t.dtype}")
     sh, st = t.shape, t.stride()
     if len(sh) == 4 and sh[3] == HD and (sh[2] == 1 or st[2] == HD):
@@ -612,25 +635,38 @@ def _heads(t: torch.Tensor, name: str, B: int, T: int, HD: int) -> tuple[int, in
     return heads, (0 if B == 1 else st[0]), (0 if T == 1 else st[1])
 
 
-def _need_kv8(data: torch.Tensor, scale: torch.Tensor) -> tuple[int, int, int, int]:
-    """(B, HKV, cap, HD) of an 8-bit cache: data int8 [2, B, HKV, cap, HD], scale fp32 [2, B, HKV, cap]."""
-    _need(data, torch.int8, "data")
-    _need(scale, torch.float32, "scale")
-    if data.dim() != 5 or data.shape[0] != 2 or scale.shape != data.shape[:4]:
+def _tokens(t, name: str) -> int:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if t.dim() not in (3, 4):
+        raise ValueError(f"{name} must be [B, T, heads * HD] or [B, T, heads, HD], got {tuple(t.shape)}")
+    return t.shape[1]
+
+
+def _need_kv8(data: torch.Tensor, scale: torch.Tensor, dev: int) -> tuple:
+    """(B, HKV, cap, HD, address of data, of scale) of an 8-bit cache: data int8 [2, B, HKV, cap, HD], scale
+    fp32 [2, B, HKV, cap]."""
+    at, sat = _fits(data, torch.int8, dev, "data", 1), _fits(scale, torch.float32, dev, "scale", 1)
+    sh = data.shape
+    if len(sh) != 5 or sh[0] != 2 or scale.shape != sh[:4]:
         raise ValueError(f"an 8-bit cache is data [2, B, HKV, cap, HD] with scale [2, B, HKV, cap], got "
                          f"{tuple(data.shape)} and {tuple(scale.shape)}")
-    return tuple(data.shape[1:])
+    return sh[1], sh[2], sh[3], sh[4], at, sat
 
 
-def _need_lens(lens, dev_pos, B: int) -> int | None:
+def _lens_ptr(lens, dev_pos, B: int, dev: int) -> int:
     if lens is None:
-        return None
+        return 0
     if dev_pos is not None:
         raise ValueError("lens and a device step position exclude each other")
-    _need(lens, torch.int32, "lens")
-    if lens.shape != (B,):
+    at = _fits(lens, torch.int32, dev, "lens", 1)
+    if lens.dim() != 1 or lens.shape[0] != B:
         raise ValueError(f"lens must be [{B}], got {tuple(lens.shape)}")
-    return lens.data_ptr()
+    return at
+
+
+def _pos_fields(dev_pos) -> tuple:
+    return (0, 0, 0) if dev_pos is None else (dev_pos.word.data_ptr(), dev_pos.ref, dev_pos.span)
 
 
 def kv8_append(*, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, data: torch.Tensor, scale: torch.Tensor,
@@ -642,28 +678,25 @@ def kv8_append(*, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, data: torch
     (weights q_norm, k_norm fp32 [HD]; None: no norm), rotate-half RoPE at position pos0 + t (inv_freq fp32
     [HD / 2]; None: no rotation), k and v quantised into rows n .. n + T - 1. Returns the rotated queries,
     bf16 [B, T, H, HD]. With `lens` (int32 [B] on the device) sequence b appends at row lens[b] and position
-    pos0 + lens[b] - n; lens[b] = -1 skips it (its queries are 0)."""
-    B, HKV, cap, HD = _need_kv8(data, scale)
-    if not isinstance(q, torch.Tensor) or q.dim() < 3:
-        raise ValueError("q must be [B, T, H * HD] or [B, T, H, HD]")
-    T = q.shape[1]
-    H, q_sb, q_st = _heads(q, "q", B, T, HD)
-    hk, k_sb, k_st = _heads(k, "k", B, T, HD)
-    hv, v_sb, v_st = _heads(v, "v", B, T, HD)
+    pos0 + lens[b] - n; lens[b] = -1 skips it (its queries are 0). A length on the device that leaves no room
+    skips its sequence too and sets status bit 8."""
+    dev = _here()
+    T = _tokens(q, "q")
+    B, HKV, cap, HD, at, sat = _need_kv8(data, scale, dev)
+    H, q_sb, q_st = _heads(q, "q", B, T, HD, dev)
+    _tokens(k, "k"), _tokens(v, "v")
+    hk, k_sb, k_st = _heads(k, "k", B, T, HD, dev)
+    hv, v_sb, v_st = _heads(v, "v", B, T, HD, dev)
     if hk != HKV or hv != HKV:
         raise ValueError(f"k and v hold {hk} and {hv} heads, the cache {HKV}")
     if q_out is None:
-        q_out = torch.empty(B, T, H, HD, dtype=torch.bfloat16, device=q.device)
-    else:
-        _need(q_out, torch.bfloat16, "q_out", B * T * H * HD)
-    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        _opt(w, torch.float32, name, HD)
-    _opt(inv_freq, torch.float32, "inv_freq", HD // 2)
-    a = _lib.Kv8AppendArgs(B, T, H, HKV, HD, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_sb, q_st, k_sb, k_st, v_sb,
-                           v_st, _ptr(q_norm), _ptr(k_norm), eps, _ptr(inv_freq), q_out.data_ptr(), data.data_ptr(),
-                           scale.data_ptr(), cap, n, pos0, _need_lens(lens, dev_pos, B), _status(status))
-    _set_dev_pos(a, dev_pos)
-    _lib.check(_lib.load().bolt3_kv8_append(ctypes.byref(a), _stream()), "bolt3_kv8_append")
+        q_out = torch.empty((B, T, H, HD), dtype=torch.bfloat16, device=q.device)
+    _lib.kv8_append(
+        torch._C._cuda_getCurrentRawStream(dev), B, T, H, HKV, HD, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_sb, q_st, k_sb,
+        k_st, v_sb, v_st, _maybe(q_norm, torch.float32, dev, "q_norm", HD), _maybe(k_norm, torch.float32, dev, "k_norm", HD),
+        eps, _maybe(inv_freq, torch.float32, dev, "inv_freq", HD // 2),
+        _fits(q_out, torch.bfloat16, dev, "q_out", B * T * H * HD), at, sat, cap, n, pos0, _lens_ptr(lens, dev_pos, B, dev),
+        _status_ptr(status), *_pos_fields(dev_pos))
     _count(1)
     return q_out
 
@@ -672,14 +705,12 @@ def kv8_read(data: torch.Tensor, scale: torch.Tensor, t0: int, T: int, lens: tor
              out: torch.Tensor | None = None, status=None) -> torch.Tensor:
     """Rows t0 .. t0 + T - 1 (with `lens`: from row lens[b]) of an 8-bit cache as bf16 [2, B, HKV, T, HD]
     (bolt3_kv8_read): keys, then values."""
-    B, HKV, cap, HD = _need_kv8(data, scale)
+    dev = _here()
+    B, HKV, cap, HD, at, sat = _need_kv8(data, scale, dev)
     if out is None:
-        out = torch.empty(2, B, HKV, T, HD, dtype=torch.bfloat16, device=data.device)
-    else:
-        _need(out, torch.bfloat16, "out", 2 * B * HKV * T * HD)
-    a = _lib.Kv8ReadArgs(B, HKV, HD, T, data.data_ptr(), scale.data_ptr(), cap, t0, _need_lens(lens, None, B),
-                         out.data_ptr(), _status(status))
-    _lib.check(_lib.load().bolt3_kv8_read(ctypes.byref(a), _stream()), "bolt3_kv8_read")
+        out = torch.empty((2, B, HKV, T, HD), dtype=torch.bfloat16, device=data.device)
+    _lib.kv8_read(torch._C._cuda_getCurrentRawStream(dev), B, HKV, HD, T, at, sat, cap, t0, _lens_ptr(lens, None, B, dev),
+                  _fits(out, torch.bfloat16, dev, "out", 2 * B * HKV * T * HD), _status_ptr(status))
     _count(1)
     return out
 
@@ -691,28 +722,34 @@ def kv8_attend(*, q: torch.Tensor, data: torch.Tensor, scale: torch.Tensor, n: i
     that holds n rows before them and has them appended (bolt3_kv8_attend): query t sees rows 0 .. n + t.
     With `lens` sequence b holds lens[b] rows before them (-1: idle, its outputs are 0) and n is the longest
     length to expect. Returns y, bf16 [B, T, H * HD]."""
-    B, HKV, cap, HD = _need_kv8(data, scale)
-    if not isinstance(q, torch.Tensor) or q.dim() < 3:
-        raise ValueError("q must be [B, T, H * HD] or [B, T, H, HD]")
-    T = q.shape[1]
-    H, q_sb, q_st = _heads(q, "q", B, T, HD)
+    dev = _here()
+    T = _tokens(q, "q")
+    B, HKV, cap, HD, at, sat = _need_kv8(data, scale, dev)
+    H, q_sb, q_st = _heads(q, "q", B, T, HD, dev)
     if y is None:
-        y = torch.empty(B, T, H * HD, dtype=torch.bfloat16, device=q.device)
-    else:
-        _need(y, torch.bfloat16, "y", B * T * H * HD)
-    lib = _lib.load()
-    nbytes = lib.bolt3_kv8_attend_workspace(B, T, H, HKV, HD, n)
+        y = torch.empty((B, T, H * HD), dtype=torch.bfloat16, device=q.device)
+    nbytes = _attend_workspace(B, T, H, HKV, HD, n)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    a = _lib.Kv8AttendArgs(B, T, H, HKV, HD, q.data_ptr(), q_sb, q_st, data.data_ptr(), scale.data_ptr(), cap, n,
-                           _need_lens(lens, dev_pos, B), y.data_ptr(), HD ** -0.5 if sm_scale is None else sm_scale,
-                           _ptr(ws), nbytes, _status(status))
-    _set_dev_pos(a, dev_pos)
-    _lib.check(lib.bolt3_kv8_attend(ctypes.byref(a), _stream()), "bolt3_kv8_attend")
+    _lib.kv8_attend(
+        torch._C._cuda_getCurrentRawStream(dev), B, T, H, HKV, HD, q.data_ptr(), q_sb, q_st, at, sat, cap, n,
+        _lens_ptr(lens, dev_pos, B, dev), _fits(y, torch.bfloat16, dev, "y", B * T * H * HD),
+        HD ** -0.5 if sm_scale is None else sm_scale, 0 if ws is None else ws.data_ptr(), nbytes, _status_ptr(status),
+        *_pos_fields(dev_pos))
     _count(2 if nbytes else 1)
     return y
 
 
+@functools.lru_cache(maxsize=1024)
+def _attend_workspace(B: int, T: int, H: int, HKV: int, HD: int, n: int) -> int:
+    return _lib.load().bolt3_kv8_attend_workspace(B, T, H, HKV, HD, n)
+
+
 # ---- beam search (include/bolt3.h: bolt3_beam_*)
+
+@functools.lru_cache(maxsize=256)
+def _select_workspace(B: int, K: int, V: int) -> int:
+    return _lib.load().bolt3_beam_select_workspace(B, K, V)
+
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | None = None,
                 eos_ids: tuple = (), out: tuple | None = None) -> tuple:
@@ -724,47 +761,46 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
     write instead of new ones (scores and finished may be the inputs)."""
     if not isinstance(logits, torch.Tensor) or logits.dim() not in (2, 3):
         raise ValueError("logits must be [B, K, V] or [B * K, V]")
-    if not logits.is_cuda or logits.device.index != torch.cuda.current_device():
+    dev = _here()
+    if logits.get_device() != dev:
         raise RuntimeError("logits must be on the current CUDA device (beam selection has no CPU implementation)")
-    if logits.dtype not in (torch.bfloat16, torch.float32):
+    fp32 = logits.dtype is torch.float32
+    if not fp32 and logits.dtype is not torch.bfloat16:
         raise TypeError(f"logits must be bfloat16 or float32, got {logits.dtype}")
-    _need(scores, torch.float32, "scores")
+    s_at = _fits(scores, torch.float32, dev, "scores", 1)
     if scores.dim() != 2:
         raise ValueError(f"scores must be [B, K], got {tuple(scores.shape)}")
     B, K = scores.shape
-    V = logits.shape[-1]
-    if logits.numel() != B * K * V or (logits.dim() == 3 and logits.shape[0] != B):
-        raise ValueError(f"logits {tuple(logits.shape)} do not match {B} groups of {K} beams")
-    st = logits.stride()
+    sh, st = logits.shape, logits.stride()
+    V = sh[-1]
+    if (sh[0] != B * K) if len(sh) == 2 else (sh[0] != B or sh[1] != K):
+        raise ValueError(f"logits {tuple(sh)} do not match {B} groups of {K} beams")
     if st[-1] != 1 and V > 1:
         raise ValueError("the logits' rows must be dense")
-    if logits.dim() == 3 and B > 1 and K > 1 and st[0] != K * st[1]:
+    if len(sh) == 3 and B > 1 and K > 1 and st[0] != K * st[1]:
         raise ValueError("the logits' rows must be evenly spaced")
-    stride = V if B * K == 1 else (st[0] if logits.dim() == 2 or K == 1 else st[1])
+    stride = V if B * K == 1 else (st[0] if len(sh) == 2 or K == 1 else st[1])
+    f_at = 0
     if finished is not None:
-        _need(finished, finished.dtype if finished.dtype in (torch.bool, torch.uint8) else torch.bool, "finished", B * K)
-    eos_ids = tuple(int(e) for e in eos_ids)
+        f_at = _fits(finished, torch.uint8 if finished.dtype is torch.uint8 else torch.bool, dev, "finished", B * K)
+        if not eos_ids:
+            raise ValueError("finished beams need an end-of-sequence id to go on with")
     if len(eos_ids) > 8:
         raise ValueError(f"at most 8 end-of-sequence ids, got {len(eos_ids)}")
-    if finished is not None and not eos_ids:
-        raise ValueError("finished beams need an end-of-sequence id to go on with")
-    if any(e < 0 or e >= V for e in eos_ids):
-        raise ValueError(f"end-of-sequence ids {eos_ids} must lie in [0, {V})")
+    eos = [int(e) for e in eos_ids]
+    if any(e < 0 or e >= V for e in eos):
+        raise ValueError(f"end-of-sequence ids {eos} must lie in [0, {V})")
     if out is None:
-        dev = logits.device
-        out = (torch.empty(B, K, dtype=torch.float32, device=dev), torch.empty(B, K, dtype=torch.int32, device=dev),
-               torch.empty(B, K, dtype=torch.int64, device=dev), torch.empty(B, K, dtype=torch.bool, device=dev))
-    else:
-        for t, dt, name in zip(out, (torch.float32, torch.int32, torch.int64, torch.bool),
-                               ("out scores", "out parent", "out token", "out finished")):
-            _need(t, dt, name, B * K)
-    lib = _lib.load()
-    nbytes = lib.bolt3_beam_select_workspace(B, K, V)
+        at = logits.device
+        out = (torch.empty((B, K), dtype=torch.float32, device=at), torch.empty((B, K), dtype=torch.int32, device=at),
+               torch.empty((B, K), dtype=torch.int64, device=at), torch.empty((B, K), dtype=torch.bool, device=at))
+    nbytes = _select_workspace(B, K, V)
     ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=logits.device)
-    a = _lib.BeamSelectArgs(B, K, V, logits.data_ptr(), stride, int(logits.dtype == torch.float32), scores.data_ptr(),
-                            _ptr(finished), (ctypes.c_int64 * 8)(*eos_ids), len(eos_ids), out[0].data_ptr(),
-                            out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(), ws.data_ptr(), nbytes)
-    _lib.check(lib.bolt3_beam_select(ctypes.byref(a), _stream()), "bolt3_beam_select")
+    _lib.beam_select(
+        torch._C._cuda_getCurrentRawStream(dev), B, K, V, logits.data_ptr(), stride, fp32, s_at, f_at,
+        *eos, *[0] * (8 - len(eos)), len(eos), _fits(out[0], torch.float32, dev, "out scores", B * K),
+        _fits(out[1], torch.int32, dev, "out parent", B * K), _fits(out[2], torch.int64, dev, "out token", B * K),
+        _fits(out[3], torch.bool, dev, "out finished", B * K), ws.data_ptr(), nbytes)
     _count(2)
     return out
 
@@ -780,53 +816,46 @@ class BeamReorder:
         if groups < 1 or beams < 1:
             raise ValueError(f"{groups} groups of {beams} beams")
         self.groups, self.beams, n = groups, beams, groups * beams
-        self.tensors = [it[0] for it in items]
-        self.items = (_lib.BeamItem * max(1, len(items)))()
-        self.max_tokens = None
-        spans = []
-        for x, (t, beam_dim, token_dim) in zip(self.items, items):
-            _need(t, t.dtype, "state tensor")
-            sh, es = tuple(t.shape), t.element_size()
-            if not 0 <= beam_dim < len(sh) or sh[beam_dim] == 0 or sh[beam_dim] % n:
-                raise ValueError(f"dimension {beam_dim} of a state {sh} does not hold {groups} x {beams} beams")
-            if token_dim is not None and not beam_dim < token_dim < len(sh):
-                raise ValueError(f"token dimension {token_dim} of a state {sh} must come after its beam dimension {beam_dim}")
-            if t.numel() == 0:
-                raise ValueError(f"a state of shape {sh} is empty")
-            rows, outer = sh[beam_dim] // n, 1
-            for s in sh[:beam_dim]:
-                outer *= s
-            beam_bytes = es * rows
-            for s in sh[beam_dim + 1:]:
-                beam_bytes *= s
-            x.base, x.n_outer, x.outer_stride, x.beam_stride = t.data_ptr(), outer, beam_bytes * n, beam_bytes
+        self.tensors, self.max_tokens = [it[0] for it in items], None
+        dev, spans, blocks = _here(), [], []
+        for t, beam_dim, token_dim in items:
+            at = _fits(t, t.dtype, dev, "state tensor", 1)
+            sh, es = t.shape, t.element_size()
+            if not 0 <= beam_dim < len(sh) or sh[beam_dim] % n:
+                raise ValueError(f"dimension {beam_dim} of a state {tuple(sh)} does not hold {groups} x {beams} beams")
+            beam_bytes = es * math.prod(sh[beam_dim:]) // n
             if token_dim is None:
-                x.n_row, x.row_stride, x.row_bytes, x.token_bytes = 1, beam_bytes, beam_bytes, 0
-            else:
-                token = es
-                for s in sh[token_dim + 1:]:
-                    token *= s
-                x.row_bytes = x.row_stride = token * sh[token_dim]
-                x.n_row, x.token_bytes = beam_bytes // x.row_bytes, token
+                rows, row_bytes, token = 1, beam_bytes, 0
+            elif beam_dim < token_dim < len(sh):
+                token = es * math.prod(sh[token_dim + 1:])
+                row_bytes = token * sh[token_dim]
+                rows = beam_bytes // row_bytes
                 self.max_tokens = min(self.max_tokens or sh[token_dim], sh[token_dim])
-            grain = x.base | x.beam_stride | (x.token_bytes or x.row_bytes)
-            x.unit = 16 if grain % 16 == 0 else 4 if grain % 4 == 0 else 1
-            spans.append((x.base, x.base + t.numel() * es))
+            else:
+                raise ValueError(f"token dimension {token_dim} of a state {tuple(sh)} must come after its beam "
+                                 f"dimension {beam_dim}")
+            grain = at | beam_bytes | (token or row_bytes)
+            unit = 16 if grain % 16 == 0 else 4 if grain % 4 == 0 else 1
+            blocks.append(_lib.beam_item.pack(at, beam_bytes * n, beam_bytes, row_bytes, row_bytes, token,
+                                              math.prod(sh[:beam_dim]), rows, unit, 0))
+            spans.append((at, at + t.numel() * es))
         spans.sort()
-        if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+        if any(y[0] < x[1] for x, y in zip(spans, spans[1:])):
             raise ValueError("the state tensors of a reordering must not overlap")
+        self._items = ctypes.create_string_buffer(b"".join(blocks), max(1, sum(map(len, blocks))))
+        self._items_at = ctypes.addressof(self._items)
 
     def __call__(self, parent: torch.Tensor, t0: int = 0, t1: int = 0, status=None) -> None:
         """Every state of beam j of group b becomes that of beam parent[b, j] (int32 [groups, beams] on the
         device, any map), in place."""
-        _need(parent, torch.int32, "parent")
-        if tuple(parent.shape) != (self.groups, self.beams):
+        dev = _here()
+        at = _fits(parent, torch.int32, dev, "parent", 1)
+        if parent.dim() != 2 or parent.shape[0] != self.groups or parent.shape[1] != self.beams:
             raise ValueError(f"parent must be [{self.groups}, {self.beams}], got {tuple(parent.shape)}")
         if self.max_tokens is not None and not 0 <= t0 <= t1 <= self.max_tokens:
             raise ValueError(f"tokens [{t0}, {t1}) are not within the states' {self.max_tokens}")
-        a = _lib.BeamReorderArgs(self.groups, self.beams, parent.data_ptr(), self.items, len(self.tensors), t0, t1,
-                                 _status(status))
-        _lib.check(_lib.load().bolt3_beam_reorder(ctypes.byref(a), _stream()), "bolt3_beam_reorder")
+        _lib.beam_reorder(torch._C._cuda_getCurrentRawStream(dev), self.groups, self.beams, at, self._items_at,
+                          len(self.tensors), t0, t1, _status_ptr(status))
         _count(-(-len(self.tensors) // 128))
 
 
