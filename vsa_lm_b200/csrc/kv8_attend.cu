@@ -23,6 +23,7 @@
 // m16n8k16 on f16, output dimensions permuted likewise, P^T being S^T transposed by movmatrix.
 #include "../../include/bolt3.h"
 #include "kv8.cuh"
+#include "kv8_prompt.cuh"
 #include "tc5.cuh"
 #include "trace.h"
 
@@ -784,6 +785,9 @@ bool encode_cache(CUtensorMap* m, const bolt3_kv8_attend_args* a) {
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// whether a call's rows go to the kernel for many rows
+bool many_rows(int T, int H, int HKV) { return (int64_t)T * (H / HKV) > 32; }
+
 bool shape_ok(int B, int T, int H, int HKV, int HD) {
   return B > 0 && T > 0 && HKV > 0 && H > 0 && H % HKV == 0 && H / HKV <= 16 && (HD == 64 || HD == 128) &&
          T <= 65535 / (H / HKV) && (int64_t)B * HKV <= 0x3fffffff;
@@ -793,7 +797,7 @@ bool shape_ok(int B, int T, int H, int HKV, int HD) {
 
 extern "C" size_t bolt3_kv8_attend_workspace(int B, int T, int H, int HKV, int HD, int64_t n) {
   if (!shape_ok(B, T, H, HKV, HD) || n < 0) return 0;
-  return plan_of(B, T, H, HKV, HD, n).bytes;
+  return many_rows(T, H, HKV) ? kv8_prompt_workspace(B, T, H, HKV, HD, n) : plan_of(B, T, H, HKV, HD, n).bytes;
 }
 
 extern "C" int bolt3_kv8_attend(const bolt3_kv8_attend_args* a, void* stream) {
@@ -806,12 +810,14 @@ extern "C" int bolt3_kv8_attend(const bolt3_kv8_attend_args* a, void* stream) {
   if (a->n < 0 || a->cap < a->T || a->cap > 0x7fffffff || (a->lens == nullptr && a->n > a->cap - a->T - dmax)) return BOLT3_ERR_CAPACITY;
   const uintptr_t al = (uintptr_t)a->q | (uintptr_t)a->data | (uintptr_t)a->scale | (uintptr_t)a->y | (uintptr_t)a->workspace;
   if ((al & 15) || ((a->q_sb | a->q_st) & 7)) return BOLT3_ERR_ALIGN;
+  const Length len{a->lens, a->pos_dev, a->n, a->pos_ref, a->pos_span, a->cap, a->T};
+  if (many_rows(a->T, a->H, a->HKV)) return kv8_prompt_launch(a, len, (cudaStream_t)stream);
   const Plan pl = plan_of(a->B, a->T, a->H, a->HKV, a->HD, a->n);
   if (pl.bytes > 0 && (a->workspace == nullptr || a->workspace_bytes < pl.bytes)) return BOLT3_ERR_CAPACITY;
   Params p;
   if (!encode_cache(&p.map, a)) return BOLT3_ERR_CUDA;
   p.a = *a;
-  p.len = Length{a->lens, a->pos_dev, a->n, a->pos_ref, a->pos_span, a->cap, a->T};
+  p.len = len;
   p.G = a->H / a->HKV;
   p.rows = a->T * p.G;
   cudaStream_t s = (cudaStream_t)stream;

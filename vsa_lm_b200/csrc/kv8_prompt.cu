@@ -1,0 +1,542 @@
+// Softmax attention of many query rows (prompt slices) over the 8-bit KV cache, on the tensor cores' TMEM path.
+//
+// The mathematics and its roundings are those of kv8_attend.cu: with t_j the score of key j in log2 units and
+// u_j = t_j + log2 scale_v[j], weights w_j = 2^(u_j - M) in f16, y = sum w_j v8_j / sum (w_j / scale_v[j]). Here a
+// query row is brought to f16 by a power of two of its own (exact down to 2^-25 of its largest value) and the int8
+// keys and values are exact in f16.
+//
+// Bound by arithmetic: 4 HD operations per (query row, key), and one exponential. A CTA holds two tiles of 128 query
+// rows (T * G rows of one KV head, token-major) and walks the keys in blocks of 128, so that a block is widened from
+// int8 to f16 once for 256 rows. Roles, which meet only at mbarriers:
+// - warps 8-11 widen: global int8 -> registers (a block ahead) -> f16 operand tiles in shared memory (two stages of K and
+//   of V), and the block's scales;
+// - one thread of warp 12 issues tcgen05.mma: S = Q K^T into TMEM, O += P V with P as the TMEM operand;
+// - warps 0-3 and 4-7 are the softmax of a tile, a thread per row, 64 keys at a time: scores out of TMEM, weights back
+//   over them, fp32 arithmetic in packed pairs. The bound M moves only when a weight would pass 2^8; only then are the
+//   sums in TMEM rescaled.
+// While one tile's softmax runs, the tensor cores work on the other tile. With few heads the keys are split over CTAs,
+// whose partial sums a second kernel joins.
+#include "../../include/bolt3.h"
+#include "kv8.cuh"
+#include "kv8_prompt.cuh"
+#include "tc5.cuh"
+#include "trace.h"
+
+namespace {
+
+using namespace b3;
+using namespace kv8;
+
+constexpr int kKeys = 128;                       // of a block
+constexpr int kThreads = 416;                    // 4 + 4 softmax warps, 4 widening warps, 1 issuing warp
+constexpr uint32_t kWaitIters = 1u << 24;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 8.f;
+
+struct Params {
+  bolt3_kv8_attend_args a;
+  Length len;
+  int G, rows, tiles, splits;                    // tiles: pairs of 128 rows of a head
+  float* part;                                   // [head][row][split][HD] sums, then [..] (bound, sum of weights)
+  float2* part_ml;
+};
+
+template <int HD>
+struct Smem {
+  unsigned char q[2][kKeys * HD * 2];            // K-major operand tiles: HD / 64 blocks of [128 rows][64 columns]
+  unsigned char k[2][kKeys * HD * 2];
+  unsigned char v[2][kKeys * HD * 2];
+  float scale[2][3][kKeys];                      // key scale, log2 and reciprocal of the value scale
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[2], p_full[2][2], pv_half[2], o_full[2];
+  uint32_t tbase;
+  int err;
+};
+
+B3_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+B3_DEV float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+B3_DEV float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+B3_DEV uint32_t pack_f16(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+// two fp32 at a time
+B3_DEV uint64_t pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+B3_DEV float2 unpair(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+B3_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+B3_DEV uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+B3_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+B3_DEV float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 16 int8 of row r, dimensions 16 c .., as f16 into an operand tile. Lanes of the upper column block store their two
+// 16-byte chunks in the other order, so that the eight lanes of a row keep off each other's banks
+B3_DEV void widen16(unsigned char* tile, int r, int c, const uint4& x) {
+  uint4 lo, hi;
+  s8x4_to_f16(x.x, lo.x, lo.y);
+  s8x4_to_f16(x.y, lo.z, lo.w);
+  s8x4_to_f16(x.z, hi.x, hi.y);
+  s8x4_to_f16(x.w, hi.z, hi.w);
+  unsigned char* block = tile + (c >> 2) * (kKeys * 128) + r * 128;
+  const int c0 = (2 * c) & 7;
+  const bool swap = c >> 2 & 1;
+  *reinterpret_cast<uint4*>(block + (((swap ? c0 + 1 : c0) ^ (r & 7)) << 4)) = swap ? hi : lo;
+  *reinterpret_cast<uint4*>(block + (((swap ? c0 : c0 + 1) ^ (r & 7)) << 4)) = swap ? lo : hi;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_constant__ Params p) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  Smem<HD>& sm = *reinterpret_cast<Smem<HD>*>(smem_raw + ((1024 - (tc5::smem_u32(smem_raw) & 1023)) & 1023));
+  const bolt3_kv8_attend_args& a = p.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int head = blockIdx.x / p.tiles, b = head / a.HKV, kvh = head % a.HKV;
+  const int row0 = (blockIdx.x % p.tiles) * 256, n_tile = min(2, (p.rows - row0 + 127) / 128);
+  const int split = blockIdx.y;
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      tc5::mbar_init(&sm.k_full[i], 128);
+      tc5::mbar_init(&sm.k_empty[i], 1);
+      tc5::mbar_init(&sm.v_full[i], 128);
+      tc5::mbar_init(&sm.v_empty[i], 1);
+      tc5::mbar_init(&sm.s_full[i], 1);
+      tc5::mbar_init(&sm.p_full[i][0], 128);
+      tc5::mbar_init(&sm.p_full[i][1], 128);
+      tc5::mbar_init(&sm.pv_half[i], 1);
+      tc5::mbar_init(&sm.o_full[i], 1);
+    }
+    tc5::mbar_fence_init();
+    sm.err = 0;
+  }
+  grid_dep_launch();
+  grid_dep_wait();
+  bool bad = false;
+  const int64_t s = p.len.rows(b, bad);
+  if (bad && tid == 0 && blockIdx.x % p.tiles == 0 && split == 0 && a.status) atomicOr(a.status, 8);
+  auto out_row = [&](int row) {
+    return reinterpret_cast<bf16*>(a.y) + (((int64_t)b * a.T + row / p.G) * a.H + kvh * p.G + row % p.G) * HD;
+  };
+  // blocks of keys that the last row of this CTA sees, and this split's share of them
+  const int last = (min(row0 + 256, p.rows) - 1) / p.G;
+  const int64_t all = s < 0 ? 0 : (s + last + kKeys) / kKeys;
+  const int64_t lo = all * split / p.splits, hi = all * (split + 1) / p.splits;
+  const int n_blk = (int)(hi - lo);
+  if (n_blk == 0) {                              // the same for all threads: nothing has been allocated
+    if (tid < 256 && row0 + tid < p.rows) {
+      if (p.splits > 1) {
+        const int64_t at = ((int64_t)head * p.rows + row0 + tid) * p.splits + split;
+        p.part_ml[at] = make_float2(neg_inf(), 0.f);
+      } else {
+        uint4* y = reinterpret_cast<uint4*>(out_row(row0 + tid));
+        for (int i = 0; i < HD / 8; ++i) y[i] = make_uint4(0, 0, 0, 0);
+      }
+    }
+    return;
+  }
+
+  // this thread's query row to f16, in the operand tile
+  float c_row = 0.f;
+  if (warp < 8) {
+    const int r = tid & 127, row = row0 + tid;
+    uint4 raw[HD / 8];
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i) {
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if (row < p.rows)
+        raw[i] = reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.q) + b * a.q_sb + (row / p.G) * a.q_st +
+                                                (int64_t)(kvh * p.G + row % p.G) * HD)[i];
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 v = unpack_bf16(w[j]);
+        m = max3(m, fabsf(v.x), fabsf(v.y));
+      }
+    }
+    // 2^-e brings the row's largest value into [1, 2): f16 keeps all of a bf16's bits down to 2^-17 of it
+    const int e = m > 0.f && m < 3e38f ? max(ilogbf(m), -100) : 0;
+    const float down = exp2f((float)-e);
+    c_row = a.sm_scale * kLog2e * exp2f((float)e);
+    unsigned char* tile = sm.q[tid >> 7];
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i) {
+      const float2 x = unpack_bf16(raw[i].x), y = unpack_bf16(raw[i].y), z = unpack_bf16(raw[i].z), w = unpack_bf16(raw[i].w);
+      uint4 o;
+      o.x = pack_f16(x.x * down, x.y * down);
+      o.y = pack_f16(y.x * down, y.y * down);
+      o.z = pack_f16(z.x * down, z.y * down);
+      o.w = pack_f16(w.x * down, w.y * down);
+      *reinterpret_cast<uint4*>(tile + (i >> 3) * (kKeys * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = o;
+    }
+  }
+  if (warp == 12) {
+    tc5::tmem_alloc(&sm.tbase, 512);
+    tc5::tmem_relinquish();
+  }
+  asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+  tc5::fence_before_sync();
+  __syncthreads();
+  tc5::fence_after_sync();
+  const uint32_t tb = sm.tbase;                  // S / P of tile i: columns 128 i; O of tile i: 256 + 128 i
+  auto wait = [&](uint64_t* bar, int phase) {
+    if (tc5::mbar_wait(bar, (uint32_t)phase & 1, kWaitIters)) return true;
+    sm.err = 1;
+    return false;
+  };
+
+  if (warp >= 8 && warp < 12) {
+    // ---- widening
+    constexpr int PPR = HD / 16, NP = kKeys * PPR / 128;          // 16-byte pieces of a row, of a thread
+    const int t = tid - 256;
+    const int8_t* kd = a.data + (int64_t)head * a.cap * HD;
+    const int8_t* vd = kd + (int64_t)a.B * a.HKV * a.cap * HD;
+    const float* ks = a.scale + (int64_t)head * a.cap;
+    const float* vs = ks + (int64_t)a.B * a.HKV * a.cap;
+    const int64_t end = a.cap - 1;                                // rows past the buffer are read as its last one and masked
+    uint4 kr[NP], vr[NP];
+    float k_sc, v_sc;
+    auto fetch = [&](const int8_t* base, int64_t key, uint4 (&x)[NP]) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int idx = i * 128 + t;
+        x[i] = __ldg(reinterpret_cast<const uint4*>(base + min(key + idx / PPR, end) * HD) + idx % PPR);
+      }
+    };
+    int64_t key = lo * kKeys;
+    fetch(kd, key, kr);
+    fetch(vd, key, vr);
+    k_sc = __ldg(ks + min(key + t, end));
+    v_sc = __ldg(vs + min(key + t, end));
+    for (int j = 0; j < n_blk; ++j) {
+      const int st = j & 1;
+      const int64_t next = key + kKeys;
+      if (j >= 2 && !wait(&sm.k_empty[st], (j >> 1) - 1)) break;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) widen16(sm.k[st], (i * 128 + t) / PPR, (i * 128 + t) % PPR, kr[i]);
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      tc5::mbar_arrive(&sm.k_full[st]);
+      if (j + 1 < n_blk) fetch(kd, next, kr);
+      if (j >= 2 && !wait(&sm.v_empty[st], (j >> 1) - 1)) break;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) widen16(sm.v[st], (i * 128 + t) / PPR, (i * 128 + t) % PPR, vr[i]);
+      sm.scale[st][0][t] = k_sc;
+      sm.scale[st][1][t] = lg2(v_sc);
+      sm.scale[st][2][t] = rcp(v_sc);
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      tc5::mbar_arrive(&sm.v_full[st]);
+      if (j + 1 < n_blk) {
+        fetch(vd, next, vr);
+        k_sc = __ldg(ks + min(next + t, end));
+        v_sc = __ldg(vs + min(next + t, end));
+      }
+      key = next;
+    }
+  } else if (warp == 12) {
+    // ---- issue
+    if (lane == 0) {
+      constexpr uint32_t kIdS = tc5::idesc_f16(128, kKeys, false, false), kIdO = tc5::idesc_f16(128, HD, false, true);
+      auto scores = [&](int i, int st) {
+        const uint32_t qa = tc5::smem_u32(sm.q[i]), ka = tc5::smem_u32(sm.k[st]);
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * (kKeys * 128) + (ks & 3) * 32;
+          tc5::mma_ss(tb + i * 128, tc5::sdesc(qa + off, 16, 1024), tc5::sdesc(ka + off, 16, 1024), kIdS, ks > 0);
+        }
+        tc5::commit(&sm.s_full[i]);
+      };
+      bool ok = wait(&sm.k_full[0], 0);
+      if (ok) {
+        tc5::fence_after_sync();
+        for (int i = 0; i < n_tile; ++i) scores(i, 0);
+        tc5::commit(&sm.k_empty[0]);
+      }
+      for (int j = 0; ok && j < n_blk; ++j) {
+        const int st = j & 1;
+        ok = wait(&sm.v_full[st], j >> 1);
+        const uint32_t va = tc5::smem_u32(sm.v[st]);
+        for (int i = 0; ok && i < n_tile; ++i) {
+          for (int h = 0; ok && h < 2; ++h) {
+            ok = wait(&sm.p_full[i][h], j);
+            if (!ok) break;
+            tc5::fence_after_sync();
+#pragma unroll
+            for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
+              tc5::mma_ts(tb + 256 + i * 128, tb + i * 128 + ks * 8, tc5::sdesc(va + ks * 2048, kKeys * 128, 1024), kIdO,
+                          j > 0 || ks > 0);
+            if (h == 0) tc5::commit(&sm.pv_half[i]);
+            else if (j + 1 == n_blk) tc5::commit(&sm.o_full[i]);
+          }
+          if (!ok) break;
+          if (j + 1 < n_blk) {
+            if (i == 0) ok = wait(&sm.k_full[st ^ 1], (j + 1) >> 1);
+            if (!ok) break;
+            tc5::fence_after_sync();
+            scores(i, st ^ 1);
+          }
+        }
+        if (ok) {
+          tc5::commit(&sm.v_empty[st]);
+          if (j + 1 < n_blk) tc5::commit(&sm.k_empty[st ^ 1]);
+        }
+      }
+    }
+    __syncwarp();
+  } else if ((warp >> 2) < n_tile) {
+    // ---- softmax of tile i: this thread's row
+    const int i = warp >> 2, row = row0 + tid;
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, ts = tb + i * 128 + lanes, to = tb + 256 + i * 128 + lanes;
+    const int64_t see = row < p.rows ? s + row / p.G + 1 : s + last + 1;          // keys this row sees
+    const int64_t see_all = s + (row0 + i * 128) / p.G + 1;                       // that every row of the tile sees
+    float M = neg_inf(), l = 0.f;
+    const uint64_t c2 = pair(c_row, c_row);
+    bool ok = true;
+    for (int j = 0; ok && j < n_blk; ++j) {
+      const int st = j & 1;
+      ok = wait(&sm.v_full[st], j >> 1);                          // the scales
+      ok = ok && wait(&sm.s_full[i], j);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc5::fence_after_sync();
+      uint64_t l2 = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t sc[2][32];
+        tc5::ld32(ts + 64 * h, sc[0]);
+        tc5::ld32(ts + 64 * h + 32, sc[1]);
+        tc5::ld_wait();
+        float t[64];
+        float m0 = neg_inf(), m1 = neg_inf();
+        const float* ks = sm.scale[st][0] + 64 * h;
+        const float* lg = sm.scale[st][1] + 64 * h;
+        const float* iv = sm.scale[st][2] + 64 * h;
+        const int64_t key = (lo + j) * kKeys + 64 * h;
+#pragma unroll
+        for (int x = 0; x < 64; x += 4) {
+          const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(ks + x), g4 = *reinterpret_cast<const ulonglong2*>(lg + x);
+          const float2 u = unpair(fma2(pair(__uint_as_float(sc[x >> 5][x & 31]), __uint_as_float(sc[x >> 5][(x & 31) + 1])),
+                                       mul2(k4.x, c2), g4.x));
+          const float2 v = unpair(fma2(pair(__uint_as_float(sc[x >> 5][(x & 31) + 2]), __uint_as_float(sc[x >> 5][(x & 31) + 3])),
+                                       mul2(k4.y, c2), g4.y));
+          t[x] = u.x; t[x + 1] = u.y; t[x + 2] = v.x; t[x + 3] = v.y;
+        }
+        const bool masked = key + 64 > see_all;                   // the same for the whole tile
+        if (masked) {
+          const int left = (int)min(max(see - key, (int64_t)0), (int64_t)64);
+#pragma unroll
+          for (int x = 0; x < 64; ++x)
+            if (x >= left) t[x] = neg_inf();
+        }
+#pragma unroll
+        for (int x = 0; x < 64; x += 4) {
+          m0 = max3(m0, t[x], t[x + 1]);
+          m1 = max3(m1, t[x + 2], t[x + 3]);
+        }
+        m0 = fmaxf(m0, m1);
+        // the bound moves only when a weight would pass 2^8 (and at the first key)
+        const bool over = m0 > M + kSlack;
+        if (__any_sync(0xffffffffu, over)) {
+          const float to_M = over ? m0 : M;
+          const float f = M == neg_inf() ? 0.f : ex2(M - to_M);   // 1 where the bound stays
+          M = to_M;
+          l *= f;
+          l2 = mul2(l2, pair(f, f));
+          if (j > 0 || h > 0) {
+            if (h > 0) {                                          // the first half's product may still be under way
+              ok = __all_sync(0xffffffffu, wait(&sm.pv_half[i], j));
+              tc5::fence_after_sync();
+            }
+            if (ok) {
+#pragma unroll 1
+              for (int d = 0; d < HD; d += 16) {
+                uint32_t o[16];
+                tc5::ld16(to + d, o);
+                tc5::ld_wait();
+#pragma unroll
+                for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                tc5::st16(to + d, o);
+              }
+              tc5::st_wait();
+            }
+          }
+        }
+        const float ref = M == neg_inf() ? 0.f : M;
+        const uint64_t minus = pair(-ref, -ref);
+        uint32_t w[32];
+#pragma unroll
+        for (int x = 0; x < 64; x += 4) {
+          const ulonglong2 i4 = *reinterpret_cast<const ulonglong2*>(iv + x);
+          const float2 u = unpair(add2(pair(t[x], t[x + 1]), minus)), v = unpair(add2(pair(t[x + 2], t[x + 3]), minus));
+          const float e0 = ex2(u.x), e1 = ex2(u.y), e2 = ex2(v.x), e3 = ex2(v.y);
+          if (masked) {                                           // an unseen key has weight 0, whatever its scale holds
+            const float2 a0 = unpair(i4.x), a1 = unpair(i4.y);
+            l += (e0 == 0.f ? 0.f : e0 * a0.x) + (e1 == 0.f ? 0.f : e1 * a0.y) + (e2 == 0.f ? 0.f : e2 * a1.x) +
+                 (e3 == 0.f ? 0.f : e3 * a1.y);
+          } else {
+            l2 = fma2(pair(e0, e1), i4.x, l2);
+            l2 = fma2(pair(e2, e3), i4.y, l2);
+          }
+          w[x / 2] = pack_f16(e0, e1);
+          w[x / 2 + 1] = pack_f16(e2, e3);
+        }
+        tc5::st32(ts + 32 * h, w);
+        tc5::st_wait();
+        tc5::fence_before_sync();
+        tc5::mbar_arrive(&sm.p_full[i][h]);
+      }
+      const float2 x = unpair(l2);
+      l += x.x + x.y;
+    }
+    ok = ok && wait(&sm.o_full[i], 0);
+    ok = __all_sync(0xffffffffu, ok);
+    if (ok) {
+      tc5::fence_after_sync();
+      const int64_t at = ((int64_t)head * p.rows + row) * p.splits + split;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+      for (int d = 0; d < HD; d += 32) {
+        uint32_t o[32];
+        tc5::ld32(to + d, o);
+        tc5::ld_wait();
+        if (row < p.rows) {
+          if (p.splits > 1) {
+            uint4* dst = reinterpret_cast<uint4*>(p.part + at * HD + d);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) dst[x] = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+          } else {
+            uint4* dst = reinterpret_cast<uint4*>(out_row(row) + d);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              uint32_t y[4];
+#pragma unroll
+              for (int z = 0; z < 4; ++z)
+                y[z] = pack_bf16(__uint_as_float(o[8 * x + 2 * z]) * inv, __uint_as_float(o[8 * x + 2 * z + 1]) * inv);
+              dst[x] = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+          }
+        }
+      }
+      if (p.splits > 1 && row < p.rows) p.part_ml[at] = make_float2(M, l);
+    }
+  }
+  tc5::fence_before_sync();
+  __syncthreads();
+  tc5::fence_after_sync();
+  if (warp == 12) tc5::tmem_dealloc(tb, 512);
+  if (tid == 0 && sm.err && a.status) atomicOr(a.status, 2);
+}
+
+// one warp per (head, query row): the splits' partial sums joined
+template <int HD>
+__global__ void __launch_bounds__(128) kv8_prompt_join_kernel(const __grid_constant__ Params p) {
+  constexpr int EPL = HD / 32;
+  const bolt3_kv8_attend_args& a = p.a;
+  const int lane = threadIdx.x & 31;
+  grid_dep_launch();
+  grid_dep_wait();
+  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (item >= (int64_t)a.B * a.HKV * p.rows) return;
+  const int head = (int)(item / p.rows), row = (int)(item % p.rows), b = head / a.HKV, kvh = head % a.HKV;
+  const int64_t at = item * p.splits;
+  float m = neg_inf(), l = 0.f, acc[EPL] = {};
+  for (int i = 0; i < p.splits; ++i) m = fmaxf(m, p.part_ml[at + i].x);
+  for (int i = 0; i < p.splits; ++i) {
+    const float2 ml = p.part_ml[at + i];
+    if (ml.x == neg_inf() && ml.y == 0.f) continue;               // no keys: its sums were not written
+    const float f = ml.x == neg_inf() ? 0.f : exp2f(ml.x - m);
+    l = fmaf(ml.y, f, l);
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) acc[e] = fmaf(p.part[(at + i) * HD + 32 * e + lane], f, acc[e]);
+  }
+  bf16* y = reinterpret_cast<bf16*>(a.y) + (((int64_t)b * a.T + row / p.G) * a.H + kvh * p.G + row % p.G) * HD;
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) y[32 * e + lane] = __float2bfloat16_rn(l == 0.f ? 0.f : acc[e] / l);
+}
+
+struct Plan {
+  int tiles, splits;
+  size_t bytes;
+};
+
+Plan plan_of(int B, int T, int H, int HKV, int HD, int64_t n) {
+  Plan pl;
+  const int64_t rows = (int64_t)T * (H / HKV), heads = (int64_t)B * HKV;
+  pl.tiles = (int)((rows + 255) / 256);
+  // as many splits as fill the machine, of four blocks or more
+  int64_t splits = 148 / (heads * pl.tiles);
+  const int64_t most = (n + T + kKeys - 1) / kKeys / 4;
+  if (splits > most) splits = most;
+  pl.splits = splits < 1 ? 1 : (int)splits;
+  pl.bytes = pl.splits > 1 ? (size_t)heads * (size_t)rows * (size_t)pl.splits * ((size_t)HD * 4 + 8) : 0;
+  return pl;
+}
+
+template <int HD>
+int launch(Params& p, const Plan& pl, cudaStream_t s) {
+  const size_t smem = sizeof(Smem<HD>) + 1024;
+  if (cudaFuncSetAttribute(kv8_prompt_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return BOLT3_ERR_CUDA;
+  const int64_t heads = (int64_t)p.a.B * p.a.HKV;
+  p.part = reinterpret_cast<float*>(p.a.workspace);
+  p.part_ml = reinterpret_cast<float2*>(p.part + (size_t)heads * p.rows * pl.splits * HD);
+  if (launch_overlapped(kv8_prompt_kernel<HD>, dim3((unsigned)(heads * pl.tiles), (unsigned)pl.splits), dim3(kThreads), smem, s,
+                        p) != cudaSuccess)
+    return BOLT3_ERR_CUDA;
+  if (pl.splits > 1 && launch_overlapped(kv8_prompt_join_kernel<HD>, dim3((unsigned)((heads * p.rows + 3) / 4)), dim3(128), 0, s,
+                                         p) != cudaSuccess)
+    return BOLT3_ERR_CUDA;
+  return BOLT3_OK;
+}
+
+}  // namespace
+
+size_t kv8_prompt_workspace(int B, int T, int H, int HKV, int HD, int64_t n) { return plan_of(B, T, H, HKV, HD, n).bytes; }
+
+int kv8_prompt_launch(const bolt3_kv8_attend_args* a, const Length& len, cudaStream_t s) {
+  const Plan pl = plan_of(a->B, a->T, a->H, a->HKV, a->HD, a->n);
+  if (pl.bytes > 0 && (a->workspace == nullptr || a->workspace_bytes < pl.bytes)) return BOLT3_ERR_CAPACITY;
+  if ((int64_t)a->B * a->HKV * pl.tiles > 0x7fffffff) return BOLT3_ERR_SHAPE;
+  Params p;
+  p.a = *a;
+  p.len = len;
+  p.G = a->H / a->HKV;
+  p.rows = a->T * p.G;
+  p.tiles = pl.tiles;
+  p.splits = pl.splits;
+  return a->HD == 128 ? launch<128>(p, pl, s) : launch<64>(p, pl, s);
+}
