@@ -28,7 +28,13 @@ using namespace b3;
 using namespace kv8;
 
 constexpr int kKeys = 128;                       // of a block
-constexpr int kThreads = 416;                    // 4 + 4 softmax warps, 4 widening warps, 1 issuing warp
+constexpr int kThreads = 512;                    // 4 + 4 softmax warps, 4 widening warps, 1 issuing warp (of 4)
+// registers of a thread by role, out of the 128 that each of the 512 is launched with: 2 * 160 + 112 + 80 = 4 * 128
+constexpr int kRegsSoftmax = 160, kRegsWiden = 112, kRegsIssue = 80;
+template <int N>
+B3_DEV void more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
+template <int N>
+B3_DEV void fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
 constexpr uint32_t kWaitIters = 1u << 24;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;
@@ -222,6 +228,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 
   if (warp >= 8 && warp < 12) {
     // ---- widening
+    fewer_regs<kRegsWiden>();
     constexpr int PPR = HD / 16, NP = kKeys * PPR / 128;          // 16-byte pieces of a row, of a thread
     const int t = tid - 256;
     const int8_t* kd = a.data + (int64_t)head * a.cap * HD;
@@ -267,9 +274,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       }
       key = next;
     }
-  } else if (warp == 12) {
+  } else if (warp >= 12) {
     // ---- issue
-    if (lane == 0) {
+    fewer_regs<kRegsIssue>();
+    if (tid == 384) {
       constexpr uint32_t kIdS = tc5::idesc_f16(128, kKeys, false, false), kIdO = tc5::idesc_f16(128, HD, false, true);
       auto scores = [&](int i, int st) {
         const uint32_t qa = tc5::smem_u32(sm.q[i]), ka = tc5::smem_u32(sm.k[st]);
@@ -317,7 +325,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       }
     }
     __syncwarp();
-  } else if ((warp >> 2) < n_tile) {
+  } else {
+    more_regs<kRegsSoftmax>();
+    if ((warp >> 2) < n_tile) {
     // ---- softmax of tile i: this thread's row
     const int i = warp >> 2, row = row0 + tid;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, ts = tb + i * 128 + lanes, to = tb + 256 + i * 128 + lanes;
@@ -333,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc5::fence_after_sync();
-      uint64_t l2 = 0;
+      uint64_t l2 = 0, l3 = 0;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t sc[2][32];
@@ -376,6 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           M = to_M;
           l *= f;
           l2 = mul2(l2, pair(f, f));
+          l3 = mul2(l3, pair(f, f));
           if (j > 0 || h > 0) {
             if (h > 0) {                                          // the first half's product may still be under way
               ok = __all_sync(0xffffffffu, wait(&sm.pv_half[i], j));
@@ -398,28 +409,31 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         const float ref = M == neg_inf() ? 0.f : M;
         const uint64_t minus = pair(-ref, -ref);
         uint32_t w[32];
+        if (masked) {                                             // an unseen key has weight 0, whatever its scale holds
 #pragma unroll
-        for (int x = 0; x < 64; x += 4) {
-          const ulonglong2 i4 = *reinterpret_cast<const ulonglong2*>(iv + x);
-          const float2 u = unpair(add2(pair(t[x], t[x + 1]), minus)), v = unpair(add2(pair(t[x + 2], t[x + 3]), minus));
-          const float e0 = ex2(u.x), e1 = ex2(u.y), e2 = ex2(v.x), e3 = ex2(v.y);
-          if (masked) {                                           // an unseen key has weight 0, whatever its scale holds
-            const float2 a0 = unpair(i4.x), a1 = unpair(i4.y);
-            l += (e0 == 0.f ? 0.f : e0 * a0.x) + (e1 == 0.f ? 0.f : e1 * a0.y) + (e2 == 0.f ? 0.f : e2 * a1.x) +
-                 (e3 == 0.f ? 0.f : e3 * a1.y);
-          } else {
-            l2 = fma2(pair(e0, e1), i4.x, l2);
-            l2 = fma2(pair(e2, e3), i4.y, l2);
+          for (int x = 0; x < 64; x += 2) {
+            const float e0 = ex2(t[x] - ref), e1 = ex2(t[x + 1] - ref);
+            l += (e0 == 0.f ? 0.f : e0 * iv[x]) + (e1 == 0.f ? 0.f : e1 * iv[x + 1]);
+            w[x / 2] = pack_f16(e0, e1);
           }
-          w[x / 2] = pack_f16(e0, e1);
-          w[x / 2 + 1] = pack_f16(e2, e3);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 64; x += 4) {
+            const ulonglong2 i4 = *reinterpret_cast<const ulonglong2*>(iv + x);
+            const float2 u = unpair(add2(pair(t[x], t[x + 1]), minus)), v = unpair(add2(pair(t[x + 2], t[x + 3]), minus));
+            const float e0 = ex2(u.x), e1 = ex2(u.y), e2 = ex2(v.x), e3 = ex2(v.y);
+            l2 = fma2(pair(e0, e1), i4.x, l2);
+            l3 = fma2(pair(e2, e3), i4.y, l3);
+            w[x / 2] = pack_f16(e0, e1);
+            w[x / 2 + 1] = pack_f16(e2, e3);
+          }
         }
         tc5::st32(ts + 32 * h, w);
         tc5::st_wait();
         tc5::fence_before_sync();
         tc5::mbar_arrive(&sm.p_full[i][h]);
       }
-      const float2 x = unpair(l2);
+      const float2 x = unpair(add2(l2, l3));
       l += x.x + x.y;
     }
     ok = ok && wait(&sm.o_full[i], 0);
@@ -452,6 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         }
       }
       if (p.splits > 1 && row < p.rows) p.part_ml[at] = make_float2(M, l);
+    }
     }
   }
   tc5::fence_before_sync();
