@@ -11,9 +11,11 @@
 // - warps 8-11 widen: global int8 -> registers (a block ahead) -> f16 operand tiles in shared memory (two stages of K and
 //   of V), and the block's scales;
 // - one thread of warp 12 issues tcgen05.mma: S = Q K^T into TMEM, O += P V with P as the TMEM operand;
-// - warps 0-3 and 4-7 are the softmax of a tile, a thread per row, 64 keys at a time: scores out of TMEM, weights back
-//   over them, fp32 arithmetic in packed pairs. The bound M moves only when a weight would pass 2^8; only then are the
-//   sums in TMEM rescaled.
+// - warps 0-3 and 4-7 are the softmax of a tile, 64 keys at a time: scores out of TMEM, weights back over them, fp32
+//   arithmetic in packed pairs. A thread takes 16 of the 64 keys of four rows (the 16x256b TMEM layout) and not 64 keys
+//   of one: what belongs to a key (its scales) is then read from shared memory once for four rows. With a thread per row
+//   these reads, the same address in all lanes, took twice the shared-memory time of the MMAs. The bound M moves only
+//   when a weight would pass 2^8; only then are the sums in TMEM rescaled.
 // While one tile's softmax runs, the tensor cores work on the other tile. With few heads the keys are split over CTAs,
 // whose partial sums a second kernel joins.
 #include "../../include/bolt3.h"
@@ -53,6 +55,7 @@ struct Smem {
   unsigned char k[2][kKeys * HD * 2];
   unsigned char v[2][kKeys * HD * 2];
   float scale[2][3][kKeys];                      // key scale, log2 and reciprocal of the value scale
+  float c[256];                                  // sm_scale log2(e) times the unit of a query row in f16
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t s_full[2], p_full[2][2], pv_half[2], o_full[2];
   uint32_t tbase;
@@ -109,6 +112,27 @@ B3_DEV float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
+}
+
+// 64 columns of 16 TMEM lanes: a thread gets columns 8 n + 2 (lane % 4) and the next one of lanes lane / 4 (registers
+// 4 n, 4 n + 1) and lane / 4 + 8 (4 n + 2, 4 n + 3)
+B3_DEV void ld_16x64(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// 32 columns of 16 TMEM lanes: column 4 n + lane % 4 of lanes lane / 4 (register 2 n) and lane / 4 + 8 (2 n + 1)
+B3_DEV void st_16x32(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
 }
 
 // 16 int8 of row r, dimensions 16 c .., as f16 into an operand tile. Lanes of the upper column block store their two
@@ -177,7 +201,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
   }
 
   // this thread's query row to f16, in the operand tile
-  float c_row = 0.f;
   if (warp < 8) {
     const int r = tid & 127, row = row0 + tid;
     uint4 raw[HD / 8];
@@ -198,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     // 2^-e brings the row's largest value into [1, 2): f16 keeps all of a bf16's bits down to 2^-17 of it
     const int e = m > 0.f && m < 3e38f ? max(ilogbf(m), -100) : 0;
     const float down = exp2f((float)-e);
-    c_row = a.sm_scale * kLog2e * exp2f((float)e);
+    sm.c[tid] = a.sm_scale * kLog2e * exp2f((float)e);
     unsigned char* tile = sm.q[tid >> 7];
 #pragma unroll
     for (int i = 0; i < HD / 8; ++i) {
@@ -275,66 +298,89 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       key = next;
     }
   } else if (warp >= 12) {
-    // ---- issue
+    // ---- issue. The whole warp runs the loop, so that addresses and descriptors are uniform over it (a lone thread in a
+    // branch of its own needed 170 cycles an MMA for moving them to where the instruction takes them); one lane issues
     fewer_regs<kRegsIssue>();
-    if (tid == 384) {
+    if (warp == 12) {
+      uint32_t one;
+      asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}\n" : "=r"(one));
       constexpr uint32_t kIdS = tc5::idesc_f16(128, kKeys, false, false), kIdO = tc5::idesc_f16(128, HD, false, true);
+      constexpr uint64_t kTile = sizeof(sm.q[0]) >> 4;            // from one tile's descriptor to the next one's
+      const uint32_t tu = __shfl_sync(0xffffffffu, tb, 0);
+      const uint64_t q_desc = tc5::sdesc(tc5::smem_u32(sm.q[0]), 16, 1024), k_desc = tc5::sdesc(tc5::smem_u32(sm.k[0]), 16, 1024);
+      const uint64_t v_desc = tc5::sdesc(tc5::smem_u32(sm.v[0]), kKeys * 128, 1024);
       auto scores = [&](int i, int st) {
-        const uint32_t qa = tc5::smem_u32(sm.q[i]), ka = tc5::smem_u32(sm.k[st]);
+        const uint64_t qd = q_desc + i * kTile, kd = k_desc + st * kTile;
+        if (one) {
 #pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * (kKeys * 128) + (ks & 3) * 32;
-          tc5::mma_ss(tb + i * 128, tc5::sdesc(qa + off, 16, 1024), tc5::sdesc(ka + off, 16, 1024), kIdS, ks > 0);
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            constexpr uint64_t kBlock = (kKeys * 128) >> 4;       // a block of 64 columns
+            tc5::mma_ss(tu + i * 128, qd + (ks >> 2) * kBlock + (ks & 3) * 2, kd + (ks >> 2) * kBlock + (ks & 3) * 2, kIdS, ks > 0);
+          }
+          tc5::commit(&sm.s_full[i]);
         }
-        tc5::commit(&sm.s_full[i]);
       };
-      bool ok = wait(&sm.k_full[0], 0);
+      auto product = [&](int i, int st, int h, bool first) {
+        const uint64_t vd = v_desc + st * kTile + 4 * h * 128;
+        const uint32_t d = tu + 256 + i * 128, pa = tu + i * 128 + 32 * h;
+        if (one) {
+          tc5::mma_ts(d, pa, vd, kIdO, !first);
+          tc5::mma_ts(d, pa + 8, vd + 128, kIdO, 1);
+          tc5::mma_ts(d, pa + 16, vd + 256, kIdO, 1);
+          tc5::mma_ts(d, pa + 24, vd + 384, kIdO, 1);
+        }
+      };
+      auto wait_all = [&](uint64_t* bar, int phase) { return __all_sync(0xffffffffu, wait(bar, phase)) != 0; };
+      bool ok = wait_all(&sm.k_full[0], 0);
       if (ok) {
         tc5::fence_after_sync();
         for (int i = 0; i < n_tile; ++i) scores(i, 0);
-        tc5::commit(&sm.k_empty[0]);
+        if (one) tc5::commit(&sm.k_empty[0]);
       }
       for (int j = 0; ok && j < n_blk; ++j) {
         const int st = j & 1;
-        ok = wait(&sm.v_full[st], j >> 1);
-        const uint32_t va = tc5::smem_u32(sm.v[st]);
+        ok = wait_all(&sm.v_full[st], j >> 1);
         for (int i = 0; ok && i < n_tile; ++i) {
-          for (int h = 0; ok && h < 2; ++h) {
-            ok = wait(&sm.p_full[i][h], j);
-            if (!ok) break;
-            tc5::fence_after_sync();
-#pragma unroll
-            for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
-              tc5::mma_ts(tb + 256 + i * 128, tb + i * 128 + ks * 8, tc5::sdesc(va + ks * 2048, kKeys * 128, 1024), kIdO,
-                          j > 0 || ks > 0);
-            if (h == 0) tc5::commit(&sm.pv_half[i]);
-            else if (j + 1 == n_blk) tc5::commit(&sm.o_full[i]);
-          }
+          ok = wait_all(&sm.p_full[i][0], j);
           if (!ok) break;
-          if (j + 1 < n_blk) {
-            if (i == 0) ok = wait(&sm.k_full[st ^ 1], (j + 1) >> 1);
+          tc5::fence_after_sync();
+          product(i, st, 0, j == 0);
+          if (one) tc5::commit(&sm.pv_half[i]);
+          ok = wait_all(&sm.p_full[i][1], j);
+          if (!ok) break;
+          tc5::fence_after_sync();
+          product(i, st, 1, false);
+          if (j + 1 == n_blk) {
+            if (one) tc5::commit(&sm.o_full[i]);
+          } else {
+            if (i == 0) ok = wait_all(&sm.k_full[st ^ 1], (j + 1) >> 1);
             if (!ok) break;
             tc5::fence_after_sync();
             scores(i, st ^ 1);
           }
         }
-        if (ok) {
+        if (ok && one) {
           tc5::commit(&sm.v_empty[st]);
           if (j + 1 < n_blk) tc5::commit(&sm.k_empty[st ^ 1]);
         }
       }
     }
-    __syncwarp();
   } else {
     more_regs<kRegsSoftmax>();
     if ((warp >> 2) < n_tile) {
-    // ---- softmax of tile i: this thread's row
+    // ---- softmax of tile i: this thread's four rows are those of TMEM lanes grp + 8 q of its warp's 32
     const int i = warp >> 2, row = row0 + tid;
+    const int grp = lane >> 2, tig = lane & 3, first_row = row0 + (tid & ~31) + grp;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, ts = tb + i * 128 + lanes, to = tb + 256 + i * 128 + lanes;
-    const int64_t see = row < p.rows ? s + row / p.G + 1 : s + last + 1;          // keys this row sees
-    const int64_t see_all = s + (row0 + i * 128) / p.G + 1;                       // that every row of the tile sees
-    float M = neg_inf(), l = 0.f;
-    const uint64_t c2 = pair(c_row, c_row);
+    const int64_t see_all = s + (row0 + i * 128) / p.G + 1;                       // keys that every row of the tile sees
+    float M[4], c[4];
+    uint64_t l[4];                                                // sums of weights over this thread's keys, in pairs
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      M[q] = neg_inf();
+      c[q] = sm.c[(tid & ~31) + grp + 8 * q];
+      l[q] = 0;
+    }
     bool ok = true;
     for (int j = 0; ok && j < n_blk; ++j) {
       const int st = j & 1;
@@ -343,55 +389,67 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc5::fence_after_sync();
-      uint64_t l2 = 0, l3 = 0;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t sc[2][32];
-        tc5::ld32(ts + 64 * h, sc[0]);
-        tc5::ld32(ts + 64 * h + 32, sc[1]);
-        tc5::ld_wait();
-        float t[64];
-        float m0 = neg_inf(), m1 = neg_inf();
-        const float* ks = sm.scale[st][0] + 64 * h;
-        const float* lg = sm.scale[st][1] + 64 * h;
-        const float* iv = sm.scale[st][2] + 64 * h;
+        uint32_t sc[2][32];                                       // rows grp, grp + 8; grp + 16, grp + 24
+        ld_16x64(ts + 64 * h, sc[0]);
+        ld_16x64(ts + 64 * h + (16u << 16), sc[1]);
+        const float* ks = sm.scale[st][0] + 64 * h + 2 * tig;
+        const float* lg = sm.scale[st][1] + 64 * h + 2 * tig;
+        const float* iv = sm.scale[st][2] + 64 * h + 2 * tig;
         const int64_t key = (lo + j) * kKeys + 64 * h;
+        float2 t[4][8];                                           // row q, keys 8 n + 2 tig and the next
+        tc5::ld_wait();
 #pragma unroll
-        for (int x = 0; x < 64; x += 4) {
-          const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(ks + x), g4 = *reinterpret_cast<const ulonglong2*>(lg + x);
-          const float2 u = unpair(fma2(pair(__uint_as_float(sc[x >> 5][x & 31]), __uint_as_float(sc[x >> 5][(x & 31) + 1])),
-                                       mul2(k4.x, c2), g4.x));
-          const float2 v = unpair(fma2(pair(__uint_as_float(sc[x >> 5][(x & 31) + 2]), __uint_as_float(sc[x >> 5][(x & 31) + 3])),
-                                       mul2(k4.y, c2), g4.y));
-          t[x] = u.x; t[x + 1] = u.y; t[x + 2] = v.x; t[x + 3] = v.y;
+        for (int n = 0; n < 8; ++n) {
+          const uint64_t k2 = *reinterpret_cast<const uint64_t*>(ks + 8 * n), g2 = *reinterpret_cast<const uint64_t*>(lg + 8 * n);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            t[q][n] = unpair(fma2(pair(__uint_as_float(sc[q >> 1][4 * n + 2 * (q & 1)]), __uint_as_float(sc[q >> 1][4 * n + 2 * (q & 1) + 1])),
+                                  mul2(k2, pair(c[q], c[q])), g2));
         }
         const bool masked = key + 64 > see_all;                   // the same for the whole tile
         if (masked) {
-          const int left = (int)min(max(see - key, (int64_t)0), (int64_t)64);
 #pragma unroll
-          for (int x = 0; x < 64; ++x)
-            if (x >= left) t[x] = neg_inf();
-        }
+          for (int q = 0; q < 4; ++q) {
+            const int r = min(first_row + 8 * q, p.rows - 1);
+            const int left = (int)min(max(s + r / p.G + 1 - key, (int64_t)0), (int64_t)64) - 2 * tig;   // seen, from this thread's first
 #pragma unroll
-        for (int x = 0; x < 64; x += 4) {
-          m0 = max3(m0, t[x], t[x + 1]);
-          m1 = max3(m1, t[x + 2], t[x + 3]);
+            for (int n = 0; n < 8; ++n) {
+              if (8 * n >= left) t[q][n].x = neg_inf();
+              if (8 * n + 1 >= left) t[q][n].y = neg_inf();
+            }
+          }
         }
-        m0 = fmaxf(m0, m1);
-        // the bound moves only when a weight would pass 2^8 (and at the first key)
-        const bool over = m0 > M + kSlack;
+        // the bounds move only when a weight would pass 2^8 (and at the first key)
+        float m[4];
+        bool over = false;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          m[q] = fmaxf(t[q][0].x, t[q][0].y);
+#pragma unroll
+          for (int n = 1; n < 8; ++n) m[q] = max3(m[q], t[q][n].x, t[q][n].y);
+          over |= m[q] > M[q] + kSlack;
+        }
         if (__any_sync(0xffffffffu, over)) {
-          const float to_M = over ? m0 : M;
-          const float f = M == neg_inf() ? 0.f : ex2(M - to_M);   // 1 where the bound stays
-          M = to_M;
-          l *= f;
-          l2 = mul2(l2, pair(f, f));
-          l3 = mul2(l3, pair(f, f));
+          float f[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            m[q] = quad_max(m[q]);
+            const float to_M = m[q] > M[q] + kSlack ? m[q] : M[q];
+            f[q] = M[q] == neg_inf() ? 0.f : ex2(M[q] - to_M);    // 1 where the bound stays
+            M[q] = to_M;
+            l[q] = mul2(l[q], pair(f[q], f[q]));
+          }
           if (j > 0 || h > 0) {
             if (h > 0) {                                          // the first half's product may still be under way
               ok = __all_sync(0xffffffffu, wait(&sm.pv_half[i], j));
               tc5::fence_after_sync();
             }
+            // lane's row is row q = lane / 8 of the threads with grp = lane % 8
+            const float f0 = __shfl_sync(0xffffffffu, f[0], 4 * (lane & 7)), f1 = __shfl_sync(0xffffffffu, f[1], 4 * (lane & 7));
+            const float f2 = __shfl_sync(0xffffffffu, f[2], 4 * (lane & 7)), f3 = __shfl_sync(0xffffffffu, f[3], 4 * (lane & 7));
+            const float fr = lane < 16 ? (lane < 8 ? f0 : f1) : (lane < 24 ? f2 : f3);
             if (ok) {
 #pragma unroll 1
               for (int d = 0; d < HD; d += 16) {
@@ -399,49 +457,63 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 tc5::ld16(to + d, o);
                 tc5::ld_wait();
 #pragma unroll
-                for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * fr);
                 tc5::st16(to + d, o);
               }
               tc5::st_wait();
             }
           }
         }
-        const float ref = M == neg_inf() ? 0.f : M;
-        const uint64_t minus = pair(-ref, -ref);
-        uint32_t w[32];
+        uint32_t w[2][16];
         if (masked) {                                             // an unseen key has weight 0, whatever its scale holds
 #pragma unroll
-          for (int x = 0; x < 64; x += 2) {
-            const float e0 = ex2(t[x] - ref), e1 = ex2(t[x + 1] - ref);
-            l += (e0 == 0.f ? 0.f : e0 * iv[x]) + (e1 == 0.f ? 0.f : e1 * iv[x + 1]);
-            w[x / 2] = pack_f16(e0, e1);
+          for (int q = 0; q < 4; ++q) {
+            const float ref = M[q] == neg_inf() ? 0.f : M[q];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+              const float e0 = ex2(t[q][n].x - ref), e1 = ex2(t[q][n].y - ref);
+              l[q] = add2(l[q], pair(e0 == 0.f ? 0.f : e0 * iv[8 * n], e1 == 0.f ? 0.f : e1 * iv[8 * n + 1]));
+              w[q >> 1][2 * n + (q & 1)] = pack_f16(e0, e1);
+            }
           }
         } else {
 #pragma unroll
-          for (int x = 0; x < 64; x += 4) {
-            const ulonglong2 i4 = *reinterpret_cast<const ulonglong2*>(iv + x);
-            const float2 u = unpair(add2(pair(t[x], t[x + 1]), minus)), v = unpair(add2(pair(t[x + 2], t[x + 3]), minus));
-            const float e0 = ex2(u.x), e1 = ex2(u.y), e2 = ex2(v.x), e3 = ex2(v.y);
-            l2 = fma2(pair(e0, e1), i4.x, l2);
-            l3 = fma2(pair(e2, e3), i4.y, l3);
-            w[x / 2] = pack_f16(e0, e1);
-            w[x / 2 + 1] = pack_f16(e2, e3);
+          for (int n = 0; n < 8; ++n) {
+            const uint64_t i2 = *reinterpret_cast<const uint64_t*>(iv + 8 * n);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const float2 u = unpair(add2(pair(t[q][n].x, t[q][n].y), pair(-M[q], -M[q])));
+              const float e0 = ex2(u.x), e1 = ex2(u.y);
+              l[q] = fma2(pair(e0, e1), i2, l[q]);
+              w[q >> 1][2 * n + (q & 1)] = pack_f16(e0, e1);
+            }
           }
         }
-        tc5::st32(ts + 32 * h, w);
+        st_16x32(ts + 32 * h, w[0]);
+        st_16x32(ts + 32 * h + (16u << 16), w[1]);
         tc5::st_wait();
         tc5::fence_before_sync();
         tc5::mbar_arrive(&sm.p_full[i][h]);
       }
-      const float2 x = unpair(add2(l2, l3));
-      l += x.x + x.y;
+    }
+    // the bound and the sum of weights of the row in this thread's TMEM lane
+    float M_row = 0.f, l_row = 0.f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float2 x = unpair(l[q]);
+      const float sum = quad_sum(x.x + x.y);
+      const float mm = __shfl_sync(0xffffffffu, M[q], 4 * (lane & 7)), ll = __shfl_sync(0xffffffffu, sum, 4 * (lane & 7));
+      if (lane >> 3 == q) {
+        M_row = mm;
+        l_row = ll;
+      }
     }
     ok = ok && wait(&sm.o_full[i], 0);
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       tc5::fence_after_sync();
       const int64_t at = ((int64_t)head * p.rows + row) * p.splits + split;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = l_row == 0.f ? 0.f : 1.f / l_row;
 #pragma unroll 1
       for (int d = 0; d < HD; d += 32) {
         uint32_t o[32];
@@ -465,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           }
         }
       }
-      if (p.splits > 1 && row < p.rows) p.part_ml[at] = make_float2(M, l);
+      if (p.splits > 1 && row < p.rows) p.part_ml[at] = make_float2(M_row, l_row);
     }
     }
   }
