@@ -1,9 +1,9 @@
 // Softmax attention of many query rows (prompt slices) over the 8-bit KV cache, on the tensor cores' TMEM path.
 //
 // The mathematics and its roundings are those of kv8_attend.cu: with t_j the score of key j in log2 units and
-// u_j = t_j + log2 scale_v[j], weights w_j = 2^(u_j - M) in f16, y = sum w_j v8_j / sum (w_j / scale_v[j]). Here a
-// query row is brought to f16 by a power of two of its own (exact down to 2^-25 of its largest value) and the int8
-// keys and values are exact in f16.
+// u_j = t_j + log2 scale_v[j], weights w_j = 2^(u_j - M) in f16, y = sum w_j v8_j / sum (w_j / scale_v[j]). Here the
+// CTA's query rows are brought to f16 by one power of two (exact down to 2^-25 of the largest value among them, which
+// moves a score by 2^-25 of the largest score's sum of magnitudes) and the int8 keys and values are exact in f16.
 //
 // Bound by arithmetic: 4 HD operations per (query row, key), and one exponential. A CTA holds two tiles of 128 query
 // rows (T * G rows of one KV head, token-major) and walks the keys in blocks of 128, so that a block is widened from
@@ -54,8 +54,9 @@ struct Smem {
   unsigned char q[2][kKeys * HD * 2];            // K-major operand tiles: HD / 64 blocks of [128 rows][64 columns]
   unsigned char k[2][kKeys * HD * 2];
   unsigned char v[2][kKeys * HD * 2];
-  float scale[2][3][kKeys];                      // key scale, log2 and reciprocal of the value scale
-  float c[256];                                  // sm_scale log2(e) times the unit of a query row in f16
+  float scale[2][3][kKeys];                      // key scale (times sm_scale log2(e) and the queries' unit), log2 and
+                                                 // reciprocal of the value scale
+  float q_max[8];
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t s_full[2], p_full[2][2], pv_half[2], o_full[2];
   uint32_t tbase;
@@ -200,10 +201,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     return;
   }
 
-  // this thread's query row to f16, in the operand tile
+  // this thread's query row to f16, in the operand tile. 2^-e brings the largest value of the CTA's rows into [1, 2)
+  uint4 raw[HD / 8];
   if (warp < 8) {
-    const int r = tid & 127, row = row0 + tid;
-    uint4 raw[HD / 8];
+    const int row = row0 + tid;
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < HD / 8; ++i) {
@@ -215,13 +216,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 v = unpack_bf16(w[j]);
-        m = max3(m, fabsf(v.x), fabsf(v.y));
+        m = max3(m, fabsf(v.x) < 3e38f ? fabsf(v.x) : 0.f, fabsf(v.y) < 3e38f ? fabsf(v.y) : 0.f);   // finite ones
       }
     }
-    // 2^-e brings the row's largest value into [1, 2): f16 keeps all of a bf16's bits down to 2^-17 of it
-    const int e = m > 0.f && m < 3e38f ? max(ilogbf(m), -100) : 0;
+    m = warp_max(m);
+    if (lane == 0) sm.q_max[warp] = m;
+  }
+  __syncthreads();
+  float q_max = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) q_max = fmaxf(q_max, sm.q_max[i]);
+  const int e = q_max > 0.f ? max(ilogbf(q_max), -100) : 0;
+  const float c_all = a.sm_scale * kLog2e * exp2f((float)e);      // goes into the key scales
+  if (warp < 8) {
+    const int r = tid & 127;
     const float down = exp2f((float)-e);
-    sm.c[tid] = a.sm_scale * kLog2e * exp2f((float)e);
     unsigned char* tile = sm.q[tid >> 7];
 #pragma unroll
     for (int i = 0; i < HD / 8; ++i) {
@@ -285,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       if (j >= 2 && !wait(&sm.v_empty[st], (j >> 1) - 1)) break;
 #pragma unroll
       for (int i = 0; i < NP; ++i) widen16(sm.v[st], (i * 128 + t) / PPR, (i * 128 + t) % PPR, vr[i]);
-      sm.scale[st][0][t] = k_sc;
+      sm.scale[st][0][t] = k_sc * c_all;
       sm.scale[st][1][t] = lg2(v_sc);
       sm.scale[st][2][t] = rcp(v_sc);
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
@@ -373,12 +382,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     const int grp = lane >> 2, tig = lane & 3, first_row = row0 + (tid & ~31) + grp;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, ts = tb + i * 128 + lanes, to = tb + 256 + i * 128 + lanes;
     const int64_t see_all = s + (row0 + i * 128) / p.G + 1;                       // keys that every row of the tile sees
-    float M[4], c[4];
+    float M[4];
     uint64_t l[4];                                                // sums of weights over this thread's keys, in pairs
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       M[q] = neg_inf();
-      c[q] = sm.c[(tid & ~31) + grp + 8 * q];
       l[q] = 0;
     }
     bool ok = true;
@@ -406,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             t[q][n] = unpair(fma2(pair(__uint_as_float(sc[q >> 1][4 * n + 2 * (q & 1)]), __uint_as_float(sc[q >> 1][4 * n + 2 * (q & 1) + 1])),
-                                  mul2(k2, pair(c[q], c[q])), g2));
+                                  k2, g2));
         }
         const bool masked = key + 64 > see_all;                   // the same for the whole tile
         if (masked) {
