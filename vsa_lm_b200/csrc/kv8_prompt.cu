@@ -8,14 +8,15 @@
 // Bound by arithmetic: 4 HD operations per (query row, key), and one exponential. A CTA holds two tiles of 128 query
 // rows (T * G rows of one KV head, token-major) and walks the keys in blocks of 128, so that a block is widened from
 // int8 to f16 once for 256 rows. Roles, which meet only at mbarriers:
-// - warps 8-11 widen: global int8 -> registers (a block ahead) -> f16 operand tiles in shared memory (two stages of K and
-//   of V), and the block's scales;
-// - one thread of warp 12 issues tcgen05.mma: S = Q K^T into TMEM, O += P V with P as the TMEM operand;
-// - warps 0-3 and 4-7 are the softmax of a tile, 64 keys at a time: scores out of TMEM, weights back over them, fp32
-//   arithmetic in packed pairs. A thread takes 16 of the 64 keys of four rows (the 16x256b TMEM layout) and not 64 keys
-//   of one: what belongs to a key (its scales) is then read from shared memory once for four rows. With a thread per row
-//   these reads, the same address in all lanes, took twice the shared-memory time of the MMAs. The bound M moves only
-//   when a weight would pass 2^8; only then are the sums in TMEM rescaled.
+// - warps 16-19 widen keys, 20-23 values: global int8 -> registers (a block ahead) -> f16 operand tiles in shared memory
+//   (two stages each); the latter also prepare the block's scales;
+// - one lane of warp 24 issues tcgen05.mma: S = Q K^T into TMEM, O += P V with P as the TMEM operand;
+// - warps 0-7 and 8-15 are the softmax of a tile, 64 keys at a time: scores out of TMEM, weights back over them, fp32
+//   arithmetic in packed pairs. A warp takes 16 TMEM lanes in the 16x256b layout, a thread 16 of the 64 keys of two rows:
+//   what belongs to a key (its scales) is then read from shared memory once for two rows, where a thread per row, all
+//   lanes reading the same address, took twice the shared-memory time of the MMAs; and with four such warps on a
+//   scheduler one's latencies are filled by the others. The bound M moves only when a weight would pass 2^8; only then
+//   are the sums in TMEM rescaled.
 // While one tile's softmax runs, the tensor cores work on the other tile. With few heads the keys are split over CTAs,
 // whose partial sums a second kernel joins.
 #include "../../include/bolt3.h"
@@ -30,9 +31,9 @@ using namespace b3;
 using namespace kv8;
 
 constexpr int kKeys = 128;                       // of a block
-constexpr int kThreads = 512;                    // 4 + 4 softmax warps, 4 widening warps, 1 issuing warp (of 4)
-// registers of a thread by role, out of the 128 that each of the 512 is launched with: 2 * 160 + 112 + 80 = 4 * 128
-constexpr int kRegsSoftmax = 160, kRegsWiden = 112, kRegsIssue = 80;
+constexpr int kThreads = 896;                    // 16 softmax warps, 4 + 4 widening warps, 1 issuing warp (of 4)
+// registers of a thread by role, out of the 72 that each of the 896 is launched with: 4 * 80 + 64 + 64 + 56 = 7 * 72
+constexpr int kRegsSoftmax = 80, kRegsWiden = 64, kRegsIssue = 56;
 template <int N>
 B3_DEV void more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
 template <int N>
@@ -56,7 +57,7 @@ struct Smem {
   unsigned char v[2][kKeys * HD * 2];
   float scale[2][3][kKeys];                      // key scale (times sm_scale log2(e) and the queries' unit), log2 and
                                                  // reciprocal of the value scale
-  float q_max[8];
+  float q_max[16];
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t s_full[2], p_full[2][2], pv_half[2], o_full[2];
   uint32_t tbase;
@@ -136,6 +137,22 @@ B3_DEV void st_16x32(uint32_t taddr, const uint32_t (&r)[16]) {
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
 }
 
+// the layout of ld_16x64, 32 columns
+B3_DEV void ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+B3_DEV void st_16x32f(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
+}
+
 // 16 int8 of row r, dimensions 16 c .., as f16 into an operand tile. Lanes of the upper column block store their two
 // 16-byte chunks in the other order, so that the eight lanes of a row keep off each other's banks
 B3_DEV void widen16(unsigned char* tile, int r, int c, const uint4& x) {
@@ -167,8 +184,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       tc5::mbar_init(&sm.v_full[i], 128);
       tc5::mbar_init(&sm.v_empty[i], 1);
       tc5::mbar_init(&sm.s_full[i], 1);
-      tc5::mbar_init(&sm.p_full[i][0], 128);
-      tc5::mbar_init(&sm.p_full[i][1], 128);
+      tc5::mbar_init(&sm.p_full[i][0], 256);
+      tc5::mbar_init(&sm.p_full[i][1], 256);
       tc5::mbar_init(&sm.pv_half[i], 1);
       tc5::mbar_init(&sm.o_full[i], 1);
     }
@@ -201,17 +218,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     return;
   }
 
-  // this thread's query row to f16, in the operand tile. 2^-e brings the largest value of the CTA's rows into [1, 2)
-  uint4 raw[HD / 8];
-  if (warp < 8) {
-    const int row = row0 + tid;
+  // this thread's half of query row tid / 2 to f16, in the operand tile. 2^-e brings the largest value of the CTA's rows
+  // into [1, 2)
+  uint4 raw[HD / 16];
+  if (warp < 16) {
+    const int row = row0 + (tid >> 1);
     float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < HD / 8; ++i) {
+    for (int i = 0; i < HD / 16; ++i) {
       raw[i] = make_uint4(0, 0, 0, 0);
       if (row < p.rows)
         raw[i] = reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.q) + b * a.q_sb + (row / p.G) * a.q_st +
-                                                (int64_t)(kvh * p.G + row % p.G) * HD)[i];
+                                                (int64_t)(kvh * p.G + row % p.G) * HD)[2 * i + (tid & 1)];
       const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -225,25 +243,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
   __syncthreads();
   float q_max = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) q_max = fmaxf(q_max, sm.q_max[i]);
+  for (int i = 0; i < 16; ++i) q_max = fmaxf(q_max, sm.q_max[i]);
   const int e = q_max > 0.f ? max(ilogbf(q_max), -100) : 0;
-  const float c_all = a.sm_scale * kLog2e * exp2f((float)e);      // goes into the key scales
-  if (warp < 8) {
-    const int r = tid & 127;
+  if (warp < 16) {
+    const int r = (tid >> 1) & 127;
     const float down = exp2f((float)-e);
-    unsigned char* tile = sm.q[tid >> 7];
+    unsigned char* tile = sm.q[tid >> 8];
 #pragma unroll
-    for (int i = 0; i < HD / 8; ++i) {
+    for (int i = 0; i < HD / 16; ++i) {
       const float2 x = unpack_bf16(raw[i].x), y = unpack_bf16(raw[i].y), z = unpack_bf16(raw[i].z), w = unpack_bf16(raw[i].w);
+      const int c = 2 * i + (tid & 1);                            // 16-byte chunk of the row
       uint4 o;
       o.x = pack_f16(x.x * down, x.y * down);
       o.y = pack_f16(y.x * down, y.y * down);
       o.z = pack_f16(z.x * down, z.y * down);
       o.w = pack_f16(w.x * down, w.y * down);
-      *reinterpret_cast<uint4*>(tile + (i >> 3) * (kKeys * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = o;
+      *reinterpret_cast<uint4*>(tile + (c >> 3) * (kKeys * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = o;
     }
   }
-  if (warp == 12) {
+  if (warp == 24) {
     tc5::tmem_alloc(&sm.tbase, 512);
     tc5::tmem_relinquish();
   }
@@ -258,59 +276,54 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     return false;
   };
 
-  if (warp >= 8 && warp < 12) {
-    // ---- widening
+  if (warp >= 16 && warp < 24) {
+    // ---- widening: keys, or values and scales
     fewer_regs<kRegsWiden>();
     constexpr int PPR = HD / 16, NP = kKeys * PPR / 128;          // 16-byte pieces of a row, of a thread
-    const int t = tid - 256;
-    const int8_t* kd = a.data + (int64_t)head * a.cap * HD;
-    const int8_t* vd = kd + (int64_t)a.B * a.HKV * a.cap * HD;
+    const bool values = warp >= 20;
+    const int t = tid & 127;
+    const int64_t side = (int64_t)a.B * a.HKV * a.cap;
+    const int8_t* base = a.data + ((int64_t)head * a.cap + (values ? side : 0)) * HD;
     const float* ks = a.scale + (int64_t)head * a.cap;
-    const float* vs = ks + (int64_t)a.B * a.HKV * a.cap;
+    const float c_all = a.sm_scale * kLog2e * exp2f((float)e);    // what a score in f16 units is worth, into the key scales
     const int64_t end = a.cap - 1;                                // rows past the buffer are read as its last one and masked
-    uint4 kr[NP], vr[NP];
-    float k_sc, v_sc;
-    auto fetch = [&](const int8_t* base, int64_t key, uint4 (&x)[NP]) {
+    uint64_t *full = values ? sm.v_full : sm.k_full, *empty = values ? sm.v_empty : sm.k_empty;
+    uint4 x[NP];
+    float k_sc = 0.f, v_sc = 0.f;
+    auto fetch = [&](int64_t key) {
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         const int idx = i * 128 + t;
         x[i] = __ldg(reinterpret_cast<const uint4*>(base + min(key + idx / PPR, end) * HD) + idx % PPR);
       }
+      if (values) {
+        k_sc = __ldg(ks + min(key + t, end));
+        v_sc = __ldg(ks + side + min(key + t, end));
+      }
     };
     int64_t key = lo * kKeys;
-    fetch(kd, key, kr);
-    fetch(vd, key, vr);
-    k_sc = __ldg(ks + min(key + t, end));
-    v_sc = __ldg(vs + min(key + t, end));
+    fetch(key);
     for (int j = 0; j < n_blk; ++j) {
       const int st = j & 1;
-      const int64_t next = key + kKeys;
-      if (j >= 2 && !wait(&sm.k_empty[st], (j >> 1) - 1)) break;
+      if (j >= 2 && !wait(&empty[st], (j >> 1) - 1)) break;
+      unsigned char* tile = values ? sm.v[st] : sm.k[st];
 #pragma unroll
-      for (int i = 0; i < NP; ++i) widen16(sm.k[st], (i * 128 + t) / PPR, (i * 128 + t) % PPR, kr[i]);
-      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-      tc5::mbar_arrive(&sm.k_full[st]);
-      if (j + 1 < n_blk) fetch(kd, next, kr);
-      if (j >= 2 && !wait(&sm.v_empty[st], (j >> 1) - 1)) break;
-#pragma unroll
-      for (int i = 0; i < NP; ++i) widen16(sm.v[st], (i * 128 + t) / PPR, (i * 128 + t) % PPR, vr[i]);
-      sm.scale[st][0][t] = k_sc * c_all;
-      sm.scale[st][1][t] = lg2(v_sc);
-      sm.scale[st][2][t] = rcp(v_sc);
-      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-      tc5::mbar_arrive(&sm.v_full[st]);
-      if (j + 1 < n_blk) {
-        fetch(vd, next, vr);
-        k_sc = __ldg(ks + min(next + t, end));
-        v_sc = __ldg(vs + min(next + t, end));
+      for (int i = 0; i < NP; ++i) widen16(tile, (i * 128 + t) / PPR, (i * 128 + t) % PPR, x[i]);
+      if (values) {
+        sm.scale[st][0][t] = k_sc * c_all;
+        sm.scale[st][1][t] = lg2(v_sc);
+        sm.scale[st][2][t] = rcp(v_sc);
       }
-      key = next;
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      tc5::mbar_arrive(&full[st]);
+      key += kKeys;
+      if (j + 1 < n_blk) fetch(key);
     }
-  } else if (warp >= 12) {
+  } else if (warp >= 24) {
     // ---- issue. The whole warp runs the loop, so that addresses and descriptors are uniform over it (a lone thread in a
     // branch of its own needed 170 cycles an MMA for moving them to where the instruction takes them); one lane issues
     fewer_regs<kRegsIssue>();
-    if (warp == 12) {
+    if (warp == 24) {
       uint32_t one;
       asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}\n" : "=r"(one));
       constexpr uint32_t kIdS = tc5::idesc_f16(128, kKeys, false, false), kIdO = tc5::idesc_f16(128, HD, false, true);
@@ -376,19 +389,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     }
   } else {
     more_regs<kRegsSoftmax>();
-    if ((warp >> 2) < n_tile) {
-    // ---- softmax of tile i: this thread's four rows are those of TMEM lanes grp + 8 q of its warp's 32
-    const int i = warp >> 2, row = row0 + tid;
-    const int grp = lane >> 2, tig = lane & 3, first_row = row0 + (tid & ~31) + grp;
-    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, ts = tb + i * 128 + lanes, to = tb + 256 + i * 128 + lanes;
+    if ((warp >> 3) < n_tile) {
+    // ---- softmax of tile i: this thread's two rows are those of TMEM lanes first_lane + grp and + grp + 8
+    const int i = warp >> 3, grp = lane >> 2, tig = lane & 3;
+    const int first_lane = 32 * (warp & 3) + 16 * (warp >> 2 & 1), first_row = row0 + 128 * i + first_lane + grp;
+    const uint32_t lanes = (uint32_t)first_lane << 16, ts = tb + i * 128 + lanes, to = tb + 256 + i * 128 + lanes;
     const int64_t see_all = s + (row0 + i * 128) / p.G + 1;                       // keys that every row of the tile sees
-    float M[4];
-    uint64_t l[4];                                                // sums of weights over this thread's keys, in pairs
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      M[q] = neg_inf();
-      l[q] = 0;
-    }
+    float M[2] = {neg_inf(), neg_inf()};
+    uint64_t l[2] = {0, 0};                                       // sums of weights over this thread's keys, in pairs
     bool ok = true;
     for (int j = 0; ok && j < n_blk; ++j) {
       const int st = j & 1;
@@ -399,27 +407,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       tc5::fence_after_sync();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t sc[2][32];                                       // rows grp, grp + 8; grp + 16, grp + 24
-        ld_16x64(ts + 64 * h, sc[0]);
-        ld_16x64(ts + 64 * h + (16u << 16), sc[1]);
+        uint32_t sc[32];
+        ld_16x64(ts + 64 * h, sc);
         const float* ks = sm.scale[st][0] + 64 * h + 2 * tig;
         const float* lg = sm.scale[st][1] + 64 * h + 2 * tig;
         const float* iv = sm.scale[st][2] + 64 * h + 2 * tig;
         const int64_t key = (lo + j) * kKeys + 64 * h;
-        float2 t[4][8];                                           // row q, keys 8 n + 2 tig and the next
+        float2 t[2][8];                                           // row q, keys 8 n + 2 tig and the next
         tc5::ld_wait();
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
           const uint64_t k2 = *reinterpret_cast<const uint64_t*>(ks + 8 * n), g2 = *reinterpret_cast<const uint64_t*>(lg + 8 * n);
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            t[q][n] = unpair(fma2(pair(__uint_as_float(sc[q >> 1][4 * n + 2 * (q & 1)]), __uint_as_float(sc[q >> 1][4 * n + 2 * (q & 1) + 1])),
-                                  k2, g2));
+          for (int q = 0; q < 2; ++q)
+            t[q][n] = unpair(fma2(pair(__uint_as_float(sc[4 * n + 2 * q]), __uint_as_float(sc[4 * n + 2 * q + 1])), k2, g2));
         }
         const bool masked = key + 64 > see_all;                   // the same for the whole tile
         if (masked) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < 2; ++q) {
             const int r = min(first_row + 8 * q, p.rows - 1);
             const int left = (int)min(max(s + r / p.G + 1 - key, (int64_t)0), (int64_t)64) - 2 * tig;   // seen, from this thread's first
 #pragma unroll
@@ -430,19 +436,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           }
         }
         // the bounds move only when a weight would pass 2^8 (and at the first key)
-        float m[4];
+        float m[2];
         bool over = false;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < 2; ++q) {
           m[q] = fmaxf(t[q][0].x, t[q][0].y);
 #pragma unroll
           for (int n = 1; n < 8; ++n) m[q] = max3(m[q], t[q][n].x, t[q][n].y);
           over |= m[q] > M[q] + kSlack;
         }
         if (__any_sync(0xffffffffu, over)) {
-          float f[4];
+          float f[2];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < 2; ++q) {
             m[q] = quad_max(m[q]);
             const float to_M = m[q] > M[q] + kSlack ? m[q] : M[q];
             f[q] = M[q] == neg_inf() ? 0.f : ex2(M[q] - to_M);    // 1 where the bound stays
@@ -454,34 +460,30 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
               ok = __all_sync(0xffffffffu, wait(&sm.pv_half[i], j));
               tc5::fence_after_sync();
             }
-            // lane's row is row q = lane / 8 of the threads with grp = lane % 8
-            const float f0 = __shfl_sync(0xffffffffu, f[0], 4 * (lane & 7)), f1 = __shfl_sync(0xffffffffu, f[1], 4 * (lane & 7));
-            const float f2 = __shfl_sync(0xffffffffu, f[2], 4 * (lane & 7)), f3 = __shfl_sync(0xffffffffu, f[3], 4 * (lane & 7));
-            const float fr = lane < 16 ? (lane < 8 ? f0 : f1) : (lane < 24 ? f2 : f3);
             if (ok) {
 #pragma unroll 1
-              for (int d = 0; d < HD; d += 16) {
+              for (int d = 0; d < HD; d += 32) {
                 uint32_t o[16];
-                tc5::ld16(to + d, o);
+                ld_16x32(to + d, o);
                 tc5::ld_wait();
 #pragma unroll
-                for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * fr);
-                tc5::st16(to + d, o);
+                for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f[x >> 1 & 1]);
+                st_16x32f(to + d, o);
               }
               tc5::st_wait();
             }
           }
         }
-        uint32_t w[2][16];
+        uint32_t w[16];
         if (masked) {                                             // an unseen key has weight 0, whatever its scale holds
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < 2; ++q) {
             const float ref = M[q] == neg_inf() ? 0.f : M[q];
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
               const float e0 = ex2(t[q][n].x - ref), e1 = ex2(t[q][n].y - ref);
               l[q] = add2(l[q], pair(e0 == 0.f ? 0.f : e0 * iv[8 * n], e1 == 0.f ? 0.f : e1 * iv[8 * n + 1]));
-              w[q >> 1][2 * n + (q & 1)] = pack_f16(e0, e1);
+              w[2 * n + q] = pack_f16(e0, e1);
             }
           }
         } else {
@@ -489,70 +491,66 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           for (int n = 0; n < 8; ++n) {
             const uint64_t i2 = *reinterpret_cast<const uint64_t*>(iv + 8 * n);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
+            for (int q = 0; q < 2; ++q) {
               const float2 u = unpair(add2(pair(t[q][n].x, t[q][n].y), pair(-M[q], -M[q])));
               const float e0 = ex2(u.x), e1 = ex2(u.y);
               l[q] = fma2(pair(e0, e1), i2, l[q]);
-              w[q >> 1][2 * n + (q & 1)] = pack_f16(e0, e1);
+              w[2 * n + q] = pack_f16(e0, e1);
             }
           }
         }
-        st_16x32(ts + 32 * h, w[0]);
-        st_16x32(ts + 32 * h + (16u << 16), w[1]);
+        st_16x32(ts + 32 * h, w);
         tc5::st_wait();
         tc5::fence_before_sync();
         tc5::mbar_arrive(&sm.p_full[i][h]);
-      }
-    }
-    // the bound and the sum of weights of the row in this thread's TMEM lane
-    float M_row = 0.f, l_row = 0.f;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float2 x = unpair(l[q]);
-      const float sum = quad_sum(x.x + x.y);
-      const float mm = __shfl_sync(0xffffffffu, M[q], 4 * (lane & 7)), ll = __shfl_sync(0xffffffffu, sum, 4 * (lane & 7));
-      if (lane >> 3 == q) {
-        M_row = mm;
-        l_row = ll;
       }
     }
     ok = ok && wait(&sm.o_full[i], 0);
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       tc5::fence_after_sync();
-      const int64_t at = ((int64_t)head * p.rows + row) * p.splits + split;
-      const float inv = l_row == 0.f ? 0.f : 1.f / l_row;
+      float sum[2], inv[2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const float2 x = unpair(l[q]);
+        sum[q] = quad_sum(x.x + x.y);
+        inv[q] = sum[q] == 0.f ? 0.f : 1.f / sum[q];
+      }
 #pragma unroll 1
       for (int d = 0; d < HD; d += 32) {
-        uint32_t o[32];
-        tc5::ld32(to + d, o);
+        uint32_t o[16];
+        ld_16x32(to + d, o);
         tc5::ld_wait();
-        if (row < p.rows) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int row = first_row + 8 * q;
+          if (row >= p.rows) continue;
           if (p.splits > 1) {
-            uint4* dst = reinterpret_cast<uint4*>(p.part + at * HD + d);
+            float* dst = p.part + (((int64_t)head * p.rows + row) * p.splits + split) * HD + d + 2 * tig;
 #pragma unroll
-            for (int x = 0; x < 8; ++x) dst[x] = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+            for (int n = 0; n < 4; ++n) *reinterpret_cast<uint2*>(dst + 8 * n) = make_uint2(o[4 * n + 2 * q], o[4 * n + 2 * q + 1]);
           } else {
-            uint4* dst = reinterpret_cast<uint4*>(out_row(row) + d);
+            bf16* dst = out_row(row) + d + 2 * tig;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              uint32_t y[4];
-#pragma unroll
-              for (int z = 0; z < 4; ++z)
-                y[z] = pack_bf16(__uint_as_float(o[8 * x + 2 * z]) * inv, __uint_as_float(o[8 * x + 2 * z + 1]) * inv);
-              dst[x] = make_uint4(y[0], y[1], y[2], y[3]);
-            }
+            for (int n = 0; n < 4; ++n)
+              *reinterpret_cast<uint32_t*>(dst + 8 * n) =
+                  pack_bf16(__uint_as_float(o[4 * n + 2 * q]) * inv[q], __uint_as_float(o[4 * n + 2 * q + 1]) * inv[q]);
           }
         }
       }
-      if (p.splits > 1 && row < p.rows) p.part_ml[at] = make_float2(M_row, l_row);
+      if (p.splits > 1 && tig == 0) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          if (first_row + 8 * q < p.rows)
+            p.part_ml[((int64_t)head * p.rows + first_row + 8 * q) * p.splits + split] = make_float2(M[q], sum[q]);
+      }
     }
     }
   }
   tc5::fence_before_sync();
   __syncthreads();
   tc5::fence_after_sync();
-  if (warp == 12) tc5::tmem_dealloc(tb, 512);
+  if (warp == 24) tc5::tmem_dealloc(tb, 512);
   if (tid == 0 && sm.err && a.status) atomicOr(a.status, 2);
 }
 
