@@ -153,19 +153,15 @@ B3_DEV void st_16x32f(uint32_t taddr, const uint32_t (&r)[16]) {
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
 }
 
-// 16 int8 of row r, dimensions 16 c .., as f16 into an operand tile. Lanes of the upper column block store their two
-// 16-byte chunks in the other order, so that the eight lanes of a row keep off each other's banks
-B3_DEV void widen16(unsigned char* tile, int r, int c, const uint4& x) {
+// 16 int8 as f16 to a row's 16-byte chunks 2 c and 2 c + 1 (the address of the first, swizzled; the other one is beside it)
+B3_DEV void widen16(unsigned char* at, const uint4& x) {
   uint4 lo, hi;
   s8x4_to_f16(x.x, lo.x, lo.y);
   s8x4_to_f16(x.y, lo.z, lo.w);
   s8x4_to_f16(x.z, hi.x, hi.y);
   s8x4_to_f16(x.w, hi.z, hi.w);
-  unsigned char* block = tile + (c >> 2) * (kKeys * 128) + r * 128;
-  const int c0 = (2 * c) & 7;
-  const bool swap = c >> 2 & 1;
-  *reinterpret_cast<uint4*>(block + (((swap ? c0 + 1 : c0) ^ (r & 7)) << 4)) = swap ? hi : lo;
-  *reinterpret_cast<uint4*>(block + (((swap ? c0 : c0 + 1) ^ (r & 7)) << 4)) = swap ? lo : hi;
+  *reinterpret_cast<uint4*>(at) = lo;
+  *reinterpret_cast<uint4*>((uintptr_t)at ^ 16) = hi;
 }
 
 template <int HD>
@@ -279,36 +275,49 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
   if (warp >= 16 && warp < 24) {
     // ---- widening: keys, or values and scales
     fewer_regs<kRegsWiden>();
-    constexpr int PPR = HD / 16, NP = kKeys * PPR / 128;          // 16-byte pieces of a row, of a thread
+    // piece i of thread t: 16 bytes t % 4 (+ 4 for odd i at HD 128) of row t / 4 + 32 (i / KC). The eight lanes of a phase
+    // of a store then hold two neighbouring rows' chunks of one column block: all banks differ
+    constexpr int KC = HD / 64, NP = 4 * KC;
     const bool values = warp >= 20;
-    const int t = tid & 127;
+    const int t = tid & 127, r0 = t >> 2;
     const int64_t side = (int64_t)a.B * a.HKV * a.cap;
-    const int8_t* base = a.data + ((int64_t)head * a.cap + (values ? side : 0)) * HD;
-    const float* ks = a.scale + (int64_t)head * a.cap;
+    const int8_t* base = a.data + ((int64_t)head * a.cap + (values ? side : 0) + lo * kKeys) * HD + 16 * (t & 3);
+    const float* ks = a.scale + (int64_t)head * a.cap + lo * kKeys + t;
     const float c_all = a.sm_scale * kLog2e * exp2f((float)e);    // what a score in f16 units is worth, into the key scales
-    const int64_t end = a.cap - 1;                                // rows past the buffer are read as its last one and masked
+    const int end = (int)min(a.cap - 1 - lo * kKeys, (int64_t)0x7fffff00);   // the buffer's last row
     uint64_t *full = values ? sm.v_full : sm.k_full, *empty = values ? sm.v_empty : sm.k_empty;
+    unsigned char* out = (values ? sm.v[0] : sm.k[0]) + r0 * 128 + (((2 * (t & 3)) ^ (r0 & 7)) << 4);
     uint4 x[NP];
     float k_sc = 0.f, v_sc = 0.f;
-    auto fetch = [&](int64_t key) {
+    auto fetch = [&](int j) {
+      if (j * kKeys + kKeys - 1 <= end) {
+        const int8_t* src = base + ((int64_t)j * kKeys + r0) * HD;
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const int idx = i * 128 + t;
-        x[i] = __ldg(reinterpret_cast<const uint4*>(base + min(key + idx / PPR, end) * HD) + idx % PPR);
-      }
-      if (values) {
-        k_sc = __ldg(ks + min(key + t, end));
-        v_sc = __ldg(ks + side + min(key + t, end));
+        for (int i = 0; i < NP; ++i) x[i] = __ldg(reinterpret_cast<const uint4*>(src + 32 * (i / KC) * HD + 64 * (i % KC)));
+        if (values) {
+          k_sc = __ldg(ks + j * kKeys);
+          v_sc = __ldg(ks + side + j * kKeys);
+        }
+      } else {                                                    // rows past the buffer are read as its last one and masked
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const int row = min(j * kKeys + r0 + 32 * (i / KC), end);
+          x[i] = __ldg(reinterpret_cast<const uint4*>(base + (int64_t)row * HD + 64 * (i % KC)));
+        }
+        if (values) {
+          const int row = min(j * kKeys + t, end) - t;
+          k_sc = __ldg(ks + row);
+          v_sc = __ldg(ks + side + row);
+        }
       }
     };
-    int64_t key = lo * kKeys;
-    fetch(key);
+    fetch(0);
     for (int j = 0; j < n_blk; ++j) {
       const int st = j & 1;
       if (j >= 2 && !wait(&empty[st], (j >> 1) - 1)) break;
-      unsigned char* tile = values ? sm.v[st] : sm.k[st];
+      unsigned char* to = out + st * sizeof(sm.k[0]);
 #pragma unroll
-      for (int i = 0; i < NP; ++i) widen16(tile, (i * 128 + t) / PPR, (i * 128 + t) % PPR, x[i]);
+      for (int i = 0; i < NP; ++i) widen16(to + (i % KC) * (kKeys * 128) + 32 * (i / KC) * 128, x[i]);
       if (values) {
         sm.scale[st][0][t] = k_sc * c_all;
         sm.scale[st][1][t] = lg2(v_sc);
@@ -316,8 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       }
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       tc5::mbar_arrive(&full[st]);
-      key += kKeys;
-      if (j + 1 < n_blk) fetch(key);
+      if (j + 1 < n_blk) fetch(j + 1);
     }
   } else if (warp >= 24) {
     // ---- issue. The whole warp runs the loop, so that addresses and descriptors are uniform over it (a lone thread in a
@@ -394,7 +402,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     const int i = warp >> 3, grp = lane >> 2, tig = lane & 3;
     const int first_lane = 32 * (warp & 3) + 16 * (warp >> 2 & 1), first_row = row0 + 128 * i + first_lane + grp;
     const uint32_t lanes = (uint32_t)first_lane << 16, ts = tb + i * 128 + lanes, to = tb + 256 + i * 128 + lanes;
-    const int64_t see_all = s + (row0 + i * 128) / p.G + 1;                       // keys that every row of the tile sees
+    const int seen = (int)min(s + 1 - lo * kKeys, (int64_t)0x7fffff00);           // keys of this split that token 0 sees
+    const int see_all = seen + (row0 + i * 128) / p.G;                            // that every row of the tile sees
     float M[2] = {neg_inf(), neg_inf()};
     uint64_t l[2] = {0, 0};                                       // sums of weights over this thread's keys, in pairs
     bool ok = true;
@@ -412,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         const float* ks = sm.scale[st][0] + 64 * h + 2 * tig;
         const float* lg = sm.scale[st][1] + 64 * h + 2 * tig;
         const float* iv = sm.scale[st][2] + 64 * h + 2 * tig;
-        const int64_t key = (lo + j) * kKeys + 64 * h;
+        const int key = j * kKeys + 64 * h;
         float2 t[2][8];                                           // row q, keys 8 n + 2 tig and the next
         tc5::ld_wait();
 #pragma unroll
@@ -427,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             const int r = min(first_row + 8 * q, p.rows - 1);
-            const int left = (int)min(max(s + r / p.G + 1 - key, (int64_t)0), (int64_t)64) - 2 * tig;   // seen, from this thread's first
+            const int left = seen + r / p.G - key - 2 * tig;   // seen, from this thread's first
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
               if (8 * n >= left) t[q][n].x = neg_inf();
