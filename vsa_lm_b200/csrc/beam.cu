@@ -8,8 +8,9 @@
 //   Chunks with many equal logits (more than the list holds) take K rounds of a block maximum instead.
 // - select_group_kernel: a block per group merges the chunks' sums and lists, scores, ranks and assigns slots.
 // reorder. Bound by HBM: the bytes of every beam that is not its own parent are read from the parent and
-// written. A thread holds its bytes of all parents of the group before it writes any, so the move is in
-// place for any map. Blocks cover the items' bytes flattened, so that many small arrays are one launch.
+// written, in place for any map: where a parent is moved itself, a thread holds its bytes of all parents of the
+// group before it writes any; where none is (the maps that select gives), beams are copied one by one, eight
+// 16-byte loads ahead. Blocks cover the items' bytes flattened, so that many small arrays are one launch.
 #include "../../include/bolt3.h"
 #include "common.cuh"
 #include "trace.h"
@@ -410,41 +411,63 @@ struct MoveParams {
   MoveItem item[kMaxItems];
 };
 
-template <typename V, int KM, int U>
-B3_DEV void move_units(const MoveItem& it, unsigned char* group, uint32_t blk, int K, const int (&par)[KM], unsigned moved) {
-  const int64_t i0 = (int64_t)blk * (kMoveThreads * U) + threadIdx.x;
-  V v[KM][U];
-  int64_t off[U];
+constexpr int kMoveAhead = 8;         // units of a thread
+
+// off: byte offset of a thread's unit u within a beam, -1 past the end
+template <typename V, int KM>
+B3_DEV void move_units(const MoveItem& it, unsigned char* group, uint32_t blk, const int (&par)[KM], unsigned moved, bool chained) {
+  int64_t off[kMoveAhead];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int64_t i = i0 + u * kMoveThreads;
-    const int64_t r = i / it.row_units;
-    off[u] = i < it.units ? r * it.row_stride + it.lo + (i - r * it.row_units) * (int64_t)sizeof(V) : -1;
+  for (int u = 0; u < kMoveAhead; ++u) {
+    const int64_t i = (int64_t)blk * (kMoveThreads * kMoveAhead) + u * kMoveThreads + threadIdx.x;
+    if (it.units == it.row_units) {
+      off[u] = i < it.units ? it.lo + i * (int64_t)sizeof(V) : -1;
+    } else {
+      const int64_t r = i / it.row_units;
+      off[u] = i < it.units ? r * it.row_stride + it.lo + (i - r * it.row_units) * (int64_t)sizeof(V) : -1;
+    }
   }
+  if (chained) {
+#pragma unroll 1
+    for (int u = 0; u < kMoveAhead; ++u) {
+      int64_t at = -1;
 #pragma unroll
-  for (int j = 0; j < KM; ++j)
-    if (moved >> j & 1) {
-      const unsigned char* src = group + par[j] * it.beam_stride;
+      for (int x = 0; x < kMoveAhead; ++x)
+        if (x == u) at = off[x];
+      if (at < 0) continue;
+      V v[KM];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (off[u] >= 0) v[j][u] = *reinterpret_cast<const V*>(src + off[u]);
+      for (int j = 0; j < KM; ++j)
+        if (moved >> j & 1) v[j] = *reinterpret_cast<const V*>(group + par[j] * it.beam_stride + at);
+#pragma unroll
+      for (int j = 0; j < KM; ++j)
+        if (moved >> j & 1) *reinterpret_cast<V*>(group + j * it.beam_stride + at) = v[j];
     }
+    return;
+  }
+#pragma unroll 1
+  for (int j = 0; j < KM; ++j) {
+    if (!(moved >> j & 1)) continue;
+    int from = 0;
 #pragma unroll
-  for (int j = 0; j < KM; ++j)
-    if (moved >> j & 1) {
-      unsigned char* dst = group + j * it.beam_stride;
+    for (int x = 0; x < KM; ++x)
+      if (x == j) from = par[x];
+    const unsigned char* src = group + from * it.beam_stride;
+    unsigned char* dst = group + j * it.beam_stride;
+    V v[kMoveAhead];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (off[u] >= 0) *reinterpret_cast<V*>(dst + off[u]) = v[j][u];
-    }
+    for (int u = 0; u < kMoveAhead; ++u)
+      if (off[u] >= 0) v[u] = *reinterpret_cast<const V*>(src + off[u]);
+#pragma unroll
+    for (int u = 0; u < kMoveAhead; ++u)
+      if (off[u] >= 0) *reinterpret_cast<V*>(dst + off[u]) = v[u];
+  }
 }
 
 template <int KM>
-constexpr int units_per_thread() { return KM <= 4 ? 4 : KM <= 8 ? 2 : 1; }
-
-template <int KM>
 __global__ void __launch_bounds__(kMoveThreads) reorder_kernel(const __grid_constant__ MoveParams p) {
-  constexpr int U = units_per_thread<KM>();
+  grid_dep_launch();
+  grid_dep_wait();
   // the item of this block: the last one that starts at or before it
   int lo = 0, hi = p.n_items - 1;
   while (lo < hi) {
@@ -473,15 +496,17 @@ __global__ void __launch_bounds__(kMoveThreads) reorder_kernel(const __grid_cons
   }
   if (moved == 0) return;
   unsigned char* group = it.base + outer * it.outer_stride + (int64_t)g * p.K * it.beam_stride;
-  if (it.unit == 16) move_units<uint4, KM, U>(it, group, blk, p.K, par, moved);
-  else if (it.unit == 4) move_units<uint32_t, KM, U>(it, group, blk, p.K, par, moved);
-  else move_units<unsigned char, KM, U>(it, group, blk, p.K, par, moved);
+  bool chained = false;                 // whether a parent is moved itself
+#pragma unroll
+  for (int j = 0; j < KM; ++j) chained |= (moved >> par[j] & 1) && (moved >> j & 1);
+  if (it.unit == 16) move_units<uint4, KM>(it, group, blk, par, moved, chained);
+  else if (it.unit == 4) move_units<uint32_t, KM>(it, group, blk, par, moved, chained);
+  else move_units<unsigned char, KM>(it, group, blk, par, moved, chained);
 }
 
 template <int KM>
 int launch_reorder(const MoveParams& p, uint32_t blocks, cudaStream_t s) {
-  reorder_kernel<KM><<<blocks, kMoveThreads, 0, s>>>(p);
-  return cudaGetLastError() == cudaSuccess ? BOLT3_OK : BOLT3_ERR_CUDA;
+  return launch_overlapped(reorder_kernel<KM>, dim3(blocks), dim3(kMoveThreads), 0, s, p) == cudaSuccess ? BOLT3_OK : BOLT3_ERR_CUDA;
 }
 
 }  // namespace
@@ -542,7 +567,7 @@ extern "C" int bolt3_beam_reorder(const bolt3_beam_reorder_args* a, void* stream
     if (m & (it.unit - 1)) return BOLT3_ERR_ALIGN;
   }
   const int km = a->K <= 4 ? 4 : a->K <= 8 ? 8 : 16;
-  const int per_block = kMoveThreads * (km == 4 ? units_per_thread<4>() : km == 8 ? units_per_thread<8>() : units_per_thread<16>());
+  const int per_block = kMoveThreads * kMoveAhead;
   cudaStream_t s = (cudaStream_t)stream;
   MoveParams p;
   p.parent = a->parent;

@@ -6,8 +6,9 @@
 // a key or value row goes to int8 with scale = max(max |x| / 127, 2^-40).
 // Bound by HBM: per token (H + 2 HKV) HD bf16 in, H HD bf16 and 2 HKV (HD + 4) bytes out.
 // A row is HD / 8 lanes of 16 bytes: the norm's sum and the row's maximum are shuffles within these lanes,
-// and the rotation's partner is HD / 16 lanes away. A block is one token's rows (or a share of them), so
-// that a sine and a cosine are taken once per (token, frequency).
+// and the rotation's partner is HD / 16 lanes away. A block takes four tokens (few tokens: a share of one token's
+// rows), so that a sine and a cosine are taken once per (token, frequency), by all threads at once, while the
+// first four rows of every thread are on their way.
 #include "../../include/bolt3.h"
 #include "kv8.cuh"
 #include "trace.h"
@@ -32,97 +33,131 @@ B3_DEV float row_max_nan(float v) {
   return v;
 }
 
-// blockIdx.x = token, blockIdx.y = share of its rows
-template <int HD>
-__global__ void __launch_bounds__(kThreads) kv8_append_kernel(const bolt3_kv8_append_args a, const Length len,
-                                                              int rows_per_block) {
+constexpr int kAhead = 4;                            // rows that a thread has in flight
+
+// blockIdx.x = TPB tokens, blockIdx.y = share of their rows
+template <int HD, int TPB>
+__global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_constant__ bolt3_kv8_append_args a,
+                                                              const __grid_constant__ Length len, int rows_per_block) {
   constexpr int LPR = HD / 8;                        // lanes of a row
   constexpr int RPI = kThreads / LPR;                // rows of one iteration
-  __shared__ float2 trig[HD / 2];
+  __shared__ float2 trig[TPB][HD / 2];
+  __shared__ int64_t s_row[TPB];                     // the token's cache row, or -1
   const int tid = threadIdx.x, part = tid % LPR;
-  const int64_t tok = blockIdx.x;
-  const int b = (int)(tok / a.T), t = (int)(tok % a.T);
-  bool bad = false;
-  const int64_t s = len.rows(b, bad);
-  if (bad && tid == 0 && a.status) atomicOr(a.status, 8);
-  if (a.inv_freq != nullptr) {
-    if (tid < HD / 2 && s >= 0) {
-      const float ang = __fmul_rn((float)(a.pos0 + (s - a.n) + t), a.inv_freq[tid]);
-      float sn, cs;
-      sincosf(ang, &sn, &cs);
-      trig[tid] = make_float2(cs, sn);
-    }
-    __syncthreads();
-  }
+  const int64_t tok0 = (int64_t)blockIdx.x * TPB, tokens = (int64_t)a.B * a.T;
   const int n_rows = a.H + 2 * a.HKV;
-  const int r_end = min(n_rows, ((int)blockIdx.y + 1) * rows_per_block);
-  // whole groups of LPR lanes leave the loop together, but the shuffles name the warp: rows past the end
-  // compute on zeros and store nothing
-  for (int r0 = blockIdx.y * rows_per_block; r0 < r_end; r0 += RPI) {
-    const int r = r0 + tid / LPR;
-    const bool live = r < r_end;
-    const bool is_q = r < a.H, is_k = !is_q && r < a.H + a.HKV;
-    const int h = is_q ? r : is_k ? r - a.H : r - a.H - a.HKV;
-    const bf16* src = reinterpret_cast<const bf16*>(is_q ? a.q : is_k ? a.k : a.v);
-    src += b * (is_q ? a.q_sb : is_k ? a.k_sb : a.v_sb) + t * (is_q ? a.q_st : is_k ? a.k_st : a.v_st) + (int64_t)h * HD;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (live && s >= 0) raw = reinterpret_cast<const uint4*>(src)[part];
-    float x[8];
-    {
-      const float2 p0 = unpack_bf16(raw.x), p1 = unpack_bf16(raw.y), p2 = unpack_bf16(raw.z), p3 = unpack_bf16(raw.w);
-      x[0] = p0.x; x[1] = p0.y; x[2] = p1.x; x[3] = p1.y; x[4] = p2.x; x[5] = p2.y; x[6] = p3.x; x[7] = p3.y;
+  const int first = TPB == 1 ? blockIdx.y * rows_per_block : 0;
+  const int end = TPB == 1 ? min(n_rows, first + rows_per_block) : (int)min((int64_t)TPB, tokens - tok0) * n_rows;
+  grid_dep_launch();
+  grid_dep_wait();
+  if (tid < TPB && tok0 + tid < tokens) {
+    bool bad = false;
+    const int b = (int)((tok0 + tid) / a.T), t = (int)((tok0 + tid) % a.T);
+    const int64_t s = len.rows(b, bad);
+    if (bad && a.status) atomicOr(a.status, 8);
+    s_row[tid] = s < 0 ? -1 : s + t;
+  }
+  __syncthreads();
+  for (int i = tid; a.inv_freq != nullptr && i < TPB * (HD / 2); i += kThreads) {
+    const int k = i / (HD / 2), f = i % (HD / 2);
+    if (tok0 + k < tokens && s_row[k] >= 0) {
+      float sn, cs;
+      sincosf(__fmul_rn((float)(a.pos0 + (s_row[k] - a.n)), a.inv_freq[f]), &sn, &cs);
+      trig[k][f] = make_float2(cs, sn);
     }
-    const float* w = is_q ? a.q_norm_w : is_k ? a.k_norm_w : nullptr;
-    float ss = 0.f;
+  }
+  // whole groups of LPR lanes share a row, but the shuffles name the warp: rows past the end compute on zeros
+  // and store nothing
+  for (int r0 = first; r0 < end; r0 += kAhead * RPI) {
+    uint4 raw[kAhead];
+    int row[kAhead], tk[kAhead];                     // row of its token, token of the block
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-    ss = row_sum<LPR>(ss);
-    if (w != nullptr) {
-      const float inv = rsqrtf(ss * (1.f / HD) + a.eps);
-      const float4 w0 = reinterpret_cast<const float4*>(w)[2 * part], w1 = reinterpret_cast<const float4*>(w)[2 * part + 1];
-      const float ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * ww[i];
+    for (int u = 0; u < kAhead; ++u) {
+      const int item = r0 + u * RPI + tid / LPR;
+      const bool live = item < end;
+      tk[u] = TPB == 1 || !live ? 0 : item / n_rows;
+      const int r = live ? item - tk[u] * n_rows : 0;
+      row[u] = live ? r : -1;
+      const bool is_q = r < a.H, is_k = !is_q && r < a.H + a.HKV;
+      const int h = is_q ? r : is_k ? r - a.H : r - a.H - a.HKV;
+      const int64_t tok = tok0 + tk[u], b = tok / a.T, t = tok - b * a.T;
+      const bf16* src = reinterpret_cast<const bf16*>(is_q ? a.q : is_k ? a.k : a.v);
+      src += b * (is_q ? a.q_sb : is_k ? a.k_sb : a.v_sb) + t * (is_q ? a.q_st : is_k ? a.k_st : a.v_st) + (int64_t)h * HD;
+      raw[u] = make_uint4(0, 0, 0, 0);
+      if (live && s_row[tk[u]] >= 0) raw[u] = __ldg(reinterpret_cast<const uint4*>(src) + part);
     }
-    if (a.inv_freq != nullptr) {
-      const bool second = part >= LPR / 2;           // this lane's values are the pairs' second halves
-      const int f = (second ? part - LPR / 2 : part) * 8;
+    if (r0 == first) __syncthreads();                // the sines and cosines
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float o = __shfl_xor_sync(0xffffffffu, x[i], LPR / 2);
-        const float2 cs = trig[f + i];
-        if (is_q || is_k) x[i] = second ? fmaf(x[i], cs.x, o * cs.y) : fmaf(x[i], cs.x, -o * cs.y);
+    for (int u = 0; u < kAhead; ++u) {
+      if (r0 + u * RPI >= end) break;                // the same for all threads
+      const int r = row[u];
+      const bool is_q = r < a.H, is_k = !is_q && r < a.H + a.HKV;
+      const int64_t at = s_row[tk[u]];
+      float x[8];
+      {
+        const float2 p0 = unpack_bf16(raw[u].x), p1 = unpack_bf16(raw[u].y), p2 = unpack_bf16(raw[u].z), p3 = unpack_bf16(raw[u].w);
+        x[0] = p0.x; x[1] = p0.y; x[2] = p1.x; x[3] = p1.y; x[4] = p2.x; x[5] = p2.y; x[6] = p3.x; x[7] = p3.y;
       }
-    }
-    float m = 0.f;
+      const float* w = is_q ? a.q_norm_w : is_k ? a.k_norm_w : nullptr;
+      float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(x[i]));
-    m = row_max_nan<LPR>(m);
-    if (!live) continue;
-    if (is_q) {
-      uint4 o;
-      o.x = pack_bf16(x[0], x[1]); o.y = pack_bf16(x[2], x[3]); o.z = pack_bf16(x[4], x[5]); o.w = pack_bf16(x[6], x[7]);
-      if (s < 0) o = make_uint4(0, 0, 0, 0);
-      reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.q_out) + (tok * a.H + h) * HD)[part] = o;
-    } else if (s >= 0) {
-      const float sc = max_nan(__fdiv_rn(m, 127.f), kScaleFloor);
-      const int64_t row = (((int64_t)(is_k ? 0 : a.B) + b) * a.HKV + h) * a.cap + s + t;
-      uint32_t lo = 0, hi = 0;
+      for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+      ss = row_sum<LPR>(ss);
+      if (w != nullptr) {
+        const float inv = rsqrtf(ss * (1.f / HD) + a.eps);
+        const float4 w0 = reinterpret_cast<const float4*>(w)[2 * part], w1 = reinterpret_cast<const float4*>(w)[2 * part + 1];
+        const float ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        lo |= ((uint32_t)__float2int_rn(__fdiv_rn(x[i], sc)) & 255u) << (8 * i);
-        hi |= ((uint32_t)__float2int_rn(__fdiv_rn(x[4 + i], sc)) & 255u) << (8 * i);
+        for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * ww[i];
       }
-      reinterpret_cast<uint2*>(a.data + row * HD)[part] = make_uint2(lo, hi);
-      if (part == 0) a.scale[row] = sc;
+      if (a.inv_freq != nullptr) {
+        const bool second = part >= LPR / 2;         // this lane's values are the pairs' second halves
+        const float4* cs = reinterpret_cast<const float4*>(trig[tk[u]] + (second ? part - LPR / 2 : part) * 8);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const float4 z = cs[i / 2];                // cos, sin of this value, cos, sin of the next
+          const float o0 = __shfl_xor_sync(0xffffffffu, x[i], LPR / 2), o1 = __shfl_xor_sync(0xffffffffu, x[i + 1], LPR / 2);
+          if (is_q || is_k) {
+            x[i] = second ? fmaf(x[i], z.x, o0 * z.y) : fmaf(x[i], z.x, -o0 * z.y);
+            x[i + 1] = second ? fmaf(x[i + 1], z.z, o1 * z.w) : fmaf(x[i + 1], z.z, -o1 * z.w);
+          }
+        }
+      }
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(x[i]));
+      m = row_max_nan<LPR>(m);
+      if (r < 0) continue;
+      const int64_t tok = tok0 + tk[u];
+      const int h = is_q ? r : is_k ? r - a.H : r - a.H - a.HKV;
+      if (is_q) {
+        uint4 o;
+        o.x = pack_bf16(x[0], x[1]); o.y = pack_bf16(x[2], x[3]); o.z = pack_bf16(x[4], x[5]); o.w = pack_bf16(x[6], x[7]);
+        if (at < 0) o = make_uint4(0, 0, 0, 0);
+        reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.q_out) + (tok * a.H + h) * HD)[part] = o;
+      } else if (at >= 0) {
+        const float sc = max_nan(__fdiv_rn(m, 127.f), kScaleFloor);
+        const int64_t out = (((int64_t)(is_k ? 0 : a.B) + tok / a.T) * a.HKV + h) * a.cap + at;
+        uint32_t lo = 0, hi = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          lo |= ((uint32_t)__float2int_rn(__fdiv_rn(x[i], sc)) & 255u) << (8 * i);
+          hi |= ((uint32_t)__float2int_rn(__fdiv_rn(x[4 + i], sc)) & 255u) << (8 * i);
+        }
+        reinterpret_cast<uint2*>(a.data + out * HD)[part] = make_uint2(lo, hi);
+        if (part == 0) a.scale[out] = sc;
+      }
     }
   }
 }
 
 // a thread is 16 values of a row: blockIdx.x runs over a (keys / values, sequence, head)'s T * HD / 16 pieces
 template <int HD>
-__global__ void __launch_bounds__(kThreads) kv8_read_kernel(const bolt3_kv8_read_args a, const Length len) {
+__global__ void __launch_bounds__(kThreads) kv8_read_kernel(const __grid_constant__ bolt3_kv8_read_args a,
+                                                            const __grid_constant__ Length len) {
   constexpr int PPR = HD / 16;
+  grid_dep_launch();
+  grid_dep_wait();
   const int b = (int)((blockIdx.y / a.HKV) % a.B);
   bool bad = false;
   const int64_t s = len.rows(b, bad);
@@ -171,16 +206,15 @@ extern "C" int bolt3_kv8_append(const bolt3_kv8_append_args* a, void* stream) {
   if ((al & 15) || (st & 7)) return BOLT3_ERR_ALIGN;
   const Length len{a->lens, a->pos_dev, a->n, a->pos_ref, a->pos_span, a->cap, a->T};
   const int rows = a->H + 2 * a->HKV, rpi = kThreads / (a->HD / 8);
-  // few tokens: a block per iteration's rows, so that a one-token step still fills the machine
-  const int iters = (rows + rpi - 1) / rpi;
+  // few tokens: a block per iteration's rows, so that a one-token step still fills the machine; from two blocks of four
+  // tokens for every SM on, blocks of four
   const int64_t tokens = (int64_t)a->B * a->T;
-  const int shares = tokens >= 1024 ? 1 : iters;
-  const int per = (iters + shares - 1) / shares * rpi;
-  const dim3 grid((unsigned)tokens, (unsigned)((rows + per - 1) / per));
+  const bool few = tokens < 148 * 8;
+  const dim3 grid((unsigned)(few ? tokens : (tokens + 3) / 4), (unsigned)(few ? (rows + rpi - 1) / rpi : 1));
   cudaStream_t s = (cudaStream_t)stream;
-  if (a->HD == 128) kv8_append_kernel<128><<<grid, kThreads, 0, s>>>(*a, len, per);
-  else kv8_append_kernel<64><<<grid, kThreads, 0, s>>>(*a, len, per);
-  return cudaGetLastError() == cudaSuccess ? BOLT3_OK : BOLT3_ERR_CUDA;
+  auto kern = a->HD == 128 ? (few ? kv8_append_kernel<128, 1> : kv8_append_kernel<128, 4>)
+                           : (few ? kv8_append_kernel<64, 1> : kv8_append_kernel<64, 4>);
+  return launch_overlapped(kern, grid, dim3(kThreads), 0, s, *a, len, rpi) == cudaSuccess ? BOLT3_OK : BOLT3_ERR_CUDA;
 }
 
 extern "C" int bolt3_kv8_read(const bolt3_kv8_read_args* a, void* stream) {
@@ -195,7 +229,6 @@ extern "C" int bolt3_kv8_read(const bolt3_kv8_read_args* a, void* stream) {
   const Length len{a->lens, nullptr, a->t0, 0, 0, a->cap, a->T};
   const dim3 grid((unsigned)blocks, (unsigned)(2 * a->B * a->HKV));
   cudaStream_t s = (cudaStream_t)stream;
-  if (a->HD == 128) kv8_read_kernel<128><<<grid, kThreads, 0, s>>>(*a, len);
-  else kv8_read_kernel<64><<<grid, kThreads, 0, s>>>(*a, len);
-  return cudaGetLastError() == cudaSuccess ? BOLT3_OK : BOLT3_ERR_CUDA;
+  return launch_overlapped(a->HD == 128 ? kv8_read_kernel<128> : kv8_read_kernel<64>, grid, dim3(kThreads), 0, s, *a, len) ==
+                 cudaSuccess ? BOLT3_OK : BOLT3_ERR_CUDA;
 }
