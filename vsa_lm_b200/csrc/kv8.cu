@@ -5,8 +5,8 @@
 // (i, i + HD/2) by the angle fp32(position) * inv_freq[i], all in fp32. A query row is rounded to bf16 once;
 // a key or value row goes to int8 with scale = max(max |x| / 127, 2^-40).
 // Bound by HBM: per token (H + 2 HKV) HD bf16 in, H HD bf16 and 2 HKV (HD + 4) bytes out.
-// A row is HD / 8 lanes of 16 bytes: the norm's sum and the row's maximum are shuffles within these lanes,
-// and the rotation's partner is HD / 16 lanes away. A block takes four tokens (few tokens: a share of one token's
+// A row is HD / 8 lanes, a lane holding four neighbouring values of each half: a rotation's pair is in one lane,
+// the norm's sum and the row's maximum are shuffles within the row's lanes. A block takes four tokens (few tokens: a share of one token's
 // rows), so that a sine and a cosine are taken once per (token, frequency), by all threads at once, while the
 // first four rows of every thread are on their way.
 #include "../../include/bolt3.h"
@@ -42,7 +42,8 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_const
   constexpr int LPR = HD / 8;                        // lanes of a row
   constexpr int RPI = kThreads / LPR;                // rows of one iteration
   __shared__ float2 trig[TPB][HD / 2];
-  __shared__ int64_t s_row[TPB];                     // the token's cache row, or -1
+  // of each token: its cache row (-1: idle), its first q, k and v element, and the cache row of its first head's keys
+  __shared__ int64_t s_row[TPB], s_src[TPB][3], s_out[TPB];
   const int tid = threadIdx.x, part = tid % LPR;
   const int64_t tok0 = (int64_t)blockIdx.x * TPB, tokens = (int64_t)a.B * a.T;
   const int n_rows = a.H + 2 * a.HKV;
@@ -56,6 +57,10 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_const
     const int64_t s = len.rows(b, bad);
     if (bad && a.status) atomicOr(a.status, 8);
     s_row[tid] = s < 0 ? -1 : s + t;
+    s_src[tid][0] = b * a.q_sb + t * a.q_st;
+    s_src[tid][1] = b * a.k_sb + t * a.k_st;
+    s_src[tid][2] = b * a.v_sb + t * a.v_st;
+    s_out[tid] = (int64_t)b * a.HKV * a.cap + s + t;
   }
   __syncthreads();
   for (int i = tid; a.inv_freq != nullptr && i < TPB * (HD / 2); i += kThreads) {
@@ -66,25 +71,37 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_const
       trig[k][f] = make_float2(cs, sn);
     }
   }
+  const bool norms = a.q_norm_w != nullptr || a.k_norm_w != nullptr;
   // whole groups of LPR lanes share a row, but the shuffles name the warp: rows past the end compute on zeros
   // and store nothing
+  int item_r = first + tid / LPR, item_t = 0;        // row and token of this thread's next item
+  if (TPB > 1) {
+    item_t = item_r / n_rows;
+    item_r -= item_t * n_rows;
+  }
   for (int r0 = first; r0 < end; r0 += kAhead * RPI) {
-    uint4 raw[kAhead];
-    int row[kAhead], tk[kAhead];                     // row of its token, token of the block
+    uint2 raw[kAhead][2];
+    int row[kAhead], tk[kAhead];                     // row of its token (-1: past the end), token of the block
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int item = r0 + u * RPI + tid / LPR;
-      const bool live = item < end;
-      tk[u] = TPB == 1 || !live ? 0 : item / n_rows;
-      const int r = live ? item - tk[u] * n_rows : 0;
+      const bool live = r0 + u * RPI + tid / LPR < end;
+      tk[u] = live ? item_t : 0;
+      const int r = live ? item_r : 0;
       row[u] = live ? r : -1;
       const bool is_q = r < a.H, is_k = !is_q && r < a.H + a.HKV;
       const int h = is_q ? r : is_k ? r - a.H : r - a.H - a.HKV;
-      const int64_t tok = tok0 + tk[u], b = tok / a.T, t = tok - b * a.T;
-      const bf16* src = reinterpret_cast<const bf16*>(is_q ? a.q : is_k ? a.k : a.v);
-      src += b * (is_q ? a.q_sb : is_k ? a.k_sb : a.v_sb) + t * (is_q ? a.q_st : is_k ? a.k_st : a.v_st) + (int64_t)h * HD;
-      raw[u] = make_uint4(0, 0, 0, 0);
-      if (live && s_row[tk[u]] >= 0) raw[u] = __ldg(reinterpret_cast<const uint4*>(src) + part);
+      const bf16* src = reinterpret_cast<const bf16*>(is_q ? a.q : is_k ? a.k : a.v) + s_src[tk[u]][is_q ? 0 : is_k ? 1 : 2] + h * HD;
+      raw[u][0] = raw[u][1] = make_uint2(0, 0);
+      if (live && s_row[tk[u]] >= 0) {
+        raw[u][0] = __ldg(reinterpret_cast<const uint2*>(src) + part);
+        raw[u][1] = __ldg(reinterpret_cast<const uint2*>(src + HD / 2) + part);
+      }
+      item_r += RPI;
+      if (TPB > 1)
+        while (item_r >= n_rows) {
+          item_r -= n_rows;
+          ++item_t;
+        }
     }
     if (r0 == first) __syncthreads();                // the sines and cosines
 #pragma unroll
@@ -93,58 +110,73 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_const
       const int r = row[u];
       const bool is_q = r < a.H, is_k = !is_q && r < a.H + a.HKV;
       const int64_t at = s_row[tk[u]];
-      float x[8];
+      float x[8];                                    // values 4 part .., HD / 2 + 4 part ..
       {
-        const float2 p0 = unpack_bf16(raw[u].x), p1 = unpack_bf16(raw[u].y), p2 = unpack_bf16(raw[u].z), p3 = unpack_bf16(raw[u].w);
+        const float2 p0 = unpack_bf16(raw[u][0].x), p1 = unpack_bf16(raw[u][0].y), p2 = unpack_bf16(raw[u][1].x), p3 = unpack_bf16(raw[u][1].y);
         x[0] = p0.x; x[1] = p0.y; x[2] = p1.x; x[3] = p1.y; x[4] = p2.x; x[5] = p2.y; x[6] = p3.x; x[7] = p3.y;
       }
-      const float* w = is_q ? a.q_norm_w : is_k ? a.k_norm_w : nullptr;
-      float ss = 0.f;
+      if (norms) {
+        const float* w = is_q ? a.q_norm_w : is_k ? a.k_norm_w : nullptr;
+        float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-      ss = row_sum<LPR>(ss);
-      if (w != nullptr) {
-        const float inv = rsqrtf(ss * (1.f / HD) + a.eps);
-        const float4 w0 = reinterpret_cast<const float4*>(w)[2 * part], w1 = reinterpret_cast<const float4*>(w)[2 * part + 1];
-        const float ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+        ss = row_sum<LPR>(ss);
+        if (w != nullptr) {
+          const float inv = rsqrtf(ss * (1.f / HD) + a.eps);
+          const float4 w0 = reinterpret_cast<const float4*>(w)[part], w1 = reinterpret_cast<const float4*>(w + HD / 2)[part];
+          const float ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * ww[i];
-      }
-      if (a.inv_freq != nullptr) {
-        const bool second = part >= LPR / 2;         // this lane's values are the pairs' second halves
-        const float4* cs = reinterpret_cast<const float4*>(trig[tk[u]] + (second ? part - LPR / 2 : part) * 8);
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          const float4 z = cs[i / 2];                // cos, sin of this value, cos, sin of the next
-          const float o0 = __shfl_xor_sync(0xffffffffu, x[i], LPR / 2), o1 = __shfl_xor_sync(0xffffffffu, x[i + 1], LPR / 2);
-          if (is_q || is_k) {
-            x[i] = second ? fmaf(x[i], z.x, o0 * z.y) : fmaf(x[i], z.x, -o0 * z.y);
-            x[i + 1] = second ? fmaf(x[i + 1], z.z, o1 * z.w) : fmaf(x[i + 1], z.z, -o1 * z.w);
-          }
+          for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * ww[i];
         }
       }
+      if (a.inv_freq != nullptr && (is_q || is_k)) {
+        const float4* cs = reinterpret_cast<const float4*>(trig[tk[u]] + 4 * part);
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const float4 z = cs[i / 2];                // cos, sin of pair i, cos, sin of the next
+          const float a0 = x[i], b0 = x[4 + i], a1 = x[i + 1], b1 = x[5 + i];
+          x[i] = fmaf(a0, z.x, -b0 * z.y);
+          x[4 + i] = fmaf(b0, z.x, a0 * z.y);
+          x[i + 1] = fmaf(a1, z.z, -b1 * z.w);
+          x[5 + i] = fmaf(b1, z.z, a1 * z.w);
+        }
+      }
+      const int h = is_q ? r : is_k ? r - a.H : r - a.H - a.HKV;
+      if (is_q && r >= 0) {
+        uint2 o0 = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+        uint2 o1 = make_uint2(pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+        if (at < 0) o0 = o1 = make_uint2(0, 0);
+        bf16* out = reinterpret_cast<bf16*>(a.q_out) + ((tok0 + tk[u]) * a.H + h) * HD;
+        reinterpret_cast<uint2*>(out)[part] = o0;
+        reinterpret_cast<uint2*>(out + HD / 2)[part] = o1;
+      }
+      const bool stores = r >= 0 && !is_q && at >= 0;
+      if (!__any_sync(0xffffffffu, stores)) continue;
       float m = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(x[i]));
       m = row_max_nan<LPR>(m);
-      if (r < 0) continue;
-      const int64_t tok = tok0 + tk[u];
-      const int h = is_q ? r : is_k ? r - a.H : r - a.H - a.HKV;
-      if (is_q) {
-        uint4 o;
-        o.x = pack_bf16(x[0], x[1]); o.y = pack_bf16(x[2], x[3]); o.z = pack_bf16(x[4], x[5]); o.w = pack_bf16(x[6], x[7]);
-        if (at < 0) o = make_uint4(0, 0, 0, 0);
-        reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.q_out) + (tok * a.H + h) * HD)[part] = o;
-      } else if (at >= 0) {
-        const float sc = max_nan(__fdiv_rn(m, 127.f), kScaleFloor);
-        const int64_t out = (((int64_t)(is_k ? 0 : a.B) + tok / a.T) * a.HKV + h) * a.cap + at;
-        uint32_t lo = 0, hi = 0;
+      const float sc = max_nan(__fdiv_rn(m, 127.f), kScaleFloor);
+      // x / sc to the nearest integer: by the reciprocal, whose product is within 127 * 2^-22 of the quotient; only where
+      // that leaves the rounding open (and for rows that are not finite) by division
+      const float inv = __frcp_rn(sc);
+      uint32_t word[2] = {0, 0};
+      bool open = !(m < 3e38f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          lo |= ((uint32_t)__float2int_rn(__fdiv_rn(x[i], sc)) & 255u) << (8 * i);
-          hi |= ((uint32_t)__float2int_rn(__fdiv_rn(x[4 + i], sc)) & 255u) << (8 * i);
-        }
-        reinterpret_cast<uint2*>(a.data + out * HD)[part] = make_uint2(lo, hi);
+      for (int i = 0; i < 8; ++i) {
+        const float y = x[i] * inv, z = y + 12582912.f;   // 1.5 * 2^23: the integer stands in the low bits
+        open |= fabsf(fabsf(y - (z - 12582912.f)) - 0.5f) < 1e-4f;
+        word[i / 4] |= (__float_as_uint(z) & 255u) << (8 * (i & 3));
+      }
+      if (open) {
+        word[0] = word[1] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) word[i / 4] |= ((uint32_t)__float2int_rn(__fdiv_rn(x[i], sc)) & 255u) << (8 * (i & 3));
+      }
+      if (stores) {
+        const int64_t out = s_out[tk[u]] + ((int64_t)(is_k ? 0 : a.B) * a.HKV + h) * a.cap;
+        reinterpret_cast<uint32_t*>(a.data + out * HD)[part] = word[0];
+        reinterpret_cast<uint32_t*>(a.data + out * HD + HD / 2)[part] = word[1];
         if (part == 0) a.scale[out] = sc;
       }
     }
