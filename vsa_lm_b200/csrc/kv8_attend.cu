@@ -646,26 +646,29 @@ __global__ void __launch_bounds__(32 * kWarps<NT>) kv8_stream_kernel(const __gri
   }
 }
 
-// one block per (head, query row): the runs' partial sums joined, a warp to a run's row at a time
+// The runs' partial sums of a (head, query row) joined: by one warp where a head has few of them (ROWS = 4 rows a block),
+// else by all warps of a block (ROWS = 1)
 constexpr int kMaxJoinWarps = 16;
 
-template <int HD, int NC>
-__global__ void __launch_bounds__(32 * kMaxJoinWarps) kv8_join_kernel(const __grid_constant__ Params p) {
+template <int HD, int NC, int ROWS>
+__global__ void __launch_bounds__(ROWS == 1 ? 32 * kMaxJoinWarps : 32 * ROWS) kv8_join_kernel(const __grid_constant__ Params p) {
   constexpr int EPL = HD / 32;                                  // dimensions of a lane
-  __shared__ float s_acc[kMaxJoinWarps][HD], s_m[kMaxJoinWarps], s_l[kMaxJoinWarps];
+  __shared__ float s_acc[ROWS == 1 ? kMaxJoinWarps : 1][HD], s_m[kMaxJoinWarps], s_l[kMaxJoinWarps];
   const bolt3_kv8_attend_args& a = p.a;
-  const int head = blockIdx.x, b = head / a.HKV, kvh = head % a.HKV, row = blockIdx.y;
-  const int d = threadIdx.x, warp = d >> 5, lane = d & 31, n_warps = blockDim.x >> 5;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_warps = ROWS == 1 ? blockDim.x >> 5 : 1;
+  const int head = blockIdx.x, b = head / a.HKV, kvh = head % a.HKV, row = blockIdx.y * ROWS + (ROWS == 1 ? 0 : warp);
   const int tile = row / NC, r = row % NC;
   grid_dep_launch();
   grid_dep_wait();
+  if (row >= p.rows) return;
   bool bad = false;
   const bool idle = p.len.rows(b, bad) < 0;
   const int2 span = p.span[(int64_t)tile * gridDim.x + head];
   bf16* y = out_row<HD>(p, b, kvh, row);
   const int r0 = span.x >> 1;
   if (idle || (span.x >= 0 && (span.x >= 2 * p.n_runs || span.y < r0 || span.y >= p.n_runs))) {   // (the latter: a run gave up)
-    for (int i = d; i < HD; i += blockDim.x) y[i] = __float2bfloat16_rn(0.f);
+    if (warp == 0 || ROWS > 1)
+      for (int i = lane; i < HD; i += 32) y[i] = __float2bfloat16_rn(0.f);
     return;
   }
   if (span.x < 0) return;                                       // the run wrote the output itself
@@ -673,7 +676,7 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) kv8_join_kernel(const __gr
   const int n = span.y - r0 + 1;
   float m = neg_inf(), l = 0.f, acc[EPL] = {};
   constexpr int kBatch = 4;
-  for (int i0 = warp; i0 < n; i0 += kBatch * n_warps) {
+  for (int i0 = ROWS == 1 ? warp : 0; i0 < n; i0 += kBatch * n_warps) {
     float2 ml[kBatch];
     float x[kBatch][EPL];
 #pragma unroll
@@ -694,24 +697,29 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) kv8_join_kernel(const __gr
       for (int e = 0; e < EPL; ++e) acc[e] = fmaf(acc[e], f0, x[j][e] * f1);
     }
   }
+  if constexpr (ROWS > 1) {
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) s_acc[warp][32 * e + lane] = acc[e];
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
-  }
-  __syncthreads();
-  for (int i = d; i < HD; i += blockDim.x) {
-    m = neg_inf();
-    for (int w = 0; w < n_warps; ++w) m = fmaxf(m, s_m[w]);
-    float sum = 0.f;
-    l = 0.f;
-    for (int w = 0; w < n_warps; ++w) {
-      const float g = s_m[w] == neg_inf() ? 0.f : exp2f(s_m[w] - m);
-      sum = fmaf(s_acc[w][i], g, sum);
-      l = fmaf(s_l[w], g, l);
+    for (int e = 0; e < EPL; ++e) y[32 * e + lane] = __float2bfloat16_rn(l == 0.f ? 0.f : acc[e] / l);
+  } else {
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) s_acc[warp][32 * e + lane] = acc[e];
+    if (lane == 0) {
+      s_m[warp] = m;
+      s_l[warp] = l;
     }
-    y[i] = __float2bfloat16_rn(l == 0.f ? 0.f : sum / l);
+    __syncthreads();
+    for (int i = threadIdx.x; i < HD; i += blockDim.x) {
+      m = neg_inf();
+      for (int w = 0; w < n_warps; ++w) m = fmaxf(m, s_m[w]);
+      float sum = 0.f;
+      l = 0.f;
+      for (int w = 0; w < n_warps; ++w) {
+        const float g = s_m[w] == neg_inf() ? 0.f : exp2f(s_m[w] - m);
+        sum = fmaf(s_acc[w][i], g, sum);
+        l = fmaf(s_l[w], g, l);
+      }
+      y[i] = __float2bfloat16_rn(l == 0.f ? 0.f : sum / l);
+    }
   }
 }
 
@@ -728,10 +736,12 @@ Plan plan_of(int B, int T, int H, int HKV, int HD, int64_t n) {
   pl.tiles = (int)((rows + 8 * pl.nt - 1) / (8 * pl.nt));
   const int64_t warps = pl.nt == 1 ? kWarps<1> : kWarps<2>;
   const int64_t per_head = (n + T + kBlock - 1) / kBlock, blocks = heads * per_head;
-  // a CTA per head where that fills the machine, or gives each warp two blocks at most; else every warp a run of two
-  // blocks or more
+  // A CTA per head where all are on the machine at once and a warp gets five blocks at most (32 query heads on 8, HD 128:
+  // one sequence of 1000 tokens 8.9 us against 10.9 in runs, of 2000 12.8 against 12.3, of 4000 20 against 11.8; 64
+  // sequences of 200 tokens, 512 heads, 22.5 against 17.1). Else every warp a run, of two blocks or more
   int64_t runs = 0;
-  if (heads * pl.tiles < 148 * 4 && per_head > 2 * warps) runs = blocks / 2 < 148 * warps ? blocks / 2 : 148 * warps;
+  if (heads * pl.tiles > 148 || per_head > 5 * warps) runs = blocks / 2 < 148 * warps ? blocks / 2 : 148 * warps;
+  if (runs < 1 && heads * pl.tiles > 148) runs = 1;
   pl.runs = (int)runs;
   pl.bytes = 0;
   if (runs > 0)
@@ -752,10 +762,12 @@ int launch_stream(Params p, const Plan& pl, cudaStream_t s) {
   const unsigned heads = (unsigned)(p.a.B * p.a.HKV), ctas = pl.runs == 0 ? heads : (unsigned)((pl.runs + kWarps<NT> - 1) / kWarps<NT>);
   if (launch_overlapped(kv8_stream_kernel<HD, NT>, dim3(ctas, (unsigned)pl.tiles), dim3(32 * kWarps<NT>), smem, s, p) != cudaSuccess)
     return BOLT3_ERR_CUDA;
-  // enough warps for the partial sums that a head has on average
-  const int per_head = pl.runs / (int)heads + 2, join_warps = per_head >= 32 ? 16 : per_head >= 8 ? 8 : 4;
-  if (pl.runs && launch_overlapped(kv8_join_kernel<HD, NC>, dim3(heads, (unsigned)p.rows), dim3(32 * join_warps), 0, s, p) != cudaSuccess)
-    return BOLT3_ERR_CUDA;
+  if (pl.runs == 0) return BOLT3_OK;
+  const int per_head = pl.runs / (int)heads + 2;                // partial sums that a head has on average, about
+  const cudaError_t e = per_head <= 8
+      ? launch_overlapped(kv8_join_kernel<HD, NC, 4>, dim3(heads, (unsigned)((p.rows + 3) / 4)), dim3(128), 0, s, p)
+      : launch_overlapped(kv8_join_kernel<HD, NC, 1>, dim3(heads, (unsigned)p.rows), dim3(per_head >= 32 ? 512 : 256), 0, s, p);
+  if (e != cudaSuccess) return BOLT3_ERR_CUDA;
   return BOLT3_OK;
 }
 
@@ -785,7 +797,8 @@ bool encode_cache(CUtensorMap* m, const bolt3_kv8_attend_args* a) {
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// whether a call's rows go to the kernel for many rows
+// Whether a call's rows go to the kernel for many rows, which works on tiles of 128 (64 sequences of 2304 tokens, 32 heads
+// on 8, HD 128: 32 rows of a head 168 us here against 239 there, 64 rows 333 against 239)
 bool many_rows(int T, int H, int HKV) { return (int64_t)T * (H / HKV) > 32; }
 
 bool shape_ok(int B, int T, int H, int HKV, int HD) {
