@@ -91,6 +91,27 @@ def test_anchor_attention_over_int8_cache(qk_norm, HD, HKV):
 
 
 @pytest.mark.gpu
+def test_int8_cache_reports_its_kernels_errors():
+    """A device step position past the span of its launches is found by Bolt3Decoder.check_status, once."""
+    cfg = dict(dim=256, num_heads=8, num_kv_heads=2, head_dim=64, rope_theta=1e4, eps=1e-6, qk_norm=False)
+    ly = SoftmaxAttn(cfg).to(device="cuda", dtype=torch.bfloat16).eval()
+    cache = AnchorKV8(1, 2, 200, 64, "cuda")
+    pos = K.DevicePosition("cuda")
+    pos.ref, pos.span = 0, 4
+    h = torch.randn(1, 1, 256, device="cuda").bfloat16()
+    with torch.no_grad():
+        pos.set(3)
+        cache.attention(ly, h, 0, pos)
+        Bolt3Decoder.check_status([cache])
+        pos.set(4)
+        y = cache.attention(ly, h, 0, pos)
+        assert bool((y == 0).all())
+        with pytest.raises(RuntimeError, match="out of range|outside the range"):
+            Bolt3Decoder.check_status([cache])
+        Bolt3Decoder.check_status([cache])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shape", ["small_lm", "tiny_lm"])
 def test_int8_step_graph_equals_eager_steps(shape):
     mcfg, model = _model(shape)

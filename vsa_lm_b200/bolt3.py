@@ -595,6 +595,8 @@ class Bolt3Decoder:
         for st in kv_caches:
             if isinstance(st, Bolt3LayerState):
                 st.status.check(block)
+            elif isinstance(st, AnchorKV8):
+                st.check_status(block)
 
     # ---- decode state in the reference's format (bolt3.py:302-319 creates it, :343-425 fills it):
     # per Bolt-3 layer a dict with the bank (ak/av [b*HKV, S, HD], mass/util/pm fp32 [b*HKV, S], act
@@ -1241,6 +1243,17 @@ class AnchorKV8:
         self.data = torch.empty(2, B, HKV, cap, HD, device=dev, dtype=torch.int8)
         self.scale = torch.empty(2, B, HKV, cap, device=dev, dtype=torch.float32)
         self.n = 0
+        # status word of this cache's kernels (an expired wait, a device position out of range)
+        self.status = K.DeviceStatus(dev) if self.data.is_cuda else None
+
+    def check_status(self, block: bool = True) -> None:
+        """Raise RuntimeError if a kernel of an earlier step reported an error (block=False: only if the copy
+        asked for by the last such call has arrived with one)."""
+        if self.status is not None:
+            self.status.check(block)
+            self.status.arm("8-bit anchor cache")
+            if block:
+                self.status.check(True)
 
     @property
     def capacity(self) -> int:
@@ -1283,7 +1296,7 @@ class AnchorKV8:
         """A copy whose sequences are this cache's, each `times` times in a row."""
         new = AnchorKV8.__new__(AnchorKV8)
         new.data, new.scale = (t.repeat_interleave(times, dim=1) for t in (self.data, self.scale))
-        new.n = self.n
+        new.n, new.status = self.n, K.DeviceStatus(self.data.device) if self.data.is_cuda else None
         return new
 
     def attention(self, ly, h: torch.Tensor, pos_start: int, dev_pos: "K.DevicePosition | None" = None) -> torch.Tensor:
@@ -1299,8 +1312,9 @@ class AnchorKV8:
                          inv_freq=_fp32_inv_freq(ly.rope, h.device),
                          q_norm=_fp32_weight(ly.q_norm, h.device) if norm else None,
                          k_norm=_fp32_weight(ly.k_norm, h.device) if norm else None,
-                         eps=ly.q_norm.eps if norm else 0.0, dev_pos=dev_pos)
-        y = K.kv8_attend(q=q, data=self.data, scale=self.scale, n=self.n, sm_scale=ly.HD ** -0.5, dev_pos=dev_pos)
+                         eps=ly.q_norm.eps if norm else 0.0, status=self.status, dev_pos=dev_pos)
+        y = K.kv8_attend(q=q, data=self.data, scale=self.scale, n=self.n, sm_scale=ly.HD ** -0.5, status=self.status,
+                         dev_pos=dev_pos)
         if dev_pos is None:
             self.n += t
         return y
