@@ -285,6 +285,35 @@ def test_attend_nan_stays_in_its_sequence(T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 4, 100])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), float("-inf")])
+def test_attend_unbounded_query_spoils_its_own_row(T, what):
+    B, H, HKV, HD, n = 2, 4, 2, 64, 50
+    data, scale = random_cache(21, B, HKV, n + T, HD)
+    q = randn(22, B, T, H, HD, dtype=torch.bfloat16)
+    clean = K.kv8_attend(q=q.cuda(), data=data.cuda(), scale=scale.cuda(), n=n).cpu().view(B, T, H, HD)
+    q[1, T // 2, 3, 7] = what
+    y = K.kv8_attend(q=q.cuda(), data=data.cuda(), scale=scale.cuda(), n=n).cpu().view(B, T, H, HD)
+    assert bool(y[1, T // 2, 3].isnan().all())
+    keep = torch.ones(B, T, H, dtype=torch.bool)
+    keep[1, T // 2, 3] = False
+    check = y.clone()
+    check[1, T // 2, 3] = 0
+    assert bool(check.isfinite().all()) and torch.equal(y[keep], clean[keep])
+
+
+@pytest.mark.gpu
+def test_attend_a_long_prompt_at_once():
+    """More rows than a grid's second dimension holds: 20000 tokens of 4 heads on one KV head, checked at a few rows."""
+    H, HD, T = 4, 64, 20000
+    data, scale = random_cache(23, 1, 1, T, HD)
+    q = randn(24, 1, T, H, HD, dtype=torch.bfloat16)
+    y = K.kv8_attend(q=q.cuda(), data=data.cuda(), scale=scale.cuda(), n=0).cpu()
+    for t in (0, 1, 127, 5000, T - 1):
+        check_attend(q[:, t:t + 1], data, scale, t, None, HD ** -0.5, y[:, t:t + 1])
+
+
+@pytest.mark.gpu
 def test_attend_rows_past_32_bit_offsets():
     """Rows whose byte offset in the cache passes 2^31 and whose element offset of the values 2^32."""
     HKV, HD, cap = 8, 128, 2_200_000
@@ -437,8 +466,10 @@ def test_entry_points_reject_bad_arguments_without_a_gpu():
         return lib.bolt3_kv8_read(ctypes.byref(a), None)
 
     assert read(out=0) == 1 and read(T=0) == 2 and read(t0=7) == 4 and read(T=9) == 4 and read(out=fake + 2) == 3
-    assert read(B=40000) == 2
+    assert read(B=1 << 30, HKV=4) == 2
     assert lib.bolt3_kv8_attend_workspace(1, 1, 4, 3, 64, 100) == 0
+    assert lib.bolt3_kv8_attend_workspace(1, 1, 4, 2, 64, 1 << 50) == 0 and attend(lens=fake, n=9) == 4
+    assert attend(T=1 << 23, cap=1 << 24, n=0, H=8) == 2
 
 
 def test_cpu_tensors_are_refused():

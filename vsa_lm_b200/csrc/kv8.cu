@@ -183,24 +183,26 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_const
   }
 }
 
-// a thread is 16 values of a row: blockIdx.x runs over a (keys / values, sequence, head)'s T * HD / 16 pieces
+// a thread is 16 values of a row; `per` blocks for the T * HD / 16 pieces of a (keys / values, sequence, head)
 template <int HD>
 __global__ void __launch_bounds__(kThreads) kv8_read_kernel(const __grid_constant__ bolt3_kv8_read_args a,
-                                                            const __grid_constant__ Length len) {
+                                                            const __grid_constant__ Length len, unsigned per) {
   constexpr int PPR = HD / 16;
+  const int64_t slice = blockIdx.x / per;
+  const unsigned blk = blockIdx.x - (unsigned)slice * per;
   grid_dep_launch();
   grid_dep_wait();
-  const int b = (int)((blockIdx.y / a.HKV) % a.B);
+  const int b = (int)((slice / a.HKV) % a.B);
   bool bad = false;
   const int64_t s = len.rows(b, bad);
-  if (bad && blockIdx.x == 0 && threadIdx.x == 0 && a.status) atomicOr(a.status, 8);
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (bad && blk == 0 && threadIdx.x == 0 && a.status) atomicOr(a.status, 8);
+  const int64_t i = (int64_t)blk * kThreads + threadIdx.x;
   if (i >= a.T * PPR) return;
   const int64_t t = i / PPR;
   const int p = (int)(i % PPR);
   uint4 o0 = make_uint4(0, 0, 0, 0), o1 = o0;
   if (s >= 0) {
-    const int64_t row = (int64_t)blockIdx.y * a.cap + s + t;
+    const int64_t row = slice * a.cap + s + t;
     const uint4 raw = reinterpret_cast<const uint4*>(a.data + row * HD)[p];
     const float sc = a.scale[row];
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -214,7 +216,7 @@ __global__ void __launch_bounds__(kThreads) kv8_read_kernel(const __grid_constan
     o0 = make_uint4(o[0], o[1], o[2], o[3]);
     o1 = make_uint4(o[4], o[5], o[6], o[7]);
   }
-  uint4* dst = reinterpret_cast<uint4*>(a.out) + ((int64_t)blockIdx.y * a.T * PPR + i) * 2;
+  uint4* dst = reinterpret_cast<uint4*>(a.out) + (slice * a.T * PPR + i) * 2;
   dst[0] = o0;
   dst[1] = o1;
 }
@@ -253,14 +255,14 @@ extern "C" int bolt3_kv8_read(const bolt3_kv8_read_args* a, void* stream) {
   const b3::TraceRange trace_range("bolt3_kv8_read");
   if (!a || !a->data || !a->scale || !a->out) return BOLT3_ERR_ARG;
   if (a->B <= 0 || a->HKV <= 0 || a->T <= 0 || (a->HD != 64 && a->HD != 128)) return BOLT3_ERR_SHAPE;
-  if ((int64_t)a->B * a->HKV > 32767) return BOLT3_ERR_SHAPE;   // 2 B HKV blocks in grid.y
   if (a->t0 < 0 || a->T > a->cap || (a->lens == nullptr && a->t0 > a->cap - a->T)) return BOLT3_ERR_CAPACITY;
   if (((uintptr_t)a->data | (uintptr_t)a->out | (uintptr_t)a->scale) & 15) return BOLT3_ERR_ALIGN;
-  const int64_t blocks = (a->T * (a->HD / 16) + kThreads - 1) / kThreads;
-  if (blocks > 0x7fffffff) return BOLT3_ERR_SHAPE;
+  const int64_t slices = 2 * (int64_t)a->B * a->HKV, per = (a->T * (a->HD / 16) + kThreads - 1) / kThreads;
+  if (per > 0x7fffffff / slices) return BOLT3_ERR_SHAPE;
   const Length len{a->lens, nullptr, a->t0, 0, 0, a->cap, a->T};
-  const dim3 grid((unsigned)blocks, (unsigned)(2 * a->B * a->HKV));
+  const dim3 grid((unsigned)(slices * per));
   cudaStream_t s = (cudaStream_t)stream;
-  return launch_overlapped(a->HD == 128 ? kv8_read_kernel<128> : kv8_read_kernel<64>, grid, dim3(kThreads), 0, s, *a, len) ==
+  return launch_overlapped(a->HD == 128 ? kv8_read_kernel<128> : kv8_read_kernel<64>, grid, dim3(kThreads), 0, s, *a, len,
+                           (unsigned)per) ==
                  cudaSuccess ? BOLT3_OK : BOLT3_ERR_CUDA;
 }

@@ -803,13 +803,13 @@ bool many_rows(int T, int H, int HKV) { return (int64_t)T * (H / HKV) > 32; }
 
 bool shape_ok(int B, int T, int H, int HKV, int HD) {
   return B > 0 && T > 0 && HKV > 0 && H > 0 && H % HKV == 0 && H / HKV <= 16 && (HD == 64 || HD == 128) &&
-         T <= 65535 / (H / HKV) && (int64_t)B * HKV <= 0x3fffffff;
+         T <= (1 << 24) / (H / HKV) && (int64_t)B * HKV <= 0x3fffffff;
 }
 
 }  // namespace
 
 extern "C" size_t bolt3_kv8_attend_workspace(int B, int T, int H, int HKV, int HD, int64_t n) {
-  if (!shape_ok(B, T, H, HKV, HD) || n < 0) return 0;
+  if (!shape_ok(B, T, H, HKV, HD) || n < 0 || n > 0x7fffffff) return 0;
   return many_rows(T, H, HKV) ? kv8_prompt_workspace(B, T, H, HKV, HD, n) : plan_of(B, T, H, HKV, HD, n).bytes;
 }
 
@@ -820,7 +820,7 @@ extern "C" int bolt3_kv8_attend(const bolt3_kv8_attend_args* a, void* stream) {
   if (a->pos_dev != nullptr && a->pos_span < 1) return BOLT3_ERR_ARG;
   if (!shape_ok(a->B, a->T, a->H, a->HKV, a->HD)) return BOLT3_ERR_SHAPE;
   const int64_t dmax = a->pos_dev != nullptr ? a->pos_span - 1 : 0;
-  if (a->n < 0 || a->cap < a->T || a->cap > 0x7fffffff || (a->lens == nullptr && a->n > a->cap - a->T - dmax)) return BOLT3_ERR_CAPACITY;
+  if (a->n < 0 || a->n > a->cap || a->cap < a->T || a->cap > 0x7fffffff || (a->lens == nullptr && a->n > a->cap - a->T - dmax)) return BOLT3_ERR_CAPACITY;
   const uintptr_t al = (uintptr_t)a->q | (uintptr_t)a->data | (uintptr_t)a->scale | (uintptr_t)a->y | (uintptr_t)a->workspace;
   if ((al & 15) || ((a->q_sb | a->q_st) & 7)) return BOLT3_ERR_ALIGN;
   const Length len{a->lens, a->pos_dev, a->n, a->pos_ref, a->pos_span, a->cap, a->T};
