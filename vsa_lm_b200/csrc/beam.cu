@@ -3,7 +3,8 @@
 // select. With lse_k = log sum_v e^x_kv, continuation (k, v) scores s_k + (x_kv - lse_k); the K best of a
 // group's K * V survive. Bound by HBM: the logits are read once. Within a beam the order is the logits',
 // so the pass that sums the exponentials also finds each chunk's K best logits:
-// - select_chunk_kernel: a block holds a chunk of one row in registers (8192 fp32 or 16384 bf16 logits). Maximum and sum of exponentials, then a threshold: the K-th largest of 16 half-warp maxima is no larger than the chunk's
+// - select_chunk_kernel: a block holds a chunk of 8192 logits of one row in registers. Maximum and
+//   sum of exponentials, then a threshold: the K-th largest of its 16 quarter-warps' maxima is no larger than the chunk's
 //   K-th largest logit, so the few logits at or above it contain the K best; they are ranked by counting.
 //   Chunks with many equal logits (more than the list holds) take K rounds of a block maximum instead.
 // - select_group_kernel: a block per group merges the chunks' sums and lists, scores, ranks and assigns slots.
@@ -24,15 +25,16 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // ------------------------------------------------------------------------------------------- select
 
-constexpr int kSelThreads = 256;
-constexpr int kMinChunk = 8192;                       // logits of a block: fp32; bf16 twice that
+// Blocks of four warps, ten on an SM (blocks of eight with chunks of 16384, five on an SM, take the same time). At 256 rows
+// of 151936 bf16 logits, a fifth of them finished, the kernel is busy for 14.5 us: exponentials 7.3, instructions 7.7, DRAM
+// 9.5 of them
+constexpr int kSelThreads = 128;
+constexpr int kPerThread = 64;
+constexpr int kChunk = kSelThreads * kPerThread;      // logits of a block
 template <bool FP32>
-constexpr int kPerThread = FP32 ? 32 : 64;
-template <bool FP32>
-constexpr int kChunk = kSelThreads * kPerThread<FP32>;
-constexpr int kSelBlocks = 5;                         // of an SM
+constexpr int kSelBlocks = FP32 ? 5 : 10;             // of an SM
 constexpr int kListCap = 256;                         // candidates at or above the threshold
-constexpr int64_t kMaxV = 64 * kMinChunk;             // (with a slip a row may have 65 chunks)
+constexpr int64_t kMaxV = 64 * kChunk;             // (with a slip a row may have 65 chunks)
 
 // the float of an fkey
 B3_DEV float unkey(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
@@ -93,7 +95,7 @@ B3_DEV uint32_t max_bf16x2(uint32_t a, uint32_t b) {
 template <bool FP32>
 struct Logits {
   static constexpr int EPL = FP32 ? 4 : 8;            // logits of a 16-byte load
-  static constexpr int NW = 32;
+  static constexpr int NW = FP32 ? 64 : 32;
   static constexpr uint32_t kNone = FP32 ? 0xff800000u : 0xff80ff80u;   // -infinity in every place
   uint32_t w[NW];
   B3_DEV float largest() const {                      // NaNs left out
@@ -114,12 +116,12 @@ struct Logits {
     if constexpr (FP32) return __uint_as_float(w[i]);
     else return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
   }
-  // of words 16 h .. 16 h + 15 (bf16) or all (fp32): a bit for every logit at or above t, a bf16 value where they are
+  // of logits 32 h .. 32 h + 31: a bit for every one at or above t, a bf16 value where they are
   B3_DEV uint32_t at_least(float t, int h) const {
     uint32_t mask = 0;
     if constexpr (FP32) {
 #pragma unroll
-      for (int i = 0; i < NW; ++i) mask |= __uint_as_float(w[i]) >= t ? 1u << i : 0u;
+      for (int i = 0; i < 32; ++i) mask |= __uint_as_float(w[32 * h + i]) >= t ? 1u << i : 0u;
     } else {
       const __nv_bfloat162 tt = __float2bfloat162_rn(t);
 #pragma unroll
@@ -128,14 +130,14 @@ struct Logits {
     }
     return mask;
   }
-  static B3_DEV int of_bit(int bit, int h) { return FP32 ? bit : 32 * h + (bit & 15) * 2 + (bit >> 4); }
+  static B3_DEV int of_bit(int bit, int h) { return 32 * h + (FP32 ? bit : (bit & 15) * 2 + (bit >> 4)); }
 };
 
 template <bool FP32>
-__global__ void __launch_bounds__(kSelThreads, kSelBlocks) select_chunk_kernel(const __grid_constant__ SelParams p) {
+__global__ void __launch_bounds__(kSelThreads, kSelBlocks<FP32>) select_chunk_kernel(const __grid_constant__ SelParams p) {
   using L = Logits<FP32>;
-  constexpr int EPL = L::EPL, kBytes = FP32 ? 4 : 2, kPer = kPerThread<FP32>;
-  __shared__ float s_max[16], s_sum[8];
+  constexpr int EPL = L::EPL, kBytes = FP32 ? 4 : 2, kPer = kPerThread;
+  __shared__ float s_max[16], s_sum[4];
   __shared__ int s_count;
   __shared__ Cand s_list[kListCap];
   const bolt3_beam_select_args& a = p.a;
@@ -144,9 +146,9 @@ __global__ void __launch_bounds__(kSelThreads, kSelBlocks) select_chunk_kernel(c
   // Chunks are cut at 16-byte boundaries whatever the row's alignment: logit e of the chunk is logit lo + e of the row,
   // lo < 0 where the row begins within the chunk's first 16 bytes
   const char* row = reinterpret_cast<const char*>(a.logits) + r * a.row_stride * kBytes;
-  const int lo = (int)blockIdx.y * kChunk<FP32> - (int)(reinterpret_cast<uintptr_t>(row) & 15) / kBytes;
+  const int lo = (int)blockIdx.y * kChunk - (int)(reinterpret_cast<uintptr_t>(row) & 15) / kBytes;
   row += (int64_t)lo * kBytes;
-  const int from = max(0, -lo), n = min(kChunk<FP32>, (int)a.V - lo);   // logits of the chunk: [from, n)
+  const int from = max(0, -lo), n = min(kChunk, (int)a.V - lo);   // logits of the chunk: [from, n)
   grid_dep_launch();
   grid_dep_wait();
   if (!row_live(a, r)) return;
@@ -198,16 +200,17 @@ __global__ void __launch_bounds__(kSelThreads, kSelBlocks) select_chunk_kernel(c
         if (place(i) >= from && place(i) < n) sum += ex2(fmaf(fmaxf(value(place(i)), neg_inf()), kLog2e, -off));
     }
   }
-  float g = m;                                        // maximum of the half-warp, of the warp
+  float g = m;                                        // maximum of the quarter-warp, of the warp
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-  if ((lane & 15) == 0) s_max[warp * 2 + (lane >> 4)] = g;
+  for (int o = 4; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+  if ((lane & 7) == 0) s_max[warp * 4 + (lane >> 3)] = g;
+  g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 8));
   g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 16));
   sum = warp_sum(m > neg_inf() ? sum * ex2((m - g) * kLog2e) : 0.f);
   if (lane == 0) s_sum[warp] = sum;
   if (tid == 0) s_count = 0;
   __syncthreads();
-  // tau: the K-th largest of the 16 half-warps' maxima (one of them leaves per round)
+  // tau: the K-th largest of the 16 quarter-warps' maxima (one of them leaves per round)
   uint32_t key = lane < 16 ? fkey(s_max[lane]) : 0;
   uint32_t best = __reduce_max_sync(0xffffffffu, key);
   const float top = unkey(best);
@@ -220,7 +223,7 @@ __global__ void __launch_bounds__(kSelThreads, kSelBlocks) select_chunk_kernel(c
   if (m >= tau && m > neg_inf()) {
     // tau is one of the logits, or -infinity: then any logit above that counts
     const float t = tau > neg_inf() ? tau : FP32 ? -3.4028235e38f : -3.3895314e38f;
-    uint32_t mask[2] = {l.at_least(t, 0), FP32 ? 0u : l.at_least(t, 1)};
+    uint32_t mask[2] = {l.at_least(t, 0), l.at_least(t, 1)};
     const bool one = __popc(mask[0]) + __popc(mask[1]) == 1;         // then it is the largest
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -236,15 +239,15 @@ __global__ void __launch_bounds__(kSelThreads, kSelBlocks) select_chunk_kernel(c
   if (tid == 0) {
     float t = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float g = fmaxf(s_max[2 * i], s_max[2 * i + 1]);
+    for (int i = 0; i < 4; ++i) {
+      const float g = fmaxf(fmaxf(s_max[4 * i], s_max[4 * i + 1]), fmaxf(s_max[4 * i + 2], s_max[4 * i + 3]));
       if (g > neg_inf()) t = fmaf(s_sum[i], ex2((g - top) * kLog2e), t);
     }
     p.sums[item] = make_float2(top, t);
   }
   if (count <= kListCap) {
-    if (tid < count) {
-      const Cand c = s_list[tid];
+    for (int j = tid; j < count; j += kSelThreads) {
+      const Cand c = s_list[j];
       int better = 0;
       for (int i = 0; i < count; ++i) better += before(s_list[i], c);
       if (better < a.K) out[better] = c;
@@ -513,7 +516,7 @@ int launch_reorder(const MoveParams& p, uint32_t blocks, cudaStream_t s) {
 
 extern "C" size_t bolt3_beam_select_workspace(int B, int K, int64_t V) {
   if (B <= 0 || K <= 0 || K > kMaxK || V <= 0 || V > kMaxV) return 0;
-  const size_t rows = (size_t)B * K, nc = (size_t)((V + 3 + kMinChunk - 1) / kMinChunk);
+  const size_t rows = (size_t)B * K, nc = (size_t)((V + 7 + kChunk - 1) / kChunk);
   return align16(rows * nc * sizeof(float2)) + align16(rows * nc * K * sizeof(Cand));
 }
 
@@ -533,9 +536,8 @@ extern "C" int bolt3_beam_select(const bolt3_beam_select_args* a, void* stream) 
     if (a->eos_ids[i] < 0 || a->eos_ids[i] >= a->V) return BOLT3_ERR_ARG;
   SelParams p;
   p.a = *a;
-  const int chunk = a->logits_fp32 ? kChunk<true> : kChunk<false>;
   const int slip = a->logits_fp32 ? 3 : 7;            // logits by which a row may begin after a 16-byte boundary
-  p.n_chunks = (int)((a->V + slip + chunk - 1) / chunk);
+  p.n_chunks = (int)((a->V + slip + kChunk - 1) / kChunk);
   const size_t rows = (size_t)a->B * a->K;
   p.sums = reinterpret_cast<float2*>(a->workspace);
   p.cands = reinterpret_cast<Cand*>(reinterpret_cast<char*>(a->workspace) + align16(rows * p.n_chunks * sizeof(float2)));
