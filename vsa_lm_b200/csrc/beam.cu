@@ -36,15 +36,20 @@ constexpr int kSelBlocks = FP32 ? 5 : 10;             // of an SM
 constexpr int kListCap = 256;                         // candidates at or above the threshold
 constexpr int64_t kMaxV = 64 * kChunk;             // (with a slip a row may have 65 chunks)
 
-// the float of an fkey
-B3_DEV float unkey(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
-
 struct Cand {
   float x;
   int32_t v;
 };
 // a before b in the order of a row: larger logit, then lower index
 B3_DEV bool before(Cand a, Cand b) { return a.x > b.x || (a.x == b.x && a.v < b.v); }
+
+// the number of candidates of the list before c
+B3_DEV int rank_of(Cand c, const Cand* list, int count) {
+  int rank = 0;
+#pragma unroll 4
+  for (int i = 0; i < count; ++i) rank += before(list[i], c);
+  return rank;
+}
 
 struct SelParams {
   bolt3_beam_select_args a;
@@ -137,7 +142,7 @@ template <bool FP32>
 __global__ void __launch_bounds__(kSelThreads, kSelBlocks<FP32>) select_chunk_kernel(const __grid_constant__ SelParams p) {
   using L = Logits<FP32>;
   constexpr int EPL = L::EPL, kBytes = FP32 ? 4 : 2, kPer = kPerThread;
-  __shared__ float s_max[16], s_sum[4];
+  __shared__ float s_max[kSelThreads / 2], s_sum[kSelThreads / 32];
   __shared__ int s_count;
   __shared__ Cand s_list[kListCap];
   const bolt3_beam_select_args& a = p.a;
@@ -200,38 +205,46 @@ __global__ void __launch_bounds__(kSelThreads, kSelBlocks<FP32>) select_chunk_ke
         if (place(i) >= from && place(i) < n) sum += ex2(fmaf(fmaxf(value(place(i)), neg_inf()), kLog2e, -off));
     }
   }
-  float g = m;                                        // maximum of the quarter-warp, of the warp
-#pragma unroll
-  for (int o = 4; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-  if ((lane & 7) == 0) s_max[warp * 4 + (lane >> 3)] = g;
-  g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 8));
-  g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 16));
-  sum = warp_sum(m > neg_inf() ? sum * ex2((m - g) * kLog2e) : 0.f);
-  if (lane == 0) s_sum[warp] = sum;
+  // column c: the threads tid = c mod 16, all of them with logits once 16 threads have some
+  const float col = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+  if (lane < 16) s_max[warp * 16 + lane] = col;
   if (tid == 0) s_count = 0;
   __syncthreads();
-  // tau: the K-th largest of the 16 quarter-warps' maxima (one of them leaves per round)
-  uint32_t key = lane < 16 ? fkey(s_max[lane]) : 0;
-  uint32_t best = __reduce_max_sync(0xffffffffu, key);
-  const float top = unkey(best);
-#pragma unroll 1
-  for (int i = 1; i < a.K; ++i) {
-    if (lane == __ffs(__ballot_sync(0xffffffffu, key == best)) - 1) key = 0;
-    best = __reduce_max_sync(0xffffffffu, key);
-  }
-  const float tau = unkey(best);
-  if (m >= tau && m > neg_inf()) {
-    // tau is one of the logits, or -infinity: then any logit above that counts
-    const float t = tau > neg_inf() ? tau : FP32 ? -3.4028235e38f : -3.3895314e38f;
-    uint32_t mask[2] = {l.at_least(t, 0), l.at_least(t, 1)};
-    const bool one = __popc(mask[0]) + __popc(mask[1]) == 1;         // then it is the largest
+  // tau: the K-th largest of the 16 columns' maxima, found by lane i as the one that K - 1 others are ahead of
+  float own = neg_inf();
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      for (; mask[h]; mask[h] &= mask[h] - 1) {
-        const int e = place(L::of_bit(__ffs(mask[h]) - 1, h));
-        const int at = atomicAdd(&s_count, 1);        // the list's order does not matter: it is ranked below
-        if (at < kListCap) s_list[at] = Cand{one ? m : value(e), lo + e};
-      }
+  for (int i = 0; i < kSelThreads / 32; ++i) own = fmaxf(own, s_max[i * 16 + (lane & 15)]);
+  int rank = 0;
+  float top = own;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) {
+    const float o = __shfl_xor_sync(0xffffffffu, own, i);
+    rank += o > own || (o == own && ((lane ^ i) & 15) < (lane & 15));
+    top = fmaxf(top, o);
+  }
+  const float tau = __shfl_sync(0xffffffffu, own, __ffs(__ballot_sync(0xffffffffu, rank == a.K - 1)) - 1);
+  sum = warp_sum(m > neg_inf() ? sum * ex2((m - top) * kLog2e) : 0.f);
+  if (lane == 0) s_sum[warp] = sum;
+  const bool any = m >= tau && m > neg_inf();
+  const unsigned some = __ballot_sync(0xffffffffu, any);
+  if (some != 0) {                                    // the list's order does not matter: it is ranked below
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&s_count, __popc(some));
+    at = __shfl_sync(0xffffffffu, at, 0) + __popc(some & ((1u << lane) - 1));
+    if (any) {
+      // tau is one of the logits, or -infinity: then any logit above that counts
+      const float t = tau > neg_inf() ? tau : FP32 ? -3.4028235e38f : -3.3895314e38f;
+      uint32_t mask[2] = {l.at_least(t, 0), l.at_least(t, 1)};
+      const bool one = __popc(mask[0]) + __popc(mask[1]) == 1;       // then it is the largest
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        for (; mask[h]; mask[h] &= mask[h] - 1) {
+          const int e = place(L::of_bit(__ffs(mask[h]) - 1, h));
+          if (at < 0) at = atomicAdd(&s_count, 1);    // the place of a thread's first is taken above
+          if (at < kListCap) s_list[at] = Cand{one ? m : value(e), lo + e};
+          at = -1;
+        }
+    }
   }
   __syncthreads();
   const int count = s_count;
@@ -239,17 +252,13 @@ __global__ void __launch_bounds__(kSelThreads, kSelBlocks<FP32>) select_chunk_ke
   if (tid == 0) {
     float t = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float g = fmaxf(fmaxf(s_max[4 * i], s_max[4 * i + 1]), fmaxf(s_max[4 * i + 2], s_max[4 * i + 3]));
-      if (g > neg_inf()) t = fmaf(s_sum[i], ex2((g - top) * kLog2e), t);
-    }
+    for (int i = 0; i < kSelThreads / 32; ++i) t += s_sum[i];
     p.sums[item] = make_float2(top, t);
   }
   if (count <= kListCap) {
     for (int j = tid; j < count; j += kSelThreads) {
       const Cand c = s_list[j];
-      int better = 0;
-      for (int i = 0; i < count; ++i) better += before(s_list[i], c);
+      const int better = rank_of(c, s_list, count);
       if (better < a.K) out[better] = c;
     }
     if (tid >= count && tid < a.K) out[tid] = Cand{neg_inf(), -1};
@@ -287,7 +296,6 @@ __global__ void __launch_bounds__(32 * kMaxK) select_group_kernel(const __grid_c
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float c_score[kMaxK * kMaxK];
   __shared__ int32_t c_token[kMaxK * kMaxK];
-  __shared__ int s_pick[kMaxK];
   __shared__ bool s_done[kMaxK];
   const bolt3_beam_select_args& a = p.a;
   const int K = a.K, tid = threadIdx.x, lane = tid & 31, k = tid >> 5;
@@ -298,7 +306,6 @@ __global__ void __launch_bounds__(32 * kMaxK) select_group_kernel(const __grid_c
   grid_dep_wait();
   const bool done = a.finished != nullptr && a.finished[r];
   const float own = a.scores[r];
-  if (tid < kMaxK) s_pick[tid] = -1;
   if (lane == 0) s_done[k] = done;       // the outputs may be the inputs: nothing of these is read later
   if (!done && own > neg_inf()) {
     for (int i = lane; i < per_row; i += 32) all[i] = p.cands[r * per_row + i];
@@ -313,54 +320,63 @@ __global__ void __launch_bounds__(32 * kMaxK) select_group_kernel(const __grid_c
     s = warp_sum(s);
     const float lse = m + logf(s);
     __syncwarp();
-    // each lane walks the sorted lists of three chunks (at most 65 in all); the order is (logit, lowest index) as a pair of
-    // integers (x + 0 makes one of the two zeros)
-    int at[3] = {0, 0, 0};
-    for (int i = 0; i < K; ++i) {
-      uint32_t key[3] = {0, 0, 0};
-      int32_t v[3] = {0x7fffffff, 0x7fffffff, 0x7fffffff};
+    // each lane walks the sorted lists of three chunks (at most 65 in all), their heads in registers; the order is (logit,
+    // lowest index) as a pair of integers (x + 0 makes one of the two zeros; key 0 is the end of a list)
+    int at[3];
+    uint32_t key[3];
+    Cand head[3];
 #pragma unroll
-      for (int j = 0; j < 3; ++j) {
-        const int c = lane + 32 * j;
-        if (c < p.n_chunks && at[j] < K) {
-          const Cand h = all[c * K + at[j]];
-          if (h.v >= 0) {
-            key[j] = fkey(h.x + 0.f);
-            v[j] = h.v;
-          }
-        }
-      }
+    for (int j = 0; j < 3; ++j) {
+      at[j] = (lane + 32 * j) * K;
+      head[j] = lane + 32 * j < p.n_chunks ? all[at[j]] : Cand{neg_inf(), -1};
+      key[j] = head[j].v >= 0 ? fkey(head[j].x + 0.f) : 0;
+    }
+    int n = 0;
+    for (; n < K; ++n) {
       const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(key[0], key[1]), key[2]));
-      const int32_t win = __reduce_min_sync(0xffffffffu, min(min(key[0] == top ? v[0] : 0x7fffffff, key[1] == top ? v[1] : 0x7fffffff),
-                                                             key[2] == top ? v[2] : 0x7fffffff));
+      if (top == 0) break;
+      uint32_t low = 0xffffffffu;
 #pragma unroll
       for (int j = 0; j < 3; ++j)
-        if (key[j] == top && v[j] == win && win != 0x7fffffff) {
-          const float sc = own + (all[(lane + 32 * j) * K + at[j]].x - lse);
-          c_score[k * K + i] = sc != sc ? neg_inf() : sc;
-          c_token[k * K + i] = win;
-          at[j]++;
+        if (key[j] == top) low = min(low, (uint32_t)head[j].v);
+      const uint32_t win = __reduce_min_sync(0xffffffffu, low);
+#pragma unroll
+      for (int j = 0; j < 3; ++j)
+        if (key[j] == top && (uint32_t)head[j].v == win) {
+          const float sc = own + (head[j].x - lse);
+          c_score[k * K + n] = sc != sc ? neg_inf() : sc;
+          c_token[k * K + n] = (int32_t)win;
+          head[j] = ++at[j] < (lane + 32 * j + 1) * K ? all[at[j]] : Cand{neg_inf(), -1};
+          key[j] = head[j].v >= 0 ? fkey(head[j].x + 0.f) : 0;
         }
-      if (win == 0x7fffffff && lane == 0) c_score[k * K + i] = neg_inf();
     }
+    if (lane >= n && lane < K) c_score[k * K + lane] = neg_inf();
   } else if (lane < K) {
     const float sc = done && lane == 0 ? own : neg_inf();
     c_score[k * K + lane] = sc != sc ? neg_inf() : sc;
     c_token[k * K + lane] = (int32_t)a.eos_ids[0];
   }
   __syncthreads();
-  // rank of every candidate: score, then beam, then its place in the beam's list
-  for (int i = tid; i < K * K; i += blockDim.x) {
-    const float sc = c_score[i];
-    if (!(sc > neg_inf())) continue;
-    int better = 0;
-    for (int j = 0; j < K * K; ++j) better += c_score[j] > sc || (c_score[j] == sc && j < i);
-    if (better < K) s_pick[better] = i;
-  }
-  __syncthreads();
   if (tid >= 32) return;
+  // the K best of the beams' sorted lists: lane k stands at beam k's list; the order is score, then beam, then place in it
+  int at = lane * K, c = -1;             // lane i gets the candidate of rank i
+  auto head = [&] {
+    const float x = lane < K && at < (lane + 1) * K ? c_score[at] : neg_inf();
+    return x > neg_inf() ? fkey(x + 0.f) : 0;
+  };
+  uint32_t key = head();
+  for (int i = 0; i < K; ++i) {
+    const uint32_t best = __reduce_max_sync(0xffffffffu, key);
+    if (best == 0) break;
+    const int from = __ffs(__ballot_sync(0xffffffffu, key == best)) - 1;
+    const int pick = __shfl_sync(0xffffffffu, at, from);
+    if (lane == i) c = pick;
+    if (lane == from) {
+      ++at;
+      key = head();
+    }
+  }
   // lane i: the continuation of rank i. The first child of a parent takes the parent's slot, the others what is left
-  const int c = lane < K ? s_pick[lane] : -1;
   const int par = c < 0 ? 32 + lane : c / K;
   const unsigned same = __match_any_sync(0xffffffffu, par);
   const bool first = c >= 0 && __ffs(same) - 1 == lane;
