@@ -50,4 +50,11 @@ B3_DEV void s8x4_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
   asm("sub.f16x2 %0, %0, %1;\n" : "+r"(hi) : "r"(0x64806480u));
 }
 
+// as two bf16 pairs, exactly: 128 + the low seven bits, minus 128, or minus 256 for a negative one
+B3_DEV void s8x4_to_bf16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t x = __byte_perm(w, 0x43434343u, 0x4140), y = __byte_perm(w, 0x43434343u, 0x4342);
+  asm("sub.rn.bf16x2 %0, %1, %2;\n" : "=r"(lo) : "r"(x & 0xff7fff7fu), "r"(x & 0xff80ff80u));
+  asm("sub.rn.bf16x2 %0, %1, %2;\n" : "=r"(hi) : "r"(y & 0xff7fff7fu), "r"(y & 0xff80ff80u));
+}
+
 }  // namespace kv8

@@ -1,14 +1,13 @@
 // Softmax attention of many query rows (prompt slices) over the 8-bit KV cache, on the tensor cores' TMEM path.
 //
 // The mathematics and its roundings are those of kv8_attend.cu: with t_j the score of key j in log2 units and
-// u_j = t_j + log2 scale_v[j], weights w_j = 2^(u_j - M) in f16, y = sum w_j v8_j / sum (w_j / scale_v[j]). Here the
-// CTA's query rows are brought to f16 by one power of two (exact down to 2^-25 of the largest value among them, which
-// moves a score by 2^-25 of the largest score's sum of magnitudes) and the int8 keys and values are exact in f16.
+// u_j = t_j + log2 scale_v[j], weights w_j = 2^(u_j - M) in f16, y = sum w_j v8_j / sum (w_j / scale_v[j]). The int8 keys
+// are exact in bf16, so the scores are products of the queries as they are; the int8 values are exact in f16.
 //
 // Bound by arithmetic: 4 HD operations per (query row, key), and one exponential. A CTA holds two tiles of 128 query
 // rows (T * G rows of one KV head, token-major) and walks the keys in blocks of 128, so that a block is widened from
-// int8 to f16 once for 256 rows. Roles, which meet only at mbarriers:
-// - warps 16-19 widen keys, 20-23 values: global int8 -> registers (a block ahead) -> f16 operand tiles in shared memory
+// int8 once for 256 rows. Roles, which meet only at mbarriers:
+// - warps 16-19 widen keys, 20-23 values: global int8 -> registers (a block ahead) -> operand tiles in shared memory
 //   (two stages each); the latter also prepare the block's scales;
 // - one lane of warp 24 issues tcgen05.mma: S = Q K^T into TMEM, O += P V with P as the TMEM operand;
 // - warps 0-7 and 8-15 are the softmax of a tile, 64 keys at a time: scores out of TMEM, weights back over them, fp32
@@ -55,9 +54,8 @@ struct Smem {
   unsigned char q[2][kKeys * HD * 2];            // K-major operand tiles: HD / 64 blocks of [128 rows][64 columns]
   unsigned char k[2][kKeys * HD * 2];
   unsigned char v[2][kKeys * HD * 2];
-  float scale[2][3][kKeys];                      // key scale (times sm_scale log2(e) and the queries' unit), log2 and
+  float scale[2][3][kKeys];                      // key scale (times sm_scale log2(e)), log2 and
                                                  // reciprocal of the value scale
-  float q_max[16];
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t s_full[2], p_full[2][2], pv_half[2], o_full[2];
   uint32_t tbase;
@@ -153,13 +151,16 @@ B3_DEV void st_16x32f(uint32_t taddr, const uint32_t (&r)[16]) {
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
 }
 
-// 16 int8 as f16 to a row's 16-byte chunks 2 c and 2 c + 1 (the address of the first, swizzled; the other one is beside it)
+// 16 int8, keys as bf16, values as f16, to a row's 16-byte chunks 2 c and 2 c + 1 (the address of the first, swizzled; the
+// other one is beside it)
+template <bool KEYS>
 B3_DEV void widen16(unsigned char* at, const uint4& x) {
+  auto widen = [](uint32_t w, uint32_t& lo, uint32_t& hi) { KEYS ? s8x4_to_bf16(w, lo, hi) : s8x4_to_f16(w, lo, hi); };
   uint4 lo, hi;
-  s8x4_to_f16(x.x, lo.x, lo.y);
-  s8x4_to_f16(x.y, lo.z, lo.w);
-  s8x4_to_f16(x.z, hi.x, hi.y);
-  s8x4_to_f16(x.w, hi.z, hi.w);
+  widen(x.x, lo.x, lo.y);
+  widen(x.y, lo.z, lo.w);
+  widen(x.z, hi.x, hi.y);
+  widen(x.w, hi.z, hi.w);
   *reinterpret_cast<uint4*>(at) = lo;
   *reinterpret_cast<uint4*>((uintptr_t)at ^ 16) = hi;
 }
@@ -214,58 +215,32 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     return;
   }
 
-  // this thread's half of query row tid / 2 to f16, in the operand tile. 2^-e brings the largest value of the CTA's rows
-  // into [1, 2)
-  uint4 raw[HD / 16];
+  // the query rows into their operand tiles; the other warps are at their first loads meanwhile
   if (warp < 16) {
-    const int row = row0 + (tid >> 1);
-    float m = 0.f;
+    constexpr int CPR = HD / 8, RPW = 32 / CPR;                   // 16-byte chunks of a row, rows of a warp's instruction
+    const int c = lane % CPR;
+    int r = warp * 16 + lane / CPR, t = (row0 + r) / p.G, g = (row0 + r) % p.G;
 #pragma unroll
-    for (int i = 0; i < HD / 16; ++i) {
-      raw[i] = make_uint4(0, 0, 0, 0);
-      if (row < p.rows)
-        raw[i] = reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.q) + b * a.q_sb + (row / p.G) * a.q_st +
-                                                (int64_t)(kvh * p.G + row % p.G) * HD)[2 * i + (tid & 1)];
-      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 v = unpack_bf16(w[j]);
-        m = max3(m, fabsf(v.x) < 3e38f ? fabsf(v.x) : 0.f, fabsf(v.y) < 3e38f ? fabsf(v.y) : 0.f);   // finite ones
-      }
+    for (int i = 0; i < 16 / RPW; ++i, r += RPW) {
+      const bool in = row0 + r < p.rows;
+      const bf16* src = reinterpret_cast<const bf16*>(a.q) + b * a.q_sb + (int64_t)(kvh * p.G) * HD;
+      if (in) src += t * a.q_st + g * HD + 8 * c;
+      cp_async16(sm.q[0] + (r >> 7) * sizeof(sm.q[0]) + (c >> 3) * (kKeys * 128) + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4), src, in);
+      for (g += RPW; g >= p.G; g -= p.G) ++t;
     }
-    m = warp_max(m);
-    if (lane == 0) sm.q_max[warp] = m;
-  }
-  __syncthreads();
-  float q_max = 0.f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) q_max = fmaxf(q_max, sm.q_max[i]);
-  const int e = q_max > 0.f ? max(ilogbf(q_max), -100) : 0;
-  if (warp < 16) {
-    const int r = (tid >> 1) & 127;
-    const float down = exp2f((float)-e);
-    unsigned char* tile = sm.q[tid >> 8];
-#pragma unroll
-    for (int i = 0; i < HD / 16; ++i) {
-      const float2 x = unpack_bf16(raw[i].x), y = unpack_bf16(raw[i].y), z = unpack_bf16(raw[i].z), w = unpack_bf16(raw[i].w);
-      const int c = 2 * i + (tid & 1);                            // 16-byte chunk of the row
-      uint4 o;
-      o.x = pack_f16(x.x * down, x.y * down);
-      o.y = pack_f16(y.x * down, y.y * down);
-      o.z = pack_f16(z.x * down, z.y * down);
-      o.w = pack_f16(w.x * down, w.y * down);
-      *reinterpret_cast<uint4*>(tile + (c >> 3) * (kKeys * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = o;
-    }
+    asm volatile("cp.async.wait_all;\nfence.proxy.async.shared::cta;\n" ::: "memory");
   }
   if (warp == 24) {
     tc5::tmem_alloc(&sm.tbase, 512);
     tc5::tmem_relinquish();
   }
-  asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-  tc5::fence_before_sync();
-  __syncthreads();
-  tc5::fence_after_sync();
-  const uint32_t tb = sm.tbase;                  // S / P of tile i: columns 128 i; O of tile i: 256 + 128 i
+  // every warp comes here once: the queries are in place, the barriers and the TMEM are there
+  auto all_ready = [&] {
+    tc5::fence_before_sync();
+    asm volatile("bar.sync 0;\n" ::: "memory");
+    tc5::fence_after_sync();
+    return sm.tbase;                             // S / P of tile i: columns 128 i; O of tile i: 256 + 128 i
+  };
   auto wait = [&](uint64_t* bar, int phase) {
     if (tc5::mbar_wait(bar, (uint32_t)phase & 1, kWaitIters)) return true;
     sm.err = 1;
@@ -283,7 +258,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     const int64_t side = (int64_t)a.B * a.HKV * a.cap;
     const int8_t* base = a.data + ((int64_t)head * a.cap + (values ? side : 0) + lo * kKeys) * HD + 16 * (t & 3);
     const float* ks = a.scale + (int64_t)head * a.cap + lo * kKeys + t;
-    const float c_all = a.sm_scale * kLog2e * exp2f((float)e);    // what a score in f16 units is worth, into the key scales
     const int end = (int)min(a.cap - 1 - lo * kKeys, (int64_t)0x7fffff00);   // the buffer's last row
     uint64_t *full = values ? sm.v_full : sm.k_full, *empty = values ? sm.v_empty : sm.k_empty;
     unsigned char* out = (values ? sm.v[0] : sm.k[0]) + r0 * 128 + (((2 * (t & 3)) ^ (r0 & 7)) << 4);
@@ -312,13 +286,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       }
     };
     fetch(0);
+    all_ready();
+    const float c_all = a.sm_scale * kLog2e;                      // into the key scales
     for (int j = 0; j < n_blk; ++j) {
       const int st = j & 1;
       if (j >= 2 && !wait(&empty[st], (j >> 1) - 1)) break;
       unsigned char* to = out + st * sizeof(sm.k[0]);
+      auto at = [&](int i) { return to + (i % KC) * (kKeys * 128) + 32 * (i / KC) * 128; };
+      if (!values) {
 #pragma unroll
-      for (int i = 0; i < NP; ++i) widen16(to + (i % KC) * (kKeys * 128) + 32 * (i / KC) * 128, x[i]);
-      if (values) {
+        for (int i = 0; i < NP; ++i) widen16<true>(at(i), x[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) widen16<false>(at(i), x[i]);
         sm.scale[st][0][t] = k_sc * c_all;
         sm.scale[st][1][t] = lg2(v_sc);
         sm.scale[st][2][t] = rcp(v_sc);
@@ -331,10 +311,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     // ---- issue. The whole warp runs the loop, so that addresses and descriptors are uniform over it (a lone thread in a
     // branch of its own needed 170 cycles an MMA for moving them to where the instruction takes them); one lane issues
     fewer_regs<kRegsIssue>();
+    const uint32_t tb = all_ready();
     if (warp == 24) {
       uint32_t one;
       asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}\n" : "=r"(one));
-      constexpr uint32_t kIdS = tc5::idesc_f16(128, kKeys, false, false), kIdO = tc5::idesc_f16(128, HD, false, true);
+      constexpr uint32_t kIdS = tc5::idesc_bf16(128, kKeys, false, false), kIdO = tc5::idesc_f16(128, HD, false, true);
       constexpr uint64_t kTile = sizeof(sm.q[0]) >> 4;            // from one tile's descriptor to the next one's
       const uint32_t tu = __shfl_sync(0xffffffffu, tb, 0);
       const uint64_t q_desc = tc5::sdesc(tc5::smem_u32(sm.q[0]), 16, 1024), k_desc = tc5::sdesc(tc5::smem_u32(sm.k[0]), 16, 1024);
@@ -396,6 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
       }
     }
   } else {
+    const uint32_t tb = all_ready();
     more_regs<kRegsSoftmax>();
     if ((warp >> 3) < n_tile) {
     // ---- softmax of tile i: this thread's two rows are those of TMEM lanes first_lane + grp and + grp + 8
@@ -514,17 +496,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         tc5::mbar_arrive(&sm.p_full[i][h]);
       }
     }
+    float sum[2], inv[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const float2 x = unpair(l[q]);
+      sum[q] = quad_sum(x.x + x.y);
+      inv[q] = sum[q] == 0.f ? 0.f : 1.f / sum[q];
+    }
     ok = ok && wait(&sm.o_full[i], 0);
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       tc5::fence_after_sync();
-      float sum[2], inv[2];
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const float2 x = unpair(l[q]);
-        sum[q] = quad_sum(x.x + x.y);
-        inv[q] = sum[q] == 0.f ? 0.f : 1.f / sum[q];
-      }
+      // bf16 rows by way of this warp's sixteen rows of the query tile, whose products are done: whole rows to a store (4 bytes
+      // of 8 rows to a store took 5000 cycles)
+      unsigned char* out = sm.q[i] + first_lane * HD * 2;
 #pragma unroll 1
       for (int d = 0; d < HD; d += 32) {
         uint32_t o[16];
@@ -532,19 +517,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         tc5::ld_wait();
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const int row = first_row + 8 * q;
-          if (row >= p.rows) continue;
           if (p.splits > 1) {
+            const int row = first_row + 8 * q;
             float* dst = p.part + (((int64_t)head * p.rows + row) * p.splits + split) * HD + d + 2 * tig;
 #pragma unroll
-            for (int n = 0; n < 4; ++n) *reinterpret_cast<uint2*>(dst + 8 * n) = make_uint2(o[4 * n + 2 * q], o[4 * n + 2 * q + 1]);
+            for (int n = 0; n < 4; ++n)
+              if (row < p.rows) *reinterpret_cast<uint2*>(dst + 8 * n) = make_uint2(o[4 * n + 2 * q], o[4 * n + 2 * q + 1]);
           } else {
-            bf16* dst = out_row(row) + d + 2 * tig;
 #pragma unroll
             for (int n = 0; n < 4; ++n)
-              *reinterpret_cast<uint32_t*>(dst + 8 * n) =
+              *reinterpret_cast<uint32_t*>(out + (grp + 8 * q) * HD * 2 + (((d / 8 + n) ^ grp) << 4) + 4 * tig) =
                   pack_bf16(__uint_as_float(o[4 * n + 2 * q]) * inv[q], __uint_as_float(o[4 * n + 2 * q + 1]) * inv[q]);
           }
+        }
+      }
+      if (p.splits == 1) {
+        constexpr int CPR = HD / 8, RPW = 32 / CPR;
+        const int c = lane % CPR;
+        __syncwarp();
+#pragma unroll
+        for (int r = lane / CPR; r < 16; r += RPW) {
+          const int row = row0 + 128 * i + first_lane + r;
+          if (row < p.rows) reinterpret_cast<uint4*>(out_row(row))[c] = *reinterpret_cast<uint4*>(out + r * HD * 2 + ((c ^ (r & 7)) << 4));
         }
       }
       if (p.splits > 1 && tig == 0) {
@@ -559,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
   tc5::fence_before_sync();
   __syncthreads();
   tc5::fence_after_sync();
-  if (warp == 24) tc5::tmem_dealloc(tb, 512);
+  if (warp == 24) tc5::tmem_dealloc(sm.tbase, 512);
   if (tid == 0 && sm.err && a.status) atomicOr(a.status, 2);
 }
 
