@@ -45,6 +45,7 @@ struct Params {
   bolt3_kv8_attend_args a;
   Length len;
   int G, rows, tiles, splits;                    // tiles: pairs of 128 rows of a head
+  uint32_t per_G;                                // ceil(2^32 / G), 0 for G = 1
   float* part;                                   // [head][row][split][HD] sums, then [..] (bound, sum of weights)
   float2* part_ml;
 };
@@ -61,6 +62,9 @@ struct Smem {
   uint32_t tbase;
   int err;
 };
+
+// the token of a query row (exact for rows below 2^28)
+B3_DEV int token_of(const Params& p, int row) { return p.per_G == 0 ? row : (int)__umulhi((uint32_t)row, p.per_G); }
 
 B3_DEV float ex2(float x) {
   float y;
@@ -195,10 +199,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
   const int64_t s = p.len.rows(b, bad);
   if (bad && tid == 0 && blockIdx.x % p.tiles == 0 && split == 0 && a.status) atomicOr(a.status, 8);
   auto out_row = [&](int row) {
-    return reinterpret_cast<bf16*>(a.y) + (((int64_t)b * a.T + row / p.G) * a.H + kvh * p.G + row % p.G) * HD;
+    const int t = token_of(p, row), g = row - t * p.G;
+    return reinterpret_cast<bf16*>(a.y) + ((int64_t)b * a.T * a.H + kvh * p.G) * HD + (int64_t)t * (a.H * HD) + g * HD;
   };
   // blocks of keys that the last row of this CTA sees, and this split's share of them
-  const int last = (min(row0 + 256, p.rows) - 1) / p.G;
+  const int last = token_of(p, min(row0 + 256, p.rows) - 1);
   const int64_t all = s < 0 ? 0 : (s + last + kKeys) / kKeys;
   const int64_t lo = all * split / p.splits, hi = all * (split + 1) / p.splits;
   const int n_blk = (int)(hi - lo);
@@ -219,14 +224,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
   if (warp < 16) {
     constexpr int CPR = HD / 8, RPW = 32 / CPR;                   // 16-byte chunks of a row, rows of a warp's instruction
     const int c = lane % CPR;
-    int r = warp * 16 + lane / CPR, t = (row0 + r) / p.G, g = (row0 + r) % p.G;
+    const bf16* q = reinterpret_cast<const bf16*>(a.q) + b * a.q_sb + (int64_t)(kvh * p.G) * HD + 8 * c;
 #pragma unroll
-    for (int i = 0; i < 16 / RPW; ++i, r += RPW) {
+    for (int i = 0; i < 16 / RPW; ++i) {
+      const int r = warp * 16 + lane / CPR + i * RPW, t = token_of(p, row0 + r), g = row0 + r - t * p.G;
       const bool in = row0 + r < p.rows;
-      const bf16* src = reinterpret_cast<const bf16*>(a.q) + b * a.q_sb + (int64_t)(kvh * p.G) * HD;
-      if (in) src += t * a.q_st + g * HD + 8 * c;
-      cp_async16(sm.q[0] + (r >> 7) * sizeof(sm.q[0]) + (c >> 3) * (kKeys * 128) + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4), src, in);
-      for (g += RPW; g >= p.G; g -= p.G) ++t;
+      cp_async16(sm.q[0] + (r >> 7) * sizeof(sm.q[0]) + (c >> 3) * (kKeys * 128) + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4),
+                 in ? q + t * a.q_st + g * HD : q, in);
     }
     asm volatile("cp.async.wait_all;\nfence.proxy.async.shared::cta;\n" ::: "memory");
   }
@@ -385,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     const int first_lane = 32 * (warp & 3) + 16 * (warp >> 2 & 1), first_row = row0 + 128 * i + first_lane + grp;
     const uint32_t lanes = (uint32_t)first_lane << 16, ts = tb + i * 128 + lanes, to = tb + 256 + i * 128 + lanes;
     const int seen = (int)min(s + 1 - lo * kKeys, (int64_t)0x7fffff00);           // keys of this split that token 0 sees
-    const int see_all = seen + (row0 + i * 128) / p.G;                            // that every row of the tile sees
+    const int see_all = seen + token_of(p, row0 + i * 128);                          // that every row of the tile sees
     float M[2] = {neg_inf(), neg_inf()};
     uint64_t l[2] = {0, 0};                                       // sums of weights over this thread's keys, in pairs
     bool ok = true;
@@ -418,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             const int r = min(first_row + 8 * q, p.rows - 1);
-            const int left = seen + r / p.G - key - 2 * tig;   // seen, from this thread's first
+            const int left = seen + token_of(p, r) - key - 2 * tig;   // seen, from this thread's first
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
               if (8 * n >= left) t[q][n].x = neg_inf();
@@ -631,6 +635,7 @@ int kv8_prompt_launch(const bolt3_kv8_attend_args* a, const Length& len, cudaStr
   p.a = *a;
   p.len = len;
   p.G = a->H / a->HKV;
+  p.per_G = p.G == 1 ? 0 : 0xffffffffu / p.G + 1;
   p.rows = a->T * p.G;
   p.tiles = pl.tiles;
   p.splits = pl.splits;
