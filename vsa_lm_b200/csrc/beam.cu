@@ -3,15 +3,20 @@
 // select. With lse_k = log sum_v e^x_kv, continuation (k, v) scores s_k + (x_kv - lse_k); the K best of a
 // group's K * V survive. Bound by HBM: the logits are read once. Within a beam the order is the logits',
 // so the pass that sums the exponentials also finds each chunk's K best logits:
-// - select_chunk_kernel: a block holds a chunk of 8192 logits of one row in registers. Maximum and
-//   sum of exponentials, then a threshold: the K-th largest of its 16 quarter-warps' maxima is no larger than the chunk's
-//   K-th largest logit, so the few logits at or above it contain the K best; they are ranked by counting.
-//   Chunks with many equal logits (more than the list holds) take K rounds of a block maximum instead.
-// - select_group_kernel: a block per group merges the chunks' sums and lists, scores, ranks and assigns slots.
+// - select_chunk_kernel: a block holds a chunk of 8192 logits of one row in registers. Maximum and sum of exponentials,
+//   then a threshold: the K-th largest of the maxima of 16 columns of threads is no larger than the chunk's K-th largest
+//   logit, so the few logits at or above it contain the K best; they are ranked by counting. Chunks with many equal
+//   logits (more than the list holds) take K rounds of a block maximum instead.
+// - select_group_kernel: a block per group merges the chunks' sums and lists, a warp per beam, and then the beams' lists:
+//   both are sorted, so a lane stands at the head of a list and the best head of the warp is next (8 x 16 beams of 34000
+//   fp32 logits: 31 us; with all K^2 continuations ranked by counting 38).
+// Measured on a B200: 64 x 4 beams of 151936 bf16 logits, a fifth finished, 24 us (2.6 TB/s; see below what it is busy
+// with); 64 x 16 beams of 34000 fp32 logits 57 us (2.5 TB/s); 1 x 4 of 32000 fp32 8 us (two launches and their latency).
 // reorder. Bound by HBM: the bytes of every beam that is not its own parent are read from the parent and
 // written, in place for any map: where a parent is moved itself, a thread holds its bytes of all parents of the
 // group before it writes any; where none is (the maps that select gives), beams are copied one by one, eight
-// 16-byte loads ahead. Blocks cover the items' bytes flattened, so that many small arrays are one launch.
+// 16-byte loads ahead. Blocks cover the items' bytes flattened, so that many small arrays are one launch. Measured:
+// 16 x 4 beams, a Bolt-3 layer's state and 256 tokens of an anchor cache in one launch, 23 us (6.0 TB/s).
 #include "../../include/bolt3.h"
 #include "common.cuh"
 #include "trace.h"

@@ -5,9 +5,11 @@
 // The value scale goes into the exponent: u_j = t_j log2(e) + log2 scale_v[j], w_j = 2^(u_j - M) with M a
 // bound on the u_j seen so far, numerator sum w_j v8_j, denominator sum w_j / scale_v[j]. So the f16 weights
 // of the product are relative to the largest weighted value, however far the scales of two tokens lie apart.
-// Sums and the outputs are fp32. Roundings: w_j to f16 (2^-11 relative) for the product with the int8 values,
-// which f16 holds exactly; a query row to 16-bit integers, relative to its largest value (2^-16 of it; bf16 has
-// already rounded that value to 2^-9), as q = 256 hi + lo, so that q . k8 is two int8 products summed exactly.
+// A weight more than 2^126 below the bound is zero in both sums; that matters only where two tokens' value scales
+// lie more than 2^100 apart. Sums and the outputs are fp32. Roundings: w_j to f16 (2^-11 relative) for the product
+// with the int8 values, which f16 holds exactly; a query row to 16-bit integers, relative to its largest value
+// (2^-16 of it; bf16 has already rounded that value to 2^-9), as q = 256 hi + lo, so that q . k8 is two int8
+// products summed exactly.
 //
 // Bound by HBM: 2 (HD + 4) bytes per key and KV head. The cache is read in blocks of 32 keys, for 8 or 16 query
 // rows at once (T * G of them, token-major; more rows: more passes). All blocks of all (sequence, KV head)s are
@@ -21,6 +23,9 @@
 // dimensions in M and the query rows in N (no padding for up to 8 rows): S^T = K Q^T by mma.sync m16n8k32 on the int8
 // keys as they are, with the dimensions permuted so that a lane's 16 bytes feed two products; O^T = V^T P^T by
 // m16n8k16 on f16, output dimensions permuted likewise, P^T being S^T transposed by movmatrix.
+//
+// Measured on a B200, 32 heads on 8 of 128, one token: 131072 keys 57.7 us (4.8 TB/s; 49 of it streaming, the rest the
+// join of 1776 runs), 64 sequences of up to 2304 keys 51 us (4.6 TB/s).
 #include "../../include/bolt3.h"
 #include "kv8.cuh"
 #include "kv8_prompt.cuh"
