@@ -266,6 +266,19 @@ def test_attend_value_ranges(T, H, HKV, HD, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,HD", [(3, 64), (100, 64), (40, 128)])
+def test_attend_rows_of_very_different_sizes(T, HD):
+    """Query rows 2^26 times larger than their neighbours leave those as they are."""
+    B, H, HKV, n = 2, 8, 2, 300
+    data, scale = random_cache(25, B, HKV, n + T, HD)
+    q = randn(26, B, T, H, HD)
+    q.view(B, T * H, HD)[:, ::3] *= 2.0 ** 26
+    q = q.to(torch.bfloat16)
+    y = K.kv8_attend(q=q.cuda(), data=data.cuda(), scale=scale.cuda(), n=n).cpu()
+    check_attend(q, data, scale, n, None, HD ** -0.5, y)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [1, 100])
 def test_attend_nan_stays_in_its_sequence(T):
     """A NaN key or value that a query sees spoils that query; what no query of a sequence sees does not."""
