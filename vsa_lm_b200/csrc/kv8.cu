@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_const
                                                               const __grid_constant__ Length len, int rows_per_block) {
   constexpr int LPR = HD / 8;                        // lanes of a row
   constexpr int RPI = kThreads / LPR;                // rows of one iteration
-  __shared__ float2 trig[TPB][HD / 2];
+  __shared__ float4 trig[TPB][HD / 4];               // cos, sin of a pair of dimensions, cos, sin of the next
   // of each token: its cache row (-1: idle), its first q, k and v element, and the cache row of its first head's keys
   __shared__ int64_t s_row[TPB], s_src[TPB][3], s_out[TPB];
   const int tid = threadIdx.x, part = tid % LPR;
@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_const
     if (tok0 + k < tokens && s_row[k] >= 0) {
       float sn, cs;
       sincosf(__fmul_rn((float)(a.pos0 + (s_row[k] - a.n)), a.inv_freq[f]), &sn, &cs);
-      trig[k][f] = make_float2(cs, sn);
+      reinterpret_cast<float2*>(trig[k])[f] = make_float2(cs, sn);
     }
   }
   const bool norms = a.q_norm_w != nullptr || a.k_norm_w != nullptr;
@@ -137,10 +137,10 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_const
         }
       }
       if (a.inv_freq != nullptr && (is_q || is_k)) {
-        const float4* cs = reinterpret_cast<const float4*>(trig[tk[u]] + 4 * part);
+        const float4* cs = trig[tk[u]] + 2 * part;
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
-          const float4 z = cs[i / 2];                // cos, sin of pair i, cos, sin of the next
+          const float4 z = cs[i / 2];                // of pairs i and i + 1
           const float a0 = x[i], b0 = x[4 + i], a1 = x[i + 1], b1 = x[5 + i];
           x[i] = fmaf(a0, z.x, -b0 * z.y);
           x[4 + i] = fmaf(b0, z.x, a0 * z.y);
