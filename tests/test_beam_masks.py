@@ -1,0 +1,65 @@
+"""Beam search's selection over logits that are masked with the type's lowest value, with large negative numbers,
+or lie at the ends of fp32's range.
+
+The reference takes log_softmax as (x - max) - log(sum e^(x - max)) in 64 bits. Tolerance of a score: three fp32
+roundings of terms no larger than |s| + |x - max| + |log sum| (2^-22 of that), and 2e-6 for the logarithm of the sum.
+"""
+import math
+
+import pytest
+import torch
+
+from vsa_lm_b200 import kernels as K
+
+
+def plain(logits, scores):
+    """(score, parent, token) of the K best continuations by slot, from [B, K, V] logits, in 64 bits."""
+    B, Kb, V = logits.shape
+    x = logits.double()
+    d = x - x.amax(-1, keepdim=True)
+    ls = torch.log(torch.exp(d).sum(-1, keepdim=True))
+    cand = (scores.double()[..., None] + (d - ls)).view(B, -1)
+    size = (scores.double()[..., None].abs() + d.abs() + ls.abs()).view(B, -1)
+    size = torch.where(size.isfinite(), size, 0.0)
+    best, at = torch.sort(cand, dim=1, descending=True, stable=True)
+    out = torch.full((B, Kb), -math.inf, dtype=torch.float64), torch.arange(Kb).repeat(B, 1), torch.zeros(B, Kb).long()
+    tol = torch.zeros(B, Kb, dtype=torch.float64)
+    for b in range(B):
+        free, later = list(range(Kb)), []
+        chosen = [i for i in range(Kb) if best[b, i] > -math.inf]
+        for i in chosen:
+            p = int(at[b, i]) // V
+            later.append(i) if p not in free else (free.remove(p), put(out, tol, b, p, best, at, size, i, V))
+        for i in later:
+            put(out, tol, b, free.pop(0), best, at, size, i, V)
+    return out, 2e-6 + 2 ** -22 * tol
+
+
+def put(out, tol, b, slot, best, at, size, i, V):
+    c = int(at[b, i])
+    out[0][b, slot], out[1][b, slot], out[2][b, slot], tol[b, slot] = best[b, i], c // V, c % V, size[b, c]
+
+
+def check(logits, scores):
+    got = [t.cpu() for t in K.beam_select(logits.cuda(), scores.cuda())]
+    ref, tol = plain(logits, scores)
+    live = ref[0] > -math.inf
+    assert torch.equal(got[0] > -math.inf, live)
+    assert torch.equal(got[1].long()[live], ref[1][live]) and torch.equal(got[2][live], ref[2][live])
+    assert bool(((got[0].double() - ref[0]).abs()[live] <= tol[live]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [100, 8192, 34000])
+@pytest.mark.parametrize("mask", ["lowest", -1e9, -1e10, -3e38, -1e30, -70000.0])
+def test_masked_vocabulary(dtype, V, mask):
+    """A few allowed tokens: whole threads, and whole chunks, hold nothing but the mask."""
+    g = torch.Generator().manual_seed(5)
+    B, Kb = 3, 4
+    x = torch.full((B, Kb, V), torch.finfo(dtype).min if mask == "lowest" else mask, dtype=dtype)
+    for b in range(B):
+        for k in range(Kb):
+            at = torch.randperm(V, generator=g)[:6]
+            x[b, k, at] = torch.arange(6, dtype=dtype) + 7 * b + k / 8
+    check(x, -3 * torch.rand(B, Kb, generator=g))

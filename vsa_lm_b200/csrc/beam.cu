@@ -187,10 +187,17 @@ __global__ void __launch_bounds__(kSelThreads, kSelBlocks<FP32>) select_chunk_ke
     }
     l.w[4 * i] = q.x; l.w[4 * i + 1] = q.y; l.w[4 * i + 2] = q.z; l.w[4 * i + 3] = q.w;
   }
-  // every thread sums against its own maximum: nothing here waits for another warp
+  // every thread sums against its own maximum: nothing here waits for another warp. The exponents are x log2(e) - off with
+  // off = m log2(e) rounded, whose remainder (up to 64 at the bound) is the same for all of them and taken out of the sum.
+  // From 2^30 on, fp32 neighbours are 64 apart: what is below m adds nothing, and the sum is the number of logits equal to m
   const float m = l.largest();
   float sum = 0.f;
-  if (m > neg_inf()) {
+  if (fabsf(m) >= 0x1p30f) {
+    if (m > neg_inf()) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) sum += l.x(i) == m ? 1.f : 0.f;
+    }
+  } else {
     const float off = m * kLog2e;
     const uint64_t l2e = pair(kLog2e, kLog2e), minus = pair(-off, -off);
     uint64_t s0 = 0, s1 = 0;
@@ -209,6 +216,7 @@ __global__ void __launch_bounds__(kSelThreads, kSelBlocks<FP32>) select_chunk_ke
       for (int i = 0; i < kPer; ++i)
         if (place(i) >= from && place(i) < n) sum += ex2(fmaf(fmaxf(value(place(i)), neg_inf()), kLog2e, -off));
     }
+    sum *= ex2(-fmaf(m, kLog2e, -off));
   }
   // column c: the threads tid = c mod 16, all of them with logits once 16 threads have some
   const float col = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
