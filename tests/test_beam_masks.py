@@ -63,3 +63,31 @@ def test_masked_vocabulary(dtype, V, mask):
             at = torch.randperm(V, generator=g)[:6]
             x[b, k, at] = torch.arange(6, dtype=dtype) + 7 * b + k / 8
     check(x, -3 * torch.rand(B, Kb, generator=g))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [100, 20000])
+@pytest.mark.parametrize("at", ["lowest", "highest", -1e9, -1e10, 1e9, 1e10, 4e4, -4e4, 2.0 ** 30, -2.0 ** 30])
+def test_beam_of_equal_logits_of_any_size(dtype, V, at):
+    """Equal logits, whatever they are, are a uniform distribution: such a beam scores its own score less log V."""
+    big = torch.finfo(dtype)
+    x = torch.full((2, 2, V), {"lowest": big.min, "highest": big.max}.get(at, at), dtype=dtype)
+    x[:, 1] = torch.linspace(-4, 4, V).to(dtype)
+    x[1, 1] = x[1, 0]
+    x[0, 1, V // 2] = 24.0                           # that beam's own first token has nearly all of its probability
+    check(x, torch.tensor([[0.0, -1.0], [-2.0, -0.5]]))
+
+
+@pytest.mark.gpu
+def test_neighbours_at_large_magnitudes():
+    """Logits a few units in the last place apart, from 2^17 to 2^30: the gaps count."""
+    B, Kb, V = 14, 2, 3000
+    g = torch.Generator().manual_seed(6)
+    x = torch.empty(B, Kb, V)
+    for b in range(B):
+        base = 2.0 ** (17 + b) * (1 if b % 2 else -1)
+        step = 2.0 ** (17 + b - 23)
+        x[b] = base - step * torch.randint(1, 40, (Kb, V), generator=g).float()
+        x[b, :, 17 + b], x[b, :, 40 + b], x[b, :, 90 + b] = base, base - step, base
+    check(x, torch.tensor([[0.0, -0.37]]).repeat(B, 1))

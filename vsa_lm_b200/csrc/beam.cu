@@ -331,7 +331,10 @@ __global__ void __launch_bounds__(32 * kMaxK) select_group_kernel(const __grid_c
       if (c.x > neg_inf()) s += c.y * exp2f((c.x - m) * kLog2e);
     }
     s = warp_sum(s);
-    const float lse = m + logf(s);
+    // The log-sum-exp m + log s is rounded to 2^-18 or better for logits below 64, which also takes up in which order the
+    // sum was made (it goes by the row's alignment); larger ones would round log s away and are measured from m
+    const float log_s = logf(s), lse = m + log_s;
+    const bool from_m = !(fabsf(m) < 64.f);
     __syncwarp();
     // each lane walks the sorted lists of three chunks (at most 65 in all), their heads in registers; the order is (logit,
     // lowest index) as a pair of integers (x + 0 makes one of the two zeros; key 0 is the end of a list)
@@ -356,7 +359,7 @@ __global__ void __launch_bounds__(32 * kMaxK) select_group_kernel(const __grid_c
 #pragma unroll
       for (int j = 0; j < 3; ++j)
         if (key[j] == top && (uint32_t)head[j].v == win) {
-          const float sc = own + (head[j].x - lse);
+          const float sc = own + (from_m ? (head[j].x - m) - log_s : head[j].x - lse);
           c_score[k * K + n] = sc != sc ? neg_inf() : sc;
           c_token[k * K + n] = (int32_t)win;
           head[j] = ++at[j] < (lane + 32 * j + 1) * K ? all[at[j]] : Cand{neg_inf(), -1};
