@@ -1,14 +1,17 @@
 """Beam search's selection over logits that are masked with the type's lowest value, with large negative numbers,
-or lie at the ends of fp32's range.
+or lie at the ends of fp32's range; and selections of different sizes at once.
 
 The reference takes log_softmax as (x - max) - log(sum e^(x - max)) in 64 bits. Tolerance of a score: three fp32
 roundings of terms no larger than |s| + |x - max| + |log sum| (2^-22 of that), and 2e-6 for the logarithm of the sum.
 """
+import ctypes
 import math
+import threading
 
 import pytest
 import torch
 
+from vsa_lm_b200 import _lib
 from vsa_lm_b200 import kernels as K
 
 
@@ -91,3 +94,40 @@ def test_neighbours_at_large_magnitudes():
         x[b] = base - step * torch.randint(1, 40, (Kb, V), generator=g).float()
         x[b, :, 17 + b], x[b, :, 40 + b], x[b, :, 90 + b] = base, base - step, base
     check(x, torch.tensor([[0.0, -0.37]]).repeat(B, 1))
+
+
+@pytest.mark.gpu
+def test_selections_of_different_sizes_from_many_threads():
+    """Calls whose second kernel takes 43 or 133 KB of shared memory, from eight host threads that do nothing else."""
+    lib = _lib.load()
+    failed = []
+
+    def work(i):
+        try:
+            select_often(i, 524288 if i % 2 else 170000)
+        except Exception as e:
+            failed.append(repr(e))
+
+    def select_often(i, V):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            x = torch.randn(16, V, generator=torch.Generator().manual_seed(i)).cuda()
+            s = torch.linspace(0, -5, 16, device="cuda").view(1, 16)
+            first = K.beam_select(x, s)
+            out = tuple(torch.empty_like(t) for t in first)
+            nbytes = lib.bolt3_beam_select_workspace(1, 16, V)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+            a = _lib.BeamSelectArgs(B=1, K=16, V=V, logits=x.data_ptr(), row_stride=V, logits_fp32=1, scores=s.data_ptr(),
+                                    out_scores=out[0].data_ptr(), out_parent=out[1].data_ptr(), out_token=out[2].data_ptr(),
+                                    out_finished=out[3].data_ptr(), workspace=ws.data_ptr(), workspace_bytes=nbytes)
+            at, stream = ctypes.byref(a), torch.cuda.current_stream().cuda_stream
+            rc = [lib.bolt3_beam_select(at, stream) for _ in range(3000)]
+            torch.cuda.current_stream().synchronize()
+            if any(rc) or not all(torch.equal(p, q) for p, q in zip(first, out)):
+                failed.append((V, sum(map(bool, rc))))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed

@@ -39,7 +39,8 @@ constexpr int kChunk = kSelThreads * kPerThread;      // logits of a block
 template <bool FP32>
 constexpr int kSelBlocks = FP32 ? 5 : 10;             // of an SM
 constexpr int kListCap = 256;                         // candidates at or above the threshold
-constexpr int64_t kMaxV = 64 * kChunk;             // (with a slip a row may have 65 chunks)
+constexpr int64_t kMaxV = 64 * kChunk;
+constexpr int kMaxChunks = 65;                        // of a row, which may begin after a 16-byte boundary
 
 struct Cand {
   float x;
@@ -578,9 +579,11 @@ extern "C" int bolt3_beam_select(const bolt3_beam_select_args* a, void* stream) 
   if (launch_overlapped(a->logits_fp32 ? select_chunk_kernel<true> : select_chunk_kernel<false>, grid, dim3(kSelThreads), 0,
                         s, p) != cudaSuccess)
     return BOLT3_ERR_CUDA;
+  // the limit is the largest call's, not this one's: it is the kernel's, and another thread may set it before this launch
   const size_t smem = (size_t)a->K * p.n_chunks * a->K * sizeof(Cand);
   if (smem > 40 * 1024 &&
-      cudaFuncSetAttribute(select_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+      cudaFuncSetAttribute(select_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           (int)(kMaxK * kMaxK * kMaxChunks * sizeof(Cand))) != cudaSuccess)
     return BOLT3_ERR_CUDA;
   return launch_overlapped(select_group_kernel, dim3((unsigned)a->B), dim3(32 * a->K), smem, s, p) == cudaSuccess
              ? BOLT3_OK : BOLT3_ERR_CUDA;
