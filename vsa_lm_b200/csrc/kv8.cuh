@@ -7,6 +7,12 @@ namespace kv8 {
 
 constexpr float kScaleFloor = 0x1p-40f;
 
+// The weights of the attention kernels are 2^(u - M) in f16, whose range is 2^-24 .. 2^15. M is set 2^7 below the largest u
+// seen and moves only when a weight would pass 2^15, so that the usual step has no rescaling. A weight is then rounded to
+// 2^-11 of itself or to within 2^-32 of the largest one, whichever is more. (With M at the largest, what lies below 2^-25 of
+// it was lost from the numerator: many thousand such keys are a visible share of the output.)
+constexpr float kHeadroom = 7.f, kMostWeight = 15.f;
+
 // Rows sequence b holds before the call, or -1 for an idle one. `bad` is set for a length that is
 // neither idle nor leaves room for T rows.
 struct Length {

@@ -6,10 +6,10 @@
 // bound on the u_j seen so far, numerator sum w_j v8_j, denominator sum w_j / scale_v[j]. So the f16 weights
 // of the product are relative to the largest weighted value, however far the scales of two tokens lie apart.
 // A weight more than 2^126 below the bound is zero in both sums; that matters only where two tokens' value scales
-// lie more than 2^100 apart. Sums and the outputs are fp32. Roundings: w_j to f16 (2^-11 relative) for the product
-// with the int8 values, which f16 holds exactly; a query row to 16-bit integers, relative to its largest value
-// (2^-16 of it; bf16 has already rounded that value to 2^-9), as q = 256 hi + lo, so that q . k8 is two int8
-// products summed exactly.
+// lie more than 2^100 apart. Sums and the outputs are fp32. Roundings: w_j to f16 (2^-11 relative, or 2^-32 of the
+// largest weighted value: kHeadroom) for the product with the int8 values, which f16 holds exactly; a query row to
+// 16-bit integers, relative to its largest value (2^-16 of it; bf16 has already rounded that value to 2^-9), as
+// q = 256 hi + lo, so that q . k8 is two int8 products summed exactly.
 //
 // Bound by HBM: 2 (HD + 4) bytes per key and KV head. The cache is read in blocks of 32 keys, for 8 or 16 query
 // rows at once (T * G of them, token-major; more rows: more passes). All blocks of all (sequence, KV head)s are
@@ -44,7 +44,6 @@ using namespace kv8;
 constexpr uint32_t kWaitIters = 1u << 24;
 constexpr int kBlock = 32;      // keys of a block: two 16-key halves of the products
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kSlack = 8.f;   // a weight may exceed its bound by 2^8 before the bound moves: f16 holds 2^15
 
 template <int NT>
 constexpr int kWarps = NT == 1 ? 12 : 8;        // one CTA per SM; 168 or 255 registers a thread
@@ -381,14 +380,14 @@ B3_DEV void walk(const Params& p, RingState& rs, int b, int kvh, int64_t s, int 
         }
       }
     }
-    // the bounds move only when a weight would pass 2^8 (and at the first key a row sees)
+    // the bounds move only when a weight would pass 2^15 (and at the first key a row sees)
     bool over = false;
     float m0[NT], m1[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       m0[n] = fmaxf(fmaxf(t[0][n][0], t[0][n][2]), fmaxf(t[1][n][0], t[1][n][2]));
       m1[n] = fmaxf(fmaxf(t[0][n][1], t[0][n][3]), fmaxf(t[1][n][1], t[1][n][3]));
-      over |= m0[n] > f.M0[n] + kSlack || m1[n] > f.M1[n] + kSlack;
+      over |= m0[n] > f.M0[n] + kMostWeight || m1[n] > f.M1[n] + kMostWeight;
     }
     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
@@ -398,8 +397,8 @@ B3_DEV void walk(const Params& p, RingState& rs, int b, int kvh, int64_t s, int 
           m0[n] = fmaxf(m0[n], __shfl_xor_sync(0xffffffffu, m0[n], x));
           m1[n] = fmaxf(m1[n], __shfl_xor_sync(0xffffffffu, m1[n], x));
         }
-        m0[n] = fmaxf(f.M0[n], m0[n]);
-        m1[n] = fmaxf(f.M1[n], m1[n]);
+        m0[n] = fmaxf(f.M0[n], m0[n] - kHeadroom);
+        m1[n] = fmaxf(f.M1[n], m1[n] - kHeadroom);
         const float f0 = f.M0[n] == neg_inf() ? 0.f : ex2(f.M0[n] - m0[n]), f1 = f.M1[n] == neg_inf() ? 0.f : ex2(f.M1[n] - m1[n]);
         f.M0[n] = m0[n];
         f.M1[n] = m1[n];

@@ -14,7 +14,7 @@
 //   arithmetic in packed pairs. A warp takes 16 TMEM lanes in the 16x256b layout, a thread 16 of the 64 keys of two rows:
 //   what belongs to a key (its scales) is then read from shared memory once for two rows, where a thread per row, all
 //   lanes reading the same address, took twice the shared-memory time of the MMAs; and with four such warps on a
-//   scheduler one's latencies are filled by the others. The bound M moves only when a weight would pass 2^8; only then
+//   scheduler one's latencies are filled by the others. The bound M moves only when a weight would pass 2^15; only then
 //   are the sums in TMEM rescaled.
 // While one tile's softmax runs, the tensor cores work on the other tile. With few heads the keys are split over CTAs,
 // whose partial sums a second kernel joins.
@@ -46,7 +46,6 @@ template <int N>
 B3_DEV void fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
 constexpr uint32_t kWaitIters = 1u << 24;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kSlack = 8.f;
 
 struct Params {
   bolt3_kv8_attend_args a;
@@ -437,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             }
           }
         }
-        // the bounds move only when a weight would pass 2^8 (and at the first key)
+        // the bounds move only when a weight would pass 2^15 (and at the first key)
         float m[2];
         bool over = false;
 #pragma unroll
@@ -445,14 +444,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
           m[q] = fmaxf(t[q][0].x, t[q][0].y);
 #pragma unroll
           for (int n = 1; n < 8; ++n) m[q] = max3(m[q], t[q][n].x, t[q][n].y);
-          over |= m[q] > M[q] + kSlack;
+          over |= m[q] > M[q] + kMostWeight;
         }
         if (__any_sync(0xffffffffu, over)) {
           float f[2];
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             m[q] = quad_max(m[q]);
-            const float to_M = m[q] > M[q] + kSlack ? m[q] : M[q];
+            const float to_M = m[q] > M[q] + kMostWeight ? m[q] - kHeadroom : M[q];
             f[q] = M[q] == neg_inf() ? 0.f : ex2(M[q] - to_M);    // 1 where the bound stays
             M[q] = to_M;
             l[q] = mul2(l[q], pair(f[q], f[q]));
