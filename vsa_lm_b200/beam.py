@@ -52,6 +52,7 @@ def expand_beams(model, states, kv_caches, beams: int):
                 new.bank[k].copy_(_repeat(t, 0, c.HKV, beams))
         new.slot_pos, new.cur_slot, new.cur_len = list(c.slot_pos), c.cur_slot, c.cur_len
         new.prev_slot, new.sinks_set, new.n_filled = c.prev_slot, c.sinks_set, c.n_filled
+        new.status.word.copy_(c.status.word)      # an error of the kernels that made this state
         if c.big_prev is not None:
             new.big_prev = {k: _repeat(t, 0, c.HKV, beams) if isinstance(t, torch.Tensor) else t
                             for k, t in c.big_prev.items()}

@@ -591,10 +591,11 @@ class Bolt3Decoder:
     @staticmethod
     def check_status(kv_caches, block: bool = True) -> None:
         """Raise RuntimeError if a kernel of an earlier step reported an error (an expired bounded
-        wait or a failed bounds check). Steps already check at every chunk boundary."""
+        wait or a failed bounds check): with block, any kernel launched so far. Steps already check at
+        every chunk boundary."""
         for st in kv_caches:
             if isinstance(st, Bolt3LayerState):
-                st.status.check(block)
+                st.status.settle("Bolt-3 decode steps") if block else st.status.check(block)
             elif isinstance(st, AnchorKV8):
                 st.check_status(block)
 
@@ -1250,10 +1251,11 @@ class AnchorKV8:
         """Raise RuntimeError if a kernel of an earlier step reported an error (block=False: only if the copy
         asked for by the last such call has arrived with one)."""
         if self.status is not None:
-            self.status.check(block)
-            self.status.arm("8-bit anchor cache")
             if block:
-                self.status.check(True)
+                self.status.settle("8-bit anchor cache")
+            else:
+                self.status.check(False)
+                self.status.arm("8-bit anchor cache")
 
     @property
     def capacity(self) -> int:
@@ -1293,10 +1295,14 @@ class AnchorKV8:
             self.data, self.scale = data, scale
 
     def repeated(self, times: int) -> "AnchorKV8":
-        """A copy whose sequences are this cache's, each `times` times in a row."""
+        """A copy whose sequences are this cache's, each `times` times in a row (an error that its kernels
+        reported is the copy's too)."""
         new = AnchorKV8.__new__(AnchorKV8)
         new.data, new.scale = (t.repeat_interleave(times, dim=1) for t in (self.data, self.scale))
-        new.n, new.status = self.n, K.DeviceStatus(self.data.device) if self.data.is_cuda else None
+        new.n, new.status = self.n, None
+        if self.status is not None:
+            new.status = K.DeviceStatus(self.data.device)
+            new.status.word.copy_(self.status.word)
         return new
 
     def attention(self, ly, h: torch.Tensor, pos_start: int, dev_pos: "K.DevicePosition | None" = None) -> torch.Tensor:

@@ -153,6 +153,12 @@ class DeviceStatus:
             why = "; ".join(msg for b, msg in _lib.DEVICE_STATUS_BITS.items() if bits & b) or "unknown bits"
             raise RuntimeError(f"{self.what}: device status {bits:#x} ({why}); the outputs of that call are invalid")
 
+    def settle(self, what: str) -> None:
+        """Wait for every kernel launched with this status so far and raise if one reported an error."""
+        self.check(block=True)
+        self.arm(what)
+        self.check(block=True)
+
 
 def prep(proj: torch.Tensor, *, B: int, T: int, H: int, HKV: int, HD: int, inv_freq: torch.Tensor,
          eps: float, q_norm_w: torch.Tensor | None, k_norm_w: torch.Tensor | None, pos0: int,
