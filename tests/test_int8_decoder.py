@@ -2,6 +2,8 @@
 
 The errors are made on the host: a status word is set as a kernel would set it. No kernel fails here.
 """
+import copy
+
 import pytest
 import torch
 
@@ -46,3 +48,71 @@ def test_beam_search_reports_errors_of_its_prompt(kind):
     _fail_prefill(dec, kind)
     with pytest.raises(RuntimeError, match="bounded wait"):
         dec.beam_search(ids, 2, 3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("graphs", [True, False])
+@pytest.mark.parametrize("call", ["generate_batch", "generate", "continue_generate"])
+def test_generation_reports_errors_of_the_anchors(call, graphs):
+    """The last tokens' too: fewer than a chunk are generated."""
+    mcfg, dec = _decoder(cuda_graphs=graphs)
+    ids = _ids(mcfg, 1, 40)
+    if call == "continue_generate":
+        _, states, kv = dec.prefill(ids)
+        more = _ids(mcfg, 1, 5, 2)
+        _, states, kv, pos = dec.continue_generate(more, states, kv, 40, 3)
+        _anchor(kv).status.word.fill_(2)
+        with pytest.raises(RuntimeError, match="bounded wait"):
+            dec.continue_generate(more, states, kv, pos, 3)
+        return
+    getattr(dec, call)(ids, 3, temperature=0.0)
+    _fail_prefill(dec, AnchorKV8)
+    with pytest.raises(RuntimeError, match="bounded wait"):
+        getattr(dec, call)(ids, 3, temperature=0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("graphs", [True, False])
+def test_steps_report_errors_of_the_anchors(graphs):
+    """A caller's own loop of steps hears of an error within two chunks of tokens."""
+    mcfg, dec = _decoder()
+    ids = _ids(mcfg, 2, 40)
+    h, states, kv = dec.prefill(ids)
+    runner = dec.step_graph(states, kv) if graphs else None
+    tok = _ids(mcfg, 2, 1, 3)
+
+    def step(i):
+        runner.step(tok, 40 + i) if graphs else dec.step(tok, 40 + i, states, kv)
+
+    for i in range(10):
+        step(i)
+    _anchor(kv).status.word.fill_(2)
+    with pytest.raises(RuntimeError, match="bounded wait"):
+        for i in range(10, 10 + 2 * dec.C):
+            step(i)
+    if runner is not None:
+        runner.close()
+
+
+@pytest.mark.gpu
+def test_prompt_slices_report_errors_of_the_anchors():
+    mcfg, dec = _decoder()
+    _, states, kv = dec.prefill(_ids(mcfg, 1, 128))
+    _anchor(kv).status.word.fill_(8)
+    more = _ids(mcfg, 1, 128, 4)
+    with pytest.raises(RuntimeError, match="outside the range"):
+        for i in range(3):
+            dec.step(more, 128 * (i + 1), states, kv)
+
+
+@pytest.mark.gpu
+def test_copied_states_keep_their_errors():
+    mcfg, dec = _decoder()
+    _, states, kv = dec.prefill(_ids(mcfg, 1, 150))       # past a chunk: a status copy is under way
+    clean = copy.deepcopy(_anchor(kv))
+    _anchor(kv).status.word.fill_(2)
+    spoiled = copy.deepcopy(_anchor(kv))
+    clean.check_status()
+    for c in (spoiled, _anchor(kv)):
+        with pytest.raises(RuntimeError, match="bounded wait"):
+            c.check_status()

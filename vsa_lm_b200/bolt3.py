@@ -599,6 +599,11 @@ class Bolt3Decoder:
             elif isinstance(st, AnchorKV8):
                 st.check_status(block)
 
+    @staticmethod
+    def _check_anchors(kv_caches) -> None:
+        """check_status of the 8-bit anchor caches alone, at the end of a generation."""
+        Bolt3Decoder.check_status([c for c in kv_caches if isinstance(c, AnchorKV8)])
+
     # ---- decode state in the reference's format (bolt3.py:302-319 creates it, :343-425 fills it):
     # per Bolt-3 layer a dict with the bank (ak/av [b*HKV, S, HD], mass/util/pm fp32 [b*HKV, S], act
     # bool, n_filled), the sinks [b, HKV, 4, HD], and the previous / current chunk windows
@@ -984,6 +989,8 @@ class Bolt3Decoder:
         for li, blk in enumerate(self.model.blocks):
             if hasattr(blk, "vsa"):
                 self._layer_advance(blk.vsa, kv_caches[li], t, pos_start, states[li])
+            elif isinstance(kv_caches[li], AnchorKV8):
+                kv_caches[li].advance(t)
             else:
                 kv_caches[li].n += t
 
@@ -1072,6 +1079,7 @@ class Bolt3Decoder:
             logits = self.model.lm_head(h[:, -1, :])
         if runner is not None:
             runner.close()
+        self._check_anchors(kv)
         return torch.cat(toks, dim=1), lengths
 
     def beam_search(self, ids: torch.Tensor, beams: int, max_new_tokens: int, eos_ids=()):
@@ -1112,6 +1120,7 @@ class Bolt3Decoder:
             pos += 1
         if runner is not None:
             runner.close()
+        self._check_anchors(kv_caches)
         out = torch.cat(toks, dim=1) if toks else torch.empty(ids.shape[0], 0, dtype=torch.long, device=ids.device)
         return out, states, kv_caches, pos
 
@@ -1239,6 +1248,8 @@ class AnchorKV8:
     csrc/kv8_attend.cu); `k` and `v` read the held tokens back as bf16 copies. GPU only. The capacity is
     max_kv_len rounded up to a multiple of 256 tokens and doubles when an append does not fit."""
 
+    CHECK_TOKENS = 128
+
     def __init__(self, B: int, HKV: int, Tmax: int, HD: int, dev):
         cap = max(256, -(-int(Tmax) // 256) * 256)
         self.data = torch.empty(2, B, HKV, cap, HD, device=dev, dtype=torch.int8)
@@ -1294,6 +1305,15 @@ class AnchorKV8:
             scale[:, :, :, :self.n].copy_(self.scale[:, :, :, :self.n])
             self.data, self.scale = data, scale
 
+    def advance(self, t: int) -> None:
+        """t more tokens are held. At every CHECK_TOKENS of them an error of the kernels before the last such
+        point is raised (their status copy finished long ago), as the Bolt-3 layers do at a chunk's end."""
+        chunks = self.n // self.CHECK_TOKENS
+        self.n += t
+        if self.status is not None and self.n // self.CHECK_TOKENS != chunks:
+            self.status.check(block=True)
+            self.status.arm(f"8-bit anchor cache at {self.n} tokens")
+
     def repeated(self, times: int) -> "AnchorKV8":
         """A copy whose sequences are this cache's, each `times` times in a row (an error that its kernels
         reported is the copy's too)."""
@@ -1322,7 +1342,7 @@ class AnchorKV8:
         y = K.kv8_attend(q=q, data=self.data, scale=self.scale, n=self.n, sm_scale=ly.HD ** -0.5, status=self.status,
                          dev_pos=dev_pos)
         if dev_pos is None:
-            self.n += t
+            self.advance(t)
         return y
 
 

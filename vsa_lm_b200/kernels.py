@@ -153,6 +153,12 @@ class DeviceStatus:
             why = "; ".join(msg for b, msg in _lib.DEVICE_STATUS_BITS.items() if bits & b) or "unknown bits"
             raise RuntimeError(f"{self.what}: device status {bits:#x} ({why}); the outputs of that call are invalid")
 
+    def __deepcopy__(self, memo) -> "DeviceStatus":
+        """A word of its own with the same bits (an event, and with it a copy under way, cannot be copied)."""
+        new = memo[id(self)] = DeviceStatus(self.word.device)
+        new.word.copy_(self.word)
+        return new
+
     def settle(self, what: str) -> None:
         """Wait for every kernel launched with this status so far and raise if one reported an error."""
         self.check(block=True)
