@@ -116,3 +116,18 @@ def test_copied_states_keep_their_errors():
     for c in (spoiled, _anchor(kv)):
         with pytest.raises(RuntimeError, match="bounded wait"):
             c.check_status()
+
+
+@pytest.mark.gpu
+def test_beam_search_pads_with_the_first_of_its_ids():
+    mcfg, dec = _decoder()
+    ids = _ids(mcfg, 1, 40)
+    h, _, _ = dec.prefill(ids)
+    best = int(dec.model.lm_head(h[:, -1]).argmax())
+    first = best + 1 if best + 1 < mcfg["vocab_size"] else best - 1
+    for eos in ((max(best, first), min(best, first)), [min(best, first), max(best, first)]):
+        toks, _, lengths = dec.beam_search(ids, 1, 20, eos_ids=eos)
+        end = int(lengths[0, 0])
+        assert end < toks.shape[2] and int(toks[0, 0, end - 1]) in eos and bool((toks[0, 0, end:] == eos[0]).all())
+    toks, _, lengths = dec.beam_search(ids, 1, 20, eos_ids={best, first})       # a set has no first: the lowest
+    assert bool((toks[0, 0, int(lengths[0, 0]):] == min(best, first)).all())

@@ -112,11 +112,11 @@ def beam_search(dec, ids: torch.Tensor, beams: int, max_new_tokens: int, eos_ids
     """The `beams` best continuations of every row of ids [B, T] by the sum of their tokens' log
     probabilities, up to max_new_tokens tokens each or through the first of `eos_ids`. Returns (tokens
     [B, beams, n], scores fp32 [B, beams], lengths [B, beams]), best first; positions past a length hold
-    eos_ids[0]. A finished beam keeps its score and its place among the beams. Stops early once all beams
-    have finished (looked at every 16 tokens)."""
+    eos_ids[0] (of a set, which has no order, the lowest). A finished beam keeps its score and its place
+    among the beams. Stops early once all beams have finished (looked at every 16 tokens)."""
     if beams < 1 or beams > 16 or max_new_tokens < 1:
         raise ValueError(f"{beams} beams and {max_new_tokens} tokens: 1 to 16 beams, at least one token")
-    eos = tuple(sorted(int(e) for e in eos_ids))
+    eos = tuple(int(e) for e in (sorted(eos_ids) if isinstance(eos_ids, (set, frozenset)) else eos_ids))
     B, T = ids.shape
     dev = ids.device
     h, states, kv = dec.prefill(ids, max_kv_len=T + max_new_tokens + 64)
