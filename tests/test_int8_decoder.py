@@ -1,4 +1,5 @@
-"""A decoder with 8-bit anchor caches: errors that its kernels report on the device reach the caller.
+"""A decoder with 8-bit anchor caches: errors that its kernels report on the device reach the caller, a beam search
+pads with the id it was given first, and models that it cannot serve are refused when it is made.
 
 The errors are made on the host: a status word is set as a kernel would set it. No kernel fails here.
 """
@@ -131,3 +132,20 @@ def test_beam_search_pads_with_the_first_of_its_ids():
         assert end < toks.shape[2] and int(toks[0, 0, end - 1]) in eos and bool((toks[0, 0, end:] == eos[0]).all())
     toks, _, lengths = dec.beam_search(ids, 1, 20, eos_ids={best, first})       # a set has no first: the lowest
     assert bool((toks[0, 0, int(lengths[0, 0]):] == min(best, first)).all())
+
+
+def test_models_that_8_bit_caches_cannot_serve_are_refused_at_once():
+    def model(**kw):
+        cfg = dict(vocab_size=32, dim=64, num_layers=1, num_heads=2, num_kv_heads=1, head_dim=64, intermediate=64,
+                   layer_types=["softmax"])
+        return Bolt3LM(**{**cfg, **kw})
+
+    Bolt3Decoder(model(), kv_cache="int8")
+    Bolt3Decoder.blank_state(model(num_heads=16), 1, "cpu", kv_cache="int8")
+    for bad in (model(head_dim=32), model(head_dim=96), model(num_heads=17), model(num_heads=34, num_kv_heads=2)):
+        Bolt3Decoder(bad)                                        # bf16 caches hold them
+        Bolt3Decoder.blank_state(bad, 1, "cpu")
+        with pytest.raises(ValueError, match="8-bit"):
+            Bolt3Decoder(bad, kv_cache="int8")
+        with pytest.raises(ValueError, match="8-bit"):
+            Bolt3Decoder.blank_state(bad, 1, "cpu", kv_cache="int8")

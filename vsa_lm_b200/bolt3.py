@@ -546,7 +546,7 @@ class Bolt3Decoder:
     def __init__(self, model, wrap_positions: bool = False, max_cache_pos: int = 65536, cuda_graphs: bool = True,
                  kv_cache: str = "bf16", **kwargs):
         self.model = model.eval()
-        _check_kv_cache(kv_cache)
+        _check_kv_cache(kv_cache, model)
         self.kv_cache = kv_cache          # the anchors' caches: "bf16" (as the reference) or "int8" (AnchorKV8)
         self.max_T = model.config["max_T"]
         self.max_cache_pos = max_cache_pos
@@ -574,7 +574,7 @@ class Bolt3Decoder:
         M_res [B, HKV, HD, HD] in states and a Bolt3LayerState in kv_caches; per softmax anchor an
         AnchorKV (kv_cache "int8": an AnchorKV8) with room for max_kv_len tokens. M_res is always fp32 (the
         kernels update it in place)."""
-        _check_kv_cache(kv_cache)
+        _check_kv_cache(kv_cache, model)
         states, kv_caches = [], []
         for blk in model.blocks:
             if hasattr(blk, "vsa"):
@@ -1157,9 +1157,16 @@ class Bolt3Decoder:
         return states
 
 
-def _check_kv_cache(kind: str) -> None:
+def _check_kv_cache(kind: str, model=None) -> None:
+    """`kind` is a kind of cache and, with a model, one whose kernels serve the model's anchors."""
     if kind not in ("bf16", "int8"):
         raise ValueError(f"kv_cache must be 'bf16' or 'int8', got {kind!r}")
+    if kind == "int8" and model is not None:
+        for blk in model.blocks:
+            a = getattr(blk, "attn", None)
+            if a is not None and (a.HD not in (64, 128) or a.H % a.HKV or a.H // a.HKV > 16 or a.H + 2 * a.HKV > 4096):
+                raise ValueError(f"8-bit caches hold heads of 64 or 128, at most 16 query heads to a KV head, got "
+                                 f"{a.H} on {a.HKV} of {a.HD}; use kv_cache='bf16'")
 
 
 def _fp32_weight(norm: "LlamaRMSNorm", device) -> torch.Tensor:
