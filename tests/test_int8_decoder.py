@@ -149,3 +149,19 @@ def test_models_that_8_bit_caches_cannot_serve_are_refused_at_once():
             Bolt3Decoder(bad, kv_cache="int8")
         with pytest.raises(ValueError, match="8-bit"):
             Bolt3Decoder.blank_state(bad, 1, "cpu", kv_cache="int8")
+
+
+def test_scales_of_rows_without_a_token_are_zero():
+    """Whatever the memory held: torch fills new memory with NaN here."""
+    torch.use_deterministic_algorithms(True)
+    try:
+        assert torch.utils.deterministic.fill_uninitialized_memory and bool(torch.empty(3).isnan().all())
+        c = AnchorKV8(2, 3, 100, 64, "cpu")
+        assert bool((c.scale == 0).all())
+        c.scale.uniform_()
+        c.n = 250
+        c.reserve(7)
+        assert c.capacity == 512 and bool((c.scale[:, :, :, 250:] == 0).all())
+        assert torch.equal(c.repeated(2).scale[:, 3], c.scale[:, 1])
+    finally:
+        torch.use_deterministic_algorithms(False)

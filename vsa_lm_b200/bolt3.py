@@ -1260,7 +1260,8 @@ class AnchorKV8:
     def __init__(self, B: int, HKV: int, Tmax: int, HD: int, dev):
         cap = max(256, -(-int(Tmax) // 256) * 256)
         self.data = torch.empty(2, B, HKV, cap, HD, device=dev, dtype=torch.int8)
-        self.scale = torch.empty(2, B, HKV, cap, device=dev, dtype=torch.float32)
+        # zeros: a scale of a row that holds no token yet is a number too, so that copies of a cache compare equal
+        self.scale = torch.zeros(2, B, HKV, cap, device=dev, dtype=torch.float32)
         self.n = 0
         # status word of this cache's kernels (an expired wait, a device position out of range)
         self.status = K.DeviceStatus(dev) if self.data.is_cuda else None
@@ -1307,7 +1308,7 @@ class AnchorKV8:
             while cap < self.n + L:
                 cap *= 2
             data = self.data.new_empty(*self.data.shape[:3], cap, self.data.shape[4])
-            scale = self.scale.new_empty(*self.scale.shape[:3], cap)
+            scale = self.scale.new_zeros(*self.scale.shape[:3], cap)
             data[:, :, :, :self.n].copy_(self.data[:, :, :, :self.n])
             scale[:, :, :, :self.n].copy_(self.scale[:, :, :, :self.n])
             self.data, self.scale = data, scale
