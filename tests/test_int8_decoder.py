@@ -165,3 +165,47 @@ def test_scales_of_rows_without_a_token_are_zero():
         assert torch.equal(c.repeated(2).scale[:, 3], c.scale[:, 1])
     finally:
         torch.use_deterministic_algorithms(False)
+
+
+def _edit(model, how, factor):
+    for blk in model.blocks:
+        if not hasattr(blk, "vsa"):
+            for norm in (blk.attn.q_norm, blk.attn.k_norm):
+                w = norm.weight
+                if how == "data":
+                    w.data.mul_(factor)                       # no version of the parameter changes
+                elif how == "in place":
+                    with torch.no_grad():
+                        w.mul_(factor)
+                else:
+                    norm.weight = torch.nn.Parameter(w.detach() * factor)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how,graphs", [("data", True), ("data", False), ("in place", True), ("in place", False),
+                                        ("replaced", False)])
+def test_edited_norm_weights_are_used_at_once(how, graphs):
+    """An edit between two steps, in eager steps and (edits that keep the parameter's memory) in a captured graph."""
+    mcfg, dec = _decoder("small_lm")
+    ids, tok = _ids(mcfg, 1, 130), _ids(mcfg, 1, 1, 2)
+
+    def run(factor_before, factor_between):
+        _, states, kv = dec.prefill(ids)
+        runner = dec.step_graph(states, kv) if graphs else None
+        step = lambda i: runner.step(tok, 130 + i) if graphs else dec.step(tok, 130 + i, states, kv)
+        _edit(dec.model, how, factor_before)
+        step(0)
+        _edit(dec.model, how, factor_between)
+        step(1)
+        c = _anchor(kv)
+        rows = [t[:, :, :, 130:132].clone() for t in (c.data, c.scale)]
+        _edit(dec.model, how, 1.0 / (factor_before * factor_between))
+        if runner is not None:
+            runner.close()
+        return rows
+
+    plain, edited = run(1.0, 1.0), run(1.0, 2.0)
+    for a, b in zip(plain, edited):
+        assert torch.equal(a[..., 0, :] if a.dim() == 5 else a[..., 0], b[..., 0, :] if b.dim() == 5 else b[..., 0])
+    # twice the weights: the key's scale doubles, exactly
+    assert torch.equal(edited[1][0, ..., 1], 2 * plain[1][0, ..., 1]) and torch.equal(edited[0], plain[0])

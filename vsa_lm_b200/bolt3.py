@@ -1170,15 +1170,9 @@ def _check_kv_cache(kind: str, model=None) -> None:
 
 
 def _fp32_weight(norm: "LlamaRMSNorm", device) -> torch.Tensor:
-    """A norm's weight as a contiguous fp32 tensor on `device`, kept between calls (made again when the
-    parameter is replaced or changed in place)."""
-    t = norm.weight
-    key = (t.data_ptr(), t._version, t.dtype, str(torch.device(device)))
-    cached = getattr(norm, "_fp32_cache", None)
-    if cached is None or cached[0] != key:
-        cached = (key, t.detach().to(device=device, dtype=torch.float32).contiguous())
-        norm._fp32_cache = cached
-    return cached[1]
+    """A norm's weight as a contiguous fp32 tensor on `device`: the parameter itself where it is one, else converted
+    at every call (in a captured step: at every replay), so that no edit of the parameter goes unseen."""
+    return norm.weight.detach().to(device=device, dtype=torch.float32).contiguous()
 
 
 def _fp32_inv_freq(rope: "LlamaRoPE", device) -> torch.Tensor:
