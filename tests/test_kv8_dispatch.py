@@ -115,3 +115,12 @@ def test_device_position_in_runs_and_splits(B, T, H, HKV, HD, n):
     assert K._attend_workspace(B, T, H, HKV, HD, n) > 0
     y = K.kv8_attend(q=q.cuda(), data=data.cuda(), scale=scale.cuda(), n=n, dev_pos=pos).cpu()
     base.check_attend(q, data, scale, n + 33, None, HD ** -0.5, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [
+    (3, 1, 8, 2, 128, 10, 400, (399, -1, 77)),       # a block per head
+    (2, 60, 4, 2, 64, 10, 900, (840, 3)),            # prompt kernel
+])
+def test_lengths_above_the_expected_one(case):
+    check(*case)
