@@ -256,8 +256,9 @@ int bolt3_kv8_read(const bolt3_kv8_read_args* a, void* stream);
 /* Softmax attention of the T newest tokens (already appended) over the cache: query t of sequence b sees
  * rows 0 .. s_b + t. q: bf16, head h of token t of sequence b at q + b * q_sb + t * q_st + h * HD; y: bf16
  * [B][T][H][HD], rounded once, not overlapping q; 0 for an idle sequence. Query values below 2^100 in magnitude
- * (the products with the int8 keys are summed in fp32; a NaN or an infinity spoils its own row). H a multiple of
- * HKV, G = H / HKV <= 16, T * G <= 2^24. With `lens`, n <= cap is the longest length to expect (it sizes the split
+ * (the products with the int8 keys are summed in fp32; a NaN or an infinity spoils its own row). Up to T * G = 32 a
+ * query value is rounded to 2^-16 of its row's largest. Softmax weights are rounded to 2^-11 of themselves, or to 2^-32 of
+ * the largest weighted value. H a multiple of HKV, G = H / HKV <= 16, T * G <= 2^24. With `lens`, n <= cap is the longest length to expect (it sizes the split
  * of the cache, nothing else).
  * `workspace`: device memory of bolt3_kv8_attend_workspace(...) bytes, 16-byte aligned, used only
  * within the call (0 bytes: none needed). */

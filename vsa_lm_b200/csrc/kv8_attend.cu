@@ -741,8 +741,9 @@ Plan plan_of(int B, int T, int H, int HKV, int HD, int64_t n) {
   const int64_t warps = pl.nt == 1 ? kWarps<1> : kWarps<2>;
   const int64_t per_head = (n + T + kBlock - 1) / kBlock, blocks = heads * per_head;
   // A CTA per head where all are on the machine at once and a warp gets five blocks at most (32 query heads on 8, HD 128:
-  // one sequence of 1000 tokens 8.9 us against 10.9 in runs, of 2000 12.8 against 12.3, of 4000 20 against 11.8; 64
-  // sequences of 200 tokens, 512 heads, 22.5 against 17.1). Else every warp a run, of two blocks or more
+  // one sequence of 1000 tokens 9.0 us against 10.7 in runs, of 2000 13.4 against 12.4, of 4000 21.1 against 13.1; with
+  // 16 rows a head, of 800 13.3 against 14.3, of 1200 15.6 against 14.5; 64 sequences of 200 tokens, 512 heads, 25.3
+  // against 16.0). Else every warp a run, of two blocks or more
   int64_t runs = 0;
   if (heads * pl.tiles > 148 || per_head > 5 * warps) runs = blocks / 2 < 148 * warps ? blocks / 2 : 148 * warps;
   if (runs < 1 && heads * pl.tiles > 148) runs = 1;
@@ -801,8 +802,10 @@ bool encode_cache(CUtensorMap* m, const bolt3_kv8_attend_args* a) {
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Whether a call's rows go to the kernel for many rows, which works on tiles of 128 (64 sequences of 2304 tokens, 32 heads
-// on 8, HD 128: 32 rows of a head 168 us here against 239 there, 64 rows 333 against 239)
+// Whether a call's rows go to the kernel for many rows, which works on tiles of 128. Measured at 32 heads on 8, HD 128, 32 and
+// 48 rows of a head: 64 sequences of 2304 tokens 143 and 214 us here, 198 and 199 there; of 300 tokens 48 and 70, 51 and 51;
+// one sequence of 2304 18 and 22, 19 and 20. Not everywhere the better one: 16 sequences take 31 us here at 32 rows and 300
+// tokens, 13 there, 65 at 2304 tokens, 51 there
 bool many_rows(int T, int H, int HKV) { return (int64_t)T * (H / HKV) > 32; }
 
 bool shape_ok(int B, int T, int H, int HKV, int HD) {

@@ -19,8 +19,8 @@
 // While one tile's softmax runs, the tensor cores work on the other tile. With few heads the keys are split over CTAs,
 // whose partial sums a second kernel joins.
 //
-// Measured on a B200: 64 x 128 tokens after 2048, 32 heads on 8 of 128, 370 us (0.77 PFLOP/s; 173 us at the machine's
-// bf16 rate). A CTA is ready for its first scores after 6000 cycles, takes 5100 for a block of 128 keys (the MMAs of its
+// Measured on a B200: 64 x 128 tokens after 2048, 32 heads on 8 of 128, 370 to 385 us by the clock under load (0.77 to
+// 0.74 PFLOP/s; 173 us at the machine's bf16 rate). A CTA is ready for its first scores after 6000 cycles, takes 5100 for a block of 128 keys (the MMAs of its
 // two tiles 2048, their exponentials 2048) and 3700 for its output. The softmax warps bound it: 64 keys take them about
 // 1900 cycles, the four of a scheduler issuing half of the time, at 72 to 80 registers with little to overlap within a
 // warp. (Scores are waited for 900 cycles of a block, but bringing them earlier, 64 keys at a time into the columns that
