@@ -277,6 +277,86 @@ typedef struct bolt3_kv8_attend_args {
 int bolt3_kv8_attend(const bolt3_kv8_attend_args* a, void* stream);
 size_t bolt3_kv8_attend_workspace(int B, int T, int H, int HKV, int HD, int64_t n);
 
+/* ---- Paged bf16 KV cache of a softmax anchor layer, and its bound by accumulated attention weight. No counterpart in
+ * the reference, whose caches are one contiguous buffer that grows with the text (vsa_lm/decode.py:88-106).
+ * Layout: `pages` bf16 [2][n_pages][HKV][page][HD] (keys, then values); `table` int32 [B][width], rows `table_stride`
+ * elements apart: row r of sequence b is row r % page of page table[b][r / page]. page 16, 32, 64 or 128; HD 64 or 128;
+ * n_pages * HKV < 2^30. A sequence holds at most cap = width * page rows. Entries behind a sequence's last row are not
+ * read. An entry in use that is not in [0, n_pages) ORs 8 into `status`: nothing is written there, nothing read outside the
+ * pool, and the outputs of that call are invalid. Sequences may share pages that are only read; a page that a call writes must belong to one sequence.
+ * Records, one value per row and KV head: `weight` fp32 [B][HKV][cap], the softmax weight that the row got so far;
+ * `order` int32 [B][HKV][cap], the position of the row's token.
+ * Lengths as for the 8-bit cache: sequence b holds s_b rows before the call, s_b = n, or n + *pos_dev - pos_ref, or
+ * lens[b] (-1: idle). With `lens`, n is a bound: a length above it makes its sequence idle and ORs 8 into `status`, as one
+ * that leaves no room in the table does. Pointers 16-byte aligned (table, lens and pos: 4). */
+
+/* T new tokens of every sequence into the pages: per-head RMSNorm of q and k (optional), rotate-half RoPE of q and k
+ * (optional) at position pos0 + (s_b - n) + t, or pos[b] + t where `pos` (device int32 [B], with `lens`) is given: of a
+ * cache that dropped rows the position is not the row. q rounded once to q_out (0 for an idle sequence), k once to its page,
+ * v as it is. fp32; the angle is position * inv_freq to fp32's precision of the turn, however far the position. `weight`
+ * and `order` (both or none) of the new rows become 0 and the position. q, k, v as in bolt3_kv8_append. H + 2 HKV <= 4096. */
+typedef struct bolt3_paged_append_args {
+  int B, T, H, HKV, HD;
+  const void* q; const void* k; const void* v;
+  int64_t q_sb, q_st, k_sb, k_st, v_sb, v_st;
+  const float* q_norm_w; const float* k_norm_w; float eps;
+  const float* inv_freq;
+  void* q_out;                         /* bf16 [B][T][H][HD] */
+  void* pages; int64_t n_pages; int page;
+  const int32_t* table; int64_t table_stride, width;
+  float* weight; int32_t* order;       /* optional */
+  int64_t n; int64_t pos0;
+  const int32_t* lens; const int32_t* pos;
+  int32_t* status;                     /* optional */
+  const int64_t* pos_dev; int64_t pos_ref; int64_t pos_span;
+} bolt3_paged_append_args;
+int bolt3_paged_append(const bolt3_paged_append_args* a, void* stream);
+
+/* Softmax attention of the T newest tokens (already appended) over the pages: query t of sequence b sees rows
+ * 0 .. s_b + t. q and y as in bolt3_kv8_attend. Scores, sums and the running maximum in fp32; the softmax weights enter the
+ * product with the values as two bf16 terms (up to T * G = 32), or rounded to bf16. With `weight`, every row's softmax
+ * weights over all T * G query rows of its head are added to its record, in a fixed order. A key or value that is not finite
+ * spoils every query row that sees it, and, of the T newest tokens, also rows before it in the same call; rows behind a
+ * sequence's length may hold anything. H a multiple of HKV, G = H / HKV <= 16, T * G <= 2^24; sm_scale > 0 and finite.
+ * `workspace`: device memory of bolt3_paged_attend_workspace(...) bytes (weigh: whether `weight` is given), 16-byte
+ * aligned, used only within the call. */
+typedef struct bolt3_paged_attend_args {
+  int B, T, H, HKV, HD;
+  const void* q; int64_t q_sb, q_st;
+  const void* pages; int64_t n_pages; int page;
+  const int32_t* table; int64_t table_stride, width;
+  float* weight;                       /* optional */
+  int64_t n;
+  const int32_t* lens;
+  void* y;
+  float sm_scale;
+  void* workspace; size_t workspace_bytes;
+  int32_t* status;                     /* optional; also OR-ed with 2 if a bounded wait expired */
+  const int64_t* pos_dev; int64_t pos_ref; int64_t pos_span;
+} bolt3_paged_attend_args;
+int bolt3_paged_attend(const bolt3_paged_attend_args* a, void* stream);
+size_t bolt3_paged_attend_workspace(int B, int T, int H, int HKV, int HD, int64_t n, int weigh);
+
+/* Every (sequence, KV head) with more than `keep` rows drops all but `keep` of them, in place: it keeps the rows whose
+ * `order` is above its largest order minus `recent`, then those of the largest `weight` (a NaN counts as +infinity), equal
+ * ones by the lowest row; where more than `keep` rows are that new, the same order decides among them. Of the dropped rows
+ * below `keep`, the i-th (ascending) receives keys, values, weight and order of the i-th kept row at or above `keep`; what
+ * stands at rows >= keep is left as it is. Here n (or lens[b] <= n) is the number of rows held; lens_out (optional, int32
+ * [B]) becomes min(rows, keep), -1 for an idle sequence. Pages must not be shared between sequences. 0 <= recent <= keep,
+ * keep >= 1. `workspace`: bolt3_paged_evict_workspace(...) bytes, 16-byte aligned, used only within the call. */
+typedef struct bolt3_paged_evict_args {
+  int B, HKV, HD;
+  void* pages; int64_t n_pages; int page;
+  const int32_t* table; int64_t table_stride, width;
+  float* weight; int32_t* order;
+  int64_t n, keep, recent;
+  const int32_t* lens; int32_t* lens_out;
+  void* workspace; size_t workspace_bytes;
+  int32_t* status;                     /* optional */
+} bolt3_paged_evict_args;
+int bolt3_paged_evict(const bolt3_paged_evict_args* a, void* stream);
+size_t bolt3_paged_evict_workspace(int B, int HKV, int64_t n, int64_t keep);
+
 /* ---- Beam search. No counterpart in the reference, which samples (vsa_lm/config/bolt3.py:321-333).
  * One selection step of B groups of K beams over V tokens. Continuation (k, v) of a group scores
  * scores[k] + log_softmax(logits[k])[v]; a finished beam has one continuation, eos_ids[0] at its own
@@ -369,8 +449,8 @@ int bolt3_prefill_fwd_noalloc(const bolt3_prefill_args* a, void* stream);
 int bolt3_abi_version(void);
 const char* bolt3_status_string(int status);
 /* sizeof of an argument struct (0 prep, 1 consolidate, 2 attend, 3 prefill, 4 anchor, 5 rmsnorm,
- * 6 silu_mul, 8 kv8_append, 9 kv8_read, 10 kv8_attend, 11 beam_select, 12 beam_item, 13 beam_reorder;
- * 0 for others), so a binding can check its own layout of the structs against the compiled one */
+ * 6 silu_mul, 8 kv8_append, 9 kv8_read, 10 kv8_attend, 11 beam_select, 12 beam_item, 13 beam_reorder,
+ * 14 paged_append, 15 paged_attend, 16 paged_evict; 0 for others), so a binding can check its own layout of the structs against the compiled one */
 size_t bolt3_args_size(int which);
 /* Host-only: reorder indices 0..n-1 of `vals` into the order CPU torch.topk(vals, k, largest)
  * returns (first k written to out_idx). Returns 0, or 1 if a bounds check fired. */

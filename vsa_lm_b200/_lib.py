@@ -23,7 +23,7 @@ STATUS = {0: "ok", 1: "invalid argument", 2: "unsupported shape", 3: "misaligned
 DEVICE_STATUS_BITS = {1: "a bounds check of the consolidation's tie-order emulation fired",
                       2: "a bounded wait in an attention kernel expired",
                       4: "a bounded wait in the consolidation scan expired",
-                      8: "a decode step's device position (or a sequence length or beam parent on the device) was "
+                      8: "a decode step's device position (or a sequence length, page or beam parent on the device) was "
                          "outside the range its launch was built for"}
 
 
@@ -182,6 +182,54 @@ class BeamReorderArgs(ctypes.Structure):
     ]
 
 
+class PagedAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", _I), ("T", _I), ("H", _I), ("HKV", _I), ("HD", _I),
+        ("q", _P), ("k", _P), ("v", _P),
+        ("q_sb", _I64), ("q_st", _I64), ("k_sb", _I64), ("k_st", _I64), ("v_sb", _I64), ("v_st", _I64),
+        ("q_norm_w", _P), ("k_norm_w", _P), ("eps", _F),
+        ("inv_freq", _P),
+        ("q_out", _P),
+        ("pages", _P), ("n_pages", _I64), ("page", _I),
+        ("table", _P), ("table_stride", _I64), ("width", _I64),
+        ("weight", _P), ("order", _P),
+        ("n", _I64), ("pos0", _I64),
+        ("lens", _P), ("pos", _P),
+        ("status", _P),
+        ("pos_dev", _P), ("pos_ref", _I64), ("pos_span", _I64),
+    ]
+
+
+class PagedAttendArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", _I), ("T", _I), ("H", _I), ("HKV", _I), ("HD", _I),
+        ("q", _P), ("q_sb", _I64), ("q_st", _I64),
+        ("pages", _P), ("n_pages", _I64), ("page", _I),
+        ("table", _P), ("table_stride", _I64), ("width", _I64),
+        ("weight", _P),
+        ("n", _I64),
+        ("lens", _P),
+        ("y", _P),
+        ("sm_scale", _F),
+        ("workspace", _P), ("workspace_bytes", _SZ),
+        ("status", _P),
+        ("pos_dev", _P), ("pos_ref", _I64), ("pos_span", _I64),
+    ]
+
+
+class PagedEvictArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", _I), ("HKV", _I), ("HD", _I),
+        ("pages", _P), ("n_pages", _I64), ("page", _I),
+        ("table", _P), ("table_stride", _I64), ("width", _I64),
+        ("weight", _P), ("order", _P),
+        ("n", _I64), ("keep", _I64), ("recent", _I64),
+        ("lens", _P), ("lens_out", _P),
+        ("workspace", _P), ("workspace_bytes", _SZ),
+        ("status", _P),
+    ]
+
+
 class PrefillArgs(ctypes.Structure):
     _fields_ = [
         ("B", _I), ("T", _I), ("H", _I), ("HKV", _I), ("HD", _I),
@@ -213,6 +261,11 @@ SIGNATURES = {
     "bolt3_beam_select": ([ctypes.POINTER(BeamSelectArgs), _P], _I),
     "bolt3_beam_select_workspace": ([_I, _I, _I64], _SZ),
     "bolt3_beam_reorder": ([ctypes.POINTER(BeamReorderArgs), _P], _I),
+    "bolt3_paged_append": ([ctypes.POINTER(PagedAppendArgs), _P], _I),
+    "bolt3_paged_attend": ([ctypes.POINTER(PagedAttendArgs), _P], _I),
+    "bolt3_paged_attend_workspace": ([_I, _I, _I, _I, _I, _I64, _I], _SZ),
+    "bolt3_paged_evict": ([ctypes.POINTER(PagedEvictArgs), _P], _I),
+    "bolt3_paged_evict_workspace": ([_I, _I, _I64, _I64], _SZ),
     "bolt3_prefill_fwd": ([ctypes.POINTER(PrefillArgs), _P], _I),
     "bolt3_prefill_fwd_noalloc": ([ctypes.POINTER(PrefillArgs), _P], _I),
     "bolt3_prefill_workspace_size": ([_I, _I64, _I], _SZ),
@@ -225,7 +278,7 @@ SIGNATURES = {
 # number of each struct for bolt3_args_size
 ARG_STRUCTS = {0: PrepArgs, 1: ConsolidateArgs, 2: AttendArgs, 3: PrefillArgs, 4: AnchorArgs, 5: RMSNormArgs,
                6: SiluMulArgs, 8: Kv8AppendArgs, 9: Kv8ReadArgs, 10: Kv8AttendArgs, 11: BeamSelectArgs, 12: BeamItem,
-               13: BeamReorderArgs}
+               13: BeamReorderArgs, 14: PagedAppendArgs, 15: PagedAttendArgs, 16: PagedEvictArgs}
 
 ABI_VERSION = 10   # BOLT3_ABI_VERSION in include/bolt3.h
 
@@ -298,6 +351,9 @@ kv8_read = Packed("bolt3_kv8_read", Kv8ReadArgs)
 kv8_attend = Packed("bolt3_kv8_attend", Kv8AttendArgs)
 beam_select = Packed("bolt3_beam_select", BeamSelectArgs)
 beam_reorder = Packed("bolt3_beam_reorder", BeamReorderArgs)
+paged_append = Packed("bolt3_paged_append", PagedAppendArgs)
+paged_attend = Packed("bolt3_paged_attend", PagedAttendArgs)
+paged_evict = Packed("bolt3_paged_evict", PagedEvictArgs)
 beam_item = _packer(BeamItem)
 
 

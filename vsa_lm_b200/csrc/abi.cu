@@ -51,6 +51,9 @@ extern "C" size_t bolt3_args_size(int which) {
     case 11: return sizeof(bolt3_beam_select_args);
     case 12: return sizeof(bolt3_beam_item);
     case 13: return sizeof(bolt3_beam_reorder_args);
+    case 14: return sizeof(bolt3_paged_append_args);
+    case 15: return sizeof(bolt3_paged_attend_args);
+    case 16: return sizeof(bolt3_paged_evict_args);
     default: return 0;
   }
 }

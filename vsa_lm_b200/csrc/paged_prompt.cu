@@ -1,0 +1,805 @@
+// Softmax attention of many query rows (prompt slices) over the pages of a bf16 KV cache, on the tensor cores' TMEM path,
+// and the record of the weights that the cached rows got.
+//
+// The mathematics is that of paged_attend.cu, with weights rounded to bf16 for the product with the values.
+//
+// attend. Bound by arithmetic: 4 HD operations per (query row, key), and one exponential; at HD 128 the MMAs of a block of 128
+// keys by 256 rows take 2048 cycles of an SM, its exponentials 2048. A CTA holds two tiles of 128 query rows (T * G rows of one
+// KV head, token-major) and walks the keys in blocks of 128. Roles, which meet only at mbarriers:
+// - warp 16 brings keys and values by TMA, a box for each page that a block touches, two stages each;
+// - one lane of warp 17 issues tcgen05.mma: S = Q K^T into TMEM, O += P V with P as the TMEM operand;
+// - warp 18 clears the value rows of the last block that no query row of the CTA sees (a page's unused rows may hold
+//   anything, and 0 times a NaN is one);
+// - warps 0-7 and 8-15 are the softmax of a tile, 64 keys at a time: scores out of TMEM, weights back over them. A warp takes
+//   16 TMEM lanes in the 16x256b layout, so that a row's reference is shared by a quad of lanes alone. The reference moves only
+//   when a weight would pass 2^kMost; only then are the sums in TMEM rescaled.
+// While one tile's softmax runs, the tensor cores work on the other tile. With few heads the keys are split over CTAs, whose
+// partial sums a second kernel joins.
+//
+// record. A key's weight needs the rows' sums over all keys, so the scores are computed again once these are known, this time
+// with the keys in the TMEM lanes: S^T = K Q^T, a thread per key, which sums 2^(t - lse) over the query columns in registers; no
+// two threads add to one record, whatever the split. A CTA holds up to 512 query rows of a head and walks a range of its keys.
+// Bound by the exponentials: 4096 cycles of an SM for 128 keys by 512 rows, against 2048 of its MMAs.
+#include "paged.cuh"
+#include "tc5.cuh"
+#include "trace.h"
+
+namespace {
+
+using namespace paged;
+
+constexpr int kKeys = 128;                       // of a block
+constexpr float kMost = 20.f;                    // log2 of the largest weight relative to the reference
+constexpr int kThreads = 608;                    // 16 softmax warps, loads, MMAs, clearing
+constexpr int kRows = 512;                       // query rows of a CTA of the record kernel
+constexpr int kRecordThreads = 576;              // 16 summing warps, loads, MMAs
+
+struct Params {
+  CUtensorMap map;                               // the pool's rows, boxes of 64 columns and a page
+  Attend c;
+  int tiles, splits;                             // tiles: pairs of 128 rows of a head
+  uint32_t per_G;                                // ceil(2^32 / G), 0 for G = 1
+  float* part;                                   // [head][row][split][HD] sums, then [..] (reference, sum of weights)
+  float2* part_ml;
+  float* lse;                                    // [head][row] log2 of the sum of 2^t, +inf for an idle sequence; null: no record
+  int ranges;                                    // of keys of a head, each a CTA of the record kernel
+};
+
+template <int HD>
+struct Smem {
+  unsigned char q[2][kKeys * HD * 2];            // K-major operand tiles: HD / 64 blocks of [128 rows][64 columns]
+  unsigned char k[2][kKeys * HD * 2];
+  unsigned char v[2][kKeys * HD * 2];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], v_last, v_clean;
+  uint64_t s_full[2], p_full[2][2], pv_half[2], o_full[2];
+  uint32_t tbase;
+  int err;
+};
+
+template <int HD>
+struct RecordSmem {
+  unsigned char q[kRows / kKeys][kKeys * HD * 2];
+  unsigned char k[2][kKeys * HD * 2];
+  float lse[kRows];
+  int token[kRows];
+  float sum[2][kRows / kKeys][kKeys];
+  uint64_t k_full[2], k_empty[2], s_full[kRows / kKeys], s_empty[kRows / kKeys];
+  uint32_t tbase;
+  int err;
+};
+
+// the token of a query row (exact for rows below 2^28)
+B3_DEV int token_of(const Params& p, int row) { return p.per_G == 0 ? row : (int)__umulhi((uint32_t)row, p.per_G); }
+
+// 64 columns of 16 TMEM lanes: a thread gets columns 8 n + 2 (lane % 4) and the next one of lanes lane / 4 (registers
+// 4 n, 4 n + 1) and lane / 4 + 8 (4 n + 2, 4 n + 3)
+B3_DEV void ld_16x64(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// 32 columns of 16 TMEM lanes: column 4 n + lane % 4 of lanes lane / 4 (register 2 n) and lane / 4 + 8 (2 n + 1)
+B3_DEV void st_16x32(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
+}
+// the layout of ld_16x64, 32 columns
+B3_DEV void ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+B3_DEV void st_16x32f(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
+}
+// All threads of the CTA meet. bar.sync in a string is the aligned form, which takes a warp's first lanes to arrive for the
+// whole warp, and the compiler does not bring a warp together for it that parted before (a page looked up by some lanes): the
+// others then went on before the tensor memory was there
+B3_DEV void meet_all() {
+  __syncwarp();
+  asm volatile("barrier.sync 0;\n" ::: "memory");
+  __syncwarp();
+}
+B3_DEV bool elected() {
+  uint32_t one;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}\n" : "=r"(one));
+  return one != 0;
+}
+
+// query rows row0 + r0 .. of head (b, kvh) into K-major operand tiles, 16 rows by each of the calling warps (r0 = 16 warp)
+template <int HD>
+B3_DEV void copy_queries(const Params& p, unsigned char* tiles, int b, int kvh, int row0, int r0, int lane) {
+  constexpr int CPR = HD / 8, RPW = 32 / CPR;                     // 16-byte chunks of a row, rows of a warp's instruction
+  const bolt3_paged_attend_args& a = p.c.a;
+  const int c = lane % CPR;
+  const bf16* q = reinterpret_cast<const bf16*>(a.q) + b * a.q_sb + (int64_t)(kvh * p.c.G) * HD + 8 * c;
+#pragma unroll
+  for (int i = 0; i < 16 / RPW; ++i) {
+    const int r = r0 + lane / CPR + i * RPW, t = token_of(p, row0 + r), g = row0 + r - t * p.c.G;
+    const bool in = row0 + r < p.c.rows;
+    cp_async16(tiles + (r >> 7) * (kKeys * HD * 2) + (c >> 3) * (kKeys * 128) + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4),
+               in ? q + t * a.q_st + (int64_t)g * HD : q, in);
+  }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_constant__ Params p) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  Smem<HD>& sm = *reinterpret_cast<Smem<HD>*>(smem_raw + ((1024 - (tc5::smem_u32(smem_raw) & 1023)) & 1023));
+  const bolt3_paged_attend_args& a = p.c.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int head = blockIdx.x / p.tiles, b = head / a.HKV, kvh = head % a.HKV;
+  const int row0 = (blockIdx.x % p.tiles) * 256, n_tile = min(2, (p.c.rows - row0 + 127) / 128);
+  const int split = blockIdx.y;
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      tc5::mbar_init(&sm.k_full[i], 1);
+      tc5::mbar_init(&sm.k_empty[i], 1);
+      tc5::mbar_init(&sm.v_full[i], 1);
+      tc5::mbar_init(&sm.v_empty[i], 1);
+      tc5::mbar_init(&sm.s_full[i], 1);
+      tc5::mbar_init(&sm.p_full[i][0], 256);
+      tc5::mbar_init(&sm.p_full[i][1], 256);
+      tc5::mbar_init(&sm.pv_half[i], 1);
+      tc5::mbar_init(&sm.o_full[i], 1);
+    }
+    tc5::mbar_init(&sm.v_last, 1);
+    tc5::mbar_init(&sm.v_clean, 32);
+    tc5::mbar_fence_init();
+    sm.err = 0;
+  }
+  grid_dep_launch();
+  grid_dep_wait();
+  bool bad = false;
+  const int64_t s = p.c.len.rows(b, bad);
+  if (bad && tid == 0 && blockIdx.x % p.tiles == 0 && split == 0 && a.status) atomicOr(a.status, 8);
+  auto out_row = [&](int row) {
+    const int t = token_of(p, row), g = row - t * p.c.G;
+    return reinterpret_cast<bf16*>(a.y) + ((int64_t)b * a.T * a.H + kvh * p.c.G) * HD + (int64_t)t * (a.H * HD) + g * HD;
+  };
+  // blocks of keys that the last row of this CTA sees, and this split's share of them
+  const int last = token_of(p, min(row0 + 256, p.c.rows) - 1);
+  const int64_t all = s < 0 ? 0 : (s + last + kKeys) / kKeys;
+  const int64_t lo = all * split / p.splits, hi = all * (split + 1) / p.splits;
+  const int n_blk = (int)(hi - lo);
+  if (n_blk == 0) {                              // the same for all threads: nothing has been allocated
+    if (tid < 256 && row0 + tid < p.c.rows) {
+      const int64_t row = (int64_t)head * p.c.rows + row0 + tid;
+      if (p.splits > 1) {
+        p.part_ml[row * p.splits + split] = make_float2(neg_inf(), 0.f);
+      } else {
+        uint4* y = reinterpret_cast<uint4*>(out_row(row0 + tid));
+        for (int i = 0; i < HD / 8; ++i) y[i] = make_uint4(0, 0, 0, 0);
+        if (p.lse != nullptr) p.lse[row] = -neg_inf();
+      }
+    }
+    return;
+  }
+  const int seen = (int)min(s + 1 - lo * kKeys, (int64_t)0x7fffff00);             // keys of this split that token 0 sees
+  const int seen_last = (int)min(s + 1 + last - lo * kKeys, (int64_t)0x7fffff00);   // that the CTA's last row sees
+  const bool ragged = seen_last < n_blk * kKeys;  // the last block ends with rows that no row sees
+
+  // the query rows into their operand tiles; the first loads are under way meanwhile
+  if (warp < 16) {
+    copy_queries<HD>(p, sm.q[0], b, kvh, row0, warp * 16, lane);
+    asm volatile("cp.async.wait_all;\nfence.proxy.async.shared::cta;\n" ::: "memory");
+  }
+  if (warp == 17) {
+    tc5::tmem_alloc(&sm.tbase, 512);
+    tc5::tmem_relinquish();
+  }
+  // every warp comes here once: the queries are in place, the barriers and the TMEM are there
+  auto all_ready = [&] {
+    tc5::fence_before_sync();
+    meet_all();
+    tc5::fence_after_sync();
+    return sm.tbase;                             // S / P of tile i: columns 128 i; O of tile i: 256 + 128 i
+  };
+  auto wait = [&](uint64_t* bar, int phase) {
+    if (tc5::mbar_wait(bar, (uint32_t)phase & 1, kWaitIters)) return true;
+    sm.err = 1;
+    return false;
+  };
+  auto wait_all = [&](uint64_t* bar, int phase) {
+    const bool ok = __all_sync(0xffffffffu, wait(bar, phase)) != 0;
+    __syncwarp();                                // what follows is for a whole warp (tcgen05.ld, barriers)
+    return ok;
+  };
+
+  if (warp == 16) {
+    // ---- loads: lane l < CB boxes brings columns 64 (l % CB) of box l / CB
+    constexpr int CB = HD / 64;
+    const Pages& pages = p.c.pages;
+    const int log = 7 - pages.log;               // log2 of the boxes of a block, a page each
+    const bool issues = lane < CB << log;
+    const int cb = lane % CB, unit = lane / CB;
+    const uint32_t to = cb * (kKeys * 128) + (unit << (pages.log + 7));
+    // the first row of the pool that this lane's box of block j is, of its head's keys. Without a page (behind the last row, or
+    // a bad entry) that is the pool's first: no row of it counts
+    const int first = ((int)lo << log) + unit, end = issues ? min((int)hi << log, (int)((s + a.T - 1) >> pages.log) + 1) : 0;   // pages
+    auto lookup = [&](int j) {
+      const int i = first + (j << log);
+      if (i >= end) return kvh;
+      const int pg = pages.page_of(b, (int64_t)i << pages.log);
+      if (pg < 0 && a.status) atomicOr(a.status, 8);
+      return max(pg, 0) * a.HKV + kvh;
+    };
+    int next = lookup(0);
+    all_ready();
+    int done = 0;                                // blocks whose loads were issued
+    bool ok = true;
+    for (int j = 0; ok && j < n_blk; ++j) {
+      const int st = j & 1, z = next;
+      next = lookup(j + 1);
+      ok = j < 2 || wait_all(&sm.k_empty[st], (j >> 1) - 1);
+      if (!ok) break;
+      if (lane == 0) tc5::mbar_expect_tx(&sm.k_full[st], kKeys * HD * 2);
+      __syncwarp();
+      if (issues) tc5::tma_load_3d(sm.k[st] + to, &p.map, 64 * cb, 0, z, &sm.k_full[st]);
+      ok = j < 2 || wait_all(&sm.v_empty[st], (j >> 1) - 1);
+      if (!ok) {                                 // give the keys' copies one more bounded wait before leaving
+        wait(&sm.k_full[st], j >> 1);
+        break;
+      }
+      // the values that are cleared have a barrier of their own: who waits for it has not followed the others' phases
+      uint64_t* bar = ragged && j + 1 == n_blk ? &sm.v_last : &sm.v_full[st];
+      if (lane == 0) tc5::mbar_expect_tx(bar, kKeys * HD * 2);
+      __syncwarp();
+      if (issues) tc5::tma_load_3d(sm.v[st] + to, &p.map, 64 * cb, 0, z + (int)(pages.n_pages * a.HKV), bar);
+      done = j + 1;
+    }
+    for (int j = max(0, done - 2); j < done; ++j) {   // no copy is in flight when the CTA ends
+      wait(&sm.k_full[j & 1], j >> 1);
+      if (ragged && j + 1 == n_blk) wait(&sm.v_last, 0);
+      else wait(&sm.v_full[j & 1], j >> 1);
+    }
+  } else if (warp == 17) {
+    // ---- issue. The whole warp runs the loop, so that addresses and descriptors are uniform over it; one lane issues
+    const uint32_t tb = all_ready();
+    const bool one = elected();
+    constexpr uint32_t kIdS = tc5::idesc_bf16(128, kKeys, false, false), kIdO = tc5::idesc_bf16(128, HD, false, true);
+    constexpr uint64_t kTile = sizeof(sm.q[0]) >> 4;              // from one tile's descriptor to the next one's
+    const uint32_t tu = __shfl_sync(0xffffffffu, tb, 0);
+    const uint64_t q_desc = tc5::sdesc(tc5::smem_u32(sm.q[0]), 16, 1024), k_desc = tc5::sdesc(tc5::smem_u32(sm.k[0]), 16, 1024);
+    const uint64_t v_desc = tc5::sdesc(tc5::smem_u32(sm.v[0]), kKeys * 128, 1024);
+    // Step after step: the products of tile i with block j's values, then its scores of block j + 1 (j = -1: scores alone). One
+    // place in the code for either: with the first scores before the loop, in a copy of their own, the loop's were issued twice at
+    // HD 64
+    bool ok = true;
+    int i = 0;
+#pragma unroll 1
+    for (int j = -1; ok && j < n_blk;) {
+      const int st = j & 1;
+      if (j >= 0) {
+        if (i == 0) ok = ragged && j + 1 == n_blk ? wait_all(&sm.v_clean, 0) : wait_all(&sm.v_full[st], j >> 1);
+#pragma unroll 1
+        for (int h = 0; ok && h < 2; ++h) {
+          ok = wait_all(&sm.p_full[i][h], j);
+          if (!ok) break;
+          tc5::fence_after_sync();
+          const uint64_t vd = v_desc + st * kTile + 4 * h * 128;
+          const uint32_t d = tu + 256 + i * 128, pa = tu + i * 128 + 32 * h;
+          if (one) {
+            tc5::mma_ts(d, pa, vd, kIdO, j > 0 || h > 0);
+            tc5::mma_ts(d, pa + 8, vd + 128, kIdO, 1);
+            tc5::mma_ts(d, pa + 16, vd + 256, kIdO, 1);
+            tc5::mma_ts(d, pa + 24, vd + 384, kIdO, 1);
+            if (h == 0) tc5::commit(&sm.pv_half[i]);
+            else if (j + 1 == n_blk) tc5::commit(&sm.o_full[i]);
+          }
+        }
+        if (!ok) break;
+      }
+      const bool last_tile = i + 1 == n_tile;
+      if (j + 1 < n_blk) {
+        if (i == 0) ok = wait_all(&sm.k_full[st ^ 1], (j + 1) >> 1);
+        if (!ok) break;
+        tc5::fence_after_sync();
+        const uint64_t qd = q_desc + i * kTile, kd = k_desc + (st ^ 1) * kTile;
+        if (one) {
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            constexpr uint64_t kBlock = (kKeys * 128) >> 4;       // a block of 64 columns
+            tc5::mma_ss(tu + i * 128, qd + (ks >> 2) * kBlock + (ks & 3) * 2, kd + (ks >> 2) * kBlock + (ks & 3) * 2, kIdS, ks > 0);
+          }
+          tc5::commit(&sm.s_full[i]);
+          if (last_tile) tc5::commit(&sm.k_empty[st ^ 1]);
+        }
+      }
+      if (last_tile && j >= 0 && one) tc5::commit(&sm.v_empty[st]);
+      i = last_tile ? 0 : i + 1;
+      j += last_tile;
+    }
+    if (ok) wait_all(&sm.v_empty[(n_blk - 1) & 1], (n_blk - 1) >> 1);   // no arrival is under way when the CTA ends
+  } else if (warp >= 18) {
+    all_ready();
+    if (ragged) {
+      const int j = n_blk - 1, st = j & 1, first = seen_last - j * kKeys;
+      // also where a wait ran out: the arrival must come, or the issuing warp waits for it in vain
+      if (wait(&sm.v_last, 0)) {
+        for (int i = lane; i < (kKeys - first) * (HD / 8); i += 32) {
+          const int r = first + i / (HD / 8), c = i % (HD / 8);
+          *reinterpret_cast<uint4*>(sm.v[st] + (c >> 3) * (kKeys * 128) + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      tc5::mbar_arrive(&sm.v_clean);
+    }
+  } else {
+    const uint32_t tb = all_ready();
+    if ((warp >> 3) < n_tile) {
+      // ---- softmax of tile i: this thread's two rows are those of TMEM lanes first_lane + grp and + grp + 8
+      const int i = warp >> 3, grp = lane >> 2, tig = lane & 3;
+      const int first_lane = 32 * (warp & 3) + 16 * (warp >> 2 & 1), first_row = row0 + 128 * i + first_lane + grp;
+      const uint32_t lanes = (uint32_t)first_lane << 16, ts = tb + i * 128 + lanes, to = tb + 256 + i * 128 + lanes;
+      const int see_all = seen + token_of(p, row0 + i * 128);       // that every row of the tile sees
+      const float scale = a.sm_scale * kLog2e;
+      float M[2] = {neg_inf(), neg_inf()};
+      uint64_t l[2] = {0, 0};                                       // sums of weights over this thread's keys, in pairs
+      bool ok = true;
+      for (int j = 0; ok && j < n_blk; ++j) {
+        ok = wait_all(&sm.s_full[i], j);
+        if (!ok) break;
+        tc5::fence_after_sync();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t sc[32];
+          ld_16x64(ts + 64 * h, sc);
+          const int key = j * kKeys + 64 * h;
+          tc5::ld_wait();
+          if (key + 64 > see_all) {                                 // the same for the whole tile
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const int left = seen + token_of(p, min(first_row + 8 * q, p.c.rows - 1)) - key - 2 * tig;   // seen, from this thread's first
+#pragma unroll
+              for (int n = 0; n < 8; ++n) {
+                if (8 * n >= left) sc[4 * n + 2 * q] = 0xff800000u;
+                if (8 * n + 1 >= left) sc[4 * n + 2 * q + 1] = 0xff800000u;
+              }
+            }
+          }
+          // the references move only when a weight would pass 2^kMost (and at the first key)
+          float m[2];
+          bool over = false;
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            m[q] = fmaxf(__uint_as_float(sc[2 * q]), __uint_as_float(sc[2 * q + 1]));
+#pragma unroll
+            for (int n = 1; n < 8; ++n) m[q] = max3(m[q], __uint_as_float(sc[4 * n + 2 * q]), __uint_as_float(sc[4 * n + 2 * q + 1]));
+            m[q] *= scale;
+            over |= m[q] > M[q] + kMost;
+          }
+          if (__any_sync(0xffffffffu, over)) {
+            float f[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              m[q] = quad_max(m[q]);
+              const float to_M = m[q] > M[q] + kMost ? m[q] : M[q];
+              f[q] = M[q] == neg_inf() ? 0.f : ex2(M[q] - to_M);    // 1 where the reference stays
+              M[q] = to_M;
+              l[q] = mul2(l[q], pair(f[q], f[q]));
+            }
+            if (j > 0 || h > 0) {
+              if (h > 0) {                                          // the first half's product may still be under way
+                ok = wait_all(&sm.pv_half[i], j);
+                tc5::fence_after_sync();
+              }
+              if (ok) {
+#pragma unroll 1
+                for (int d = 0; d < HD; d += 32) {
+                  uint32_t o[16];
+                  ld_16x32(to + d, o);
+                  tc5::ld_wait();
+#pragma unroll
+                  for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f[x >> 1 & 1]);
+                  st_16x32f(to + d, o);
+                }
+                tc5::st_wait();
+              }
+            }
+          }
+          uint32_t w[16];
+          const float r0 = M[0] == neg_inf() ? 0.f : -M[0], r1 = M[1] == neg_inf() ? 0.f : -M[1];
+          const uint64_t ref[2] = {pair(r0, r0), pair(r1, r1)};
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const float2 u = unpair(fma2(pair(__uint_as_float(sc[4 * n + 2 * q]), __uint_as_float(sc[4 * n + 2 * q + 1])), pair(scale, scale), ref[q]));
+              const float e0 = ex2(u.x), e1 = ex2(u.y);
+              l[q] = add2(l[q], pair(e0, e1));
+              w[2 * n + q] = pack_bf16(e0, e1);
+            }
+          st_16x32(ts + 32 * h, w);
+          tc5::st_wait();
+          tc5::fence_before_sync();
+          tc5::mbar_arrive(&sm.p_full[i][h]);
+        }
+      }
+      float sum[2], inv[2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const float2 x = unpair(l[q]);
+        sum[q] = quad_sum(x.x + x.y);
+        inv[q] = sum[q] == 0.f ? 0.f : 1.f / sum[q];
+      }
+      ok = ok && wait(&sm.o_full[i], 0);
+      ok = __all_sync(0xffffffffu, ok);
+      __syncwarp();
+      if (ok) {
+        tc5::fence_after_sync();
+        // bf16 rows by way of this warp's sixteen rows of the query tile, whose products are done: whole rows to a store
+        unsigned char* out = sm.q[i] + first_lane * HD * 2;
+#pragma unroll 1
+        for (int d = 0; d < HD; d += 32) {
+          uint32_t o[16];
+          ld_16x32(to + d, o);
+          tc5::ld_wait();
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            if (p.splits > 1) {
+              const int row = first_row + 8 * q;
+              float* dst = p.part + (((int64_t)head * p.c.rows + row) * p.splits + split) * HD + d + 2 * tig;
+#pragma unroll
+              for (int n = 0; n < 4; ++n)
+                if (row < p.c.rows) *reinterpret_cast<uint2*>(dst + 8 * n) = make_uint2(o[4 * n + 2 * q], o[4 * n + 2 * q + 1]);
+            } else {
+#pragma unroll
+              for (int n = 0; n < 4; ++n)
+                *reinterpret_cast<uint32_t*>(out + (grp + 8 * q) * HD * 2 + (((d / 8 + n) ^ grp) << 4) + 4 * tig) =
+                    pack_bf16(__uint_as_float(o[4 * n + 2 * q]) * inv[q], __uint_as_float(o[4 * n + 2 * q + 1]) * inv[q]);
+            }
+          }
+        }
+        if (p.splits == 1) {
+          constexpr int CPR = HD / 8, RPW = 32 / CPR;
+          const int c = lane % CPR;
+          __syncwarp();
+#pragma unroll
+          for (int r = lane / CPR; r < 16; r += RPW) {
+            const int row = row0 + 128 * i + first_lane + r;
+            if (row < p.c.rows) reinterpret_cast<uint4*>(out_row(row))[c] = *reinterpret_cast<uint4*>(out + r * HD * 2 + ((c ^ (r & 7)) << 4));
+          }
+        }
+        if (tig == 0) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            if (first_row + 8 * q >= p.c.rows) continue;
+            const int64_t row = (int64_t)head * p.c.rows + first_row + 8 * q;
+            if (p.splits > 1) p.part_ml[row * p.splits + split] = make_float2(M[q], sum[q]);
+            else if (p.lse != nullptr) p.lse[row] = sum[q] == 0.f ? -neg_inf() : M[q] + log2f(sum[q]);
+          }
+        }
+      }
+    }
+  }
+  tc5::fence_before_sync();
+  meet_all();
+  tc5::fence_after_sync();
+  if (warp == 17) tc5::tmem_dealloc(sm.tbase, 512);
+  if (tid == 0 && sm.err && a.status) atomicOr(a.status, 2);
+}
+
+// one warp per (head, query row): the splits' partial sums joined
+template <int HD>
+__global__ void __launch_bounds__(128) paged_prompt_join_kernel(const __grid_constant__ Params p) {
+  constexpr int EPL = HD / 32;
+  const bolt3_paged_attend_args& a = p.c.a;
+  const int lane = threadIdx.x & 31;
+  grid_dep_launch();
+  grid_dep_wait();
+  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (item >= (int64_t)a.B * a.HKV * p.c.rows) return;
+  const int head = (int)(item / p.c.rows), row = (int)(item % p.c.rows), b = head / a.HKV, kvh = head % a.HKV;
+  const int64_t at = item * p.splits;
+  float m = neg_inf(), l = 0.f, acc[EPL] = {};
+  for (int i = 0; i < p.splits; ++i) m = fmaxf(m, p.part_ml[at + i].x);
+  for (int i = 0; i < p.splits; ++i) {
+    const float2 ml = p.part_ml[at + i];
+    if (ml.x == neg_inf() && ml.y == 0.f) continue;               // no keys: its sums were not written
+    const float f = ml.x == neg_inf() ? 0.f : exp2f(ml.x - m);
+    l = fmaf(ml.y, f, l);
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) acc[e] = fmaf(p.part[(at + i) * HD + 32 * e + lane], f, acc[e]);
+  }
+  bf16* y = reinterpret_cast<bf16*>(a.y) + (((int64_t)b * a.T + row / p.c.G) * a.H + kvh * p.c.G + row % p.c.G) * HD;
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) y[32 * e + lane] = __float2bfloat16_rn(l == 0.f ? 0.f : acc[e] / l);
+  if (lane == 0 && p.lse != nullptr) p.lse[item] = l == 0.f ? -neg_inf() : m + log2f(l);
+}
+
+// the weights of a range of a head's keys, summed over its query rows, into their records
+template <int HD>
+__global__ void __launch_bounds__(kRecordThreads, 1) paged_prompt_record_kernel(const __grid_constant__ Params p) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  RecordSmem<HD>& sm = *reinterpret_cast<RecordSmem<HD>*>(smem_raw + ((1024 - (tc5::smem_u32(smem_raw) & 1023)) & 1023));
+  constexpr int NQ = kRows / kKeys;
+  const bolt3_paged_attend_args& a = p.c.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int head = blockIdx.x / p.ranges, range = blockIdx.x % p.ranges, b = head / a.HKV, kvh = head % a.HKV;
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      tc5::mbar_init(&sm.k_full[i], 1);
+      tc5::mbar_init(&sm.k_empty[i], 1);
+    }
+    for (int i = 0; i < NQ; ++i) {
+      tc5::mbar_init(&sm.s_full[i], 1);
+      tc5::mbar_init(&sm.s_empty[i], 128);
+    }
+    tc5::mbar_fence_init();
+    sm.err = 0;
+  }
+  grid_dep_launch();
+  grid_dep_wait();
+  bool bad = false;
+  const int64_t s = p.c.len.rows(b, bad);
+  const int64_t all = s < 0 ? 0 : (s + a.T + kKeys - 1) / kKeys, lo = all * range / p.ranges, hi = all * (range + 1) / p.ranges;
+  const int n_blk = (int)(hi - lo), groups = (p.c.rows + kRows - 1) / kRows;
+  if (n_blk == 0) return;                        // the same for all threads: nothing has been allocated
+  if (warp == 17) {
+    tc5::tmem_alloc(&sm.tbase, 512);
+    tc5::tmem_relinquish();
+  }
+  auto wait = [&](uint64_t* bar, int phase) {
+    if (tc5::mbar_wait(bar, (uint32_t)phase & 1, kWaitIters)) return true;
+    sm.err = 1;
+    return false;
+  };
+  auto wait_all = [&](uint64_t* bar, int phase) {
+    const bool ok = __all_sync(0xffffffffu, wait(bar, phase)) != 0;
+    __syncwarp();                                // what follows is for a whole warp (tcgen05.ld, barriers)
+    return ok;
+  };
+  const int total = groups * n_blk;              // blocks of keys that come, group after group
+  // all warps come here before a group (its queries are in place) and after the last
+  auto meet = [&] {
+    tc5::fence_before_sync();
+    meet_all();
+    tc5::fence_after_sync();
+  };
+  // the first and the last block of group g that one of its rows sees: all of them up to that of its last row
+  auto tiles_of = [&](int g) { return min(NQ, (p.c.rows - g * kRows + kKeys - 1) / kKeys); };
+
+  if (warp == 16) {
+    constexpr int CB = HD / 64;
+    const Pages& pages = p.c.pages;
+    const int log = 7 - pages.log;
+    const bool issues = lane < CB << log;
+    const int cb = lane % CB, unit = lane / CB;
+    const int first = ((int)lo << log) + unit, end = issues ? min((int)hi << log, (int)((s + a.T - 1) >> pages.log) + 1) : 0;   // pages
+    auto lookup = [&](int j) {
+      const int i = first + (j << log);
+      return i >= end ? kvh : max(pages.page_of(b, (int64_t)i << pages.log), 0) * a.HKV + kvh;
+    };
+    int done = 0;
+    bool ok = true;
+    for (int g = 0; g < groups; ++g) {
+      int next = lookup(0);
+      meet();
+      for (int j = 0; ok && j < n_blk; ++j) {
+        const int it = g * n_blk + j, st = it & 1, z = next;
+        next = lookup(j + 1);
+        ok = it < 2 || wait_all(&sm.k_empty[st], (it >> 1) - 1);
+        if (!ok) break;
+        if (lane == 0) tc5::mbar_expect_tx(&sm.k_full[st], kKeys * HD * 2);
+        __syncwarp();
+        if (issues)
+          tc5::tma_load_3d(sm.k[st] + cb * (kKeys * 128) + (unit << (pages.log + 7)), &p.map, 64 * cb, 0, z, &sm.k_full[st]);
+        done = it + 1;
+      }
+      // no copy is in flight when the CTA ends
+      if (g + 1 == groups || !ok)
+        for (int it = max(0, done - 2); it < done; ++it) wait(&sm.k_full[it & 1], it >> 1);
+    }
+  } else if (warp == 17) {
+    const bool one = elected();
+    constexpr uint32_t kId = tc5::idesc_bf16(128, kKeys, false, false);
+    constexpr uint64_t kTile = (kKeys * HD * 2) >> 4;
+    const uint64_t q_desc = tc5::sdesc(tc5::smem_u32(sm.q[0]), 16, 1024), k_desc = tc5::sdesc(tc5::smem_u32(sm.k[0]), 16, 1024);
+    uint32_t used = 0;                           // parity of each tile's next wait for its columns; a first use does not wait
+    uint32_t first = (1u << NQ) - 1;
+    bool ok = true;
+    for (int g = 0; g < groups; ++g) {
+      meet();
+      const uint32_t tu = __shfl_sync(0xffffffffu, sm.tbase, 0);
+      const int nq = tiles_of(g);
+      for (int j = 0; ok && j < n_blk; ++j) {
+        const int it = g * n_blk + j, st = it & 1;
+        ok = wait_all(&sm.k_full[st], it >> 1);
+        for (int i = 0; ok && i < nq; ++i) {
+          if (first >> i & 1) {
+            first &= ~(1u << i);
+          } else {
+            ok = wait_all(&sm.s_empty[i], (int)(used >> i & 1));
+            used ^= 1u << i;
+          }
+          if (!ok) break;
+          tc5::fence_after_sync();
+          if (one) {
+#pragma unroll
+            for (int ks = 0; ks < HD / 16; ++ks) {
+              constexpr uint64_t kBlock = (kKeys * 128) >> 4;
+              const uint64_t at = (ks >> 2) * kBlock + (ks & 3) * 2;
+              tc5::mma_ss(tu + i * 128, k_desc + st * kTile + at, q_desc + i * kTile + at, kId, ks > 0);
+            }
+            tc5::commit(&sm.s_full[i]);
+          }
+        }
+        if (ok && one) tc5::commit(&sm.k_empty[st]);
+      }
+    }
+    if (ok) wait_all(&sm.k_empty[(total - 1) & 1], (total - 1) >> 1);   // no arrival is under way when the CTA ends
+  } else {
+    // ---- a thread is key 32 (warp % 4) + lane of a block, for the rows of tile warp / 4
+    const int i = warp >> 2, key = 32 * (warp & 3) + lane;
+    const float scale = a.sm_scale * kLog2e;
+    const uint64_t scale2 = pair(scale, scale);
+    const int64_t cap = a.width * a.page;
+    float* record = a.weight + (int64_t)head * cap;
+    bool ok = true;
+    int uses = 0;                                // of this tile's columns so far
+    for (int g = 0; g < groups; ++g) {
+      const int row0 = g * kRows, nq = tiles_of(g);
+      // this group's queries, sums and tokens (its first rows' MMAs of the group before are done: their scores were read)
+      copy_queries<HD>(p, sm.q[0], b, kvh, row0, warp * 32, lane);
+      copy_queries<HD>(p, sm.q[0], b, kvh, row0, warp * 32 + 16, lane);
+      const int r = row0 + tid;
+      sm.lse[tid] = r < p.c.rows ? p.lse[(int64_t)head * p.c.rows + r] : -neg_inf();
+      sm.token[tid] = token_of(p, min(r, p.c.rows - 1));
+      asm volatile("cp.async.wait_all;\nfence.proxy.async.shared::cta;\n" ::: "memory");
+      meet();
+      const uint32_t ts = sm.tbase + i * 128 + ((uint32_t)(32 * (warp & 3)) << 16);
+      const int first_token = token_of(p, row0);
+      for (int j = 0; j < n_blk; ++j) {
+        const int64_t key0 = (lo + j) * kKeys;
+        float sum = 0.f;
+        if (i < nq) {
+          ok = ok && wait(&sm.s_full[i], uses);
+          ++uses;
+          ok = __all_sync(0xffffffffu, ok);
+          __syncwarp();
+          if (ok) {
+            tc5::fence_after_sync();
+            const bool masked = key0 + kKeys > s + 1 + first_token;     // the same for all threads
+            const int rel = (int)max(min(key0 + key - s, (int64_t)0x7fffffff), (int64_t)-1);   // the first token that sees this key
+            uint64_t acc = 0;
+#pragma unroll 1
+            for (int c = 0; c < kKeys; c += 32) {
+              uint32_t x[32];
+              tc5::ld32(ts + c, x);
+              const float4* lse = reinterpret_cast<const float4*>(sm.lse + i * kKeys + c);
+              const int4* token = reinterpret_cast<const int4*>(sm.token + i * kKeys + c);
+              tc5::ld_wait();
+#pragma unroll
+              for (int u = 0; u < 8; ++u) {
+                const float4 z = lse[u];
+                const float2 a0 = unpair(fma2(pair(__uint_as_float(x[4 * u]), __uint_as_float(x[4 * u + 1])), scale2, pair(-z.x, -z.y)));
+                const float2 a1 = unpair(fma2(pair(__uint_as_float(x[4 * u + 2]), __uint_as_float(x[4 * u + 3])), scale2, pair(-z.z, -z.w)));
+                float e0 = ex2(a0.x), e1 = ex2(a0.y), e2 = ex2(a1.x), e3 = ex2(a1.y);
+                if (masked) {
+                  const int4 t = token[u];
+                  e0 = t.x >= rel ? e0 : 0.f;
+                  e1 = t.y >= rel ? e1 : 0.f;
+                  e2 = t.z >= rel ? e2 : 0.f;
+                  e3 = t.w >= rel ? e3 : 0.f;
+                }
+                acc = add2(acc, add2(pair(e0, e1), pair(e2, e3)));
+              }
+            }
+            const float2 x = unpair(acc);
+            sum = x.x + x.y;
+          }
+          tc5::fence_before_sync();
+          tc5::mbar_arrive(&sm.s_empty[i]);
+        }
+        // the tiles' sums of a key meet, in the order of the tiles
+        sm.sum[j & 1][i][key] = sum;
+        __syncwarp();
+        asm volatile("barrier.sync 1, 512;\n" ::: "memory");
+        if (i == (j & 3) && key0 + key < s + a.T) {
+          float w = 0.f;
+#pragma unroll
+          for (int x = 0; x < NQ; ++x) w += sm.sum[j & 1][x][key];
+          record[key0 + key] += w;
+        }
+      }
+    }
+  }
+  meet();
+  if (warp == 17) tc5::tmem_dealloc(sm.tbase, 512);
+  if (tid == 0 && sm.err && a.status) atomicOr(a.status, 2);
+}
+
+struct Plan {
+  int tiles, splits, ranges;
+  size_t part, ml, lse, bytes;                   // offsets
+};
+
+Plan plan_of(int B, int T, int H, int HKV, int HD, int64_t n, bool weigh) {
+  Plan pl;
+  const int64_t rows = (int64_t)T * (H / HKV), heads = (int64_t)B * HKV, blocks = (n + T + kKeys - 1) / kKeys;
+  pl.tiles = (int)((rows + 255) / 256);
+  // as many splits as fill the machine, of four blocks or more
+  int64_t splits = 148 / (heads * pl.tiles);
+  const int64_t most = blocks / 4;
+  if (splits > most) splits = most;
+  pl.splits = splits < 1 ? 1 : (int)splits;
+  // ranges of keys: two waves of CTAs or so, of two blocks or more each
+  int64_t ranges = 2 * 148 / heads;
+  if (ranges > blocks / 2) ranges = blocks / 2;
+  pl.ranges = ranges < 1 ? 1 : (int)ranges;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t was = at;
+    at += (bytes + 15) & ~(size_t)15;
+    return was;
+  };
+  const size_t parts = pl.splits > 1 ? (size_t)heads * (size_t)rows * (size_t)pl.splits : 0;
+  pl.part = take(parts * (size_t)HD * 4);
+  pl.ml = take(parts * 8);
+  pl.lse = take(weigh ? (size_t)heads * (size_t)rows * 4 : 0);
+  pl.bytes = at;
+  return pl;
+}
+
+template <int HD>
+int launch(Params& p, const Plan& pl, cudaStream_t s) {
+  const size_t smem = sizeof(Smem<HD>) + 1024, rsmem = sizeof(RecordSmem<HD>) + 1024;
+  if (cudaFuncSetAttribute(paged_prompt_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+      cudaFuncSetAttribute(paged_prompt_record_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rsmem) != cudaSuccess)
+    return BOLT3_ERR_CUDA;
+  const int64_t heads = (int64_t)p.c.a.B * p.c.a.HKV;
+  if (launch_overlapped(paged_prompt_kernel<HD>, dim3((unsigned)(heads * pl.tiles), (unsigned)pl.splits), dim3(kThreads), smem, s,
+                        p) != cudaSuccess)
+    return BOLT3_ERR_CUDA;
+  if (pl.splits > 1 && launch_overlapped(paged_prompt_join_kernel<HD>, dim3((unsigned)((heads * p.c.rows + 3) / 4)), dim3(128), 0, s,
+                                         p) != cudaSuccess)
+    return BOLT3_ERR_CUDA;
+  if (p.lse != nullptr && launch_overlapped(paged_prompt_record_kernel<HD>, dim3((unsigned)(heads * pl.ranges)), dim3(kRecordThreads),
+                                            rsmem, s, p) != cudaSuccess)
+    return BOLT3_ERR_CUDA;
+  return BOLT3_OK;
+}
+
+}  // namespace
+
+namespace paged {
+
+size_t prompt_workspace(int B, int T, int H, int HKV, int HD, int64_t n, bool weigh) {
+  return plan_of(B, T, H, HKV, HD, n, weigh).bytes;
+}
+
+int prompt_launch(const Attend& c, cudaStream_t s) {
+  const bolt3_paged_attend_args& a = c.a;
+  const Plan pl = plan_of(a.B, a.T, a.H, a.HKV, a.HD, c.len.cap - a.T, a.weight != nullptr);
+  const int64_t heads = (int64_t)a.B * a.HKV;
+  if (heads * pl.tiles > 0x7fffffff || heads * pl.ranges > 0x7fffffff || (heads * c.rows + 3) / 4 > 0x7fffffff) return BOLT3_ERR_SHAPE;
+  Params p;
+  if (!encode_pool(&p.map, a.pages, a.n_pages, a.page, a.HKV, a.HD, a.page)) return BOLT3_ERR_CUDA;
+  p.c = c;
+  p.per_G = c.G == 1 ? 0 : 0xffffffffu / c.G + 1;
+  p.tiles = pl.tiles;
+  p.splits = pl.splits;
+  p.ranges = pl.ranges;
+  char* ws = reinterpret_cast<char*>(a.workspace);
+  p.part = reinterpret_cast<float*>(ws + pl.part);
+  p.part_ml = reinterpret_cast<float2*>(ws + pl.ml);
+  p.lse = a.weight != nullptr ? reinterpret_cast<float*>(ws + pl.lse) : nullptr;
+  return a.HD == 128 ? launch<128>(p, pl, s) : launch<64>(p, pl, s);
+}
+
+}  // namespace paged

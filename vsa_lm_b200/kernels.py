@@ -756,6 +756,129 @@ def _attend_workspace(B: int, T: int, H: int, HKV: int, HD: int, n: int) -> int:
     return _lib.load().bolt3_kv8_attend_workspace(B, T, H, HKV, HD, n)
 
 
+# ---- paged bf16 KV cache of a softmax anchor (include/bolt3.h: bolt3_paged_*)
+
+def _need_pages(pages, table, dev: int) -> tuple:
+    """(pages of the pool, HKV, rows of a page, HD, B, pages of a sequence, table's row stride, address of pages, of
+    table): pages bf16 [2, P, HKV, page, HD], table int32 [B, W] with dense rows."""
+    at = _fits(pages, torch.bfloat16, dev, "pages", 1)
+    sh = pages.shape
+    if len(sh) != 5 or sh[0] != 2 or sh[3] not in (16, 32, 64, 128) or sh[4] not in (64, 128):
+        raise ValueError(f"pages must be [2, P, HKV, 16, 32, 64 or 128, 64 or 128], got {tuple(sh)}")
+    if type(table) is not torch.Tensor or table.dtype is not torch.int32 or table.get_device() != dev:
+        _need(table, torch.int32, "table")
+    ts, st = table.shape, table.stride()
+    if len(ts) != 2 or ts[0] < 1 or ts[1] < 1 or (st[1] != 1 and ts[1] > 1):
+        raise ValueError(f"table must be [B, pages of a sequence] with dense rows, got {tuple(ts)} strides {st}")
+    return sh[1], sh[2], sh[3], sh[4], ts[0], ts[1], (ts[1] if ts[0] == 1 else st[0]), at, table.data_ptr()
+
+
+def _need_records(weight, order, B: int, HKV: int, cap: int, dev: int) -> tuple[int, int]:
+    at = [0, 0]
+    for i, (t, dtype, name) in enumerate(((weight, torch.float32, "weight"), (order, torch.int32, "order"))):
+        if t is not None:
+            at[i] = _fits(t, dtype, dev, name, 1)
+            if t.shape != (B, HKV, cap):
+                raise ValueError(f"{name} must be [{B}, {HKV}, {cap}] for these pages, got {tuple(t.shape)}")
+    return at[0], at[1]
+
+
+def paged_append(*, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, n: int,
+                 pos0: int, inv_freq: torch.Tensor | None = None, q_norm: torch.Tensor | None = None,
+                 k_norm: torch.Tensor | None = None, eps: float = 1e-6, lens: torch.Tensor | None = None,
+                 pos: torch.Tensor | None = None, weight: torch.Tensor | None = None, order: torch.Tensor | None = None,
+                 q_out: torch.Tensor | None = None, status=None, dev_pos: "DevicePosition | None" = None) -> torch.Tensor:
+    """T new tokens of every sequence into a paged cache (bolt3_paged_append): per-head RMSNorm of q and k (weights
+    q_norm, k_norm fp32 [HD]; None: no norm), rotate-half RoPE at position pos0 + t (inv_freq fp32 [HD / 2]; None: no
+    rotation), k and v into rows n .. n + T - 1. pages is the pool, bf16 [2, P, HKV, page, HD]; table int32 [B, W] names each
+    sequence's pages, in order. Returns the rotated queries, bf16 [B, T, H, HD]. With `lens` (int32 [B] on the device, at most
+    n) sequence b appends at row lens[b], at position pos0 + lens[b] - n, or pos[b] with `pos` (int32 [B]); lens[b] = -1 skips it
+    (its queries are 0). weight (fp32 [B, HKV, W * page]) and order (int32, the same shape), both or none: the new rows'
+    records become 0 and the position."""
+    dev = _here()
+    T = _tokens(q, "q")
+    P, HKV, page, HD, B, W, stride, at, tat = _need_pages(pages, table, dev)
+    H, q_sb, q_st = _heads(q, "q", B, T, HD, dev)
+    _tokens(k, "k"), _tokens(v, "v")
+    hk, k_sb, k_st = _heads(k, "k", B, T, HD, dev)
+    hv, v_sb, v_st = _heads(v, "v", B, T, HD, dev)
+    if hk != HKV or hv != HKV:
+        raise ValueError(f"k and v hold {hk} and {hv} heads, the cache {HKV}")
+    if (weight is None) != (order is None):
+        raise ValueError("weight and order are given together")
+    w_at, o_at = (0, 0) if weight is None else _need_records(weight, order, B, HKV, W * page, dev)
+    if pos is not None and lens is None:
+        raise ValueError("positions of their own (pos) go with lengths of their own (lens)")
+    if q_out is None:
+        q_out = torch.empty((B, T, H, HD), dtype=torch.bfloat16, device=q.device)
+    _lib.paged_append(
+        torch._C._cuda_getCurrentRawStream(dev), B, T, H, HKV, HD, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_sb, q_st, k_sb,
+        k_st, v_sb, v_st, _maybe(q_norm, torch.float32, dev, "q_norm", HD), _maybe(k_norm, torch.float32, dev, "k_norm", HD),
+        eps, _maybe(inv_freq, torch.float32, dev, "inv_freq", HD // 2),
+        _fits(q_out, torch.bfloat16, dev, "q_out", B * T * H * HD), at, P, page, tat, stride, W, w_at, o_at, n, pos0,
+        _lens_ptr(lens, dev_pos, B, dev), 0 if pos is None else _lens_ptr(pos, None, B, dev), _status_ptr(status),
+        *_pos_fields(dev_pos))
+    _count(1)
+    return q_out
+
+
+def paged_attend(*, q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, n: int, sm_scale: float | None = None,
+                 lens: torch.Tensor | None = None, weight: torch.Tensor | None = None, y: torch.Tensor | None = None,
+                 status=None, dev_pos: "DevicePosition | None" = None) -> torch.Tensor:
+    """Softmax attention of the T newest tokens, q = [B, T, H, HD] (or [B, T, H * HD]), over a paged cache that holds n
+    rows before them and has them appended (bolt3_paged_attend): query t sees rows 0 .. n + t. With `lens` sequence b holds
+    lens[b] rows before them (-1: idle, its outputs are 0), at most n. `weight` (fp32 [B, HKV, W * page]): the softmax weight
+    of every row, summed over the query rows of its head, is added to its record. Returns y, bf16 [B, T, H * HD]."""
+    dev = _here()
+    T = _tokens(q, "q")
+    P, HKV, page, HD, B, W, stride, at, tat = _need_pages(pages, table, dev)
+    H, q_sb, q_st = _heads(q, "q", B, T, HD, dev)
+    w_at = 0 if weight is None else _need_records(weight, None, B, HKV, W * page, dev)[0]
+    if y is None:
+        y = torch.empty((B, T, H * HD), dtype=torch.bfloat16, device=q.device)
+    nbytes, launches = _paged_workspace(B, T, H, HKV, HD, n + (0 if dev_pos is None else dev_pos.span - 1), w_at != 0)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _lib.paged_attend(
+        torch._C._cuda_getCurrentRawStream(dev), B, T, H, HKV, HD, q.data_ptr(), q_sb, q_st, at, P, page, tat, stride, W, w_at,
+        n, _lens_ptr(lens, dev_pos, B, dev), _fits(y, torch.bfloat16, dev, "y", B * T * H * HD),
+        HD ** -0.5 if sm_scale is None else sm_scale, 0 if ws is None else ws.data_ptr(), nbytes, _status_ptr(status),
+        *_pos_fields(dev_pos))
+    _count(launches)
+    return y
+
+
+@functools.lru_cache(maxsize=1024)
+def _paged_workspace(B: int, T: int, H: int, HKV: int, HD: int, n: int, weigh: bool) -> tuple[int, int]:
+    """Workspace bytes of a paged_attend call and the kernels it launches (at least: one for the attention, one to join
+    partial sums where there are any)."""
+    fn = _lib.load().bolt3_paged_attend_workspace
+    return fn(B, T, H, HKV, HD, n, int(weigh)), 2 if fn(B, T, H, HKV, HD, n, 0) else 1
+
+
+def paged_evict(*, pages: torch.Tensor, table: torch.Tensor, weight: torch.Tensor, order: torch.Tensor, n: int, keep: int,
+                recent: int = 0, lens: torch.Tensor | None = None, status=None) -> "int | torch.Tensor":
+    """Every (sequence, KV head) of a paged cache that holds more than `keep` rows drops all but `keep` of them, in place
+    (bolt3_paged_evict): it keeps those whose `order` (position) is above its newest minus `recent`, then those of the
+    largest `weight`, equal ones by the lowest row. Kept rows from behind `keep` move into the places of dropped ones, so the
+    rows of a head are in no order afterwards; `order` tells their positions. Holding n rows, or lens[b] <= n (int32 [B],
+    -1: idle). Returns the rows that are left: min(n, keep), or with `lens` a new int32 [B]."""
+    dev = _here()
+    P, HKV, page, HD, B, W, stride, at, tat = _need_pages(pages, table, dev)
+    if weight is None or order is None:
+        raise ValueError("an eviction needs weight and order")
+    w_at, o_at = _need_records(weight, order, B, HKV, W * page, dev)
+    if keep < 1 or not 0 <= recent <= keep:
+        raise ValueError(f"keep must be at least 1 and recent within [0, keep], got keep={keep} recent={recent}")
+    out = None if lens is None else torch.empty(B, dtype=torch.int32, device=pages.device)
+    nbytes = _lib.load().bolt3_paged_evict_workspace(B, HKV, n, keep)
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=pages.device)
+    _lib.paged_evict(torch._C._cuda_getCurrentRawStream(dev), B, HKV, HD, at, P, page, tat, stride, W, w_at, o_at, n, keep, recent,
+                     _lens_ptr(lens, None, B, dev), 0 if out is None else out.data_ptr(), ws.data_ptr(), nbytes,
+                     _status_ptr(status))
+    _count(1)
+    return min(n, keep) if out is None else out
+
+
 # ---- beam search (include/bolt3.h: bolt3_beam_*)
 
 @functools.lru_cache(maxsize=256)
