@@ -72,7 +72,7 @@ class BeamStates:
         self.plan = None
 
     def _items(self):
-        from .bolt3 import Bolt3LayerState
+        from .bolt3 import AnchorKVPaged, Bolt3LayerState
 
         items = []
         for s, c in zip(self.states, self.kv):
@@ -80,18 +80,24 @@ class BeamStates:
                 items += [(t, 0, None) for t in _layer_tensors(c)]
                 if c.has_bank:
                     items.append((s, 0, None))
-            else:
+            elif not isinstance(c, AnchorKVPaged):
                 items += [(t, 1, 3) for t in c.tensors()]
         return items
 
     def reorder(self, parent: torch.Tensor) -> None:
-        """Every beam's state becomes that of its parent (int32 [groups, beams], as beam_select gives it)."""
+        """Every beam's state becomes that of its parent (int32 [groups, beams], as beam_select gives it). Paged caches
+        move their tables and the page that is not full yet."""
+        from .bolt3 import AnchorKVPaged
+
         items = self._items()
         if self.plan is None or len(items) != len(self.plan.tensors) or any(
                 a[0] is not b for a, b in zip(items, self.plan.tensors)):
             self.plan = K.BeamReorder(items, self.groups, self.beams)
         n = max((c.n for c in self.kv if hasattr(c, "tensors")), default=0)
         self.plan(parent, t0=min(self.shared, n), t1=n)
+        for c in self.kv:
+            if isinstance(c, AnchorKVPaged):
+                c.reorder(parent)
 
 
 def backtrack(tokens: list, parents: list, pad: int) -> torch.Tensor:
@@ -116,6 +122,9 @@ def beam_search(dec, ids: torch.Tensor, beams: int, max_new_tokens: int, eos_ids
     among the beams. Stops early once all beams have finished (looked at every 16 tokens)."""
     if beams < 1 or beams > 16 or max_new_tokens < 1:
         raise ValueError(f"{beams} beams and {max_new_tokens} tokens: 1 to 16 beams, at least one token")
+    if dec.kv_budget is not None:
+        raise ValueError("beams share the pages of their past, which a cache with a budget moves: beam search takes a paged "
+                         "cache without one, or another kind")
     eos = tuple(int(e) for e in (sorted(eos_ids) if isinstance(eos_ids, (set, frozenset)) else eos_ids))
     B, T = ids.shape
     dev = ids.device

@@ -540,14 +540,19 @@ class Bolt3Decoder:
     """Constant-memory decoder (reference: vsa_lm/config/bolt3.py:279-557) with native Bolt-3 layers.
 
     Softmax anchor layers use a static KV cache and SDPA as in the reference (bolt3.py:426-445), or, with
-    kv_cache="int8", an 8-bit cache with kernels of its own for prompts and single tokens.
+    kv_cache="int8", an 8-bit cache, or, with kv_cache="paged", a paged one, with kernels of their own for prompts and
+    single tokens. A paged cache may be bounded: with kv_budget rows per KV head it keeps the kv_recent newest tokens (half
+    of the budget by default) and those with the most attention so far, so that the whole decode state stays constant.
     """
 
     def __init__(self, model, wrap_positions: bool = False, max_cache_pos: int = 65536, cuda_graphs: bool = True,
-                 kv_cache: str = "bf16", **kwargs):
+                 kv_cache: str = "bf16", kv_budget: int | None = None, kv_recent: int | None = None, kv_page: int = 64,
+                 **kwargs):
         self.model = model.eval()
-        _check_kv_cache(kv_cache, model)
-        self.kv_cache = kv_cache          # the anchors' caches: "bf16" (as the reference) or "int8" (AnchorKV8)
+        _check_kv_cache(kv_cache, model, kv_budget, kv_recent, kv_page)
+        # the anchors' caches: "bf16" (as the reference), "int8" (AnchorKV8) or "paged" (AnchorKVPaged)
+        self.kv_cache = kv_cache
+        self.kv_budget, self.kv_recent, self.kv_page = kv_budget, kv_recent, kv_page
         self.max_T = model.config["max_T"]
         self.max_cache_pos = max_cache_pos
         self.C = int(model.config.get("bolt3_C", 128))
@@ -556,25 +561,31 @@ class Bolt3Decoder:
         self.use_cuda_graphs = cuda_graphs
 
     @staticmethod
-    def state_bytes(model, kv_cache: str = "bf16"):
+    def state_bytes(model, kv_cache: str = "bf16", kv_budget: int | None = None, kv_page: int = 64):
         """(bytes of fixed-size state per sequence, bytes per token of the anchor layers' KV caches),
         the same pair the reference reports (bolt3.py:290-300), counted from the buffers this
         decoder actually keeps (Bolt3LayerState.bytes_per_sequence, AnchorKV's bf16 k and v or AnchorKV8's
-        int8 with a scale per row)."""
-        _check_kv_cache(kv_cache)
+        int8 with a scale per row). A paged cache with a budget is of fixed size: its pages of budget + 2 C rows, with
+        weight and position of each."""
+        _check_kv_cache(kv_cache, None, kv_budget, None, kv_page)
         fixed = sum(Bolt3LayerState.bytes_per_sequence(b.vsa) for b in model.blocks if hasattr(b, "vsa"))
         row = (lambda hd: hd + 4) if kv_cache == "int8" else (lambda hd: 2 * hd)
         per_token = sum(2 * b.attn.HKV * row(b.attn.HD) for b in model.blocks if not hasattr(b, "vsa"))
+        if kv_budget is not None:
+            rows = -(-(kv_budget + 2 * int(model.config.get("bolt3_C", 128))) // kv_page) * kv_page
+            records = sum(8 * b.attn.HKV for b in model.blocks if not hasattr(b, "vsa"))
+            return fixed + rows * (per_token + records), 0
         return fixed, per_token
 
     @staticmethod
     def blank_state(model, batch_size: int, device, max_kv_len: int = 4096, state_dtype=torch.float32,
-                    kv_cache: str = "bf16", **kwargs):
+                    kv_cache: str = "bf16", kv_budget: int | None = None, kv_recent: int | None = None, kv_page: int = 64,
+                    **kwargs):
         """(states, kv_caches) for `batch_size` sequences (bolt3.py:302-319): per Bolt-3 layer an fp32
         M_res [B, HKV, HD, HD] in states and a Bolt3LayerState in kv_caches; per softmax anchor an
-        AnchorKV (kv_cache "int8": an AnchorKV8) with room for max_kv_len tokens. M_res is always fp32 (the
-        kernels update it in place)."""
-        _check_kv_cache(kv_cache, model)
+        AnchorKV (kv_cache "int8": an AnchorKV8, "paged": an AnchorKVPaged) with room for max_kv_len tokens (with a
+        kv_budget: for what it holds at most). M_res is always fp32 (the kernels update it in place)."""
+        _check_kv_cache(kv_cache, model, kv_budget, kv_recent, kv_page)
         states, kv_caches = [], []
         for blk in model.blocks:
             if hasattr(blk, "vsa"):
@@ -584,6 +595,10 @@ class Bolt3Decoder:
             else:
                 a = blk.attn
                 states.append(None)
+                if kv_cache == "paged":
+                    kv_caches.append(AnchorKVPaged(batch_size, a.HKV, max_kv_len, a.HD, device, page=kv_page, budget=kv_budget,
+                                                   recent=kv_recent, chunk=int(model.config.get("bolt3_C", 128))))
+                    continue
                 kv_caches.append(AnchorKV8(batch_size, a.HKV, max_kv_len, a.HD, device) if kv_cache == "int8" else
                                  AnchorKV(batch_size, a.HKV, max_kv_len, a.HD, device, dt=torch.bfloat16))
         return states, kv_caches
@@ -596,13 +611,13 @@ class Bolt3Decoder:
         for st in kv_caches:
             if isinstance(st, Bolt3LayerState):
                 st.status.settle("Bolt-3 decode steps") if block else st.status.check(block)
-            elif isinstance(st, AnchorKV8):
+            elif isinstance(st, (AnchorKV8, AnchorKVPaged)):
                 st.check_status(block)
 
     @staticmethod
     def _check_anchors(kv_caches) -> None:
-        """check_status of the 8-bit anchor caches alone, at the end of a generation."""
-        Bolt3Decoder.check_status([c for c in kv_caches if isinstance(c, AnchorKV8)])
+        """check_status of the 8-bit and paged anchor caches alone, at the end of a generation."""
+        Bolt3Decoder.check_status([c for c in kv_caches if isinstance(c, (AnchorKV8, AnchorKVPaged))])
 
     # ---- decode state in the reference's format (bolt3.py:302-319 creates it, :343-425 fills it):
     # per Bolt-3 layer a dict with the bank (ak/av [b*HKV, S, HD], mass/util/pm fp32 [b*HKV, S], act
@@ -916,7 +931,7 @@ class Bolt3Decoder:
         dev_pos (a step captured into a CUDA graph) the position comes from the device and the cache's
         host count is left to the caller."""
         b, t, _ = h.shape
-        if isinstance(cache, AnchorKV8):
+        if isinstance(cache, (AnchorKV8, AnchorKVPaged)):
             y = cache.attention(ly, h, pos_start, dev_pos)
             return Bolt3Decoder._anchor_out(ly, y, partial_fp32)
         q, k, v = ly.head_qkv(h)
@@ -989,7 +1004,7 @@ class Bolt3Decoder:
         for li, blk in enumerate(self.model.blocks):
             if hasattr(blk, "vsa"):
                 self._layer_advance(blk.vsa, kv_caches[li], t, pos_start, states[li])
-            elif isinstance(kv_caches[li], AnchorKV8):
+            elif isinstance(kv_caches[li], (AnchorKV8, AnchorKVPaged)):
                 kv_caches[li].advance(t)
             else:
                 kv_caches[li].n += t
@@ -1023,7 +1038,8 @@ class Bolt3Decoder:
     def prefill(self, ids: torch.Tensor, max_kv_len: int = 4096):
         """Fresh state for ids [b, t] and the prompt run through it (bolt3.py:449-457)."""
         states, kv = self.blank_state(self.model, ids.shape[0], ids.device, max_kv_len=max(max_kv_len, ids.shape[1] + 1024),
-                                      kv_cache=self.kv_cache)
+                                      kv_cache=self.kv_cache, kv_budget=self.kv_budget, kv_recent=self.kv_recent,
+                                      kv_page=self.kv_page)
         h, _ = self._feed(ids, 0, states, kv)
         return h, states, kv
 
@@ -1157,15 +1173,21 @@ class Bolt3Decoder:
         return states
 
 
-def _check_kv_cache(kind: str, model=None) -> None:
-    """`kind` is a kind of cache and, with a model, one whose kernels serve the model's anchors."""
-    if kind not in ("bf16", "int8"):
-        raise ValueError(f"kv_cache must be 'bf16' or 'int8', got {kind!r}")
-    if kind == "int8" and model is not None:
+def _check_kv_cache(kind: str, model=None, budget: int | None = None, recent: int | None = None, page: int = 64) -> None:
+    """`kind` is a kind of cache and, with a model, one whose kernels serve the model's anchors; a budget, its recent rows and
+    the page size are a paged cache's."""
+    if kind not in ("bf16", "int8", "paged"):
+        raise ValueError(f"kv_cache must be 'bf16', 'int8' or 'paged', got {kind!r}")
+    if kind == "paged":
+        check_budget(page, budget, recent)
+    elif budget is not None or recent is not None:
+        raise ValueError(f"a budget of rows goes with kv_cache='paged', got {kind!r}")
+    if kind != "bf16" and model is not None:
+        what = "8-bit" if kind == "int8" else "paged"
         for blk in model.blocks:
             a = getattr(blk, "attn", None)
             if a is not None and (a.HD not in (64, 128) or a.H % a.HKV or a.H // a.HKV > 16 or a.H + 2 * a.HKV > 4096):
-                raise ValueError(f"8-bit caches hold heads of 64 or 128, at most 16 query heads to a KV head, got "
+                raise ValueError(f"{what} caches hold heads of 64 or 128, at most 16 query heads to a KV head, got "
                                  f"{a.H} on {a.HKV} of {a.HD}; use kv_cache='bf16'")
 
 
@@ -1367,6 +1389,7 @@ class _ChunkGraph:
     def _phase(self) -> int: ...
     def _prepare(self, span: int) -> None: ...
     def _body(self, pos: int) -> torch.Tensor: ...
+    def _trial(self, pos: int) -> None: self._body(pos)
     def _advance(self, pos: int) -> None: ...
 
     @K.traced("DecodeGraph.capture")
@@ -1379,7 +1402,7 @@ class _ChunkGraph:
         if self.captures == 0:
             # first capture: one eager run of the same launches initialises the libraries' lazy state
             # (it rewrites exactly what the replay below writes: this step's window and cache rows)
-            self._body(pos)
+            self._trial(pos)
         # captured on a side stream that joins the current one; torch.cuda.graph() would also run a
         # garbage collection and empty the allocator cache at every capture, once per chunk here
         main = torch.cuda.current_stream()
@@ -1432,11 +1455,11 @@ class DecodeGraph(_ChunkGraph):
 
     def __init__(self, dec: "Bolt3Decoder", states, kv_caches):
         bolt = [st for st in kv_caches if isinstance(st, Bolt3LayerState)]
-        anch = [c for c in kv_caches if isinstance(c, (AnchorKV, AnchorKV8))]
+        anch = [c for c in kv_caches if isinstance(c, (AnchorKV, AnchorKV8, AnchorKVPaged))]
         ref = bolt[0].ring_kp if bolt else anch[0].tensors()[0]
         super().__init__(ref.device, dec.C)
         self.dec, self.states, self.kv = dec, states, kv_caches
-        self.B = bolt[0].B if bolt else ref.shape[1]
+        self.B = bolt[0].B if bolt else anch[0].B if isinstance(anch[0], AnchorKVPaged) else ref.shape[1]
         self.tok = torch.zeros(self.B, 1, dtype=torch.long, device=self.device)
 
     def _phase(self) -> int:
@@ -1455,8 +1478,18 @@ class DecodeGraph(_ChunkGraph):
     def _body(self, pos: int) -> torch.Tensor:
         return self.dec._blocks(self.tok, pos, self.states, self.kv, dev_pos=self.pos)
 
+    def _trial(self, pos: int) -> None:
+        # records of attention weights are added to, not rewritten: the step counts once
+        records = [(c, c.weight.clone()) for c in self.kv if isinstance(c, AnchorKVPaged) and c.weight is not None]
+        self._body(pos)
+        for c, weight in records:
+            c.weight.copy_(weight)
+
     def _advance(self, pos: int) -> None:
+        n = [c.n for c in self.kv if isinstance(c, AnchorKVPaged)]
         self.dec._advance(1, pos, self.states, self.kv)
+        if any(c.n != x + 1 for c, x in zip((c for c in self.kv if isinstance(c, AnchorKVPaged)), n)):
+            self.hi = pos + 1             # a cache dropped rows: the next step's launches have other row numbers
 
     @torch.no_grad()
     def step(self, tokens: torch.Tensor, pos: int) -> torch.Tensor:
@@ -1473,6 +1506,8 @@ class DecodeGraph(_ChunkGraph):
         self.tok.copy_(tokens)
         return self._replay(pos)
 
+
+from .paged import AnchorKVPaged, check_budget  # noqa: E402  (its attention uses helpers from above)
 
 # the reference's name for the anchor-layer cache class (vsa_lm/decode.py:88)
 StaticKV = AnchorKV
