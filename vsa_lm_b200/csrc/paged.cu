@@ -4,12 +4,13 @@
 // append, per head row x of HD values: x <- x * rsqrt(mean(x^2) + eps) * w, then the rotation of the pairs (i, i + HD/2)
 // by pos * inv_freq[i], in fp32, one rounding to bf16; values are copied. The angle's product is taken in fp64 and reduced
 // to one turn before the fp32 sine: at position 100000 an fp32 product is off by 0.004 of a radian, more than a bf16 step.
-// Bound by HBM: (2 H + 4 HKV) HD bf16 per token. A row is HD / 8 lanes, a lane holding four neighbouring values of each
-// half, so that a rotation's pair is in one lane; a block takes four tokens (few tokens: a share of one token's rows).
+// Bound by HBM: (2 H + 4 HKV) HD bf16 per token. A warp takes a token's rows (few tokens: a share of them), HD / 16 lanes to a
+// row, a lane holding eight neighbouring values of each half, so that a rotation's pair is in one lane; its lanes share the
+// token's sines and cosines out among themselves and keep them for all rows.
 //
 // evict: a CTA per (sequence, KV head). The threshold weight comes from a radix selection over the weights as ordered 32-bit
-// keys (digits of 11, 11 and 10 bits, counted in shared memory); then every thread walks a stretch of rows of its own, so that
-// one block-wide sum gives the ranks of equal weights, and one those of dropped rows below `keep` and of kept rows behind it,
+// keys (digits of 11, 11 and 10 bits, counted in shared memory); then every warp walks a stretch of rows, so that one sum over
+// the warps gives the ranks of equal weights, and one those of dropped rows below `keep` and of kept rows behind it,
 // which are paired by rank. Only those rows move. Bound by HBM: 8 bytes per row, and 8 HD + 16 per moved row.
 #include <cudaTypedefs.h>
 
@@ -55,162 +56,153 @@ using namespace paged;
 // ------------------------------------------------------------------------------------------- append
 
 constexpr int kThreads = 256;
-constexpr int kAhead = 4;                            // rows that a thread has in flight
+constexpr int kAhead = 2;                            // rows that a thread has in flight
 
-template <int LPR>
-B3_DEV float row_sum(float v) {
-#pragma unroll
-  for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// blockIdx.x = TPB tokens, blockIdx.y = share of their rows
-template <int HD, int TPB>
-__global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_constant__ bolt3_paged_append_args a,
+// A warp takes rows [c rows_per, ..) of the H + 2 HKV rows of a token, of `chunks` such stretches
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 3) paged_append_kernel(const __grid_constant__ bolt3_paged_append_args a,
                                                                 const __grid_constant__ Length len,
-                                                                const __grid_constant__ Pages pages, int rows_per_block) {
-  constexpr int LPR = HD / 8;                        // lanes of a row
-  constexpr int RPI = kThreads / LPR;                // rows of one iteration
-  __shared__ float4 trig[TPB][HD / 4];               // cos, sin of a pair of dimensions, cos, sin of the next
-  // of each token: its cache row (-1: idle), its position, its first q, k and v element, the pool row of its first head's key
-  // (-1: no page), the record of its first head
-  __shared__ int64_t s_row[TPB], s_pos[TPB], s_src[TPB][3], s_out[TPB], s_rec[TPB];
-  const int tid = threadIdx.x, part = tid % LPR;
-  const int64_t tok0 = (int64_t)blockIdx.x * TPB, tokens = (int64_t)a.B * a.T;
-  const int n_rows = a.H + 2 * a.HKV;
-  const int first = TPB == 1 ? blockIdx.y * rows_per_block : 0;
-  const int end = TPB == 1 ? min(n_rows, first + rows_per_block) : (int)min((int64_t)TPB, tokens - tok0) * n_rows;
-  const int64_t cap = a.width * a.page;
+                                                                const __grid_constant__ Pages pages, int chunks, int rows_per) {
+  constexpr int LPR = HD / 16, RPI = 32 / LPR;       // lanes of a row, rows of an iteration
+  constexpr int PPG = 8 / RPI;                       // pairs of a lane's eight whose angle it takes itself
+  __shared__ float4 s_turn[kThreads / 32][HD / 4];   // of a warp's token: cos, sin of a pair of dimensions, cos, sin of the next
+  __shared__ float4 s_norm[2][HD / 4];               // of queries, of keys
+  const int lane = threadIdx.x & 31, part = lane % LPR, sub = lane / LPR;
+  const int64_t item = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), token = item / chunks;
   grid_dep_launch();
   grid_dep_wait();
-  if (tid < TPB && tok0 + tid < tokens) {
-    bool bad = false;
-    const int b = (int)((tok0 + tid) / a.T), t = (int)((tok0 + tid) % a.T);
-    const int64_t s = len.rows(b, bad);
-    int pg = -1;
-    if (s >= 0) {
-      pg = pages.page_of(b, s + t);
-      bad |= pg < 0;
-    }
-    if (bad && a.status) atomicOr(a.status, 8);
-    s_row[tid] = s < 0 ? -1 : s + t;
-    s_pos[tid] = a.pos != nullptr ? (int64_t)a.pos[b] + t : a.pos0 + (s + t - a.n);
-    s_src[tid][0] = b * a.q_sb + t * a.q_st;
-    s_src[tid][1] = b * a.k_sb + t * a.k_st;
-    s_src[tid][2] = b * a.v_sb + t * a.v_st;
-    s_out[tid] = pg < 0 ? -1 : (int64_t)pg * a.HKV * a.page + ((s + t) & (a.page - 1));
-    s_rec[tid] = (int64_t)b * a.HKV * cap + s + t;
-  }
-  __syncthreads();
-  for (int i = tid; a.inv_freq != nullptr && i < TPB * (HD / 2); i += kThreads) {
-    const int k = i / (HD / 2), f = i % (HD / 2);
-    if (tok0 + k < tokens && s_row[k] >= 0) {
-      const double turn = (double)s_pos[k] * (double)a.inv_freq[f] * 0.15915494309189533577;   // 1 / (2 pi)
-      float sn, cs;
-      sincosf((float)((turn - rint(turn)) * 6.28318530717958647693), &sn, &cs);
-      reinterpret_cast<float2*>(trig[k])[f] = make_float2(cs, sn);
-    }
-  }
   const bool norms = a.q_norm_w != nullptr || a.k_norm_w != nullptr;
-  // whole groups of LPR lanes share a row, but the shuffles name the warp: rows past the end compute on zeros
-  // and store nothing
-  int item_r = first + tid / LPR, item_t = 0;        // row and token of this thread's next item
-  if (TPB > 1) {
-    item_t = item_r / n_rows;
-    item_r -= item_t * n_rows;
-  }
-  for (int r0 = first; r0 < end; r0 += kAhead * RPI) {
-    uint2 raw[kAhead][2];
-    int row[kAhead], tk[kAhead];                     // row of its token (-1: past the end), token of the block
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const bool live = r0 + u * RPI + tid / LPR < end;
-      tk[u] = live ? item_t : 0;
-      const int r = live ? item_r : 0;
-      row[u] = live ? r : -1;
-      const bool is_q = r < a.H, is_k = !is_q && r < a.H + a.HKV;
-      const int h = is_q ? r : is_k ? r - a.H : r - a.H - a.HKV;
-      const bf16* src = reinterpret_cast<const bf16*>(is_q ? a.q : is_k ? a.k : a.v) + s_src[tk[u]][is_q ? 0 : is_k ? 1 : 2] + h * HD;
-      raw[u][0] = raw[u][1] = make_uint2(0, 0);
-      if (live && s_row[tk[u]] >= 0) {
-        raw[u][0] = __ldg(reinterpret_cast<const uint2*>(src) + part);
-        raw[u][1] = __ldg(reinterpret_cast<const uint2*>(src + HD / 2) + part);
-      }
-      item_r += RPI;
-      if (TPB > 1)
-        while (item_r >= n_rows) {
-          item_r -= n_rows;
-          ++item_t;
-        }
+  if (norms) {
+    if (threadIdx.x < HD / 2) {
+      const float* w = threadIdx.x < HD / 4 ? a.q_norm_w : a.k_norm_w;
+      if (w != nullptr) s_norm[0][threadIdx.x] = __ldg(reinterpret_cast<const float4*>(w) + threadIdx.x % (HD / 4));
     }
-    if (r0 == first) __syncthreads();                // the sines and cosines
+    __syncthreads();
+  }
+  if (token >= (int64_t)a.B * a.T) return;
+  const int c = (int)(item - token * chunks), b = (int)(token / a.T), t = (int)(token - (int64_t)b * a.T);
+  const int n_rows = a.H + 2 * a.HKV, first = c * rows_per, end = min(n_rows, first + rows_per);
+  const bf16* q = reinterpret_cast<const bf16*>(a.q) + b * a.q_sb + t * a.q_st + 8 * part;
+  const bf16* k = reinterpret_cast<const bf16*>(a.k) + b * a.k_sb + t * a.k_st + 8 * part;
+  const bf16* v = reinterpret_cast<const bf16*>(a.v) + b * a.v_sb + t * a.v_st + 8 * part;
+  uint4 raw[kAhead][2];                              // values 8 part .., HD / 2 + 8 part ..
+  auto fetch = [&](int u, int r) {
+    if (r >= end) return;
+    const bf16* src = r < a.H ? q + r * HD : r < a.H + a.HKV ? k + (r - a.H) * HD : v + (r - a.H - a.HKV) * HD;
+    raw[u][0] = __ldg(reinterpret_cast<const uint4*>(src));
+    raw[u][1] = __ldg(reinterpret_cast<const uint4*>(src + HD / 2));
+  };
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) fetch(u, first + u * RPI + sub);
+  bool bad = false;
+  const int64_t s = len.rows(b, bad);                // the same for the whole warp
+  int pg = -1;
+  if (s >= 0) {
+    pg = pages.page_of(b, s + t);
+    bad |= pg < 0;
+  }
+  if (bad && lane == 0 && a.status) atomicOr(a.status, 8);
+  const int64_t pos = s < 0 ? 0 : a.pos != nullptr ? (int64_t)a.pos[b] + t : a.pos0 + (s + t - a.n);
+  if (first < a.H + a.HKV) {
+    float2* turns = reinterpret_cast<float2*>(s_turn[threadIdx.x >> 5]) + 8 * part + PPG * sub;
+#pragma unroll
+    for (int i = 0; i < PPG; ++i) {                  // the row groups share the work
+      float sn = 0.f, cs = 1.f;
+      if (a.inv_freq != nullptr) {
+        const double turn = (double)pos * (double)a.inv_freq[8 * part + PPG * sub + i] * 0.15915494309189533577;   // 1 / (2 pi)
+        __sincosf((float)((turn - rint(turn)) * 6.28318530717958647693), &sn, &cs);   // within 2^-21 of either, in [-pi, pi]
+      }
+      turns[i] = make_float2(cs, sn);
+    }
+    __syncwarp();
+  }
+  const uint32_t at_turn = (uint32_t)__cvta_generic_to_shared(s_turn[threadIdx.x >> 5] + 4 * part);
+  const uint32_t at_norm = (uint32_t)__cvta_generic_to_shared(s_norm[0] + 2 * part);
+  auto lds = [](uint32_t at) {                       // where it stands: kept in registers over the rows they cost the loads in flight
+    float4 z;
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];\n" : "=f"(z.x), "=f"(z.y), "=f"(z.z), "=f"(z.w) : "r"(at));
+    return z;
+  };
+  // rows past the end compute on what stands in the registers and store nothing: the shuffles name the warp
+  for (int r0 = first; r0 < end; r0 += kAhead * RPI) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      if (r0 + u * RPI >= end) break;                // the same for all threads
-      const int r = row[u];
+      if (r0 + u * RPI >= end) break;                // the same for the whole warp
+      const int r = r0 + u * RPI + sub;
       const bool is_q = r < a.H, is_k = !is_q && r < a.H + a.HKV;
-      uint2 o0 = raw[u][0], o1 = raw[u][1];
-      if (is_q || is_k || norms) {                   // (norms: the shuffles need whole warps)
-        float x[8];                                  // values 4 part .., HD / 2 + 4 part ..
-        const float2 p0 = unpack_bf16(o0.x), p1 = unpack_bf16(o0.y), p2 = unpack_bf16(o1.x), p3 = unpack_bf16(o1.y);
-        x[0] = p0.x; x[1] = p0.y; x[2] = p1.x; x[3] = p1.y; x[4] = p2.x; x[5] = p2.y; x[6] = p3.x; x[7] = p3.y;
+      uint4 o0 = raw[u][0], o1 = raw[u][1];
+      fetch(u, r + kAhead * RPI);
+      if (r0 + u * RPI < a.H + a.HKV) {              // the same for the whole warp: some of its rows are queries or keys
+        float x[8], y[8];                            // the pairs
+        {
+          const uint32_t w0[4] = {o0.x, o0.y, o0.z, o0.w}, w1[4] = {o1.x, o1.y, o1.z, o1.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 p0 = unpack_bf16(w0[i]), p1 = unpack_bf16(w1[i]);
+            x[2 * i] = p0.x; x[2 * i + 1] = p0.y;
+            y[2 * i] = p1.x; y[2 * i + 1] = p1.y;
+          }
+        }
         if (norms) {
-          const float* w = is_q ? a.q_norm_w : is_k ? a.k_norm_w : nullptr;
-          float ss = 0.f;
+          float ss = 0.f, s2 = 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-          ss = row_sum<LPR>(ss);
-          if (w != nullptr) {
+          for (int i = 0; i < 8; ++i) {
+            ss = fmaf(x[i], x[i], ss);
+            s2 = fmaf(y[i], y[i], s2);
+          }
+          ss += s2;
+#pragma unroll
+          for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          if (is_q ? a.q_norm_w != nullptr : is_k && a.k_norm_w != nullptr) {
             const float inv = rsqrtf(ss * (1.f / HD) + a.eps);
-            const float4 w0 = reinterpret_cast<const float4*>(w)[part], w1 = reinterpret_cast<const float4*>(w + HD / 2)[part];
-            const float ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * ww[i];
+            const uint32_t w = at_norm + (is_q ? 0 : HD * 4);
+            const float4 wa = lds(w), wb = lds(w + 16), wc = lds(w + HD * 2), wd = lds(w + HD * 2 + 16);
+            x[0] *= inv * wa.x; x[1] *= inv * wa.y; x[2] *= inv * wa.z; x[3] *= inv * wa.w;
+            x[4] *= inv * wb.x; x[5] *= inv * wb.y; x[6] *= inv * wb.z; x[7] *= inv * wb.w;
+            y[0] *= inv * wc.x; y[1] *= inv * wc.y; y[2] *= inv * wc.z; y[3] *= inv * wc.w;
+            y[4] *= inv * wd.x; y[5] *= inv * wd.y; y[6] *= inv * wd.z; y[7] *= inv * wd.w;
           }
         }
         if (is_q || is_k) {
-          if (a.inv_freq != nullptr) {
-            const float4* cs = trig[tk[u]] + 2 * part;
+          uint32_t w0[4], w1[4];
 #pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-              const float4 z = cs[i / 2];            // of pairs i and i + 1
-              const float a0 = x[i], b0 = x[4 + i], a1 = x[i + 1], b1 = x[5 + i];
-              x[i] = fmaf(a0, z.x, -b0 * z.y);
-              x[4 + i] = fmaf(b0, z.x, a0 * z.y);
-              x[i + 1] = fmaf(a1, z.z, -b1 * z.w);
-              x[5 + i] = fmaf(b1, z.z, a1 * z.w);
-            }
+          for (int i = 0; i < 4; ++i) {
+            const int e = 2 * i, f = e + 1;
+            const float4 z = lds(at_turn + 16 * i);  // of pairs e and f
+            w0[i] = pack_bf16(fmaf(x[e], z.x, -y[e] * z.y), fmaf(x[f], z.z, -y[f] * z.w));
+            w1[i] = pack_bf16(fmaf(y[e], z.x, x[e] * z.y), fmaf(y[f], z.z, x[f] * z.w));
           }
-          o0 = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
-          o1 = make_uint2(pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+          o0 = make_uint4(w0[0], w0[1], w0[2], w0[3]);
+          o1 = make_uint4(w1[0], w1[1], w1[2], w1[3]);
         }
       }
-      if (r < 0) continue;
-      const int h = is_q ? r : is_k ? r - a.H : r - a.H - a.HKV;
+      if (r >= end) continue;
       bf16* out;
       if (is_q) {
-        if (s_row[tk[u]] < 0) o0 = o1 = make_uint2(0, 0);
-        out = reinterpret_cast<bf16*>(a.q_out) + ((tok0 + tk[u]) * a.H + h) * HD;
+        if (s < 0) o0 = o1 = make_uint4(0, 0, 0, 0);
+        out = reinterpret_cast<bf16*>(a.q_out) + (token * a.H + r) * HD + 8 * part;
       } else {
-        if (s_out[tk[u]] < 0) continue;
-        out = reinterpret_cast<bf16*>(a.pages) + (s_out[tk[u]] + ((is_k ? 0 : a.n_pages * a.HKV) + h) * a.page) * HD;
+        if (pg < 0) continue;
+        const int h = is_k ? r - a.H : r - a.H - a.HKV;
+        const int64_t row = ((is_k ? 0 : a.n_pages) + pg) * a.HKV + h;
+        out = reinterpret_cast<bf16*>(a.pages) + (row * a.page + ((s + t) & (a.page - 1))) * HD + 8 * part;
+        if (is_k && part == 0 && a.weight != nullptr) {
+          const int64_t at = ((int64_t)b * a.HKV + h) * a.width * a.page + s + t;
+          a.weight[at] = 0.f;
+          a.order[at] = (int32_t)pos;
+        }
       }
-      reinterpret_cast<uint2*>(out)[part] = o0;
-      reinterpret_cast<uint2*>(out + HD / 2)[part] = o1;
-      if (is_k && part == 0 && a.weight != nullptr) {
-        const int64_t at = s_rec[tk[u]] + h * cap;
-        a.weight[at] = 0.f;
-        a.order[at] = (int32_t)s_pos[tk[u]];
-      }
+      reinterpret_cast<uint4*>(out)[0] = o0;
+      reinterpret_cast<uint4*>(out + HD / 2)[0] = o1;
     }
   }
 }
 
 // -------------------------------------------------------------------------------------------- evict
 
-constexpr int kEvictThreads = 512;
 constexpr int kBins = 2048;
-constexpr int kCached = 16384;                       // rows whose keys are kept in shared memory
+constexpr int kCached = 12288;                       // rows whose keys and positions are kept in shared memory
+constexpr int kListed = 1024;                        // moves of a head whose list is kept in shared memory
 constexpr int kInline = 512;                         // moves of a head that its own CTA makes, whatever the number of heads
 
 struct Evict {
@@ -222,28 +214,21 @@ struct Evict {
   int split;                                         // a second kernel moves the rows
 };
 
-// sum over the block's earlier threads, and over all
-B3_DEV uint64_t block_before(uint64_t v, uint64_t* s_warp, uint64_t& total) {
-  constexpr int W = kEvictThreads / 32;
+// v summed over the earlier warps of the block, and over all; v the same for all lanes of a warp
+template <int W>
+B3_DEV uint64_t warps_before(uint64_t v, uint64_t* s_warp, uint64_t& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint64_t up = v;
+  __syncthreads();
+  if (lane == 0) s_warp[warp] = v;
+  __syncthreads();
+  uint64_t up = lane < W ? s_warp[lane] : 0;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const uint64_t x = __shfl_up_sync(0xffffffffu, up, o);
     if (lane >= o) up += x;
   }
-  __syncthreads();
-  if (lane == 31) s_warp[warp] = up;
-  __syncthreads();
-  uint64_t before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    const uint64_t x = s_warp[w];
-    if (w < warp) before += x;
-    total += x;
-  }
-  return before + up - v;
+  total = __shfl_sync(0xffffffffu, up, 31);
+  return __shfl_sync(0xffffffffu, up, warp) - v;
 }
 
 // rows `to` of a head become rows `from`: lanes [0, HD / 8) a key row, the next HD / 8 its value row
@@ -285,15 +270,16 @@ B3_DEV void move_rows(const Evict& p, int b, int h, const int2* moves, int first
   }
 }
 
-template <int HD>
-__global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const __grid_constant__ Evict p) {
-  extern __shared__ uint32_t s_key[];                // keys of the first rows, then a bit per row: new enough to stay
+template <int HD, int NT>
+__global__ void __launch_bounds__(NT) paged_evict_kernel(const __grid_constant__ Evict p) {
+  constexpr int W = NT / 32;
+  extern __shared__ __align__(16) uint32_t s_dyn[];                // keys of the first rows, positions of the first rows, the list of moves
   __shared__ uint32_t s_hist[kBins];
-  __shared__ uint64_t s_warp[kEvictThreads / 32];
+  __shared__ uint64_t s_warp[32];
   __shared__ uint32_t s_digit;
-  __shared__ int s_left, s_bad;
+  __shared__ int s_left, s_whole, s_bad;
   const bolt3_paged_evict_args& a = p.a;
-  const int tid = threadIdx.x, head = blockIdx.x, b = head / a.HKV, h = head % a.HKV;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head = blockIdx.x, b = head / a.HKV, h = head % a.HKV;
   const int64_t cap = a.width * a.page;
   grid_dep_launch();
   grid_dep_wait();
@@ -310,103 +296,154 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const __grid
   const float* weight = a.weight + ((int64_t)b * a.HKV + h) * cap;
   const int32_t* order = a.order + ((int64_t)b * a.HKV + h) * cap;
   const int cached = min(n, kCached);
+  uint32_t* s_key = s_dyn;
+  int32_t* s_order = reinterpret_cast<int32_t*>(s_dyn + cached);
+  // NaN as +infinity; no key is 0
+  auto key_of = [&](float w) { return w != w ? 0xff800000u : fkey(w); };
   __syncthreads();
 
-  // every page that a row may leave or reach is in the pool
-  for (int i = tid; i <= (n - 1) >> p.pages.log; i += kEvictThreads)
-    if (p.pages.page_of(b, (int64_t)i << p.pages.log) < 0) s_bad = 1;
-  // the newest position, then how many rows are new enough to stay
+  // positions and weights into shared memory, the newest position; every page that a row may leave or reach is in the pool
   int newest = (int)0x80000000;
-  for (int i = tid; i < n; i += kEvictThreads) newest = max(newest, order[i]);
+  for (int i0 = tid; i0 < n; i0 += 4 * NT) {
+    int32_t o[4];
+    float w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * NT;
+      if (i < n) o[u] = order[i];
+      if (i < cached) w[u] = weight[i];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * NT;
+      if (i < n) newest = max(newest, o[u]);
+      if (i < cached) {
+        s_key[i] = key_of(w[u]);
+        s_order[i] = o[u];
+      }
+    }
+  }
+  for (int i = tid; i <= (n - 1) >> p.pages.log; i += NT)
+    if (p.pages.page_of(b, (int64_t)i << p.pages.log) < 0) s_bad = 1;
+  for (int i = tid; i < kBins; i += NT) s_hist[i] = 0;
   newest = __reduce_max_sync(0xffffffffu, newest);
-  if ((tid & 31) == 0) s_warp[tid >> 5] = (uint64_t)(uint32_t)newest;
+  if (lane == 0) s_warp[warp] = (uint64_t)(uint32_t)newest;
   __syncthreads();
   if (s_bad) {
     if (tid == 0 && a.status) atomicOr(a.status, 8);
     return;
   }
-#pragma unroll
-  for (int w = 0; w < kEvictThreads / 32; ++w) newest = max(newest, (int)(uint32_t)s_warp[w]);
+  newest = __reduce_max_sync(0xffffffffu, lane < W ? (int)(uint32_t)s_warp[lane] : (int)0x80000000);
   const int64_t above = (int64_t)newest - a.recent;
-  // NaN as +infinity; no key is 0
-  auto key_of = [&](float w) { return w != w ? 0xff800000u : fkey(w); };
-  int fresh = 0;
-  for (int i = tid; i < n; i += kEvictThreads) {
-    fresh += order[i] > above;
-    if (i < cached) s_key[i] = key_of(weight[i]);
-  }
-  uint64_t total;
-  block_before((uint64_t)fresh, s_warp, total);
-  const bool all_fresh_stay = (int64_t)total <= keep;
   // New rows rank before all others. Where they all stay, they need no order among themselves; where they do not, the
   // other rows are out
-  auto rank_key = [&](int i, uint32_t k) {
-    const bool f = order[i] > above;
+  uint64_t total;
+  int fresh = 0;
+  for (int i = tid; i < n; i += NT) fresh += (i < cached ? s_order[i] : order[i]) > above;
+  warps_before<W>((uint64_t)__reduce_add_sync(0xffffffffu, fresh), s_warp, total);
+  const bool all_fresh_stay = (int64_t)total <= keep;
+  auto rank_key = [&](int32_t o, uint32_t k) {
+    const bool f = o > above;
     return all_fresh_stay ? (f ? 0xffffffffu : k) : (f ? k : 0u);
   };
-  for (int i = tid; i < cached; i += kEvictThreads) s_key[i] = rank_key(i, s_key[i]);
-  auto get = [&](int i) { return i < cached ? s_key[i] : rank_key(i, key_of(weight[i])); };
+  auto get = [&](int i) { return i < cached ? s_key[i] : rank_key(order[i], key_of(weight[i])); };
 
-  // the keep-th largest key, digit by digit: rows of the digits so far are candidates, `left` of them stay
+  // the keep-th largest key, digit by digit: rows of the digits so far are candidates, `left` of them stay. Done early where a
+  // digit's rows all stay
   uint32_t prefix = 0;
   int left = keep;
+  bool whole = false;
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
+    if (whole) break;                                // the same for all threads
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
     const uint32_t mask = (1u << bits) - 1;
-    for (int i = tid; i < kBins; i += kEvictThreads) s_hist[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += kEvictThreads) {
-      const uint32_t k = get(i);
+    if (pass > 0) {
+      for (int i = tid; i < kBins; i += NT) s_hist[i] = 0;
+      __syncthreads();
+    }
+    for (int i = tid; i < n; i += NT) {
+      uint32_t k;
+      if (pass == 0 && i < cached) s_key[i] = k = rank_key(s_order[i], s_key[i]);
+      else k = get(i);
       if (pass == 0 || k >> (shift + bits) == prefix >> (shift + bits)) atomicAdd(&s_hist[(k >> shift) & mask], 1u);
     }
     __syncthreads();
-    // bins from the largest digit on, four to a thread
-    constexpr int PER = kBins / kEvictThreads;
+    // bins from the largest digit on, a few to a thread
+    constexpr int PER = kBins / NT;
     uint32_t c[PER], sum = 0;
 #pragma unroll
     for (int u = 0; u < PER; ++u) sum += c[u] = s_hist[kBins - 1 - (tid * PER + u)];
-    uint64_t before = block_before((uint64_t)sum, s_warp, total);
+    uint32_t up = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += x;
+    }
+    uint32_t before = (uint32_t)warps_before<W>((uint64_t)__shfl_sync(0xffffffffu, up, 31), s_warp, total) + up - sum;
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-      if ((int64_t)before < left && (int64_t)(before + c[u]) >= left) {
+      if ((int)before < left && (int)(before + c[u]) >= left) {
         s_digit = kBins - 1 - (tid * PER + u);
         s_left = left - (int)before;
+        s_whole = (int)(before + c[u]) == left;
       }
       before += c[u];
     }
     __syncthreads();
     prefix |= s_digit << shift;
     left = s_left;
+    whole = s_whole;
   }
-  // rows above `prefix` stay, and the first `left` of those equal to it
-  const int per = (n + kEvictThreads - 1) / kEvictThreads, i0 = min(n, tid * per), i1 = min(n, i0 + per);
-  int equal = 0;
-  for (int i = i0; i < i1; ++i) equal += get(i) == prefix;
-  int rank = (int)block_before((uint64_t)equal, s_warp, total);
-  const int rank0 = rank;
+  // rows above `prefix` stay, and the first `left` of those equal to it; a whole digit: those from it on (no key is 0, and not
+  // all rows stay, so it is not 0)
+  if (whole) {
+    prefix -= 1;
+    left = 0;
+  }
+  // a warp takes a stretch of rows, 32 at a time, so that ranks in the order of rows are sums over warps and bits before a lane's
+  const int per = (n + NT - 1) / NT * 32, i0 = min(n, warp * per), i1 = min(n, i0 + per);
+  const uint32_t lower = (1u << lane) - 1;
+  int rank0 = 0;
+  if (left > 0) {
+    int equal = 0;
+    for (int i = i0 + lane; i - lane < i1; i += 32) equal += __popc(__ballot_sync(0xffffffffu, i < i1 && get(i) == prefix));
+    rank0 = (int)warps_before<W>((uint64_t)equal, s_warp, total);
+  }
+  auto stays = [&](int i, int& rank) {
+    const uint32_t k = i < i1 ? get(i) : 0u;
+    bool st = k > prefix;
+    if (left > 0) {
+      const uint32_t eq = __ballot_sync(0xffffffffu, i < i1 && k == prefix);
+      st |= (eq >> lane & 1) && rank + __popc(eq & lower) < left;
+      rank += __popc(eq);
+    }
+    return st;
+  };
   uint64_t mine = 0;                                 // dropped rows below keep, kept rows from it on
-  for (int i = i0; i < i1; ++i) {
-    const uint32_t k = get(i);
-    const bool stays = k > prefix || (k == prefix && rank++ < left);
-    if (i < keep) mine += !stays;
-    else mine += (uint64_t)stays << 32;
+  int rank = rank0;
+  for (int i = i0 + lane; i - lane < i1; i += 32) {
+    const bool st = stays(i, rank);
+    mine += __popc(__ballot_sync(0xffffffffu, i < i1 && i < keep && !st)) +
+            ((uint64_t)__popc(__ballot_sync(0xffffffffu, i < i1 && i >= keep && st)) << 32);
   }
-  const uint64_t before = block_before(mine, s_warp, total);
+  const uint64_t before = warps_before<W>(mine, s_warp, total);
   int hole = (int)(uint32_t)before, mover = (int)(before >> 32);
-  int2* moves = p.moves + (int64_t)head * p.most;
-  rank = rank0;
-  for (int i = i0; i < i1; ++i) {
-    const uint32_t k = get(i);
-    const bool stays = k > prefix || (k == prefix && rank++ < left);
-    if (i < keep && !stays) moves[hole++].x = i;
-    if (i >= keep && stays) moves[mover++].y = i;
-  }
   const int n_moves = (int)(uint32_t)total;
+  int2* moves = !p.split && p.most <= kListed ? reinterpret_cast<int2*>(s_dyn + 2 * cached) : p.moves + (int64_t)head * p.most;
+  rank = rank0;
+  for (int i = i0 + lane; i - lane < i1; i += 32) {
+    const bool st = stays(i, rank), drops = i < i1 && i < keep && !st, moves_in = i < i1 && i >= keep && st;
+    const uint32_t d = __ballot_sync(0xffffffffu, drops), m = __ballot_sync(0xffffffffu, moves_in);
+    if (drops) moves[hole + __popc(d & lower)].x = i;
+    if (moves_in) moves[mover + __popc(m & lower)].y = i;
+    hole += __popc(d);
+    mover += __popc(m);
+  }
   if (tid == 0) p.count[head] = n_moves;
   if (p.split) return;
   __syncthreads();
-  move_rows<HD>(p, b, h, moves, tid >> 5, n_moves, kEvictThreads / 32, tid & 31);
+  move_rows<HD>(p, b, h, moves, warp, n_moves, W, lane);
 }
 
 // the moves of a head, shared by gridDim.y blocks
@@ -421,14 +458,22 @@ __global__ void __launch_bounds__(kThreads) paged_move_kernel(const __grid_const
 
 int64_t most_moves(int64_t n, int64_t keep) { return n <= keep ? 0 : n - keep < keep ? n - keep : keep; }
 
+template <int HD, int NT>
+int launch_select(const Evict& p, cudaStream_t s) {
+  const size_t cached = p.a.n < kCached ? (size_t)p.a.n : (size_t)kCached;
+  const size_t smem = cached * 8 + (!p.split && p.most <= kListed ? (size_t)p.most * 8 : 0);
+  if (cudaFuncSetAttribute(paged_evict_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCached * 8 + kListed * 8) != cudaSuccess)
+    return BOLT3_ERR_CUDA;
+  return launch_overlapped(paged_evict_kernel<HD, NT>, dim3((unsigned)(p.a.B * p.a.HKV)), dim3(NT), smem, s, p) == cudaSuccess
+             ? BOLT3_OK : BOLT3_ERR_CUDA;
+}
+
 template <int HD>
 int launch_evict(const Evict& p, cudaStream_t s) {
   const int64_t heads = (int64_t)p.a.B * p.a.HKV;
-  const size_t smem = (size_t)(p.a.n < kCached ? p.a.n : kCached) * 4;
-  if (cudaFuncSetAttribute(paged_evict_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCached * 4) != cudaSuccess)
-    return BOLT3_ERR_CUDA;
-  if (launch_overlapped(paged_evict_kernel<HD>, dim3((unsigned)heads), dim3(kEvictThreads), smem, s, p) != cudaSuccess)
-    return BOLT3_ERR_CUDA;
+  // a thread per few rows
+  const int rc = p.a.n > 4096 ? launch_select<HD, 1024>(p, s) : launch_select<HD, 512>(p, s);
+  if (rc != BOLT3_OK) return rc;
   if (!p.split) return BOLT3_OK;
   const int64_t per = kThreads / 32 * 4 * (HD == 128 ? 1 : 2), want = (p.most + per - 1) / per, fit = (148 * 4 + heads - 1) / heads;
   const unsigned slices = (unsigned)(want < fit ? want : fit);
@@ -460,16 +505,18 @@ extern "C" int bolt3_paged_append(const bolt3_paged_append_args* a, void* stream
   // with lens, n bounds the lengths and the table the rows
   const Length len{a->lens, a->pos_dev, a->n, a->pos_ref, a->pos_span,
                    a->lens != nullptr && a->n < cap - a->T ? a->n + a->T : cap, a->T};
-  const int rows = a->H + 2 * a->HKV, rpi = kThreads / (a->HD / 8);
-  // few tokens: a block per iteration's rows, so that a one-token step still fills the machine; from two blocks of four
-  // tokens for every SM on, blocks of four
+  // a warp per token, or per share of a token's rows where there are few: as long as eight warps per SM are not reached
+  const int rows = a->H + 2 * a->HKV, rpi = 32 / (a->HD / 16), groups = (rows + rpi - 1) / rpi;
   const int64_t tokens = (int64_t)a->B * a->T;
-  const bool few = tokens < 148 * 8;
-  const dim3 grid((unsigned)(few ? tokens : (tokens + 3) / 4), (unsigned)(few ? (rows + rpi - 1) / rpi : 1));
+  int64_t chunks = (148 * 16 + tokens - 1) / tokens;
+  if (chunks > groups) chunks = groups;
+  const int rows_per = (groups + (int)chunks - 1) / (int)chunks * rpi;
+  chunks = (rows + rows_per - 1) / rows_per;
+  const int64_t blocks = (tokens * chunks + kThreads / 32 - 1) / (kThreads / 32);
+  if (blocks > 0x7fffffff) return BOLT3_ERR_SHAPE;
   cudaStream_t s = (cudaStream_t)stream;
-  auto kern = a->HD == 128 ? (few ? paged_append_kernel<128, 1> : paged_append_kernel<128, 4>)
-                           : (few ? paged_append_kernel<64, 1> : paged_append_kernel<64, 4>);
-  return launch_overlapped(kern, grid, dim3(kThreads), 0, s, *a, len, pages, rpi) == cudaSuccess ? BOLT3_OK : BOLT3_ERR_CUDA;
+  return launch_overlapped(a->HD == 128 ? paged_append_kernel<128> : paged_append_kernel<64>, dim3((unsigned)blocks), dim3(kThreads), 0, s,
+                           *a, len, pages, (int)chunks, rows_per) == cudaSuccess ? BOLT3_OK : BOLT3_ERR_CUDA;
 }
 
 extern "C" size_t bolt3_paged_evict_workspace(int B, int HKV, int64_t n, int64_t keep) {

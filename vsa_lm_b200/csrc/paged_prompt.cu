@@ -7,13 +7,15 @@
 // keys by 256 rows take 2048 cycles of an SM, its exponentials 2048. A CTA holds two tiles of 128 query rows (T * G rows of one
 // KV head, token-major) and walks the keys in blocks of 128. Roles, which meet only at mbarriers:
 // - warp 16 brings keys and values by TMA, a box for each page that a block touches, two stages each;
-// - one lane of warp 17 issues tcgen05.mma: S = Q K^T into TMEM, O += P V with P as the TMEM operand;
-// - warp 18 clears the value rows of the last block that no query row of the CTA sees (a page's unused rows may hold
+// - one lane of warps 17 and 18 issues a tile's tcgen05.mma: S = Q K^T into TMEM, O += P V with P as the TMEM operand, 64 keys
+//   at a time: once a half's weights have been used, the next block's scores of that half are on their way, while the softmax is
+//   at the other half;
+// - warp 19 clears the value rows of the last block that no query row of the CTA sees (a page's unused rows may hold
 //   anything, and 0 times a NaN is one);
 // - warps 0-7 and 8-15 are the softmax of a tile, 64 keys at a time: scores out of TMEM, weights back over them. A warp takes
 //   16 TMEM lanes in the 16x256b layout, so that a row's reference is shared by a quad of lanes alone. The reference moves only
 //   when a weight would pass 2^kMost; only then are the sums in TMEM rescaled.
-// While one tile's softmax runs, the tensor cores work on the other tile. With few heads the keys are split over CTAs, whose
+// With few heads the keys are split over CTAs, whose
 // partial sums a second kernel joins.
 //
 // record. A key's weight needs the rows' sums over all keys, so the scores are computed again once these are known, this time
@@ -30,7 +32,7 @@ using namespace paged;
 
 constexpr int kKeys = 128;                       // of a block
 constexpr float kMost = 20.f;                    // log2 of the largest weight relative to the reference
-constexpr int kThreads = 608;                    // 16 softmax warps, loads, MMAs, clearing
+constexpr int kThreads = 640;                    // 16 softmax warps, loads, MMAs of either tile, clearing
 constexpr int kRows = 512;                       // query rows of a CTA of the record kernel
 constexpr int kRecordThreads = 576;              // 16 summing warps, loads, MMAs
 
@@ -51,7 +53,7 @@ struct Smem {
   unsigned char k[2][kKeys * HD * 2];
   unsigned char v[2][kKeys * HD * 2];
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], v_last, v_clean;
-  uint64_t s_full[2], p_full[2][2], pv_half[2], o_full[2];
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], o_full[2];    // of a tile, of a half of its keys
   uint32_t tbase;
   int err;
 };
@@ -148,13 +150,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       tc5::mbar_init(&sm.k_full[i], 1);
-      tc5::mbar_init(&sm.k_empty[i], 1);
+      tc5::mbar_init(&sm.k_empty[i], n_tile);
       tc5::mbar_init(&sm.v_full[i], 1);
-      tc5::mbar_init(&sm.v_empty[i], 1);
-      tc5::mbar_init(&sm.s_full[i], 1);
-      tc5::mbar_init(&sm.p_full[i][0], 256);
-      tc5::mbar_init(&sm.p_full[i][1], 256);
-      tc5::mbar_init(&sm.pv_half[i], 1);
+      tc5::mbar_init(&sm.v_empty[i], n_tile);
+      for (int h = 0; h < 2; ++h) {
+        tc5::mbar_init(&sm.s_full[i][h], 1);
+        tc5::mbar_init(&sm.p_full[i][h], 256);
+        tc5::mbar_init(&sm.pv_done[i][h], 1);
+      }
       tc5::mbar_init(&sm.o_full[i], 1);
     }
     tc5::mbar_init(&sm.v_last, 1);
@@ -207,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
     tc5::fence_before_sync();
     meet_all();
     tc5::fence_after_sync();
-    return sm.tbase;                             // S / P of tile i: columns 128 i; O of tile i: 256 + 128 i
+    return sm.tbase;                             // S of tile i: columns 128 i, weights of a half over its first 32; O of tile i: 256 + 128 i
   };
   auto wait = [&](uint64_t* bar, int phase) {
     if (tc5::mbar_wait(bar, (uint32_t)phase & 1, kWaitIters)) return true;
@@ -267,65 +270,63 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
       if (ragged && j + 1 == n_blk) wait(&sm.v_last, 0);
       else wait(&sm.v_full[j & 1], j >> 1);
     }
-  } else if (warp == 17) {
-    // ---- issue. The whole warp runs the loop, so that addresses and descriptors are uniform over it; one lane issues
+  } else if (warp == 17 || warp == 18) {
+    // ---- issue, tile i. The whole warp runs the loop, and what it counts with comes from one lane, so that addresses and
+    // descriptors are uniform over it (moving them to where the instruction takes them cost more than the MMAs); one lane issues.
+    // Step after step: the product of a half of block j, then the same half's scores of block j + 1 (j = -1: scores alone). One
+    // place in the code for either: with the first scores before the loop, in a copy of their own, the loop's were issued twice
+    // at HD 64
     const uint32_t tb = all_ready();
-    const bool one = elected();
-    constexpr uint32_t kIdS = tc5::idesc_bf16(128, kKeys, false, false), kIdO = tc5::idesc_bf16(128, HD, false, true);
+    const int i = __shfl_sync(0xffffffffu, warp, 0) - 17, blocks = __shfl_sync(0xffffffffu, i < n_tile ? n_blk : -1, 0);
+    const bool tail = __shfl_sync(0xffffffffu, (int)ragged, 0) != 0, one = elected();
+    constexpr uint32_t kIdS = tc5::idesc_bf16(128, kKeys / 2, false, false), kIdO = tc5::idesc_bf16(128, HD, false, true);
     constexpr uint64_t kTile = sizeof(sm.q[0]) >> 4;              // from one tile's descriptor to the next one's
-    const uint32_t tu = __shfl_sync(0xffffffffu, tb, 0);
-    const uint64_t q_desc = tc5::sdesc(tc5::smem_u32(sm.q[0]), 16, 1024), k_desc = tc5::sdesc(tc5::smem_u32(sm.k[0]), 16, 1024);
+    const uint32_t tu = __shfl_sync(0xffffffffu, tb, 0) + i * 128;
+    const uint64_t qd = tc5::sdesc(tc5::smem_u32(sm.q[0]), 16, 1024) + i * kTile, k_desc = tc5::sdesc(tc5::smem_u32(sm.k[0]), 16, 1024);
     const uint64_t v_desc = tc5::sdesc(tc5::smem_u32(sm.v[0]), kKeys * 128, 1024);
-    // Step after step: the products of tile i with block j's values, then its scores of block j + 1 (j = -1: scores alone). One
-    // place in the code for either: with the first scores before the loop, in a copy of their own, the loop's were issued twice at
-    // HD 64
     bool ok = true;
-    int i = 0;
 #pragma unroll 1
-    for (int j = -1; ok && j < n_blk;) {
+    for (int j = -1; ok && j < blocks; ++j) {
       const int st = j & 1;
-      if (j >= 0) {
-        if (i == 0) ok = ragged && j + 1 == n_blk ? wait_all(&sm.v_clean, 0) : wait_all(&sm.v_full[st], j >> 1);
 #pragma unroll 1
-        for (int h = 0; ok && h < 2; ++h) {
-          ok = wait_all(&sm.p_full[i][h], j);
+      for (int h = 0; ok && h < 2; ++h) {
+        if (j >= 0) {
+          if (h == 0) ok = tail && j + 1 == blocks ? wait_all(&sm.v_clean, 0) : wait_all(&sm.v_full[st], j >> 1);
+          ok = ok && wait_all(&sm.p_full[i][h], j);
           if (!ok) break;
           tc5::fence_after_sync();
           const uint64_t vd = v_desc + st * kTile + 4 * h * 128;
-          const uint32_t d = tu + 256 + i * 128, pa = tu + i * 128 + 32 * h;
+          const uint32_t d = tu + 256, pa = tu + 64 * h;
           if (one) {
             tc5::mma_ts(d, pa, vd, kIdO, j > 0 || h > 0);
             tc5::mma_ts(d, pa + 8, vd + 128, kIdO, 1);
             tc5::mma_ts(d, pa + 16, vd + 256, kIdO, 1);
             tc5::mma_ts(d, pa + 24, vd + 384, kIdO, 1);
-            if (h == 0) tc5::commit(&sm.pv_half[i]);
-            else if (j + 1 == n_blk) tc5::commit(&sm.o_full[i]);
+            tc5::commit(&sm.pv_done[i][h]);
+            if (h == 1) tc5::commit(j + 1 == blocks ? &sm.o_full[i] : &sm.v_empty[st]);
           }
         }
-        if (!ok) break;
-      }
-      const bool last_tile = i + 1 == n_tile;
-      if (j + 1 < n_blk) {
-        if (i == 0) ok = wait_all(&sm.k_full[st ^ 1], (j + 1) >> 1);
-        if (!ok) break;
-        tc5::fence_after_sync();
-        const uint64_t qd = q_desc + i * kTile, kd = k_desc + (st ^ 1) * kTile;
-        if (one) {
+        if (j + 1 < blocks) {
+          if (h == 0) ok = wait_all(&sm.k_full[st ^ 1], (j + 1) >> 1);
+          if (!ok) break;
+          tc5::fence_after_sync();
+          const uint64_t kd = k_desc + (st ^ 1) * kTile + 4 * h * 128;
+          if (one) {
 #pragma unroll
-          for (int ks = 0; ks < HD / 16; ++ks) {
-            constexpr uint64_t kBlock = (kKeys * 128) >> 4;       // a block of 64 columns
-            tc5::mma_ss(tu + i * 128, qd + (ks >> 2) * kBlock + (ks & 3) * 2, kd + (ks >> 2) * kBlock + (ks & 3) * 2, kIdS, ks > 0);
+            for (int ks = 0; ks < HD / 16; ++ks) {
+              constexpr uint64_t kBlock = (kKeys * 128) >> 4;     // a block of 64 columns
+              tc5::mma_ss(tu + 64 * h, qd + (ks >> 2) * kBlock + (ks & 3) * 2, kd + (ks >> 2) * kBlock + (ks & 3) * 2, kIdS, ks > 0);
+            }
+            tc5::commit(&sm.s_full[i][h]);
+            if (h == 1) tc5::commit(&sm.k_empty[st ^ 1]);
           }
-          tc5::commit(&sm.s_full[i]);
-          if (last_tile) tc5::commit(&sm.k_empty[st ^ 1]);
         }
       }
-      if (last_tile && j >= 0 && one) tc5::commit(&sm.v_empty[st]);
-      i = last_tile ? 0 : i + 1;
-      j += last_tile;
     }
-    if (ok) wait_all(&sm.v_empty[(n_blk - 1) & 1], (n_blk - 1) >> 1);   // no arrival is under way when the CTA ends
-  } else if (warp >= 18) {
+    // no arrival is under way when the CTA ends
+    if (ok && blocks > 0) wait_all(&sm.k_empty[(blocks - 1) & 1], (blocks - 1) >> 1);
+    if (ok && blocks > 0) wait_all(&sm.o_full[i], 0);
+  } else if (warp == 19) {
     all_ready();
     if (ragged) {
       const int j = n_blk - 1, st = j & 1, first = seen_last - j * kKeys;
@@ -352,11 +353,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
       uint64_t l[2] = {0, 0};                                       // sums of weights over this thread's keys, in pairs
       bool ok = true;
       for (int j = 0; ok && j < n_blk; ++j) {
-        ok = wait_all(&sm.s_full[i], j);
-        if (!ok) break;
-        tc5::fence_after_sync();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          ok = ok && wait_all(&sm.s_full[i][h], j);
+          if (!ok) break;
+          tc5::fence_after_sync();
           uint32_t sc[32];
           ld_16x64(ts + 64 * h, sc);
           const int key = j * kKeys + 64 * h;
@@ -394,10 +395,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
               l[q] = mul2(l[q], pair(f[q], f[q]));
             }
             if (j > 0 || h > 0) {
-              if (h > 0) {                                          // the first half's product may still be under way
-                ok = wait_all(&sm.pv_half[i], j);
-                tc5::fence_after_sync();
-              }
+              ok = h > 0 ? wait_all(&sm.pv_done[i][0], j) : wait_all(&sm.pv_done[i][1], j - 1);   // the last product
+              tc5::fence_after_sync();
               if (ok) {
 #pragma unroll 1
                 for (int d = 0; d < HD; d += 32) {
@@ -424,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
               l[q] = add2(l[q], pair(e0, e1));
               w[2 * n + q] = pack_bf16(e0, e1);
             }
-          st_16x32(ts + 32 * h, w);
+          st_16x32(ts + 64 * h, w);
           tc5::st_wait();
           tc5::fence_before_sync();
           tc5::mbar_arrive(&sm.p_full[i][h]);
@@ -738,10 +737,17 @@ Plan plan_of(int B, int T, int H, int HKV, int HD, int64_t n, bool weigh) {
   const int64_t most = blocks / 4;
   if (splits > most) splits = most;
   pl.splits = splits < 1 ? 1 : (int)splits;
-  // ranges of keys: two waves of CTAs or so, of two blocks or more each
-  int64_t ranges = 2 * 148 / heads;
-  if (ranges > blocks / 2) ranges = blocks / 2;
-  pl.ranges = ranges < 1 ? 1 : (int)ranges;
+  // ranges of keys: as many as give the shortest longest SM, a CTA costing a block and a half beside its own (its queries).
+  // 16 sequences of 17 blocks, 8 heads: 1 range 73 us, 2 of them 81
+  pl.ranges = 1;
+  double least = 0;
+  for (int64_t r = 1; r <= 32 && r <= blocks; ++r) {
+    const double waves = (double)((heads * r + 147) / 148), cost = waves * ((double)((blocks + r - 1) / r) + 1.5);
+    if (r == 1 || cost < least) {
+      least = cost;
+      pl.ranges = (int)r;
+    }
+  }
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t was = at;

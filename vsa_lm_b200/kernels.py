@@ -758,19 +758,53 @@ def _attend_workspace(B: int, T: int, H: int, HKV: int, HD: int, n: int) -> int:
 
 # ---- paged bf16 KV cache of a softmax anchor (include/bolt3.h: bolt3_paged_*)
 
+_PAGES = frozenset((16, 32, 64, 128))
+
+
 def _need_pages(pages, table, dev: int) -> tuple:
     """(pages of the pool, HKV, rows of a page, HD, B, pages of a sequence, table's row stride, address of pages, of
     table): pages bf16 [2, P, HKV, page, HD], table int32 [B, W] with dense rows."""
-    at = _fits(pages, torch.bfloat16, dev, "pages", 1)
-    sh = pages.shape
-    if len(sh) != 5 or sh[0] != 2 or sh[3] not in (16, 32, 64, 128) or sh[4] not in (64, 128):
-        raise ValueError(f"pages must be [2, P, HKV, 16, 32, 64 or 128, 64 or 128], got {tuple(sh)}")
+    if type(pages) is not torch.Tensor or pages.dtype is not torch.bfloat16 or pages.get_device() != dev or not pages.is_contiguous():
+        _need(pages, torch.bfloat16, "pages")
     if type(table) is not torch.Tensor or table.dtype is not torch.int32 or table.get_device() != dev:
         _need(table, torch.int32, "table")
-    ts, st = table.shape, table.stride()
-    if len(ts) != 2 or ts[0] < 1 or ts[1] < 1 or (st[1] != 1 and ts[1] > 1):
-        raise ValueError(f"table must be [B, pages of a sequence] with dense rows, got {tuple(ts)} strides {st}")
-    return sh[1], sh[2], sh[3], sh[4], ts[0], ts[1], (ts[1] if ts[0] == 1 else st[0]), at, table.data_ptr()
+    sh, ts = pages.shape, table.shape
+    if len(sh) != 5 or sh[0] != 2 or sh[3] not in _PAGES or sh[4] not in (64, 128) or sh[1] < 1 or sh[2] < 1:
+        raise ValueError(f"pages must be [2, P, HKV, 16, 32, 64 or 128, 64 or 128], got {tuple(sh)}")
+    _, P, HKV, page, HD = sh
+    if len(ts) != 2:
+        raise ValueError(f"table must be [B, pages of a sequence], got {tuple(ts)}")
+    B, W = ts
+    stride = W
+    if not table.is_contiguous():
+        st = table.stride()
+        if st[1] != 1 and W > 1:
+            raise ValueError(f"table must be [B, pages of a sequence] with dense rows, got {tuple(ts)} strides {st}")
+        stride = st[0]
+    if B < 1 or W < 1:
+        raise ValueError(f"table must be [B, pages of a sequence], got {tuple(ts)}")
+    return P, HKV, page, HD, B, W, stride, pages.data_ptr(), table.data_ptr()
+
+
+def _tokens_heads(t, name: str, B: int, HD: int, dev: int) -> tuple[int, int, int, int, int]:
+    """(T, heads, sequence stride, token stride, address) of `t` = [B, T, heads * HD] or [B, T, heads, HD] as in _heads."""
+    if type(t) is torch.Tensor and t.dtype is torch.bfloat16 and t.get_device() == dev:
+        sh = t.shape
+        if len(sh) == 3:
+            b, T, width = sh
+            sb, st, one = t.stride()
+            if b == B and T > 0 and one == 1 and width and width % HD == 0:
+                return T, width // HD, 0 if B == 1 else sb, 0 if T == 1 else st, t.data_ptr()
+        elif len(sh) == 4:
+            b, T, heads, hd = sh
+            sb, st, sr, one = t.stride()
+            if b == B and T > 0 and one == 1 and hd == HD and heads and (sr == HD or heads == 1):
+                return T, heads, 0 if B == 1 else sb, 0 if T == 1 else st, t.data_ptr()
+    T = _tokens(t, name)
+    return T, *_heads(t, name, B, T, HD, dev), t.data_ptr()
+
+
+_NO_POS = (0, 0, 0)
 
 
 def _need_records(weight, order, B: int, HKV: int, cap: int, dev: int) -> tuple[int, int]:
@@ -796,28 +830,30 @@ def paged_append(*, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pages: to
     (its queries are 0). weight (fp32 [B, HKV, W * page]) and order (int32, the same shape), both or none: the new rows'
     records become 0 and the position."""
     dev = _here()
-    T = _tokens(q, "q")
     P, HKV, page, HD, B, W, stride, at, tat = _need_pages(pages, table, dev)
-    H, q_sb, q_st = _heads(q, "q", B, T, HD, dev)
-    _tokens(k, "k"), _tokens(v, "v")
-    hk, k_sb, k_st = _heads(k, "k", B, T, HD, dev)
-    hv, v_sb, v_st = _heads(v, "v", B, T, HD, dev)
-    if hk != HKV or hv != HKV:
-        raise ValueError(f"k and v hold {hk} and {hv} heads, the cache {HKV}")
+    T, H, q_sb, q_st, q_at = _tokens_heads(q, "q", B, HD, dev)
+    tk, hk, k_sb, k_st, k_at = _tokens_heads(k, "k", B, HD, dev)
+    tv, hv, v_sb, v_st, v_at = _tokens_heads(v, "v", B, HD, dev)
+    if hk != HKV or hv != HKV or tk != T or tv != T:
+        raise ValueError(f"k and v hold {hk} and {hv} heads of {tk} and {tv} tokens, the cache {HKV} heads and q {T} tokens")
     if (weight is None) != (order is None):
         raise ValueError("weight and order are given together")
     w_at, o_at = (0, 0) if weight is None else _need_records(weight, order, B, HKV, W * page, dev)
     if pos is not None and lens is None:
         raise ValueError("positions of their own (pos) go with lengths of their own (lens)")
     if q_out is None:
-        q_out = torch.empty((B, T, H, HD), dtype=torch.bfloat16, device=q.device)
+        q_out = q.new_empty((B, T, H, HD))
+        out_at = q_out.data_ptr()
+    else:
+        out_at = _fits(q_out, torch.bfloat16, dev, "q_out", B * T * H * HD)
     _lib.paged_append(
-        torch._C._cuda_getCurrentRawStream(dev), B, T, H, HKV, HD, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_sb, q_st, k_sb,
-        k_st, v_sb, v_st, _maybe(q_norm, torch.float32, dev, "q_norm", HD), _maybe(k_norm, torch.float32, dev, "k_norm", HD),
-        eps, _maybe(inv_freq, torch.float32, dev, "inv_freq", HD // 2),
-        _fits(q_out, torch.bfloat16, dev, "q_out", B * T * H * HD), at, P, page, tat, stride, W, w_at, o_at, n, pos0,
-        _lens_ptr(lens, dev_pos, B, dev), 0 if pos is None else _lens_ptr(pos, None, B, dev), _status_ptr(status),
-        *_pos_fields(dev_pos))
+        torch._C._cuda_getCurrentRawStream(dev), B, T, H, HKV, HD, q_at, k_at, v_at, q_sb, q_st, k_sb, k_st, v_sb, v_st,
+        0 if q_norm is None else _fits(q_norm, torch.float32, dev, "q_norm", HD),
+        0 if k_norm is None else _fits(k_norm, torch.float32, dev, "k_norm", HD),
+        eps, 0 if inv_freq is None else _fits(inv_freq, torch.float32, dev, "inv_freq", HD // 2),
+        out_at, at, P, page, tat, stride, W, w_at, o_at, n, pos0,
+        0 if lens is None else _lens_ptr(lens, dev_pos, B, dev), 0 if pos is None else _lens_ptr(pos, None, B, dev),
+        0 if status is None else _status(status), *(_NO_POS if dev_pos is None else _pos_fields(dev_pos)))
     _count(1)
     return q_out
 
@@ -830,19 +866,24 @@ def paged_attend(*, q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, n
     lens[b] rows before them (-1: idle, its outputs are 0), at most n. `weight` (fp32 [B, HKV, W * page]): the softmax weight
     of every row, summed over the query rows of its head, is added to its record. Returns y, bf16 [B, T, H * HD]."""
     dev = _here()
-    T = _tokens(q, "q")
     P, HKV, page, HD, B, W, stride, at, tat = _need_pages(pages, table, dev)
-    H, q_sb, q_st = _heads(q, "q", B, T, HD, dev)
+    T, H, q_sb, q_st, q_at = _tokens_heads(q, "q", B, HD, dev)
     w_at = 0 if weight is None else _need_records(weight, None, B, HKV, W * page, dev)[0]
     if y is None:
-        y = torch.empty((B, T, H * HD), dtype=torch.bfloat16, device=q.device)
-    nbytes, launches = _paged_workspace(B, T, H, HKV, HD, n + (0 if dev_pos is None else dev_pos.span - 1), w_at != 0)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        y = q.new_empty((B, T, H * HD))
+        y_at = y.data_ptr()
+    else:
+        y_at = _fits(y, torch.bfloat16, dev, "y", B * T * H * HD)
+    nbytes, launches = _paged_workspace(B, T, H, HKV, HD, n if dev_pos is None else n + dev_pos.span - 1, w_at != 0)
+    if nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        ws_at = ws.data_ptr()
+    else:
+        ws_at = 0
     _lib.paged_attend(
-        torch._C._cuda_getCurrentRawStream(dev), B, T, H, HKV, HD, q.data_ptr(), q_sb, q_st, at, P, page, tat, stride, W, w_at,
-        n, _lens_ptr(lens, dev_pos, B, dev), _fits(y, torch.bfloat16, dev, "y", B * T * H * HD),
-        HD ** -0.5 if sm_scale is None else sm_scale, 0 if ws is None else ws.data_ptr(), nbytes, _status_ptr(status),
-        *_pos_fields(dev_pos))
+        torch._C._cuda_getCurrentRawStream(dev), B, T, H, HKV, HD, q_at, q_sb, q_st, at, P, page, tat, stride, W, w_at,
+        n, 0 if lens is None else _lens_ptr(lens, dev_pos, B, dev), y_at, HD ** -0.5 if sm_scale is None else sm_scale, ws_at, nbytes,
+        0 if status is None else _status(status), *(_NO_POS if dev_pos is None else _pos_fields(dev_pos)))
     _count(launches)
     return y
 
@@ -853,6 +894,11 @@ def _paged_workspace(B: int, T: int, H: int, HKV: int, HD: int, n: int, weigh: b
     partial sums where there are any)."""
     fn = _lib.load().bolt3_paged_attend_workspace
     return fn(B, T, H, HKV, HD, n, int(weigh)), 2 if fn(B, T, H, HKV, HD, n, 0) else 1
+
+
+@functools.lru_cache(maxsize=256)
+def _evict_workspace(B: int, HKV: int, n: int, keep: int) -> int:
+    return _lib.load().bolt3_paged_evict_workspace(B, HKV, n, keep)
 
 
 def paged_evict(*, pages: torch.Tensor, table: torch.Tensor, weight: torch.Tensor, order: torch.Tensor, n: int, keep: int,
@@ -870,8 +916,8 @@ def paged_evict(*, pages: torch.Tensor, table: torch.Tensor, weight: torch.Tenso
     if keep < 1 or not 0 <= recent <= keep:
         raise ValueError(f"keep must be at least 1 and recent within [0, keep], got keep={keep} recent={recent}")
     out = None if lens is None else torch.empty(B, dtype=torch.int32, device=pages.device)
-    nbytes = _lib.load().bolt3_paged_evict_workspace(B, HKV, n, keep)
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=pages.device)
+    nbytes = _evict_workspace(B, HKV, n, keep)
+    ws = torch.empty(nbytes or 16, dtype=torch.uint8, device=pages.device)
     _lib.paged_evict(torch._C._cuda_getCurrentRawStream(dev), B, HKV, HD, at, P, page, tat, stride, W, w_at, o_at, n, keep, recent,
                      _lens_ptr(lens, None, B, dev), 0 if out is None else out.data_ptr(), ws.data_ptr(), nbytes,
                      _status_ptr(status))
