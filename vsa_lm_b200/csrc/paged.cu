@@ -17,7 +17,6 @@
 #include <mutex>
 
 #include "paged.cuh"
-#include "tc5.cuh"
 #include "trace.h"
 
 namespace paged {
@@ -56,145 +55,183 @@ using namespace paged;
 // ------------------------------------------------------------------------------------------- append
 
 constexpr int kThreads = 256;
-constexpr int kAhead = 2;                            // rows that a thread has in flight
 
-// A warp takes rows [c rows_per, ..) of the H + 2 HKV rows of a token, of `chunks` such stretches
+// Where a token's rows go
+struct Token {
+  int64_t token, s, row, pos;                        // its number, the rows its sequence held (-1: idle), its row, its position
+  int b, page;                                       // -1: none
+};
+
+B3_DEV Token token_at(const bolt3_paged_append_args& a, const Length& len, const Pages& pages, int64_t token, int lane) {
+  Token tk;
+  bool bad = false;
+  tk.token = token;
+  tk.b = (int)(token / a.T);
+  const int t = (int)(token - (int64_t)tk.b * a.T);
+  tk.s = len.rows(tk.b, bad);                        // the same for the whole warp
+  tk.row = tk.s + t;
+  tk.page = -1;
+  if (tk.s >= 0) {
+    tk.page = pages.page_of(tk.b, tk.row);
+    bad |= tk.page < 0;
+  }
+  if (bad && lane == 0 && a.status) atomicOr(a.status, 8);
+  tk.pos = tk.s < 0 ? 0 : a.pos != nullptr ? (int64_t)a.pos[tk.b] + t : a.pos0 + (tk.row - a.n);
+  return tk;
+}
+
+// The norms' weights, of queries and of keys, into shared memory, the first four of every lane's eight (append_rows) before the
+// other four: a load's lanes read neighbouring 16 bytes. A __syncthreads() comes after
 template <int HD>
-__global__ void __launch_bounds__(kThreads, 3) paged_append_kernel(const __grid_constant__ bolt3_paged_append_args a,
+B3_DEV bool load_norms(const bolt3_paged_append_args& a, float4* s_norm) {
+  if (threadIdx.x < HD / 2) {
+    const float* w = threadIdx.x < HD / 4 ? a.q_norm_w : a.k_norm_w;
+    const int i = threadIdx.x % (HD / 8), at = threadIdx.x - i + i % 2 * (HD / 16) + i / 2;
+    if (w != nullptr) s_norm[at] = __ldg(reinterpret_cast<const float4*>(w) + threadIdx.x % (HD / 4));
+  }
+  return a.q_norm_w != nullptr || a.k_norm_w != nullptr;
+}
+
+// The cosines of two neighbouring pairs of dimensions of a token, then their sines, for all pairs, by the lanes of a warp; the
+// i-th 16 bytes of every lane's four (append_rows) stand together (a lane's own together: 4 banks for 8 lanes, and 50 us
+// rather than 41 for 64 x 128 tokens of 32 + 2 x 8 heads of 128)
+template <int HD>
+B3_DEV void turns_of(const bolt3_paged_append_args& a, const Token& tk, float* turns, int lane) {
+#pragma unroll
+  for (int i = lane; i < HD / 2; i += 32) {
+    float sn = 0.f, cs = 1.f;
+    if (a.inv_freq != nullptr) {
+      const double turn = (double)tk.pos * (double)a.inv_freq[i] * 0.15915494309189533577;   // 1 / (2 pi)
+      __sincosf((float)((turn - rint(turn)) * 6.28318530717958647693), &sn, &cs);   // within 2^-21 of either, in [-pi, pi]
+    }
+    float* at = turns + (i / 2 % 4 * (HD / 16) + i / 8) * 4 + i % 2;
+    at[0] = cs;
+    at[2] = sn;
+  }
+}
+
+// Rows r0 .. of a token, one for each HD / 16 lanes: this lane's values 8 part .. of row r in o0, HD / 2 + 8 part .. in o1. Rows
+// from `end` on store nothing, but their lanes take part: the shuffles name the warp
+template <int HD>
+B3_DEV void append_rows(const bolt3_paged_append_args& a, const Token& tk, uint4 o0, uint4 o1, int r0, int r, int end, uint32_t at_turn,
+                        uint32_t at_norm, bool norms) {
+  constexpr int LPR = HD / 16;
+  const int part = (threadIdx.x & 31) % LPR;
+  const bool is_q = r < a.H, is_k = !is_q && r < a.H + a.HKV;
+  auto lds = [](uint32_t at, uint64_t& lo, uint64_t& hi) {   // where it stands: kept in registers over the rows they cost the loads in flight
+    asm volatile("ld.shared.v2.b64 {%0,%1}, [%2];\n" : "=l"(lo), "=l"(hi) : "r"(at));
+  };
+  if (r0 < a.H + a.HKV) {                            // the same for the whole warp: some of its rows are queries or keys
+    uint64_t x[4], y[4];                             // the values, two neighbours at a time
+    {
+      const uint32_t w0[4] = {o0.x, o0.y, o0.z, o0.w}, w1[4] = {o1.x, o1.y, o1.z, o1.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = pair(__uint_as_float(w0[i] << 16), __uint_as_float(w0[i] & 0xffff0000u));
+        y[i] = pair(__uint_as_float(w1[i] << 16), __uint_as_float(w1[i] & 0xffff0000u));
+      }
+    }
+    if (norms) {
+      uint64_t s0 = mul2(x[0], x[0]), s1 = mul2(y[0], y[0]);
+#pragma unroll
+      for (int i = 1; i < 4; ++i) {
+        s0 = fma2(x[i], x[i], s0);
+        s1 = fma2(y[i], y[i], s1);
+      }
+      const float2 s2 = unpair(add2(s0, s1));
+      float ss = s2.x + s2.y;
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (is_q ? a.q_norm_w != nullptr : is_k && a.k_norm_w != nullptr) {
+        const float inv = rsqrtf(ss * (1.f / HD) + a.eps);
+        const uint64_t inv2 = pair(inv, inv);
+        const uint32_t w = at_norm + (is_q ? 0 : HD * 4);
+        uint64_t wx[4], wy[4];
+        lds(w, wx[0], wx[1]);
+        lds(w + HD, wx[2], wx[3]);
+        lds(w + HD * 2, wy[0], wy[1]);
+        lds(w + HD * 3, wy[2], wy[3]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = mul2(x[i], mul2(inv2, wx[i]));
+          y[i] = mul2(y[i], mul2(inv2, wy[i]));
+        }
+      }
+    }
+    if (is_q || is_k) {
+      uint32_t w0[4], w1[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint64_t c, d;                               // cosines and sines of a pair of pairs
+        lds(at_turn + HD * i, c, d);
+        const float2 u = unpair(fma2(x[i], c, mul2(y[i], d ^ 0x8000000080000000ull))), v = unpair(fma2(y[i], c, mul2(x[i], d)));
+        w0[i] = pack_bf16(u.x, u.y);
+        w1[i] = pack_bf16(v.x, v.y);
+      }
+      o0 = make_uint4(w0[0], w0[1], w0[2], w0[3]);
+      o1 = make_uint4(w1[0], w1[1], w1[2], w1[3]);
+    }
+  }
+  if (r >= end) return;
+  bf16* out;
+  if (is_q) {
+    if (tk.s < 0) o0 = o1 = make_uint4(0, 0, 0, 0);
+    out = reinterpret_cast<bf16*>(a.q_out) + (tk.token * a.H + r) * HD + 8 * part;
+  } else {
+    if (tk.page < 0) return;
+    const int h = is_k ? r - a.H : r - a.H - a.HKV;
+    const int64_t row = ((is_k ? 0 : a.n_pages) + tk.page) * a.HKV + h;
+    out = reinterpret_cast<bf16*>(a.pages) + (row * a.page + (tk.row & (a.page - 1))) * HD + 8 * part;
+    if (is_k && part == 0 && a.weight != nullptr) {
+      const int64_t at = ((int64_t)tk.b * a.HKV + h) * a.width * a.page + tk.row;
+      a.weight[at] = 0.f;
+      a.order[at] = (int32_t)tk.pos;
+    }
+  }
+  reinterpret_cast<uint4*>(out)[0] = o0;
+  reinterpret_cast<uint4*>(out + HD / 2)[0] = o1;
+}
+
+// A warp takes rows [c rows_per, ..) of the H + 2 HKV rows of a token, of `chunks` such stretches. The row after the one at work
+// is in flight, and 32 warps of an SM hide the rest: 64 x 128 tokens of 32 + 2 x 8 heads of 128 in 39 us, where a copy of as many
+// bytes takes 35 (two rows in flight and 24 warps 41 us, four and 16 48 us, 40 warps spill: 48 us; rows by bulk copies through
+// a ring of shared memory are not faster)
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(const __grid_constant__ bolt3_paged_append_args a,
                                                                 const __grid_constant__ Length len,
                                                                 const __grid_constant__ Pages pages, int chunks, int rows_per) {
   constexpr int LPR = HD / 16, RPI = 32 / LPR;       // lanes of a row, rows of an iteration
-  constexpr int PPG = 8 / RPI;                       // pairs of a lane's eight whose angle it takes itself
-  __shared__ float4 s_turn[kThreads / 32][HD / 4];   // of a warp's token: cos, sin of a pair of dimensions, cos, sin of the next
+  __shared__ float4 s_turn[kThreads / 32][HD / 4];   // of a warp's token (turns_of)
   __shared__ float4 s_norm[2][HD / 4];               // of queries, of keys
   const int lane = threadIdx.x & 31, part = lane % LPR, sub = lane / LPR;
   const int64_t item = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), token = item / chunks;
   grid_dep_launch();
   grid_dep_wait();
-  const bool norms = a.q_norm_w != nullptr || a.k_norm_w != nullptr;
-  if (norms) {
-    if (threadIdx.x < HD / 2) {
-      const float* w = threadIdx.x < HD / 4 ? a.q_norm_w : a.k_norm_w;
-      if (w != nullptr) s_norm[0][threadIdx.x] = __ldg(reinterpret_cast<const float4*>(w) + threadIdx.x % (HD / 4));
-    }
-    __syncthreads();
-  }
+  const bool norms = load_norms<HD>(a, s_norm[0]);
+  __syncthreads();
   if (token >= (int64_t)a.B * a.T) return;
   const int c = (int)(item - token * chunks), b = (int)(token / a.T), t = (int)(token - (int64_t)b * a.T);
   const int n_rows = a.H + 2 * a.HKV, first = c * rows_per, end = min(n_rows, first + rows_per);
   const bf16* q = reinterpret_cast<const bf16*>(a.q) + b * a.q_sb + t * a.q_st + 8 * part;
   const bf16* k = reinterpret_cast<const bf16*>(a.k) + b * a.k_sb + t * a.k_st + 8 * part;
   const bf16* v = reinterpret_cast<const bf16*>(a.v) + b * a.v_sb + t * a.v_st + 8 * part;
-  uint4 raw[kAhead][2];                              // values 8 part .., HD / 2 + 8 part ..
-  auto fetch = [&](int u, int r) {
+  uint4 raw[2];                                      // values 8 part .., HD / 2 + 8 part ..
+  auto fetch = [&](int r) {
     if (r >= end) return;
     const bf16* src = r < a.H ? q + r * HD : r < a.H + a.HKV ? k + (r - a.H) * HD : v + (r - a.H - a.HKV) * HD;
-    raw[u][0] = __ldg(reinterpret_cast<const uint4*>(src));
-    raw[u][1] = __ldg(reinterpret_cast<const uint4*>(src + HD / 2));
+    raw[0] = __ldg(reinterpret_cast<const uint4*>(src));
+    raw[1] = __ldg(reinterpret_cast<const uint4*>(src + HD / 2));
   };
-#pragma unroll
-  for (int u = 0; u < kAhead; ++u) fetch(u, first + u * RPI + sub);
-  bool bad = false;
-  const int64_t s = len.rows(b, bad);                // the same for the whole warp
-  int pg = -1;
-  if (s >= 0) {
-    pg = pages.page_of(b, s + t);
-    bad |= pg < 0;
-  }
-  if (bad && lane == 0 && a.status) atomicOr(a.status, 8);
-  const int64_t pos = s < 0 ? 0 : a.pos != nullptr ? (int64_t)a.pos[b] + t : a.pos0 + (s + t - a.n);
-  if (first < a.H + a.HKV) {
-    float2* turns = reinterpret_cast<float2*>(s_turn[threadIdx.x >> 5]) + 8 * part + PPG * sub;
-#pragma unroll
-    for (int i = 0; i < PPG; ++i) {                  // the row groups share the work
-      float sn = 0.f, cs = 1.f;
-      if (a.inv_freq != nullptr) {
-        const double turn = (double)pos * (double)a.inv_freq[8 * part + PPG * sub + i] * 0.15915494309189533577;   // 1 / (2 pi)
-        __sincosf((float)((turn - rint(turn)) * 6.28318530717958647693), &sn, &cs);   // within 2^-21 of either, in [-pi, pi]
-      }
-      turns[i] = make_float2(cs, sn);
-    }
-    __syncwarp();
-  }
-  const uint32_t at_turn = (uint32_t)__cvta_generic_to_shared(s_turn[threadIdx.x >> 5] + 4 * part);
-  const uint32_t at_norm = (uint32_t)__cvta_generic_to_shared(s_norm[0] + 2 * part);
-  auto lds = [](uint32_t at) {                       // where it stands: kept in registers over the rows they cost the loads in flight
-    float4 z;
-    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];\n" : "=f"(z.x), "=f"(z.y), "=f"(z.z), "=f"(z.w) : "r"(at));
-    return z;
-  };
-  // rows past the end compute on what stands in the registers and store nothing: the shuffles name the warp
-  for (int r0 = first; r0 < end; r0 += kAhead * RPI) {
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (r0 + u * RPI >= end) break;                // the same for the whole warp
-      const int r = r0 + u * RPI + sub;
-      const bool is_q = r < a.H, is_k = !is_q && r < a.H + a.HKV;
-      uint4 o0 = raw[u][0], o1 = raw[u][1];
-      fetch(u, r + kAhead * RPI);
-      if (r0 + u * RPI < a.H + a.HKV) {              // the same for the whole warp: some of its rows are queries or keys
-        float x[8], y[8];                            // the pairs
-        {
-          const uint32_t w0[4] = {o0.x, o0.y, o0.z, o0.w}, w1[4] = {o1.x, o1.y, o1.z, o1.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 p0 = unpack_bf16(w0[i]), p1 = unpack_bf16(w1[i]);
-            x[2 * i] = p0.x; x[2 * i + 1] = p0.y;
-            y[2 * i] = p1.x; y[2 * i + 1] = p1.y;
-          }
-        }
-        if (norms) {
-          float ss = 0.f, s2 = 0.f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            ss = fmaf(x[i], x[i], ss);
-            s2 = fmaf(y[i], y[i], s2);
-          }
-          ss += s2;
-#pragma unroll
-          for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          if (is_q ? a.q_norm_w != nullptr : is_k && a.k_norm_w != nullptr) {
-            const float inv = rsqrtf(ss * (1.f / HD) + a.eps);
-            const uint32_t w = at_norm + (is_q ? 0 : HD * 4);
-            const float4 wa = lds(w), wb = lds(w + 16), wc = lds(w + HD * 2), wd = lds(w + HD * 2 + 16);
-            x[0] *= inv * wa.x; x[1] *= inv * wa.y; x[2] *= inv * wa.z; x[3] *= inv * wa.w;
-            x[4] *= inv * wb.x; x[5] *= inv * wb.y; x[6] *= inv * wb.z; x[7] *= inv * wb.w;
-            y[0] *= inv * wc.x; y[1] *= inv * wc.y; y[2] *= inv * wc.z; y[3] *= inv * wc.w;
-            y[4] *= inv * wd.x; y[5] *= inv * wd.y; y[6] *= inv * wd.z; y[7] *= inv * wd.w;
-          }
-        }
-        if (is_q || is_k) {
-          uint32_t w0[4], w1[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int e = 2 * i, f = e + 1;
-            const float4 z = lds(at_turn + 16 * i);  // of pairs e and f
-            w0[i] = pack_bf16(fmaf(x[e], z.x, -y[e] * z.y), fmaf(x[f], z.z, -y[f] * z.w));
-            w1[i] = pack_bf16(fmaf(y[e], z.x, x[e] * z.y), fmaf(y[f], z.z, x[f] * z.w));
-          }
-          o0 = make_uint4(w0[0], w0[1], w0[2], w0[3]);
-          o1 = make_uint4(w1[0], w1[1], w1[2], w1[3]);
-        }
-      }
-      if (r >= end) continue;
-      bf16* out;
-      if (is_q) {
-        if (s < 0) o0 = o1 = make_uint4(0, 0, 0, 0);
-        out = reinterpret_cast<bf16*>(a.q_out) + (token * a.H + r) * HD + 8 * part;
-      } else {
-        if (pg < 0) continue;
-        const int h = is_k ? r - a.H : r - a.H - a.HKV;
-        const int64_t row = ((is_k ? 0 : a.n_pages) + pg) * a.HKV + h;
-        out = reinterpret_cast<bf16*>(a.pages) + (row * a.page + ((s + t) & (a.page - 1))) * HD + 8 * part;
-        if (is_k && part == 0 && a.weight != nullptr) {
-          const int64_t at = ((int64_t)b * a.HKV + h) * a.width * a.page + s + t;
-          a.weight[at] = 0.f;
-          a.order[at] = (int32_t)pos;
-        }
-      }
-      reinterpret_cast<uint4*>(out)[0] = o0;
-      reinterpret_cast<uint4*>(out + HD / 2)[0] = o1;
-    }
+  fetch(first + sub);
+  const Token tk = token_at(a, len, pages, token, lane);
+  if (first < a.H + a.HKV) turns_of<HD>(a, tk, reinterpret_cast<float*>(s_turn[threadIdx.x >> 5]), lane);
+  __syncwarp();
+  const uint32_t at_turn = (uint32_t)__cvta_generic_to_shared(s_turn[threadIdx.x >> 5] + part);
+  const uint32_t at_norm = (uint32_t)__cvta_generic_to_shared(s_norm[0] + part);
+  for (int r0 = first; r0 < end; r0 += RPI) {
+    const uint4 o0 = raw[0], o1 = raw[1];
+    fetch(r0 + sub + RPI);                           // rows past the end compute on what stands in the registers
+    append_rows<HD>(a, tk, o0, o1, r0, r0 + sub, end, at_turn, at_norm, norms);
   }
 }
 
@@ -209,8 +246,8 @@ struct Evict {
   bolt3_paged_evict_args a;
   Pages pages;
   int64_t most;                                      // moves that a head can have
-  int2* moves;                                       // [head][most] (to, from)
-  int32_t* count;                                    // [head]
+  int2* moves;                                       // [head][most] (to, from), where they are not listed in shared memory
+  int32_t* count;                                    // [head], where `split`
   int split;                                         // a second kernel moves the rows
 };
 
@@ -288,7 +325,7 @@ __global__ void __launch_bounds__(NT) paged_evict_kernel(const __grid_constant__
   if (tid == 0) {
     if (bad && h == 0 && a.status) atomicOr(a.status, 8);
     if (h == 0 && a.lens_out != nullptr) a.lens_out[b] = bad ? -1 : (int32_t)min(held, a.keep);
-    p.count[head] = 0;
+    if (p.split) p.count[head] = 0;
     s_bad = 0;
   }
   if (bad || held <= a.keep) return;                 // the same for all threads
@@ -440,8 +477,10 @@ __global__ void __launch_bounds__(NT) paged_evict_kernel(const __grid_constant__
     hole += __popc(d);
     mover += __popc(m);
   }
-  if (tid == 0) p.count[head] = n_moves;
-  if (p.split) return;
+  if (p.split) {
+    if (tid == 0) p.count[head] = n_moves;
+    return;
+  }
   __syncthreads();
   move_rows<HD>(p, b, h, moves, warp, n_moves, W, lane);
 }
@@ -457,6 +496,7 @@ __global__ void __launch_bounds__(kThreads) paged_move_kernel(const __grid_const
 }
 
 int64_t most_moves(int64_t n, int64_t keep) { return n <= keep ? 0 : n - keep < keep ? n - keep : keep; }
+bool split_moves(int64_t heads, int64_t most) { return most > kInline && heads < 148; }
 
 template <int HD, int NT>
 int launch_select(const Evict& p, cudaStream_t s) {
@@ -508,37 +548,40 @@ extern "C" int bolt3_paged_append(const bolt3_paged_append_args* a, void* stream
   // a warp per token, or per share of a token's rows where there are few: as long as eight warps per SM are not reached
   const int rows = a->H + 2 * a->HKV, rpi = 32 / (a->HD / 16), groups = (rows + rpi - 1) / rpi;
   const int64_t tokens = (int64_t)a->B * a->T;
+  cudaStream_t s = (cudaStream_t)stream;
   int64_t chunks = (148 * 16 + tokens - 1) / tokens;
   if (chunks > groups) chunks = groups;
   const int rows_per = (groups + (int)chunks - 1) / (int)chunks * rpi;
   chunks = (rows + rows_per - 1) / rows_per;
   const int64_t blocks = (tokens * chunks + kThreads / 32 - 1) / (kThreads / 32);
-  if (blocks > 0x7fffffff) return BOLT3_ERR_SHAPE;
-  cudaStream_t s = (cudaStream_t)stream;
   return launch_overlapped(a->HD == 128 ? paged_append_kernel<128> : paged_append_kernel<64>, dim3((unsigned)blocks), dim3(kThreads), 0, s,
                            *a, len, pages, (int)chunks, rows_per) == cudaSuccess ? BOLT3_OK : BOLT3_ERR_CUDA;
 }
 
 extern "C" size_t bolt3_paged_evict_workspace(int B, int HKV, int64_t n, int64_t keep) {
   if (B <= 0 || HKV <= 0 || n < 0 || keep < 1 || n > 0x7fffffff) return 0;
-  return (size_t)B * (size_t)HKV * ((size_t)most_moves(n, keep) * 8 + 4);
+  const int64_t heads = (int64_t)B * HKV, most = most_moves(n, keep);
+  const bool split = split_moves(heads, most);
+  return split || most > kListed ? (size_t)heads * ((size_t)most * 8 + (split ? 4 : 0)) : 0;
 }
 
 extern "C" int bolt3_paged_evict(const bolt3_paged_evict_args* a, void* stream) {
   const b3::TraceRange trace_range("bolt3_paged_evict");
-  if (!a || !a->pages || !a->table || !a->weight || !a->order || !a->workspace) return BOLT3_ERR_ARG;
+  if (!a || !a->pages || !a->table || !a->weight || !a->order) return BOLT3_ERR_ARG;
   if (a->keep < 1 || a->recent < 0 || a->recent > a->keep) return BOLT3_ERR_ARG;
   if (a->B <= 0 || (int64_t)a->B * a->HKV > 0x7fffffff) return BOLT3_ERR_SHAPE;
   Evict p;
   if (!pages_ok(a->n_pages, a->page, a->width, a->table_stride, a->HKV, a->HD, &p.pages, a->table)) return BOLT3_ERR_SHAPE;
   if (a->n < 0 || a->n > a->width * a->page) return BOLT3_ERR_CAPACITY;
-  if (a->workspace_bytes < bolt3_paged_evict_workspace(a->B, a->HKV, a->n, a->keep)) return BOLT3_ERR_CAPACITY;
+  const size_t need = bolt3_paged_evict_workspace(a->B, a->HKV, a->n, a->keep);
+  if (need > 0 && !a->workspace) return BOLT3_ERR_ARG;
+  if (a->workspace_bytes < need) return BOLT3_ERR_CAPACITY;
   if (((uintptr_t)a->pages | (uintptr_t)a->workspace) & 15) return BOLT3_ERR_ALIGN;
   p.a = *a;
   p.most = most_moves(a->n, a->keep);
   p.moves = reinterpret_cast<int2*>(a->workspace);
   p.count = reinterpret_cast<int32_t*>(p.moves + (int64_t)a->B * a->HKV * p.most);
-  p.split = p.most > kInline && (int64_t)a->B * a->HKV < 148;
+  p.split = split_moves((int64_t)a->B * a->HKV, p.most);
   cudaStream_t s = (cudaStream_t)stream;
   return a->HD == 128 ? launch_evict<128>(p, s) : launch_evict<64>(p, s);
 }

@@ -917,9 +917,9 @@ def paged_evict(*, pages: torch.Tensor, table: torch.Tensor, weight: torch.Tenso
         raise ValueError(f"keep must be at least 1 and recent within [0, keep], got keep={keep} recent={recent}")
     out = None if lens is None else torch.empty(B, dtype=torch.int32, device=pages.device)
     nbytes = _evict_workspace(B, HKV, n, keep)
-    ws = torch.empty(nbytes or 16, dtype=torch.uint8, device=pages.device)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=pages.device) if nbytes else None
     _lib.paged_evict(torch._C._cuda_getCurrentRawStream(dev), B, HKV, HD, at, P, page, tat, stride, W, w_at, o_at, n, keep, recent,
-                     _lens_ptr(lens, None, B, dev), 0 if out is None else out.data_ptr(), ws.data_ptr(), nbytes,
+                     _lens_ptr(lens, None, B, dev), 0 if out is None else out.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes,
                      _status_ptr(status))
     _count(1)
     return min(n, keep) if out is None else out
