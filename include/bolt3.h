@@ -294,7 +294,8 @@ size_t bolt3_kv8_attend_workspace(int B, int T, int H, int HKV, int HD, int64_t 
  * (optional) at position pos0 + (s_b - n) + t, or pos[b] + t where `pos` (device int32 [B], with `lens`) is given: of a
  * cache that dropped rows the position is not the row. q rounded once to q_out (0 for an idle sequence), k once to its page,
  * v as it is. fp32; the angle is position * inv_freq to fp32's precision of the turn, however far the position. `weight`
- * and `order` (both or none) of the new rows become 0 and the position. q, k, v as in bolt3_kv8_append. H + 2 HKV <= 4096. */
+ * and `order` (both or none) of the new rows become 0 and the position, which has to fit 32 bits (pos[b] + t above them counts
+ * as the largest). q, k, v as in bolt3_kv8_append. H + 2 HKV <= 4096. */
 typedef struct bolt3_paged_append_args {
   int B, T, H, HKV, HD;
   const void* q; const void* k; const void* v;

@@ -616,3 +616,111 @@ def test_a_device_position_out_of_its_range_is_skipped():
     with pytest.raises(RuntimeError, match="outside the range"):
         st["status"].check(block=True)
     assert bool((y == 0).all()) and bool((st["weight"] == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 40])
+def test_a_pool_whose_offsets_pass_32_bits(T):
+    """The same rows in pages at the start of a small pool and at the end of one of more than 2^31 values to a side."""
+    B, H, HKV, HD, page, n = 2, 4, 1, 128, 128, 300
+    W, P = 3, (1 << 31) // (128 * 128) + 9
+    x = randn(60, B, n + T, (H + 2 * HKV) * HD, dtype=torch.bfloat16).cuda()
+    cut = (0, H * HD, (H + HKV) * HD, (H + 2 * HKV) * HD)
+    small = torch.zeros(2, B * W, HKV, page, HD, dtype=torch.bfloat16, device="cuda")
+    large = torch.empty(2, P, HKV, page, HD, dtype=torch.bfloat16, device="cuda")
+    tables = [torch.arange(B * W, dtype=torch.int32, device="cuda").view(B, W)]
+    tables.append(tables[0] + (P - B * W))
+    out = []
+    for pages, table in zip((small, large), tables):
+        pages[:, table.view(-1).long()] = 0
+        rec = dict(weight=torch.zeros(B, HKV, W * page, device="cuda"), order=torch.zeros(B, HKV, W * page, dtype=torch.int32, device="cuda"))
+        for t0, t1 in ((0, n), (n, n + T)):
+            q, k, v = (x[:, t0:t1, a:b] for a, b in zip(cut, cut[1:]))
+            q = K.paged_append(q=q, k=k, v=v, pages=pages, table=table, n=t0, pos0=t0, **rec)
+        y = K.paged_attend(q=q, pages=pages, table=table, n=n, weight=rec["weight"])
+        left = K.paged_evict(pages=pages, table=table, n=n + T, keep=200, recent=9, **rec)
+        out.append((q, y, left, pages[:, table.view(-1).long()], rec["weight"], rec["order"]))
+    for a, b in zip(*out):
+        assert a == b if isinstance(a, int) else torch.equal(a, b)
+    assert bool((out[0][1] != 0).any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 40])
+def test_calls_on_two_streams_at_once(T):
+    """Two streams take steps over caches of their own at the same time; each is as it is alone."""
+    H, HKV, HD, page, n = 8, 2, 128, 32, 700
+    cap = 1024
+    x = [randn(70 + i, 3, T, (H + 2 * HKV) * HD, dtype=torch.bfloat16).cuda() for i in range(2)]
+    cut = (0, H * HD, (H + HKV) * HD, (H + 2 * HKV) * HD)
+    kv = [randn(72 + i, 2, 3 * cap // page, HKV, page, HD, dtype=torch.bfloat16).cuda() for i in range(2)]
+    table = torch.arange(3 * cap // page, dtype=torch.int32, device="cuda").view(3, -1)
+
+    def fresh(i):
+        return dict(pages=kv[i].clone(), weight=torch.zeros(3, HKV, cap, device="cuda"),
+                    order=torch.arange(cap, dtype=torch.int32, device="cuda").expand(3, HKV, cap).contiguous())
+
+    def step(i, st, j):
+        q, k, v = (x[i][..., a:b] for a, b in zip(cut, cut[1:]))
+        q = K.paged_append(q=q, k=k, v=v, table=table, n=n + j * T, pos0=n + j * T, **st)
+        return K.paged_attend(q=q, pages=st["pages"], table=table, n=n + j * T, weight=st["weight"])
+
+    def finish(st):
+        K.paged_evict(table=table, n=n + 4 * T, keep=n // 2, recent=3, **st)
+
+    want, ys = [fresh(i) for i in range(2)], [[], []]
+    for i in range(2):
+        ys[i] = [step(i, want[i], j) for j in range(4)]
+        finish(want[i])
+    got, zs = [fresh(i) for i in range(2)], [[], []]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for j in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                zs[i].append(step(i, got[i], j))
+    for i, st in enumerate(streams):
+        with torch.cuda.stream(st):
+            finish(got[i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(ys[i], zs[i]))
+        assert all(torch.equal(want[i][k], got[i][k]) for k in got[i])
+
+
+@pytest.mark.gpu
+def test_positions_are_recorded_in_32_bits():
+    """The last positions that fit are recorded, later ones refused; positions on the device count as the largest."""
+    for pos0 in (2 ** 31 - 1, -(2 ** 31) + 4):
+        calls, st = _call(pos0=pos0)
+        with pytest.raises(RuntimeError):
+            calls[0]()
+    calls, st = _call(pos0=2 ** 31 - 2)
+    calls[0]()
+    assert st["order"][:, :, 5].tolist() == [[2 ** 31 - 2] * 2] * 2
+    z = torch.zeros(2, 3, 2 * 64, dtype=torch.bfloat16, device="cuda")
+    K.paged_append(q=z, k=z, v=z, pages=st["pages"], table=st["table"], n=5, pos0=0, weight=st["weight"], order=st["order"],
+                   lens=torch.tensor([5, 0], dtype=torch.int32, device="cuda"),
+                   pos=torch.tensor([2 ** 31 - 2, -7], dtype=torch.int32, device="cuda"))
+    assert st["order"][0, 0, 5:8].tolist() == [2 ** 31 - 2, 2 ** 31 - 1, 2 ** 31 - 1]
+    assert st["order"][1, 1, 0:3].tolist() == [-7, -6, -5]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 40])
+def test_tables_and_queries_with_strides(T):
+    """Rows of a larger table, queries out of a larger tensor, and outputs that the caller gives."""
+    B, H, HKV, HD, page, n = 3, 8, 2, 64, 16, 200
+    W = -(-(n + T) // page)
+    pages = randn(80, 2, B * W, HKV, page, HD, dtype=torch.bfloat16).cuda()
+    wide = torch.full((2 * B, W + 5), -3, dtype=torch.int32, device="cuda")
+    table = torch.randperm(B * W, generator=torch.Generator().manual_seed(81)).to(torch.int32).view(B, W).cuda()
+    wide[::2, 2:W + 2] = table
+    q = randn(82, B, T, H, HD, dtype=torch.bfloat16).cuda()
+    qs = torch.full((B, 2 * T, H + 3, HD), float("nan"), dtype=torch.bfloat16, device="cuda")
+    qs[:, ::2, 1:H + 1] = q
+    weight = [torch.zeros(B, HKV, W * page, device="cuda") for _ in range(2)]
+    y = K.paged_attend(q=q, pages=pages, table=table, n=n, weight=weight[0])
+    out = torch.empty_like(y)
+    got = K.paged_attend(q=qs[:, ::2, 1:H + 1], pages=pages, table=wide[::2, 2:W + 2], n=n, weight=weight[1], y=out)
+    assert got is out and torch.equal(got, y) and torch.equal(*weight)

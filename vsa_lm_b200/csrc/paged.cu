@@ -185,7 +185,7 @@ B3_DEV void append_rows(const bolt3_paged_append_args& a, const Token& tk, uint4
     if (is_k && part == 0 && a.weight != nullptr) {
       const int64_t at = ((int64_t)tk.b * a.HKV + h) * a.width * a.page + tk.row;
       a.weight[at] = 0.f;
-      a.order[at] = (int32_t)tk.pos;
+      a.order[at] = (int32_t)min(tk.pos, (int64_t)0x7fffffff);
     }
   }
   reinterpret_cast<uint4*>(out)[0] = o0;
@@ -537,6 +537,8 @@ extern "C" int bolt3_paged_append(const bolt3_paged_append_args* a, void* stream
   Pages pages;
   if (!pages_ok(a->n_pages, a->page, a->width, a->table_stride, a->HKV, a->HD, &pages, a->table)) return BOLT3_ERR_SHAPE;
   const int64_t cap = a->width * a->page, dmax = a->pos_dev != nullptr ? a->pos_span - 1 : 0;
+  // positions are recorded in 32 bits
+  if (a->order != nullptr && a->pos == nullptr && (a->pos0 < -(1ll << 31) + a->n || a->pos0 > 0x7fffffffll - a->T - dmax)) return BOLT3_ERR_CAPACITY;
   if (a->n < 0 || cap < a->T || (a->lens == nullptr && a->n > cap - a->T - dmax)) return BOLT3_ERR_CAPACITY;
   const uintptr_t al = (uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->q_out | (uintptr_t)a->pages |
                        (uintptr_t)a->q_norm_w | (uintptr_t)a->k_norm_w;

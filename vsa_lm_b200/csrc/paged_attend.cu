@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_stream_kernel(const __grid_
       kvh = 0;
       start += nb * a.HKV;
       do {
-        ++b;
+        if (++b >= a.B) return;                                 // not reached while the lengths stand
         if (a.lens != nullptr) {
           s = p.c.len.rows(b, bad);
           nb = blocks_of(s, last);
