@@ -22,6 +22,8 @@
 // with the keys in the TMEM lanes: S^T = K Q^T, a thread per key, which sums 2^(t - lse) over the query columns in registers; no
 // two threads add to one record, whatever the split. A CTA holds up to 512 query rows of a head and walks a range of its keys.
 // Bound by the exponentials: 4096 cycles of an SM for 128 keys by 512 rows, against 2048 of its MMAs.
+#include <type_traits>
+
 #include "paged.cuh"
 #include "tc5.cuh"
 #include "trace.h"
@@ -64,8 +66,8 @@ struct RecordSmem {
   unsigned char k[2][kKeys * HD * 2];
   float lse[kRows];
   int token[kRows];
-  float sum[2][kRows / kKeys][kKeys];
-  uint64_t k_full[2], k_empty[2], s_full[kRows / kKeys], s_empty[kRows / kKeys];
+  float sum[4][kRows / kKeys][kKeys];            // of a block's keys, of each tile's rows
+  uint64_t k_full[2], k_empty[2], s_full[kRows / kKeys], s_empty[kRows / kKeys], sum_full[4][kRows / kKeys];
   uint32_t tbase;
   int err;
 };
@@ -538,6 +540,7 @@ __global__ void __launch_bounds__(kRecordThreads, 1) paged_prompt_record_kernel(
     for (int i = 0; i < NQ; ++i) {
       tc5::mbar_init(&sm.s_full[i], 1);
       tc5::mbar_init(&sm.s_empty[i], 128);
+      for (int x = 0; x < 4; ++x) tc5::mbar_init(&sm.sum_full[x][i], 4);
     }
     tc5::mbar_fence_init();
     sm.err = 0;
@@ -650,46 +653,70 @@ __global__ void __launch_bounds__(kRecordThreads, 1) paged_prompt_record_kernel(
     const int64_t cap = a.width * a.page;
     float* record = a.weight + (int64_t)head * cap;
     bool ok = true;
-    int uses = 0;                                // of this tile's columns so far
     for (int g = 0; g < groups; ++g) {
       const int row0 = g * kRows, nq = tiles_of(g);
       // this group's queries, sums and tokens (its first rows' MMAs of the group before are done: their scores were read)
       copy_queries<HD>(p, sm.q[0], b, kvh, row0, warp * 32, lane);
       copy_queries<HD>(p, sm.q[0], b, kvh, row0, warp * 32 + 16, lane);
       const int r = row0 + tid;
-      sm.lse[tid] = r < p.c.rows ? p.lse[(int64_t)head * p.c.rows + r] : -neg_inf();
+      sm.lse[tid] = r < p.c.rows ? -p.lse[(int64_t)head * p.c.rows + r] : neg_inf();   // negated
       sm.token[tid] = token_of(p, min(r, p.c.rows - 1));
       asm volatile("cp.async.wait_all;\nfence.proxy.async.shared::cta;\n" ::: "memory");
       meet();
       const uint32_t ts = sm.tbase + i * 128 + ((uint32_t)(32 * (warp & 3)) << 16);
       const int first_token = token_of(p, row0);
+      if (i >= nq) continue;
+      // The tiles' sums of a block's keys meet two blocks later, in the order of the tiles, at one tile's threads: no tile waits
+      // for another at every block. The four slots suffice: a tile comes to block j + 4 once the MMAs of block j + 3 were issued
+      // for all tiles, and so after each of them let go of the scores of block j + 2, which the one at which the sums of block j
+      // meet does after it has read them
+      float was = 0.f;                           // the record of this thread's key of the block before the last
+      auto meets_here = [&](int j) { return j >= 0 && i == min(j & 3, nq - 1); };
+      auto at = [&](int j) { return (lo + j) * kKeys + key; };
+      auto fetch = [&](int j) {
+        if (meets_here(j) && at(j) < s + a.T) was = record[at(j)];
+      };
+      auto add = [&](int j) {
+        if (!meets_here(j)) return;
+        const int it = g * n_blk + j;
+        float w = 0.f;
+        for (int x = 0; x < nq; ++x) {
+          ok = ok && wait(&sm.sum_full[it & 3][x], it >> 2);
+          w += sm.sum[it & 3][x][key];
+        }
+        if (ok && at(j) < s + a.T) record[at(j)] = was + w;
+      };
       for (int j = 0; j < n_blk; ++j) {
+        const int it = g * n_blk + j;
         const int64_t key0 = (lo + j) * kKeys;
+        add(j - 2);
         float sum = 0.f;
-        if (i < nq) {
-          ok = ok && wait(&sm.s_full[i], uses);
-          ++uses;
-          ok = __all_sync(0xffffffffu, ok);
-          __syncwarp();
-          if (ok) {
-            tc5::fence_after_sync();
-            const bool masked = key0 + kKeys > s + 1 + first_token;     // the same for all threads
-            const int rel = (int)max(min(key0 + key - s, (int64_t)0x7fffffff), (int64_t)-1);   // the first token that sees this key
-            uint64_t acc = 0;
-#pragma unroll 1
+        ok = ok && wait(&sm.s_full[i], it);
+        ok = __all_sync(0xffffffffu, ok);
+        __syncwarp();
+        if (ok) {
+          tc5::fence_after_sync();
+          const bool masked = key0 + kKeys > s + 1 + first_token;     // the same for all threads
+          const int rel = (int)max(min(key0 + key - s, (int64_t)0x7fffffff), (int64_t)-1);   // the first token that sees this key
+          uint64_t acc = 0;
+          // the next 32 scores are on their way while these are used; once the last have come, the next block's may overwrite them
+          auto run = [&](auto cut) {
+            uint32_t x[2][32];
+            tc5::ld32(ts, x[0]);
+            tc5::ld_wait();
+#pragma unroll
             for (int c = 0; c < kKeys; c += 32) {
-              uint32_t x[32];
-              tc5::ld32(ts + c, x);
-              const float4* lse = reinterpret_cast<const float4*>(sm.lse + i * kKeys + c);
+              const uint32_t(&y)[32] = x[c / 32 & 1];
+              if (c + 32 < kKeys) tc5::ld32(ts + c + 32, x[c / 32 + 1 & 1]);
+              const ulonglong2* lse = reinterpret_cast<const ulonglong2*>(sm.lse + i * kKeys + c);
               const int4* token = reinterpret_cast<const int4*>(sm.token + i * kKeys + c);
-              tc5::ld_wait();
 #pragma unroll
               for (int u = 0; u < 8; ++u) {
-                const float4 z = lse[u];
-                const float2 a0 = unpair(fma2(pair(__uint_as_float(x[4 * u]), __uint_as_float(x[4 * u + 1])), scale2, pair(-z.x, -z.y)));
-                const float2 a1 = unpair(fma2(pair(__uint_as_float(x[4 * u + 2]), __uint_as_float(x[4 * u + 3])), scale2, pair(-z.z, -z.w)));
+                const ulonglong2 z = lse[u];
+                const float2 a0 = unpair(fma2(pair(__uint_as_float(y[4 * u]), __uint_as_float(y[4 * u + 1])), scale2, z.x));
+                const float2 a1 = unpair(fma2(pair(__uint_as_float(y[4 * u + 2]), __uint_as_float(y[4 * u + 3])), scale2, z.y));
                 float e0 = ex2(a0.x), e1 = ex2(a0.y), e2 = ex2(a1.x), e3 = ex2(a1.y);
-                if (masked) {
+                if constexpr (cut) {
                   const int4 t = token[u];
                   e0 = t.x >= rel ? e0 : 0.f;
                   e1 = t.y >= rel ? e1 : 0.f;
@@ -698,24 +725,28 @@ __global__ void __launch_bounds__(kRecordThreads, 1) paged_prompt_record_kernel(
                 }
                 acc = add2(acc, add2(pair(e0, e1), pair(e2, e3)));
               }
+              if (c + 32 < kKeys) tc5::ld_wait();
+              if (c + 64 == kKeys) {
+                tc5::fence_before_sync();
+                tc5::mbar_arrive(&sm.s_empty[i]);
+              }
             }
-            const float2 x = unpair(acc);
-            sum = x.x + x.y;
-          }
-          tc5::fence_before_sync();
+          };
+          if (masked) run(std::true_type{});
+          else run(std::false_type{});
+          const float2 x = unpair(acc);
+          sum = x.x + x.y;
+        } else {
           tc5::mbar_arrive(&sm.s_empty[i]);
         }
-        // the tiles' sums of a key meet, in the order of the tiles
-        sm.sum[j & 1][i][key] = sum;
+        sm.sum[it & 3][i][key] = sum;
         __syncwarp();
-        asm volatile("barrier.sync 1, 512;\n" ::: "memory");
-        if (i == (j & 3) && key0 + key < s + a.T) {
-          float w = 0.f;
-#pragma unroll
-          for (int x = 0; x < NQ; ++x) w += sm.sum[j & 1][x][key];
-          record[key0 + key] += w;
-        }
+        if (lane == 0) tc5::mbar_arrive(&sm.sum_full[it & 3][i]);
+        fetch(j - 1);
       }
+      add(n_blk - 2);
+      fetch(n_blk - 1);
+      add(n_blk - 1);
     }
   }
   meet();
