@@ -116,6 +116,9 @@ B3_DEV void walk(const Params& p, RingState& rs, int b, int kvh, int64_t s, int 
   // lane l < 2 CB units brings box l: keys or values (bit 0), columns 64 c, unit u
   const int side = lane & 1, cb = (lane >> 1) % CB, unit = (lane >> 1) / CB;
   const bool issues = lane < 2 * CB << units_log;
+  // rows are read once: what else the call keeps in L2 (scores, partial sums) stays there. 64 sequences of 2176 keys, 8 heads: 95 -> 92 us,
+  // with records 110 -> 103
+  const uint64_t once = tc5::policy_evict_first();
   auto load = [&](int it, int stage) {
     const int at = it & ((1 << per_log) - 1);
     if (at == 0 && it > 0) {
@@ -132,7 +135,7 @@ B3_DEV void walk(const Params& p, RingState& rs, int b, int kvh, int64_t s, int 
       const int z = (int)((side * pages.n_pages + max(pg, 0)) * a.HKV + kvh);
       void* dst = reinterpret_cast<void*>(
           __cvta_shared_to_generic(rs.ring + stage * R::kStage + side * R::kSide + cb * (kBlock * 128) + (unit << (rows_log + 7))));
-      tc5::tma_load_3d(dst, &p.map, 64 * cb, (int)(row & ((1 << pages.log) - 1)), z, bar);
+      tc5::tma_load_3d(dst, &p.map, 64 * cb, (int)(row & ((1 << pages.log) - 1)), z, bar, once);
     }
   };
 #pragma unroll
@@ -339,17 +342,36 @@ B3_DEV int64_t blocks_of(int64_t s, int last) { return s < 0 ? 0 : (s + last + k
 // log2 of the sum of 2^t, from a reference and the sum relative to it
 B3_DEV float lse_of(float m, float l) { return l == 0.f ? -neg_inf() : m + log2f(l); }
 
-// the record of key `key` of a sequence with s rows before the call: its weights over the rows of a head that see it
-B3_DEV void record(const Params& p, int head, int64_t cap, int64_t s, int64_t key, const float* lse) {
-  const float* t = p.score + ((int64_t)head * p.most + key) * p.score_row;
-  const int first = key > s ? (int)(key - s) * p.c.G : 0;       // row that sees it first
-  float sum = 0.f;
-  for (int r = first & ~1; r < p.c.rows; r += 2) {
-    const float2 x = *reinterpret_cast<const float2*>(t + r);
-    if (r >= first) sum += ex2(x.x - lse[r]);
-    if (r + 1 < p.c.rows) sum += ex2(x.y - lse[r + 1]);
+// the records of keys key0, key0 + step, .. (kKeysAt of them, those below `end`) of a sequence with s rows before the call: their
+// weights over the rows of a head that see them. `lse` of the head's rows
+constexpr int kKeysAt = 4;
+B3_DEV void record(const Params& p, int head, int64_t cap, int64_t s, int64_t key0, int step, int64_t end, const float* lse) {
+  const float* t = p.score + ((int64_t)head * p.most + key0) * p.score_row;
+  float* weight = p.c.a.weight + head * cap + key0;
+  float sum[kKeysAt], was[kKeysAt];
+  int first[kKeysAt];                                           // row that sees the key first
+#pragma unroll
+  for (int u = 0; u < kKeysAt; ++u) {
+    const int64_t key = key0 + u * step;
+    first[u] = key >= end ? 0x7fffffff : key > s ? (int)(key - s) * p.c.G : 0;
+    was[u] = key < end ? weight[u * step] : 0.f;
+    sum[u] = 0.f;
   }
-  p.c.a.weight[head * cap + key] += sum;
+#pragma unroll 2
+  for (int r = 0; r < p.c.rows; r += 2) {
+    float2 x[kKeysAt];
+#pragma unroll
+    for (int u = 0; u < kKeysAt; ++u)
+      if (r + 1 >= first[u]) x[u] = *reinterpret_cast<const float2*>(t + (int64_t)u * step * p.score_row + r);
+#pragma unroll
+    for (int u = 0; u < kKeysAt; ++u) {
+      if (r >= first[u]) sum[u] += ex2(x[u].x - lse[r]);
+      if (r + 1 >= first[u] && r + 1 < p.c.rows) sum[u] += ex2(x[u].y - lse[r + 1]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kKeysAt; ++u)
+    if (key0 + u * step < end) weight[u * step] = was[u] + sum[u];
 }
 
 template <int HD, int NT>
@@ -427,7 +449,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_stream_kernel(const __grid_
       __syncthreads();
       const int64_t cap = a.width * a.page;
       if (s >= 0)
-        for (int64_t key = tid; key < s + a.T; key += 32 * kWarps) record(p, head, cap, s, key, s_lse);
+        for (int64_t key = tid; key < s + a.T; key += kKeysAt * 32 * kWarps) record(p, head, cap, s, key, 32 * kWarps, s + a.T, s_lse);
     }
     return;
   }
@@ -561,49 +583,50 @@ __global__ void __launch_bounds__(32 * kWarps) paged_stream_kernel(const __grid_
   }
 }
 
-// The runs' partial sums of a (head, query row) joined: by one warp where a head has few of them (ROWS = 4 rows a block),
-// else by all warps of a block (ROWS = 1)
-constexpr int kMaxJoinWarps = 16;
-
-template <int HD, int NC, int ROWS>
-__global__ void __launch_bounds__(ROWS == 1 ? 32 * kMaxJoinWarps : 32 * ROWS) paged_join_kernel(const __grid_constant__ Params p) {
-  constexpr int EPL = HD / 32;                                  // dimensions of a lane
-  __shared__ float s_acc[ROWS == 1 ? kMaxJoinWarps : 1][HD], s_m[kMaxJoinWarps], s_l[kMaxJoinWarps];
-  const bolt3_paged_attend_args& a = p.c.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_warps = ROWS == 1 ? blockDim.x >> 5 : 1;
-  const int head = blockIdx.x, b = head / a.HKV, kvh = head % a.HKV, row = blockIdx.y * ROWS + (ROWS == 1 ? 0 : warp);
-  const int tile = row / NC, r = row % NC;
-  grid_dep_launch();
-  grid_dep_wait();
-  if (row >= p.c.rows) return;
+// Where the partial sums of a head are: the first one's slot, the first run, their number. false: there are none, and the row's
+// output has been written (done) or is 0 (an idle sequence, or a run gave up)
+struct Parts {
+  int64_t base;
+  int x, r0, n;
+  bool done;
+};
+B3_DEV bool parts_of(const Params& p, int head, int heads, int tile, Parts& f) {
   bool bad = false;
-  const bool idle = p.c.len.rows(b, bad) < 0;
-  const int2 span = p.span[(int64_t)tile * gridDim.x + head];
-  bf16* y = out_row<HD>(p.c, b, kvh, row);
-  float* lse = p.score != nullptr ? p.lse + (int64_t)head * p.c.rows + row : nullptr;
-  const int r0 = span.x >> 1;
-  if (idle || (span.x >= 0 && (span.x >= 2 * p.n_runs || span.y < r0 || span.y >= p.n_runs))) {   // (the latter: a run gave up)
-    if (warp == 0 || ROWS > 1) {
-      for (int i = lane; i < HD; i += 32) y[i] = __float2bfloat16_rn(0.f);
-      if (lse != nullptr && lane == 0) *lse = -neg_inf();
-    }
-    return;
+  const int2 span = p.span[(int64_t)tile * heads + head];
+  f.base = (int64_t)tile * p.n_runs * 2;
+  f.x = span.x;
+  f.r0 = span.x >> 1;
+  f.n = span.y - f.r0 + 1;
+  f.done = span.x < 0;
+  if (p.c.len.rows(head / p.c.a.HKV, bad) < 0 || (span.x >= 0 && (span.x >= 2 * p.n_runs || span.y < f.r0 || span.y >= p.n_runs))) {
+    f.done = false;
+    return false;
   }
-  if (span.x < 0) return;                                       // the run wrote the output itself
-  const int64_t base = (int64_t)tile * p.n_runs * 2;
-  const int n = span.y - r0 + 1;
-  float m = neg_inf(), l = 0.f, acc[EPL] = {};
+  return !f.done;
+}
+// slot of the i-th of them: a later run's first stretch
+B3_DEV int64_t slot_of(const Parts& f, int i) { return f.base + (i == 0 ? f.x : 2 * (f.r0 + i)); }
+
+// The sums i0, i0 + step, .. of a query row (r of its tile) joined, by a warp: the reference, the sum of weights, the outputs'
+// dimensions 32 e + lane
+template <int HD, int NC>
+B3_DEV void join(const Params& p, const Parts& f, int r, int i0, int step, float& m, float& l, float (&acc)[HD / 32]) {
+  const int lane = threadIdx.x & 31;
+  m = neg_inf();
+  l = 0.f;
+#pragma unroll
+  for (int e = 0; e < HD / 32; ++e) acc[e] = 0.f;
   constexpr int kBatch = 4;
-  for (int i0 = ROWS == 1 ? warp : 0; i0 < n; i0 += kBatch * n_warps) {
+  for (; i0 < f.n; i0 += kBatch * step) {
     float2 ml[kBatch];
-    float x[kBatch][EPL];
+    float x[kBatch][HD / 32];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      const int i = i0 + j * n_warps;
-      const int64_t at = (base + (i == 0 ? span.x : 2 * (r0 + min(i, n - 1)))) * NC + r;   // a later run's first stretch
-      ml[j] = i < n ? p.part_ml[at] : make_float2(neg_inf(), 0.f);
+      const int i = i0 + j * step;
+      const int64_t at = slot_of(f, min(i, f.n - 1)) * NC + r;
+      ml[j] = i < f.n ? p.part_ml[at] : make_float2(neg_inf(), 0.f);
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) x[j][e] = i < n ? p.part[at * HD + 32 * e + lane] : 0.f;
+      for (int e = 0; e < HD / 32; ++e) x[j][e] = i < f.n ? p.part[at * HD + 32 * e + lane] : 0.f;
     }
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
@@ -612,54 +635,137 @@ __global__ void __launch_bounds__(ROWS == 1 ? 32 * kMaxJoinWarps : 32 * ROWS) pa
       m = to;
       l = fmaf(l, f0, ml[j].y * f1);
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) acc[e] = fmaf(acc[e], f0, x[j][e] * f1);
-    }
-  }
-  if constexpr (ROWS > 1) {
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) y[32 * e + lane] = __float2bfloat16_rn(l == 0.f ? 0.f : acc[e] / l);
-    if (lse != nullptr && lane == 0) *lse = lse_of(m, l);
-  } else {
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) s_acc[warp][32 * e + lane] = acc[e];
-    if (lane == 0) {
-      s_m[warp] = m;
-      s_l[warp] = l;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < HD; i += blockDim.x) {
-      m = neg_inf();
-      for (int w = 0; w < n_warps; ++w) m = fmaxf(m, s_m[w]);
-      float sum = 0.f;
-      l = 0.f;
-      for (int w = 0; w < n_warps; ++w) {
-        const float g = s_m[w] == neg_inf() ? 0.f : exp2f(s_m[w] - m);
-        sum = fmaf(s_acc[w][i], g, sum);
-        l = fmaf(s_l[w], g, l);
-      }
-      y[i] = __float2bfloat16_rn(l == 0.f ? 0.f : sum / l);
-      if (i == 0 && lse != nullptr) *lse = lse_of(m, l);
+      for (int e = 0; e < HD / 32; ++e) acc[e] = fmaf(acc[e], f0, x[j][e] * f1);
     }
   }
 }
 
-// The scores of a head's keys turned into weights and added to their records, a thread per key
-constexpr int kRecordThreads = 256;
+// A head's output row where there are no sums to join
+template <int HD>
+B3_DEV void zero_row(const Params& p, int head, int row) {
+  bf16* y = out_row<HD>(p.c, head / p.c.a.HKV, head % p.c.a.HKV, row);
+  for (int i = threadIdx.x & 31; i < HD; i += 32) y[i] = __float2bfloat16_rn(0.f);
+}
 
-__global__ void __launch_bounds__(kRecordThreads) paged_record_kernel(const __grid_constant__ Params p) {
+// The runs' partial sums of a (head, query row) where a head has few of them, joined by a warp; with records, blocks from
+// `joins` on turn the scores of kKeysAt * kJoinThreads keys of a head into weights at the same time (a launch less, and
+// neither waits for the other: 64 sequences of 2176 keys, 8 heads, 112 -> 110 us), for which they join the rows' sums of weights
+constexpr int kJoinThreads = 256;
+
+template <int HD, int NC>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ Params p, int joins, int chunks) {
+  constexpr int kJoinWarps = kJoinThreads / 32;
   __shared__ float s_lse[32];
   const bolt3_paged_attend_args& a = p.c.a;
-  const unsigned chunks = (unsigned)((p.most + kRecordThreads - 1) / kRecordThreads);
-  const int head = (int)(blockIdx.x / chunks), b = head / a.HKV;
-  const int64_t key = (int64_t)(blockIdx.x % chunks) * kRecordThreads + threadIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = a.B * a.HKV;
+  grid_dep_launch();
+  grid_dep_wait();
+  Parts f;
+  if ((int)blockIdx.x < joins) {
+    const int64_t item = (int64_t)blockIdx.x * kJoinWarps + warp;
+    if (item >= (int64_t)heads * p.c.rows) return;
+    const int head = (int)(item / p.c.rows), row = (int)(item - (int64_t)head * p.c.rows);
+    if (!parts_of(p, head, heads, row / NC, f)) {
+      if (!f.done) zero_row<HD>(p, head, row);
+      return;
+    }
+    float m, l, acc[HD / 32];
+    join<HD, NC>(p, f, row % NC, 0, 1, m, l, acc);
+    bf16* y = out_row<HD>(p.c, head / a.HKV, head % a.HKV, row);
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) y[32 * e + lane] = __float2bfloat16_rn(l == 0.f ? 0.f : acc[e] / l);
+    return;
+  }
+  const int at = blockIdx.x - joins, head = at / chunks, b = head / a.HKV;
+  bool bad = false;
+  const int64_t s = p.c.len.rows(b, bad), key = (int64_t)(at % chunks) * (kKeysAt * kJoinThreads) + threadIdx.x;
+  if (s < 0 || key - threadIdx.x >= s + a.T) return;            // the same for the whole block
+  for (int row = warp; row < p.c.rows; row += kJoinWarps) {
+    float m = neg_inf(), l = 0.f;
+    if (parts_of(p, head, heads, row / NC, f)) {
+      for (int i = lane; i < f.n; i += 32) {
+        const float2 ml = p.part_ml[slot_of(f, i) * NC + row % NC];
+        const float to = fmaxf(m, ml.x), ref = to == neg_inf() ? 0.f : to;
+        l = fmaf(l, exp2f(m - ref), ml.y * exp2f(ml.x - ref));
+        m = to;
+      }
+      float all = m;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, x));
+      l *= all == neg_inf() ? 1.f : exp2f(m - all);
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+      m = all;
+      if (lane == 0) s_lse[row] = lse_of(m, l);
+    } else if (lane == 0) {
+      s_lse[row] = f.done ? p.lse[(int64_t)head * p.c.rows + row] : -neg_inf();
+    }
+  }
+  __syncthreads();
+  record(p, head, a.width * a.page, s, key, kJoinThreads, s + a.T, s_lse);
+}
+
+// The same for heads with many partial sums: a block for each query row
+constexpr int kMaxJoinWarps = 16;
+
+template <int HD, int NC>
+__global__ void __launch_bounds__(32 * kMaxJoinWarps) paged_join_long_kernel(const __grid_constant__ Params p) {
+  __shared__ float s_acc[kMaxJoinWarps][HD], s_m[kMaxJoinWarps], s_l[kMaxJoinWarps];
+  const bolt3_paged_attend_args& a = p.c.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_warps = blockDim.x >> 5;
+  const int head = blockIdx.x, row = blockIdx.y;
+  grid_dep_launch();
+  grid_dep_wait();
+  float* lse = p.score != nullptr ? p.lse + (int64_t)head * p.c.rows + row : nullptr;
+  Parts f;
+  if (!parts_of(p, head, gridDim.x, row / NC, f)) {             // the same for the whole block
+    if (!f.done && warp == 0) {
+      zero_row<HD>(p, head, row);
+      if (lse != nullptr && lane == 0) *lse = -neg_inf();
+    }
+    return;
+  }
+  float m, l, acc[HD / 32];
+  join<HD, NC>(p, f, row % NC, warp, n_warps, m, l, acc);
+#pragma unroll
+  for (int e = 0; e < HD / 32; ++e) s_acc[warp][32 * e + lane] = acc[e];
+  if (lane == 0) {
+    s_m[warp] = m;
+    s_l[warp] = l;
+  }
+  __syncthreads();
+  bf16* y = out_row<HD>(p.c, head / a.HKV, head % a.HKV, row);
+  for (int i = threadIdx.x; i < HD; i += blockDim.x) {
+    m = neg_inf();
+    for (int w = 0; w < n_warps; ++w) m = fmaxf(m, s_m[w]);
+    float sum = 0.f;
+    l = 0.f;
+    for (int w = 0; w < n_warps; ++w) {
+      const float g = s_m[w] == neg_inf() ? 0.f : exp2f(s_m[w] - m);
+      sum = fmaf(s_acc[w][i], g, sum);
+      l = fmaf(s_l[w], g, l);
+    }
+    y[i] = __float2bfloat16_rn(l == 0.f ? 0.f : sum / l);
+    if (i == 0 && lse != nullptr) *lse = lse_of(m, l);
+  }
+}
+
+// The scores of a head's keys turned into weights and added to their records, once the rows' sums over all keys are known
+constexpr int kRecordThreads = 256;
+
+__global__ void __launch_bounds__(kRecordThreads) paged_record_kernel(const __grid_constant__ Params p, int chunks) {
+  __shared__ float s_lse[32];
+  const bolt3_paged_attend_args& a = p.c.a;
+  const int head = blockIdx.x / chunks, b = head / a.HKV;
+  const int64_t key = (int64_t)(blockIdx.x % chunks) * (kKeysAt * kRecordThreads) + threadIdx.x;
   grid_dep_launch();
   grid_dep_wait();
   bool bad = false;
-  const int64_t s = p.c.len.rows(b, bad), cap = a.width * a.page, end = s + a.T;
+  const int64_t s = p.c.len.rows(b, bad);
   if (s < 0) return;
   if (threadIdx.x < p.c.rows) s_lse[threadIdx.x] = p.lse[(int64_t)head * p.c.rows + threadIdx.x];
   __syncthreads();
-  if (key < end) record(p, head, cap, s, key, s_lse);
+  record(p, head, a.width * a.page, s, key, kRecordThreads, s + a.T, s_lse);
 }
 
 // how a call is cut: columns of a CTA (in 8), column tiles, runs
@@ -707,16 +813,19 @@ int launch_stream(Params& p, const Plan& pl, cudaStream_t s) {
   const unsigned heads = (unsigned)(p.c.a.B * p.c.a.HKV), ctas = pl.runs == 0 ? heads : (unsigned)((pl.runs + kWarps - 1) / kWarps);
   if (launch_overlapped(paged_stream_kernel<HD, NT>, dim3(ctas, (unsigned)pl.tiles), dim3(32 * kWarps), smem, s, p) != cudaSuccess)
     return BOLT3_ERR_CUDA;
-  if (pl.runs > 0) {
-    const int per_head = pl.runs / (int)heads + 2;              // partial sums that a head has on average, about
-    const cudaError_t e = per_head <= 8
-        ? launch_overlapped(paged_join_kernel<HD, NC, 4>, dim3(heads, (unsigned)((p.c.rows + 3) / 4)), dim3(128), 0, s, p)
-        : launch_overlapped(paged_join_kernel<HD, NC, 1>, dim3(heads, (unsigned)p.c.rows), dim3(per_head >= 32 ? 512 : 256), 0, s, p);
-    if (e != cudaSuccess) return BOLT3_ERR_CUDA;
+  static_assert(kJoinThreads == kRecordThreads, "of a block of records");
+  const int chunks = (int)((p.most + kKeysAt * kRecordThreads - 1) / (kKeysAt * kRecordThreads));
+  const int per_head = pl.runs / (int)heads + 2;                // partial sums that a head has on average, about
+  if (pl.runs > 0 && per_head <= 8) {
+    const unsigned joins = (unsigned)(((int64_t)heads * p.c.rows + kJoinThreads / 32 - 1) / (kJoinThreads / 32));
+    return launch_overlapped(paged_join_kernel<HD, NC>, dim3(joins + (p.score != nullptr ? heads * (unsigned)chunks : 0u)),
+                             dim3(kJoinThreads), 0, s, p, (int)joins, chunks) == cudaSuccess ? BOLT3_OK : BOLT3_ERR_CUDA;
   }
+  if (pl.runs > 0 && launch_overlapped(paged_join_long_kernel<HD, NC>, dim3(heads, (unsigned)p.c.rows), dim3(per_head >= 32 ? 512 : 256), 0,
+                                       s, p) != cudaSuccess)
+    return BOLT3_ERR_CUDA;
   if (p.score != nullptr && (pl.runs > 0 || pl.tiles > 1) &&
-      launch_overlapped(paged_record_kernel, dim3(heads * (unsigned)((p.most + kRecordThreads - 1) / kRecordThreads)),
-                        dim3(kRecordThreads), 0, s, p) != cudaSuccess)
+      launch_overlapped(paged_record_kernel, dim3(heads * (unsigned)chunks), dim3(kRecordThreads), 0, s, p, chunks) != cudaSuccess)
     return BOLT3_ERR_CUDA;
   return BOLT3_OK;
 }
@@ -760,7 +869,8 @@ extern "C" int bolt3_paged_attend(const bolt3_paged_attend_args* a, void* stream
   cudaStream_t s = (cudaStream_t)stream;
   if (many_rows(a->T, a->H, a->HKV)) return prompt_launch(p.c, s);
   if (!encode_pool(&p.map, a->pages, a->n_pages, a->page, a->HKV, a->HD, a->page < kBlock ? a->page : kBlock)) return BOLT3_ERR_CUDA;
-  if ((int64_t)a->B * a->HKV * ((n + a->T + kRecordThreads - 1) / kRecordThreads) > 0x7fffffff) return BOLT3_ERR_SHAPE;
+  // blocks of the joins (a warp for each query row) and of the records
+  if ((int64_t)a->B * a->HKV * (p.c.rows + (n + a->T + kRecordThreads - 1) / kRecordThreads) > 0x7fffffff) return BOLT3_ERR_SHAPE;
   const Plan pl = plan_of(a->B, a->T, a->H, a->HKV, a->HD, n, a->weight != nullptr);
   char* ws = reinterpret_cast<char*>(a->workspace);
   p.n_runs = pl.runs;
