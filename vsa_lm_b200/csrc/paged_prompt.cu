@@ -167,6 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
     tc5::mbar_fence_init();
     sm.err = 0;
   }
+  meet_all();                                    // the barriers are there: loads may begin
   grid_dep_launch();
   grid_dep_wait();
   bool bad = false;
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
     tc5::tmem_alloc(&sm.tbase, 512);
     tc5::tmem_relinquish();
   }
-  // every warp comes here once: the queries are in place, the barriers and the TMEM are there
+  // every warp comes here once: the queries are in place, the TMEM is there
   auto all_ready = [&] {
     tc5::fence_before_sync();
     meet_all();
@@ -244,10 +245,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
       return max(pg, 0) * a.HKV + kvh;
     };
     int next = lookup(0);
-    all_ready();
     int done = 0;                                // blocks whose loads were issued
     bool ok = true;
     for (int j = 0; ok && j < n_blk; ++j) {
+      if (j == 2) all_ready();                   // the first two blocks come while the queries do
       const int st = j & 1, z = next;
       next = lookup(j + 1);
       ok = j < 2 || wait_all(&sm.k_empty[st], (j >> 1) - 1);
@@ -267,6 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
       if (issues) tc5::tma_load_3d(sm.v[st] + to, &p.map, 64 * cb, 0, z + (int)(pages.n_pages * a.HKV), bar);
       done = j + 1;
     }
+    if (n_blk <= 2) all_ready();
     for (int j = max(0, done - 2); j < done; ++j) {   // no copy is in flight when the CTA ends
       wait(&sm.k_full[j & 1], j >> 1);
       if (ragged && j + 1 == n_blk) wait(&sm.v_last, 0);
@@ -545,6 +547,7 @@ __global__ void __launch_bounds__(kRecordThreads, 1) paged_prompt_record_kernel(
     tc5::mbar_fence_init();
     sm.err = 0;
   }
+  meet_all();                                    // the barriers are there: loads may begin
   grid_dep_launch();
   grid_dep_wait();
   bool bad = false;
@@ -591,8 +594,12 @@ __global__ void __launch_bounds__(kRecordThreads, 1) paged_prompt_record_kernel(
     bool ok = true;
     for (int g = 0; g < groups; ++g) {
       int next = lookup(0);
-      meet();
+      bool met = false;
       for (int j = 0; ok && j < n_blk; ++j) {
+        if (j == 2) {                            // the first two blocks come while the queries do
+          meet();
+          met = true;
+        }
         const int it = g * n_blk + j, st = it & 1, z = next;
         next = lookup(j + 1);
         ok = it < 2 || wait_all(&sm.k_empty[st], (it >> 1) - 1);
@@ -603,6 +610,7 @@ __global__ void __launch_bounds__(kRecordThreads, 1) paged_prompt_record_kernel(
           tc5::tma_load_3d(sm.k[st] + cb * (kKeys * 128) + (unit << (pages.log + 7)), &p.map, 64 * cb, 0, z, &sm.k_full[st]);
         done = it + 1;
       }
+      if (!met) meet();
       // no copy is in flight when the CTA ends
       if (g + 1 == groups || !ok)
         for (int it = max(0, done - 2); it < done; ++it) wait(&sm.k_full[it & 1], it >> 1);
