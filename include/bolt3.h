@@ -315,7 +315,7 @@ int bolt3_paged_append(const bolt3_paged_append_args* a, void* stream);
 
 /* Softmax attention of the T newest tokens (already appended) over the pages: query t of sequence b sees rows
  * 0 .. s_b + t. q and y as in bolt3_kv8_attend. Scores, sums and the running maximum in fp32; the softmax weights enter the
- * product with the values as two bf16 terms (up to T * G = 32), or rounded to bf16. With `weight`, every row's softmax
+ * product with the values as two bf16 terms (up to T * G = 16), or rounded to bf16. With `weight`, every row's softmax
  * weights over all T * G query rows of its head are added to its record, in a fixed order. A key or value that is not finite
  * spoils every query row that sees it, and, of the T newest tokens, also rows before it in the same call; rows behind a
  * sequence's length may hold anything. H a multiple of HKV, G = H / HKV <= 16, T * G <= 2^24; sm_scale > 0 and finite.

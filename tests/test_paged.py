@@ -8,7 +8,7 @@ Tolerances, from the arithmetic of include/bolt3.h:
 - a score t (base 2) is off by HD roundings of the products' absolute sum, times 2 for the tensor cores' truncation,
   and by a few roundings of itself and of the reference it is measured from: 2^-22 (|t| + |reference|). An error d of
   a score changes its weight by a factor of 2^d;
-- a weight in the product with the values is two bf16 terms, 2^-17 of it, up to 32 query rows per KV head; one, 2^-9,
+- a weight in the product with the values is two bf16 terms, 2^-17 of it, up to 16 query rows per KV head; one, 2^-9,
   above; ex2 is off by 2^-22; a sum of N terms by N 2^-24.
 """
 import math
@@ -176,6 +176,11 @@ ATTEND = [
     (2, 3, 15, 5, 64, 16, 45, (45, -1)),                 # a few tokens, causal among themselves
     (2, 7, 16, 4, 128, 32, 1000, (3, 1000)),             # two column tiles
     (1, 2, 16, 1, 128, 16, 2500, None),                  # 32 rows over runs
+    (1, 16, 5, 5, 64, 16, 100, None),                    # 16 rows of as many tokens
+    (1, 17, 5, 5, 64, 32, 100, None),                    # the fewest of many rows
+    (12, 1, 32, 8, 128, 64, 2500, None),                 # a CTA per head, most of the machine
+    (8, 1, 16, 8, 64, 64, 4200, None),                   # longer: its records apart
+    (8, 1, 32, 8, 64, 64, 2500, (2500, 3, 0, -1, 64, 63, 65, 1)),   # the same ragged: runs
     (2, 33, 4, 4, 64, 16, 0, None),                      # many rows: a prompt from its start
     (3, 40, 4, 2, 128, 64, 500, (500, 0, -1)),           # one tile of rows, a ragged batch
     (1, 128, 8, 2, 128, 128, 130, None),                 # two tiles
@@ -211,7 +216,7 @@ def test_attend_matches_64_bits(case, weigh):
                          lens=torch.tensor(L, dtype=torch.int32).cuda() if lens else None, weight=weight, status=status)
     assert int(status.word) == 0
     got = got.cpu().view(B, T, H, HD)
-    few = T * (H // HKV) <= 32
+    few = T * (H // HKV) <= 16
     tol = mass * (2 * (err + (2 ** -17 if few else 2 ** -9) + 2 ** -21) + (n + T) * 2 ** -23)
     for b in range(B):
         if L[b] < 0:
@@ -240,7 +245,7 @@ def test_a_key_far_above_the_others_takes_everything(T):
     y, mass, err, rec, rec_err = ref_attend(q, pages, table, [n], HD ** -0.5, HKV)
     weight = torch.zeros(B, HKV, table.shape[1] * page, device="cuda")
     got = K.paged_attend(q=q.cuda(), pages=pages.cuda(), table=table.cuda(), n=n, weight=weight).cpu().view(B, T, H, HD)
-    assert rounded_within(got, y, mass * (2 * (err + (2 ** -17 if T * H <= 32 else 2 ** -9) + 2 ** -21) + (n + T) * 2 ** -23))
+    assert rounded_within(got, y, mass * (2 * (err + (2 ** -17 if T * H <= 16 else 2 ** -9) + 2 ** -21) + (n + T) * 2 ** -23))
     assert bool(((weight.cpu().double() - rec).abs() <= rec_err + 2 ** -23 * rec).all())
     assert abs(float(y[0, 0, 0, 0]) - float(kv[1, 1700, 0])) < 1e-3
 

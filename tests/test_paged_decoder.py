@@ -155,7 +155,7 @@ def test_anchor_attention_over_a_paged_cache(qk_norm, HD, HKV, page, budget):
                                k_norm=ly.k_norm.weight.float() if qk_norm else None, eps=1e-6, weight=before.weight, order=before.order)
             n = before.n
             ref, mass, err, rec, rec_err = ref_attend(q.cpu(), before.pages.cpu(), before.table.cpu(), [n] * B, HD ** -0.5, HKV)
-            few = t * (8 // HKV) <= 32
+            few = t * (8 // HKV) <= 16
             tol = mass * (2 * (err + (2 ** -17 if few else 2 ** -9) + 2 ** -21) + (n + t) * 2 ** -23)
             assert rounded_within(y.cpu().view(B, t, 8, HD), ref, tol)
             pos += t

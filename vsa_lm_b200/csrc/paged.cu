@@ -240,7 +240,6 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(const __grid_
 constexpr int kBins = 2048;
 constexpr int kCached = 12288;                       // rows whose keys and positions are kept in shared memory
 constexpr int kListed = 1024;                        // moves of a head whose list is kept in shared memory
-constexpr int kInline = 512;                         // moves of a head that its own CTA makes, whatever the number of heads
 
 struct Evict {
   bolt3_paged_evict_args a;
@@ -467,7 +466,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) paged_evict_kernel(cons
   const uint64_t before = warps_before<W>(mine, s_warp, total);
   int hole = (int)(uint32_t)before, mover = (int)(before >> 32);
   const int n_moves = (int)(uint32_t)total;
-  int2* moves = !p.split && p.most <= kListed ? reinterpret_cast<int2*>(s_dyn + 2 * cached) : p.moves + (int64_t)head * p.most;
+  int2* moves = p.most <= kListed ? reinterpret_cast<int2*>(s_dyn + 2 * cached) : p.moves + (int64_t)head * p.most;
   rank = rank0;
   for (int i = i0 + lane; i - lane < i1; i += 32) {
     const bool st = stays(i, rank), drops = i < i1 && i < keep && !st, moves_in = i < i1 && i >= keep && st;
@@ -496,12 +495,14 @@ __global__ void __launch_bounds__(kThreads) paged_move_kernel(const __grid_const
 }
 
 int64_t most_moves(int64_t n, int64_t keep) { return n <= keep ? 0 : n - keep < keep ? n - keep : keep; }
-bool split_moves(int64_t heads, int64_t most) { return most > kInline && heads < 148; }
+// Whether a kernel of its own moves the rows, several blocks to a head: 8 heads of 6107 rows with 2011 moves each 18.5 us, moved by
+// each head's CTA 27; with 1024 moves, whose list is in shared memory, the CTA is as fast (4 heads 17.1 us, apart 17.4)
+bool split_moves(int64_t heads, int64_t most) { return most > kListed && heads < 148; }
 
 template <int HD, int NT>
 int launch_select(const Evict& p, cudaStream_t s) {
   const size_t cached = p.a.n < kCached ? (size_t)p.a.n : (size_t)kCached;
-  const size_t smem = cached * 8 + (!p.split && p.most <= kListed ? (size_t)p.most * 8 : 0);
+  const size_t smem = cached * 8 + (p.most <= kListed ? (size_t)p.most * 8 : 0);
   if (cudaFuncSetAttribute(paged_evict_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCached * 8 + kListed * 8) != cudaSuccess)
     return BOLT3_ERR_CUDA;
   return launch_overlapped(paged_evict_kernel<HD, NT>, dim3((unsigned)(p.a.B * p.a.HKV)), dim3(NT), smem, s, p) == cudaSuccess
@@ -511,8 +512,9 @@ int launch_select(const Evict& p, cudaStream_t s) {
 template <int HD>
 int launch_evict(const Evict& p, cudaStream_t s) {
   const int64_t heads = (int64_t)p.a.B * p.a.HKV;
-  // a thread per few rows, and of smaller blocks where there are more heads than the machine holds of 512 threads (two to an SM, by
-  // registers): 512 heads of 2176 rows 20 us rather than 25, 5 heads of 514 rows the other way round 6.3 rather than 6.0
+  // A thread per few rows (4 heads of 5128 rows: 1024 threads 14.7 us with the append, 512 15.7), in smaller blocks where the machine
+  // holds fewer of 512 threads than there are heads (two to an SM, by registers): 512 heads of 2176 rows 20 us, in blocks of 512 25;
+  // 288 heads 19.5, in blocks of 512 13.4
   const int rc = p.a.n > 4096 ? launch_select<HD, 1024>(p, s)
                : heads > 148 * 2 ? launch_select<HD, 256>(p, s) : launch_select<HD, 512>(p, s);
   if (rc != BOLT3_OK) return rc;
@@ -574,8 +576,7 @@ extern "C" int bolt3_paged_append(const bolt3_paged_append_args* a, void* stream
 extern "C" size_t bolt3_paged_evict_workspace(int B, int HKV, int64_t n, int64_t keep) {
   if (B <= 0 || HKV <= 0 || n < 0 || keep < 1 || n > 0x7fffffff) return 0;
   const int64_t heads = (int64_t)B * HKV, most = most_moves(n, keep);
-  const bool split = split_moves(heads, most);
-  return split || most > kListed ? (size_t)heads * ((size_t)most * 8 + (split ? 4 : 0)) : 0;
+  return most > kListed ? (size_t)heads * ((size_t)most * 8 + (split_moves(heads, most) ? 4 : 0)) : 0;
 }
 
 extern "C" int bolt3_paged_evict(const bolt3_paged_evict_args* a, void* stream) {

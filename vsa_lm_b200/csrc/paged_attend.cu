@@ -12,18 +12,19 @@
 // Bound by HBM: 4 HD bytes per key and KV head. The cache is read in blocks of 32 keys, for 8 or 16 query rows at once
 // (T * G of them, token-major). All blocks of all (sequence, KV head)s are one list, and every warp of the machine takes an
 // equal run of it, whatever the lengths of the sequences: within a run each head's stretch is a softmax of its own, finished
-// there if it is the whole cache of that head, else left in the workspace for a second kernel that joins the runs. A call
-// with little to read takes a CTA per head instead, whose warps take its blocks in turn and join in shared memory.
+// there if it is the whole cache of that head, else left in the workspace for a second kernel that joins the runs. Where the
+// heads fit the machine at once, a CTA takes one instead (plan_of), and its warps the head's blocks in turn, joined in shared
+// memory. 64 sequences of 2176 keys, 8 heads of 128: 92 us, 6.2 TB/s; one of 131072 keys: 88 us, 6.1 TB/s.
 // A warp works on its own: lanes bring the next block's keys and values by TMA, a box for each page that the block touches,
 // into a ring of the warp's own, in the 128-byte swizzle, whose ldmatrix reads are free of bank conflicts; the page numbers
 // of the next 32 boxes stand in the warp's registers, those after them are on their way. Both products have the keys or
 // dimensions in M and the query rows in N (no padding for up to 8 rows): S^T = K Q^T and O^T = V^T P^T by mma.sync m16n8k16,
-// P^T being S^T transposed by movmatrix. Value rows that no query row of the tile sees are cleared in the fragments: a page's
+// P^T being S^T transposed by movmatrix. Value rows that no query row sees are cleared in the fragments: a page's
 // unused rows may hold anything.
 //
 // The record needs the sum over all keys, which is known after the last one: the scores are left in the workspace (4 bytes
-// per key and query row, against 4 HD of the cache) and turned into weights by a third kernel, a thread per key, so that
-// no two threads add to one record.
+// per key and query row, against 4 HD of the cache) and turned into weights afterwards, a key by one thread, so that no two
+// add to one record. 64 sequences of 2176 keys, 8 heads of 128, 4 rows each: 101 us with records.
 #include "paged.cuh"
 #include "tc5.cuh"
 #include "trace.h"
@@ -39,10 +40,11 @@ constexpr float kMost = 20.f;   // log2 of the largest weight relative to the re
 struct Params {
   CUtensorMap map;              // the pool's rows, boxes of 64 columns and min(page, kBlock) rows
   Attend c;
-  int n_runs;                   // warps that share the blocks of a column tile; 0: a CTA per head
-  float* part;                  // [column tile][run][2][NC][HD] sums: a run's first stretch, its last
+  int n_runs;                   // warps that share all blocks; 0: a CTA per head
+  int apart;                    // the records are made by a kernel of their own
+  float* part;                  // [run][2][NC][HD] sums: a run's first stretch, its last
   float2* part_ml;              // [..][NC] (reference, sum of weights)
-  int2* span;                   // [column tile][head]: where its first partial sum is, its last run; -1: no partial sums
+  int2* span;                   // [head]: where its first partial sum is, its last run; -1: no partial sums
   float* lse;                   // [head][rows] log2 of the sum of 2^t over the keys, +inf for an idle sequence
   float* score;                 // [head][most keys][score_row] t
   int64_t most;                 // keys that a head can have
@@ -90,10 +92,9 @@ B3_DEV uint32_t transpose8(uint32_t x) {
   return y;
 }
 
-// Blocks blk0, blk0 + step, .. (n_it of them) of head (b, kvh), of whose keys query row r of this tile sees the first
-// s + token + 1.
+// Blocks blk0, blk0 + step, .. (n_it of them) of head (b, kvh), of whose keys query row r sees the first s + token + 1.
 template <int HD, int NT>
-B3_DEV void walk(const Params& p, RingState& rs, int b, int kvh, int64_t s, int col0, int64_t blk0, int n_it, int step,
+B3_DEV void walk(const Params& p, RingState& rs, int b, int kvh, int64_t s, int64_t blk0, int n_it, int step,
                  Softmax<HD, NT>& f) {
   using R = Ring<HD>;
   constexpr int KS = HD / 16, MT = HD / 16, CB = HD / 64, kDepth = R::kDepth;
@@ -145,14 +146,14 @@ B3_DEV void walk(const Params& p, RingState& rs, int b, int kvh, int64_t s, int 
       load(i, st >= kDepth ? st - kDepth : st);
     }
 
-  // queries as B fragments: a lane holds row grp of each n8 tile, dimensions 16 k + 2 tig, + 1, + 8, + 9. Row r of the tile
-  // is head kvh * G + r % G of token r / G
+  // queries as B fragments: a lane holds row grp of each n8 tile, dimensions 16 k + 2 tig, + 1, + 8, + 9. Row r is head
+  // kvh * G + r % G of token r / G
   uint32_t q[NT][KS][2];
   int see0[NT], see1[NT];                      // keys from blk0 on that rows 2 tig, 2 tig + 1 see (any number for a row past the last)
   const int64_t row0 = blk0 * kBlock;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int r = col0 + 8 * n + grp;
+    const int r = 8 * n + grp;
     const bool live = r < p.c.rows;
     const bf16* src = reinterpret_cast<const bf16*>(a.q) + (live ? b * a.q_sb + (r / p.c.G) * a.q_st + (int64_t)(kvh * p.c.G + r % p.c.G) * HD : 0);
 #pragma unroll
@@ -160,14 +161,13 @@ B3_DEV void walk(const Params& p, RingState& rs, int b, int kvh, int64_t s, int 
 #pragma unroll
       for (int j = 0; j < 2; ++j)
         q[n][k][j] = live ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 2 * tig + 8 * j) : 0u;
-    const int r0 = col0 + 8 * n + 2 * tig;
+    const int r0 = 8 * n + 2 * tig;
     const int64_t first = s + 1 - row0;
     see0[n] = (int)min(max(first + r0 / p.c.G, (int64_t)0), (int64_t)0x7ffffff0);
     see1[n] = (int)min(max(first + (r0 + 1) / p.c.G, (int64_t)0), (int64_t)0x7ffffff0);
   }
-  const int last = min(col0 + 8 * NT, p.c.rows) - 1;
-  const int see_all = (int)min(max(s + 1 + col0 / p.c.G - row0, (int64_t)0), (int64_t)0x7ffffff0);   // what every row sees
-  const int see_any = (int)min(max(s + 1 + last / p.c.G - row0, (int64_t)0), (int64_t)0x7ffffff0);   // what some row sees
+  const int see_all = (int)min(max(s + 1 - row0, (int64_t)0), (int64_t)0x7ffffff0);      // what every row sees
+  const int see_any = (int)min(max(s + a.T - row0, (int64_t)0), (int64_t)0x7ffffff0);    // what some row sees
   const float scale = a.sm_scale * kLog2e;
   // ldmatrix addresses within a tile: keys: row lane % 16, 16-byte chunk lane / 16; values: row lane % 8 + 8 (lane / 16),
   // chunk lane / 8 % 2. Chunk c of row r stands at c ^ r % 8
@@ -230,7 +230,7 @@ B3_DEV void walk(const Params& p, RingState& rs, int b, int kvh, int64_t s, int 
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const int r = col0 + 8 * n + 2 * tig, key = key0 + 16 * i + grp;
+          const int r = 8 * n + 2 * tig, key = key0 + 16 * i + grp;
           if (r >= p.score_row) continue;
           float* to = p.score + ((int64_t)head * p.most + row0 + key) * p.score_row + r;
           if (key < see_any) *reinterpret_cast<float2*>(to) = make_float2(t[i][n][0], t[i][n][1]);
@@ -336,8 +336,8 @@ B3_DEV bf16* out_row(const Attend& c, int b, int kvh, int row) {
   return reinterpret_cast<bf16*>(c.a.y) + (((int64_t)b * c.a.T + row / c.G) * c.a.H + kvh * c.G + row % c.G) * HD;
 }
 
-// blocks that a head of a sequence with s rows has for a tile whose last row is of token `last`
-B3_DEV int64_t blocks_of(int64_t s, int last) { return s < 0 ? 0 : (s + last + kBlock) / kBlock; }
+// blocks of a head of a sequence with s rows before the call
+B3_DEV int64_t blocks_of(int64_t s, int T) { return s < 0 ? 0 : (s + T + kBlock - 1) / kBlock; }
 
 // log2 of the sum of 2^t, from a reference and the sum relative to it
 B3_DEV float lse_of(float m, float l) { return l == 0.f ? -neg_inf() : m + log2f(l); }
@@ -383,8 +383,6 @@ __global__ void __launch_bounds__(32 * kWarps) paged_stream_kernel(const __grid_
   __shared__ float s_lse[NC];
   const bolt3_paged_attend_args& a = p.c.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane >> 2, tig = lane & 3;
-  const int tile = blockIdx.y, col0 = tile * NC;
-  const int last = (min(col0 + NC, p.c.rows) - 1) / p.c.G;      // token of the tile's last row
   unsigned char* smem = smem_raw + ((1024 - (tc5::smem_u32(smem_raw) & 1023)) & 1023);
   RingState rs;
   rs.ring = tc5::smem_u32(smem) + warp * R::kDepth * R::kStage;
@@ -402,9 +400,9 @@ __global__ void __launch_bounds__(32 * kWarps) paged_stream_kernel(const __grid_
   if (p.n_runs == 0) {
     const int b = blockIdx.x / a.HKV, kvh = blockIdx.x % a.HKV, head = blockIdx.x;
     const int64_t s = p.c.len.rows(b, bad);
-    if (bad && tid == 0 && tile == 0 && a.status) atomicOr(a.status, 8);
-    const int64_t nb = blocks_of(s, last);
-    walk<HD, NT>(p, rs, b, kvh, s, col0, warp, nb > warp ? (int)((nb - warp + kWarps - 1) / kWarps) : 0, kWarps, f);
+    if (bad && tid == 0 && a.status) atomicOr(a.status, 8);
+    const int64_t nb = blocks_of(s, a.T);
+    walk<HD, NT>(p, rs, b, kvh, s, warp, nb > warp ? (int)((nb - warp + kWarps - 1) / kWarps) : 0, kWarps, f);
     __syncthreads();                                            // the rings are read: their memory is free
     float* so = reinterpret_cast<float*>(smem);                 // [kWarps][NC][HD]
     float2* sml = reinterpret_cast<float2*>(so + kWarps * NC * HD);
@@ -425,8 +423,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_stream_kernel(const __grid_
       }
     }
     __syncthreads();
-    const int rows = min(NC, p.c.rows - col0);
-    for (int i = tid; i < rows * HD; i += 32 * kWarps) {
+    for (int i = tid; i < p.c.rows * HD; i += 32 * kWarps) {
       const int r = i / HD, d = i % HD;
       float m = neg_inf();
 #pragma unroll
@@ -439,13 +436,13 @@ __global__ void __launch_bounds__(32 * kWarps) paged_stream_kernel(const __grid_
         acc = fmaf(so[(w * NC + r) * HD + d], g, acc);
         l = fmaf(ml.y, g, l);
       }
-      out_row<HD>(p.c, b, kvh, col0 + r)[d] = __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
-      if (d == 0 && p.score != nullptr) {
-        if (gridDim.y == 1) s_lse[r] = lse_of(m, l);
-        else p.lse[(int64_t)head * p.c.rows + col0 + r] = lse_of(m, l);
+      out_row<HD>(p.c, b, kvh, r)[d] = __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
+      if (d == 0) {
+        if (p.apart) p.lse[(int64_t)head * p.c.rows + r] = lse_of(m, l);
+        else s_lse[r] = lse_of(m, l);
       }
     }
-    if (p.score != nullptr && gridDim.y == 1) {                 // all rows of the head are here
+    if (p.score != nullptr && !p.apart) {
       __syncthreads();
       const int64_t cap = a.width * a.page;
       if (s >= 0)
@@ -462,9 +459,9 @@ __global__ void __launch_bounds__(32 * kWarps) paged_stream_kernel(const __grid_
   int64_t s, nb;
   if (a.lens == nullptr) {
     s = p.c.len.rows(0, bad);
-    nb = blocks_of(s, last);
+    nb = blocks_of(s, a.T);
     total = nb * a.B * a.HKV;
-    if (bad && run == 0 && lane == 0 && tile == 0 && a.status) atomicOr(a.status, 8);
+    if (bad && run == 0 && lane == 0 && a.status) atomicOr(a.status, 8);
     const int64_t runs = min((int64_t)p.n_runs, total);         // none is empty: the join takes all from first to last
     if (run >= runs) return;
     lo = total * run / runs;
@@ -472,8 +469,8 @@ __global__ void __launch_bounds__(32 * kWarps) paged_stream_kernel(const __grid_
     b = (int)(lo / (nb * a.HKV));
     start = b * nb * a.HKV;
   } else {
-    for (int i = lane; i < a.B; i += 32) total += blocks_of(p.c.len.rows(i, bad), last);
-    if (bad && run == 0 && tile == 0 && a.status) atomicOr(a.status, 8);
+    for (int i = lane; i < a.B; i += 32) total += blocks_of(p.c.len.rows(i, bad), a.T);
+    if (bad && run == 0 && a.status) atomicOr(a.status, 8);
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
     total *= a.HKV;
@@ -483,7 +480,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_stream_kernel(const __grid_
     hi = total * (run + 1) / runs;
     // the sequence that block lo belongs to
     for (int i0 = 0;; i0 += 32) {
-      const int64_t mine = i0 + lane < a.B ? blocks_of(p.c.len.rows(i0 + lane, bad), last) * a.HKV : 0;
+      const int64_t mine = i0 + lane < a.B ? blocks_of(p.c.len.rows(i0 + lane, bad), a.T) * a.HKV : 0;
       int64_t upto = mine;
 #pragma unroll
       for (int x = 1; x < 32; x <<= 1) {
@@ -501,7 +498,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_stream_kernel(const __grid_
       if (i0 + 32 >= a.B) return;                               // not reached: lo < total
     }
     s = p.c.len.rows(b, bad);
-    nb = blocks_of(s, last);
+    nb = blocks_of(s, a.T);
   }
   int kvh = (int)((lo - start) / nb);
   bool first = true;
@@ -509,10 +506,10 @@ __global__ void __launch_bounds__(32 * kWarps) paged_stream_kernel(const __grid_
     const int64_t at0 = start + kvh * nb;                       // this head's first block in the list
     const int64_t b0 = lo - at0, b1 = min(hi - at0, nb);
     const int head = b * a.HKV + kvh;
-    walk<HD, NT>(p, rs, b, kvh, s, col0, b0, (int)(b1 - b0), 1, f);
+    walk<HD, NT>(p, rs, b, kvh, s, b0, (int)(b1 - b0), 1, f);
     const bool whole = b0 == 0 && b1 == nb;
-    int2* span = p.span + (int64_t)tile * a.B * a.HKV + head;
-    const int64_t slot = ((int64_t)tile * p.n_runs + run) * 2 + (first ? 0 : 1);
+    int2* span = p.span + head;
+    const int64_t slot = (int64_t)run * 2 + (first ? 0 : 1);
     if (lane == 0) {
       if (whole) {
         *span = make_int2(-1, -1);
@@ -524,7 +521,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_stream_kernel(const __grid_
     if (whole) {                                                // the head's whole cache: done
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const int r = col0 + 8 * n + 2 * tig;
+        const int r = 8 * n + 2 * tig;
         const float i0 = f.l0[n] == 0.f ? 0.f : 1.f / f.l0[n], i1 = f.l1[n] == 0.f ? 0.f : 1.f / f.l1[n];
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -552,11 +549,11 @@ __global__ void __launch_bounds__(32 * kWarps) paged_stream_kernel(const __grid_
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           float* at = p.part + (slot * NC + r) * HD + 16 * m + grp;
-          if (col0 + r < p.c.rows) {
+          if (r < p.c.rows) {
             at[0] = f.o[m][n][0];
             at[8] = f.o[m][n][2];
           }
-          if (col0 + r + 1 < p.c.rows) {
+          if (r + 1 < p.c.rows) {
             at[HD] = f.o[m][n][1];
             at[HD + 8] = f.o[m][n][3];
           }
@@ -576,7 +573,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_stream_kernel(const __grid_
         if (++b >= a.B) return;                                 // not reached while the lengths stand
         if (a.lens != nullptr) {
           s = p.c.len.rows(b, bad);
-          nb = blocks_of(s, last);
+          nb = blocks_of(s, a.T);
         }
       } while (nb == 0);
     }
@@ -586,14 +583,12 @@ __global__ void __launch_bounds__(32 * kWarps) paged_stream_kernel(const __grid_
 // Where the partial sums of a head are: the first one's slot, the first run, their number. false: there are none, and the row's
 // output has been written (done) or is 0 (an idle sequence, or a run gave up)
 struct Parts {
-  int64_t base;
   int x, r0, n;
   bool done;
 };
-B3_DEV bool parts_of(const Params& p, int head, int heads, int tile, Parts& f) {
+B3_DEV bool parts_of(const Params& p, int head, Parts& f) {
   bool bad = false;
-  const int2 span = p.span[(int64_t)tile * heads + head];
-  f.base = (int64_t)tile * p.n_runs * 2;
+  const int2 span = p.span[head];
   f.x = span.x;
   f.r0 = span.x >> 1;
   f.n = span.y - f.r0 + 1;
@@ -605,9 +600,9 @@ B3_DEV bool parts_of(const Params& p, int head, int heads, int tile, Parts& f) {
   return !f.done;
 }
 // slot of the i-th of them: a later run's first stretch
-B3_DEV int64_t slot_of(const Parts& f, int i) { return f.base + (i == 0 ? f.x : 2 * (f.r0 + i)); }
+B3_DEV int64_t slot_of(const Parts& f, int i) { return i == 0 ? f.x : 2 * (int64_t)(f.r0 + i); }
 
-// The sums i0, i0 + step, .. of a query row (r of its tile) joined, by a warp: the reference, the sum of weights, the outputs'
+// The sums i0, i0 + step, .. of query row r joined, by a warp: the reference, the sum of weights, the outputs'
 // dimensions 32 e + lane
 template <int HD, int NC>
 B3_DEV void join(const Params& p, const Parts& f, int r, int i0, int step, float& m, float& l, float (&acc)[HD / 32]) {
@@ -647,7 +642,8 @@ B3_DEV void zero_row(const Params& p, int head, int row) {
   for (int i = threadIdx.x & 31; i < HD; i += 32) y[i] = __float2bfloat16_rn(0.f);
 }
 
-// The runs' partial sums of a (head, query row) where a head has few of them, joined by a warp; with records, blocks from
+// The runs' partial sums of a (head, query row) where a head has few of them, joined by a warp (64 heads with 18 each: 157 us, by a block
+// 151; 256 heads with 6: the same); with records, blocks from
 // `joins` on turn the scores of kKeysAt * kJoinThreads keys of a head into weights at the same time (a launch less, and
 // neither waits for the other: 64 sequences of 2176 keys, 8 heads, 112 -> 110 us), for which they join the rows' sums of weights
 constexpr int kJoinThreads = 256;
@@ -655,7 +651,7 @@ constexpr int kJoinThreads = 256;
 template <int HD, int NC>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ Params p, int joins, int chunks) {
   constexpr int kJoinWarps = kJoinThreads / 32;
-  __shared__ float s_lse[32];
+  __shared__ float s_lse[16];
   const bolt3_paged_attend_args& a = p.c.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = a.B * a.HKV;
   grid_dep_launch();
@@ -665,12 +661,12 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     const int64_t item = (int64_t)blockIdx.x * kJoinWarps + warp;
     if (item >= (int64_t)heads * p.c.rows) return;
     const int head = (int)(item / p.c.rows), row = (int)(item - (int64_t)head * p.c.rows);
-    if (!parts_of(p, head, heads, row / NC, f)) {
+    if (!parts_of(p, head, f)) {
       if (!f.done) zero_row<HD>(p, head, row);
       return;
     }
     float m, l, acc[HD / 32];
-    join<HD, NC>(p, f, row % NC, 0, 1, m, l, acc);
+    join<HD, NC>(p, f, row, 0, 1, m, l, acc);
     bf16* y = out_row<HD>(p.c, head / a.HKV, head % a.HKV, row);
 #pragma unroll
     for (int e = 0; e < HD / 32; ++e) y[32 * e + lane] = __float2bfloat16_rn(l == 0.f ? 0.f : acc[e] / l);
@@ -682,9 +678,9 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   if (s < 0 || key - threadIdx.x >= s + a.T) return;            // the same for the whole block
   for (int row = warp; row < p.c.rows; row += kJoinWarps) {
     float m = neg_inf(), l = 0.f;
-    if (parts_of(p, head, heads, row / NC, f)) {
+    if (parts_of(p, head, f)) {
       for (int i = lane; i < f.n; i += 32) {
-        const float2 ml = p.part_ml[slot_of(f, i) * NC + row % NC];
+        const float2 ml = p.part_ml[slot_of(f, i) * NC + row];
         const float to = fmaxf(m, ml.x), ref = to == neg_inf() ? 0.f : to;
         l = fmaf(l, exp2f(m - ref), ml.y * exp2f(ml.x - ref));
         m = to;
@@ -718,7 +714,7 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) paged_join_long_kernel(con
   grid_dep_wait();
   float* lse = p.score != nullptr ? p.lse + (int64_t)head * p.c.rows + row : nullptr;
   Parts f;
-  if (!parts_of(p, head, gridDim.x, row / NC, f)) {             // the same for the whole block
+  if (!parts_of(p, head, f)) {             // the same for the whole block
     if (!f.done && warp == 0) {
       zero_row<HD>(p, head, row);
       if (lse != nullptr && lane == 0) *lse = -neg_inf();
@@ -726,7 +722,7 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) paged_join_long_kernel(con
     return;
   }
   float m, l, acc[HD / 32];
-  join<HD, NC>(p, f, row % NC, warp, n_warps, m, l, acc);
+  join<HD, NC>(p, f, row, warp, n_warps, m, l, acc);
 #pragma unroll
   for (int e = 0; e < HD / 32; ++e) s_acc[warp][32 * e + lane] = acc[e];
   if (lane == 0) {
@@ -754,7 +750,7 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) paged_join_long_kernel(con
 constexpr int kRecordThreads = 256;
 
 __global__ void __launch_bounds__(kRecordThreads) paged_record_kernel(const __grid_constant__ Params p, int chunks) {
-  __shared__ float s_lse[32];
+  __shared__ float s_lse[16];
   const bolt3_paged_attend_args& a = p.c.a;
   const int head = blockIdx.x / chunks, b = head / a.HKV;
   const int64_t key = (int64_t)(blockIdx.x % chunks) * (kKeysAt * kRecordThreads) + threadIdx.x;
@@ -768,24 +764,29 @@ __global__ void __launch_bounds__(kRecordThreads) paged_record_kernel(const __gr
   record(p, head, a.width * a.page, s, key, kRecordThreads, s + a.T, s_lse);
 }
 
-// how a call is cut: columns of a CTA (in 8), column tiles, runs
+// how a call is cut: query rows (in 8), runs
 struct Plan {
-  int nt, tiles, runs, score_row;
+  int nt, runs, apart, score_row;
   size_t part, ml, span, lse, score, bytes;                     // offsets
 };
 
-Plan plan_of(int B, int T, int H, int HKV, int HD, int64_t n, bool weigh) {
+Plan plan_of(int B, int T, int H, int HKV, int HD, int64_t n, bool ragged, bool weigh) {
   Plan pl;
   const int64_t rows = (int64_t)T * (H / HKV), heads = (int64_t)B * HKV;
   pl.nt = rows <= 8 ? 1 : 2;
-  pl.tiles = (int)((rows + 8 * pl.nt - 1) / (8 * pl.nt));
   const int64_t per_head = (n + T + kBlock - 1) / kBlock, blocks = heads * per_head;
-  // A CTA per head where all are on the machine at once and a warp gets eight blocks at most; else every warp a run, of
-  // two blocks or more
-  int64_t runs = 0;
-  if (heads * pl.tiles > 148 || per_head > 8 * kWarps) runs = blocks / 2 < 148 * kWarps ? blocks / 2 : 148 * kWarps;
-  if (runs < 1 && heads * pl.tiles > 148) runs = 1;
-  pl.runs = (int)runs;
+  // A CTA per head, which needs no join (4 us), where all are on the machine at once and none works for much longer than the
+  // machine would: a CTA streams at 1 / 58 of the machine's bandwidth, a block of each warp in 1 us. Of a ragged batch one
+  // sequence may be all there is. Else every warp a run, of two blocks or more. 3 heads of 701 keys with records 9.6 us, in runs
+  // 10.3; of 1701 15.4, in runs 10.6; 128 heads of 3001 keys 33.7, in runs 37.6
+  pl.runs = 0;
+  if (heads > 148 || per_head * (58 - min(ragged ? (int64_t)HKV : heads, (int64_t)58)) > (int64_t)(3.5 * kWarps * 58)) {
+    const int64_t runs = blocks / 2 < 148 * kWarps ? blocks / 2 : 148 * kWarps;
+    pl.runs = runs < 1 ? 1 : (int)runs;
+  }
+  // A CTA per head makes its records itself, up to 4096 keys: 24 heads of 701 keys 9.9 us in all, with a kernel apart 10.9; 64 heads of
+  // 3001 keys 25.0, apart 24.4; of 12001 keys 82, apart 75
+  pl.apart = weigh && (pl.runs > 0 || per_head > 128);
   pl.score_row = (int)((rows + 1) & ~1);
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -793,10 +794,10 @@ Plan plan_of(int B, int T, int H, int HKV, int HD, int64_t n, bool weigh) {
     at += (bytes + 15) & ~(size_t)15;
     return was;
   };
-  const size_t slots = (size_t)pl.tiles * (size_t)runs * 2 * (size_t)(8 * pl.nt);
+  const size_t slots = (size_t)pl.runs * 2 * (size_t)(8 * pl.nt);
   pl.part = take(slots * (size_t)HD * 4);
   pl.ml = take(slots * 8);
-  pl.span = take(runs > 0 ? (size_t)pl.tiles * (size_t)heads * 8 : 0);
+  pl.span = take(pl.runs > 0 ? (size_t)heads * 8 : 0);
   pl.lse = take(weigh ? (size_t)heads * (size_t)rows * 4 : 0);
   pl.score = take(weigh ? (size_t)heads * (size_t)(n + T) * (size_t)pl.score_row * 4 : 0);
   pl.bytes = at;
@@ -811,7 +812,7 @@ int launch_stream(Params& p, const Plan& pl, cudaStream_t s) {
   if (cudaFuncSetAttribute(paged_stream_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return BOLT3_ERR_CUDA;
   const unsigned heads = (unsigned)(p.c.a.B * p.c.a.HKV), ctas = pl.runs == 0 ? heads : (unsigned)((pl.runs + kWarps - 1) / kWarps);
-  if (launch_overlapped(paged_stream_kernel<HD, NT>, dim3(ctas, (unsigned)pl.tiles), dim3(32 * kWarps), smem, s, p) != cudaSuccess)
+  if (launch_overlapped(paged_stream_kernel<HD, NT>, dim3(ctas), dim3(32 * kWarps), smem, s, p) != cudaSuccess)
     return BOLT3_ERR_CUDA;
   static_assert(kJoinThreads == kRecordThreads, "of a block of records");
   const int chunks = (int)((p.most + kKeysAt * kRecordThreads - 1) / (kKeysAt * kRecordThreads));
@@ -824,14 +825,15 @@ int launch_stream(Params& p, const Plan& pl, cudaStream_t s) {
   if (pl.runs > 0 && launch_overlapped(paged_join_long_kernel<HD, NC>, dim3(heads, (unsigned)p.c.rows), dim3(per_head >= 32 ? 512 : 256), 0,
                                        s, p) != cudaSuccess)
     return BOLT3_ERR_CUDA;
-  if (p.score != nullptr && (pl.runs > 0 || pl.tiles > 1) &&
+  if (p.apart &&
       launch_overlapped(paged_record_kernel, dim3(heads * (unsigned)chunks), dim3(kRecordThreads), 0, s, p, chunks) != cudaSuccess)
     return BOLT3_ERR_CUDA;
   return BOLT3_OK;
 }
 
-// Whether a call's rows go to the kernel for many rows, which works on tiles of 128
-bool many_rows(int T, int H, int HKV) { return (int64_t)T * (H / HKV) > 32; }
+// Whether a call's rows go to the kernel for many rows, which works on tiles of 128: from 17 rows on, where this one's products
+// pass its loads. 8 sequences of 2048 keys, 8 heads: 16 rows 22.7 us, there 23.5; 32 rows (two passes over the keys) 39.1, there 24.7
+bool many_rows(int T, int H, int HKV) { return (int64_t)T * (H / HKV) > 16; }
 
 bool shape_ok(int B, int T, int H, int HKV, int HD) {
   return B > 0 && T > 0 && HKV > 0 && H > 0 && H % HKV == 0 && H / HKV <= 16 && (HD == 64 || HD == 128) &&
@@ -842,7 +844,8 @@ bool shape_ok(int B, int T, int H, int HKV, int HD) {
 
 extern "C" size_t bolt3_paged_attend_workspace(int B, int T, int H, int HKV, int HD, int64_t n, int weigh) {
   if (!shape_ok(B, T, H, HKV, HD) || n < 0 || n > 0x7fffffff) return 0;
-  return many_rows(T, H, HKV) ? prompt_workspace(B, T, H, HKV, HD, n, weigh != 0) : plan_of(B, T, H, HKV, HD, n, weigh != 0).bytes;
+  if (many_rows(T, H, HKV)) return prompt_workspace(B, T, H, HKV, HD, n, weigh != 0);
+  return max(plan_of(B, T, H, HKV, HD, n, false, weigh != 0).bytes, plan_of(B, T, H, HKV, HD, n, true, weigh != 0).bytes);
 }
 
 extern "C" int bolt3_paged_attend(const bolt3_paged_attend_args* a, void* stream) {
@@ -871,9 +874,10 @@ extern "C" int bolt3_paged_attend(const bolt3_paged_attend_args* a, void* stream
   if (!encode_pool(&p.map, a->pages, a->n_pages, a->page, a->HKV, a->HD, a->page < kBlock ? a->page : kBlock)) return BOLT3_ERR_CUDA;
   // blocks of the joins (a warp for each query row) and of the records
   if ((int64_t)a->B * a->HKV * (p.c.rows + (n + a->T + kRecordThreads - 1) / kRecordThreads) > 0x7fffffff) return BOLT3_ERR_SHAPE;
-  const Plan pl = plan_of(a->B, a->T, a->H, a->HKV, a->HD, n, a->weight != nullptr);
+  const Plan pl = plan_of(a->B, a->T, a->H, a->HKV, a->HD, n, a->lens != nullptr, a->weight != nullptr);
   char* ws = reinterpret_cast<char*>(a->workspace);
   p.n_runs = pl.runs;
+  p.apart = pl.apart;
   p.part = reinterpret_cast<float*>(ws + pl.part);
   p.part_ml = reinterpret_cast<float2*>(ws + pl.ml);
   p.span = reinterpret_cast<int2*>(ws + pl.span);

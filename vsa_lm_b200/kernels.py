@@ -874,7 +874,7 @@ def paged_attend(*, q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, n
         y_at = y.data_ptr()
     else:
         y_at = _fits(y, torch.bfloat16, dev, "y", B * T * H * HD)
-    nbytes, launches = _paged_workspace(B, T, H, HKV, HD, n if dev_pos is None else n + dev_pos.span - 1, w_at != 0)
+    nbytes = _paged_workspace(B, T, H, HKV, HD, n if dev_pos is None else n + dev_pos.span - 1, w_at != 0)
     if nbytes:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         ws_at = ws.data_ptr()
@@ -884,16 +884,13 @@ def paged_attend(*, q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, n
         torch._C._cuda_getCurrentRawStream(dev), B, T, H, HKV, HD, q_at, q_sb, q_st, at, P, page, tat, stride, W, w_at,
         n, 0 if lens is None else _lens_ptr(lens, dev_pos, B, dev), y_at, HD ** -0.5 if sm_scale is None else sm_scale, ws_at, nbytes,
         0 if status is None else _status(status), *(_NO_POS if dev_pos is None else _pos_fields(dev_pos)))
-    _count(launches)
+    _count(1)
     return y
 
 
 @functools.lru_cache(maxsize=1024)
-def _paged_workspace(B: int, T: int, H: int, HKV: int, HD: int, n: int, weigh: bool) -> tuple[int, int]:
-    """Workspace bytes of a paged_attend call and the kernels it launches (at least: one for the attention, one to join
-    partial sums where there are any)."""
-    fn = _lib.load().bolt3_paged_attend_workspace
-    return fn(B, T, H, HKV, HD, n, int(weigh)), 2 if fn(B, T, H, HKV, HD, n, 0) else 1
+def _paged_workspace(B: int, T: int, H: int, HKV: int, HD: int, n: int, weigh: bool) -> int:
+    return _lib.load().bolt3_paged_attend_workspace(B, T, H, HKV, HD, n, int(weigh))
 
 
 @functools.lru_cache(maxsize=256)
