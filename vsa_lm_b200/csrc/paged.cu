@@ -6,12 +6,14 @@
 // to one turn before the fp32 sine: at position 100000 an fp32 product is off by 0.004 of a radian, more than a bf16 step.
 // Bound by HBM: (2 H + 4 HKV) HD bf16 per token. A warp takes a token's rows (few tokens: a share of them), HD / 16 lanes to a
 // row, a lane holding eight neighbouring values of each half, so that a rotation's pair is in one lane; its lanes share the
-// token's sines and cosines out among themselves and keep them for all rows.
+// token's sines and cosines out among themselves and keep them for all rows. 64 x 128 tokens of 32 + 2 x 8 heads of 128: 38.5 us,
+// 5.2 TB/s.
 //
 // evict: a CTA per (sequence, KV head). The threshold weight comes from a radix selection over the weights as ordered 32-bit
 // keys (digits of 11, 11 and 10 bits, counted in shared memory); then every warp walks a stretch of rows, so that one sum over
 // the warps gives the ranks of equal weights, and one those of dropped rows below `keep` and of kept rows behind it,
-// which are paired by rank. Only those rows move. Bound by HBM: 8 bytes per row, and 8 HD + 16 per moved row.
+// which are paired by rank. Only those rows move. Bound by HBM: 8 bytes per row, and 8 HD + 16 per moved row. 512 heads of 2176
+// rows, 128 of them moved: 20 us.
 #include <cudaTypedefs.h>
 
 #include <mutex>

@@ -676,24 +676,19 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   bool bad = false;
   const int64_t s = p.c.len.rows(b, bad), key = (int64_t)(at % chunks) * (kKeysAt * kJoinThreads) + threadIdx.x;
   if (s < 0 || key - threadIdx.x >= s + a.T) return;            // the same for the whole block
-  for (int row = warp; row < p.c.rows; row += kJoinWarps) {
+  if (threadIdx.x < p.c.rows) {
+    const int row = threadIdx.x;
     float m = neg_inf(), l = 0.f;
     if (parts_of(p, head, f)) {
-      for (int i = lane; i < f.n; i += 32) {
+#pragma unroll 4
+      for (int i = 0; i < f.n; ++i) {
         const float2 ml = p.part_ml[slot_of(f, i) * NC + row];
         const float to = fmaxf(m, ml.x), ref = to == neg_inf() ? 0.f : to;
         l = fmaf(l, exp2f(m - ref), ml.y * exp2f(ml.x - ref));
         m = to;
       }
-      float all = m;
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, x));
-      l *= all == neg_inf() ? 1.f : exp2f(m - all);
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-      m = all;
-      if (lane == 0) s_lse[row] = lse_of(m, l);
-    } else if (lane == 0) {
+      s_lse[row] = lse_of(m, l);
+    } else {
       s_lse[row] = f.done ? p.lse[(int64_t)head * p.c.rows + row] : -neg_inf();
     }
   }
