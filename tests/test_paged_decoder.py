@@ -340,3 +340,27 @@ def test_errors_of_the_kernels_reach_the_caller(call):
         else:
             for i in range(300):
                 dec.step(ids[:, :1], 40 + i, states, kv)
+
+
+@pytest.mark.gpu
+def test_a_model_of_anchors_alone():
+    """No other state in the steps, their graphs and the beams' reordering."""
+    torch.manual_seed(3)
+    model = Bolt3LM(vocab_size=64, dim=128, num_layers=2, num_heads=4, num_kv_heads=2, head_dim=64, intermediate=128,
+                    layer_types=["softmax", "softmax"]).to("cuda", torch.bfloat16).eval()
+    ids = torch.randint(0, 64, (2, 150), generator=torch.Generator().manual_seed(4)).cuda()
+    for budget in (None, 40):
+        dec = Bolt3Decoder(model, kv_cache="paged", kv_page=16, kv_budget=budget)
+        (_, st_e, kv_e), (_, st_g, kv_g) = dec.prefill(ids), dec.prefill(ids)
+        runner = dec.step_graph(st_g, kv_g)
+        for i in range(120):
+            tok = ids[:, i:i + 1]
+            he, _, _ = dec.step(tok, 150 + i, st_e, kv_e)
+            err = (runner.step(tok, 150 + i).float() - he.float()).abs().amax()
+            assert err <= 0.05 * he.float().pow(2).mean().sqrt(), (budget, i, float(err))
+        runner.close()
+        Bolt3Decoder.check_status(kv_g)
+        # 270 tokens seen, the last chunk's end at 256
+        assert all(c.n == (270 if budget is None else 40 + 14) and c.seen == 270 for c in kv_e + kv_g)
+    toks, scores, lengths = Bolt3Decoder(model, kv_cache="paged", kv_page=16).beam_search(ids, 3, 30)
+    assert toks.shape == (2, 3, 30) and bool(scores.isfinite().all()) and bool((scores.diff(dim=1) <= 0).all())
