@@ -516,10 +516,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
   if (tid == 0 && sm.err && a.status) atomicOr(a.status, 2);
 }
 
-// one warp per (head, query row): the splits' partial sums joined
-template <int HD>
+// one warp per (head, query row): the splits' partial sums joined. A lane holds the factors of splits lane, lane + 32, .., kOf of them;
+// four splits' sums are on their way at once, of more than 32 splits eight (1 head of 20030 keys, 480 rows in 74 splits: 26.9 us, one
+// after another 33.5)
+constexpr int kMostSplits = 148;
+
+template <int HD, int kOf>
 __global__ void __launch_bounds__(128) paged_prompt_join_kernel(const __grid_constant__ Params p) {
-  constexpr int EPL = HD / 32;
+  constexpr int EPL = HD / 32, kBatch = kOf == 1 ? 4 : 8;
   const bolt3_paged_attend_args& a = p.c.a;
   const int lane = threadIdx.x & 31;
   grid_dep_launch();
@@ -528,15 +532,41 @@ __global__ void __launch_bounds__(128) paged_prompt_join_kernel(const __grid_con
   if (item >= (int64_t)a.B * a.HKV * p.c.rows) return;
   const int head = (int)(item / p.c.rows), row = (int)(item % p.c.rows), b = head / a.HKV, kvh = head % a.HKV;
   const int64_t at = item * p.splits;
-  float m = neg_inf(), l = 0.f, acc[EPL] = {};
-  for (int i = 0; i < p.splits; ++i) m = fmaxf(m, p.part_ml[at + i].x);
-  for (int i = 0; i < p.splits; ++i) {
-    const float2 ml = p.part_ml[at + i];
-    if (ml.x == neg_inf() && ml.y == 0.f) continue;               // no keys: its sums were not written
-    const float f = ml.x == neg_inf() ? 0.f : exp2f(ml.x - m);
-    l = fmaf(ml.y, f, l);
+  float2 ml[kOf];
+  float m = neg_inf(), l = 0.f, f[kOf], acc[EPL] = {};
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) acc[e] = fmaf(p.part[(at + i) * HD + 32 * e + lane], f, acc[e]);
+  for (int c = 0; c < kOf; ++c) {
+    const int i = 32 * c + lane;
+    ml[c] = i < p.splits ? p.part_ml[at + i] : make_float2(neg_inf(), 0.f);
+    m = fmaxf(m, ml[c].x);
+  }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+#pragma unroll
+  for (int c = 0; c < kOf; ++c) {
+    f[c] = ml[c].x == neg_inf() ? 0.f : exp2f(ml[c].x - m);
+    l = fmaf(ml[c].y, f[c], l);
+    if (ml[c].x == neg_inf() && ml[c].y == 0.f) f[c] = -1.f;      // no keys: its sums were not written
+  }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+#pragma unroll
+  for (int c = 0; c < kOf; ++c) {
+    const int n = min(p.splits - 32 * c, 32);
+    for (int j0 = 0; j0 < n; j0 += kBatch) {                      // the same for the whole warp
+      float x[kBatch][EPL];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) x[j][e] = p.part[(at + 32 * c + min(j0 + j, n - 1)) * HD + 32 * e + lane];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const float g = __shfl_sync(0xffffffffu, f[c], j0 + j & 31);
+        if (j0 + j >= n || g == -1.f) continue;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) acc[e] = fmaf(x[j][e], g, acc[e]);
+      }
+    }
   }
   bf16* y = reinterpret_cast<bf16*>(a.y) + (((int64_t)b * a.T + row / p.c.G) * a.H + kvh * p.c.G + row % p.c.G) * HD;
 #pragma unroll
@@ -796,11 +826,19 @@ Plan plan_of(int B, int T, int H, int HKV, int HD, int64_t n, bool weigh) {
   Plan pl;
   const int64_t rows = (int64_t)T * (H / HKV), heads = (int64_t)B * HKV, blocks = (n + T + kKeys - 1) / kKeys;
   pl.tiles = (int)((rows + 255) / 256);
-  // as many splits as fill the machine, of four blocks or more
-  int64_t splits = 148 / (heads * pl.tiles);
-  const int64_t most = blocks / 4;
-  if (splits > most) splits = most;
-  pl.splits = splits < 1 ? 1 : (int)splits;
+  // Splits of the keys, as many as fit the machine with the rows' tiles: of a few numbers the one with the shortest time, a block
+  // taking 1.65 us, a join 3.3 and its sums, written and read, their bytes at 10 TB/s. 5 heads of 396 keys, 192 rows: 4 splits
+  // 9.9 us, 1 13.0; 2 of 1700 keys, 1200 rows: 7 splits 17.2, 3 or 14 20.2; 8 of 428 keys, 512 rows: 1 split 15.1, 4 14.3
+  pl.splits = 1;
+  double best = (double)blocks * 1.65;
+  for (int64_t room = min(148 / (heads * pl.tiles), blocks); room > 1; room = room * 3 / 4) {
+    const int64_t longest = (blocks + room - 1) / room, of = (blocks + longest - 1) / longest;
+    const double cost = (double)longest * 1.65 + 3.3 + (double)(of * heads * rows * HD) * 8e-7;
+    if (cost < best) {
+      best = cost;
+      pl.splits = (int)of;
+    }
+  }
   // ranges of keys: as many as give the shortest longest SM, a CTA costing a block and a half beside its own (its queries).
   // 16 sequences of 17 blocks, 8 heads: with the attention 136 us, 2 ranges 143
   pl.ranges = 1;
@@ -836,8 +874,8 @@ int launch(Params& p, const Plan& pl, cudaStream_t s) {
   if (launch_overlapped(paged_prompt_kernel<HD>, dim3((unsigned)(heads * pl.tiles), (unsigned)pl.splits), dim3(kThreads), smem, s,
                         p) != cudaSuccess)
     return BOLT3_ERR_CUDA;
-  if (pl.splits > 1 && launch_overlapped(paged_prompt_join_kernel<HD>, dim3((unsigned)((heads * p.c.rows + 3) / 4)), dim3(128), 0, s,
-                                         p) != cudaSuccess)
+  if (pl.splits > 1 && launch_overlapped(pl.splits <= 32 ? paged_prompt_join_kernel<HD, 1> : paged_prompt_join_kernel<HD, (kMostSplits + 31) / 32>,
+                                         dim3((unsigned)((heads * p.c.rows + 3) / 4)), dim3(128), 0, s, p) != cudaSuccess)
     return BOLT3_ERR_CUDA;
   if (p.lse != nullptr && launch_overlapped(paged_prompt_record_kernel<HD>, dim3((unsigned)(heads * pl.ranges)), dim3(kRecordThreads),
                                             rsmem, s, p) != cudaSuccess)
