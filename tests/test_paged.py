@@ -181,6 +181,8 @@ ATTEND = [
     (12, 1, 32, 8, 128, 64, 2500, None),                 # a CTA per head, most of the machine
     (8, 1, 16, 8, 64, 64, 4200, None),                   # longer: its records apart
     (8, 1, 32, 8, 64, 64, 2500, (2500, 3, 0, -1, 64, 63, 65, 1)),   # the same ragged: runs
+    (2, 1, 7, 1, 64, 64, 20000, (20000, 5)),             # hundreds of partial sums of a head
+    (1, 1, 16, 1, 128, 32, 20000, None),
     (2, 33, 4, 4, 64, 16, 0, None),                      # many rows: a prompt from its start
     (3, 40, 4, 2, 128, 64, 500, (500, 0, -1)),           # one tile of rows, a ragged batch
     (1, 128, 8, 2, 128, 128, 130, None),                 # two tiles
