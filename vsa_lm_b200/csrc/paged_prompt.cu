@@ -66,8 +66,8 @@ template <int HD>
 struct RecordSmem {
   unsigned char q[kRows / kKeys][kKeys * HD * 2];
   unsigned char k[2][kKeys * HD * 2];
-  float lse[kRows];
-  int token[kRows];
+  float lse[2][kRows];                           // of even groups of rows, of odd ones
+  int token[2][kRows];
   float sum[4][kRows / kKeys][kKeys];            // of a block's keys, of each tile's rows
   uint64_t k_full[2], k_empty[2], s_full[kRows / kKeys], s_empty[kRows / kKeys], sum_full[4][kRows / kKeys];
   uint32_t tbase;
@@ -717,13 +717,17 @@ __global__ void __launch_bounds__(kRecordThreads, 1) paged_prompt_record_kernel(
     bool ok = true;
     for (int g = 0; g < groups; ++g) {
       const int row0 = g * kRows, nq = tiles_of(g);
-      // this group's queries, sums and tokens (its first rows' MMAs of the group before are done: their scores were read)
+      // This group's queries, sums and tokens. The tile's MMAs of the group before are done: this warp has read their scores. The
+      // tile's other warps may still be turning theirs into weights, by that group's sums and tokens: those of this one go beside
+      // them, where nobody has read since the meeting at the start of the group before
+      float* lse_of = sm.lse[g & 1];
+      int* tokens = sm.token[g & 1];
       copy_queries<HD>(p, sm.q[0], b, kvh, row0, warp * 32, lane);
       copy_queries<HD>(p, sm.q[0], b, kvh, row0, warp * 32 + 16, lane);
       const int r = row0 + tid;
       if (g == 0) grid_dep_wait();
-      sm.lse[tid] = r < p.c.rows ? -p.lse[(int64_t)head * p.c.rows + r] : neg_inf();   // negated
-      sm.token[tid] = token_of(p, min(r, p.c.rows - 1));
+      lse_of[tid] = r < p.c.rows ? -p.lse[(int64_t)head * p.c.rows + r] : neg_inf();   // negated
+      tokens[tid] = token_of(p, min(r, p.c.rows - 1));
       asm volatile("cp.async.wait_all;\nfence.proxy.async.shared::cta;\n" ::: "memory");
       meet();
       const uint32_t ts = sm.tbase + i * 128 + ((uint32_t)(32 * (warp & 3)) << 16);
@@ -771,8 +775,8 @@ __global__ void __launch_bounds__(kRecordThreads, 1) paged_prompt_record_kernel(
             for (int c = 0; c < kKeys; c += 32) {
               const uint32_t(&y)[32] = x[c / 32 & 1];
               if (c + 32 < kKeys) tc5::ld32(ts + c + 32, x[c / 32 + 1 & 1]);
-              const ulonglong2* lse = reinterpret_cast<const ulonglong2*>(sm.lse + i * kKeys + c);
-              const int4* token = reinterpret_cast<const int4*>(sm.token + i * kKeys + c);
+              const ulonglong2* lse = reinterpret_cast<const ulonglong2*>(lse_of + i * kKeys + c);
+              const int4* token = reinterpret_cast<const int4*>(tokens + i * kKeys + c);
 #pragma unroll
               for (int u = 0; u < 8; ++u) {
                 const ulonglong2 z = lse[u];
