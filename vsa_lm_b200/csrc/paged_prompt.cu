@@ -187,8 +187,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
     sm.err = 0;
   }
   meet_all();                                    // the barriers are there: loads may begin
+  grid_dep_launch();
   grid_dep_wait();
-  grid_dep_launch();                             // not before the wait: the record kernel counts on what is complete here
   bool bad = false;
   const int64_t s = p.c.len.rows(b, bad);
   if (bad && tid == 0 && blockIdx.x % p.tiles == 0 && split == 0 && a.status) atomicOr(a.status, 8);
@@ -526,8 +526,8 @@ __global__ void __launch_bounds__(128) paged_prompt_join_kernel(const __grid_con
   constexpr int EPL = HD / 32, kBatch = kOf == 1 ? 4 : 8;
   const bolt3_paged_attend_args& a = p.c.a;
   const int lane = threadIdx.x & 31;
+  grid_dep_launch();
   grid_dep_wait();
-  grid_dep_launch();                             // not before the wait, as above
   const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (item >= (int64_t)a.B * a.HKV * p.c.rows) return;
   const int head = (int)(item / p.c.rows), row = (int)(item % p.c.rows), b = head / a.HKV, kvh = head % a.HKV;
@@ -597,18 +597,15 @@ __global__ void __launch_bounds__(kRecordThreads, 1) paged_prompt_record_kernel(
     sm.err = 0;
   }
   meet_all();                                    // the barriers are there: loads may begin
-  // The kernels before this one let it start once they have waited for those before them: queries, pages, table and lengths are
-  // complete, and are read while the attention still runs on other SMs (8 heads of 240 keys, 40 tokens of 8 rows: 17.4 us with the
-  // attention, after a wait here 19.9). Only its sums are waited for, by every CTA before it ends
+  // Queries, keys, table and lengths come from kernels before the attention, but only this wait makes their writes visible here: read
+  // before it, while the attention still runs, they saved 2 us and rested on an order that is promised nowhere
   grid_dep_launch();
+  grid_dep_wait();
   bool bad = false;
   const int64_t s = p.c.len.rows(b, bad);
   const int64_t all = s < 0 ? 0 : (s + a.T + kKeys - 1) / kKeys, lo = all * range / p.ranges, hi = all * (range + 1) / p.ranges;
   const int n_blk = (int)(hi - lo), groups = (p.c.rows + kRows - 1) / kRows;
-  if (n_blk == 0) {                              // the same for all threads: nothing has been allocated
-    grid_dep_wait();
-    return;
-  }
+  if (n_blk == 0) return;                        // the same for all threads: nothing has been allocated
   if (warp == 17) {
     tc5::tmem_alloc(&sm.tbase, 512);
     tc5::tmem_relinquish();
@@ -725,7 +722,6 @@ __global__ void __launch_bounds__(kRecordThreads, 1) paged_prompt_record_kernel(
       copy_queries<HD>(p, sm.q[0], b, kvh, row0, warp * 32, lane);
       copy_queries<HD>(p, sm.q[0], b, kvh, row0, warp * 32 + 16, lane);
       const int r = row0 + tid;
-      if (g == 0) grid_dep_wait();
       lse_of[tid] = r < p.c.rows ? -p.lse[(int64_t)head * p.c.rows + r] : neg_inf();   // negated
       tokens[tid] = token_of(p, min(r, p.c.rows - 1));
       asm volatile("cp.async.wait_all;\nfence.proxy.async.shared::cta;\n" ::: "memory");
