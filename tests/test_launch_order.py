@@ -35,3 +35,11 @@ def test_a_kernel_waits_before_it_reads_what_earlier_ones_wrote(f, name, body):
     reads = re.search(r"\blen\.rows\(|\bpage_of\(|\bcopy_queries<|\btma_load|\bcp_async16\(|\ba\.(lens|weight|order|table|status)\b"
                       r"|\bp\.(part|part_ml|lse|span|count|moves)\[|\bparts_of\(|\btoken_at\(|\bload_norms<|\b__ldg\(|\bmove_rows<", body)
     assert reads and waits[0] < reads.start(), body[reads.start():reads.start() + 40]
+
+
+@pytest.mark.parametrize("f,name,body", [k for k in KERNELS if "tmem_alloc(" in k[2]], ids=[k[1] for k in KERNELS if "tmem_alloc(" in k[2]])
+def test_a_kernel_has_its_tensor_memory_before_the_next_one_starts(f, name, body):
+    """Else a block of the next kernel could take the columns on the same SM and wait, with them, for this grid's end. And it
+    takes none before its own wait, which the kernels before it could need."""
+    assert body.count("grid_dep_launch();") == body.count("tmem_alloc(") == 1
+    assert body.index("grid_dep_wait();") < body.index("tmem_alloc(") < body.index("grid_dep_launch();")

@@ -121,7 +121,9 @@ B3_DEV uint32_t fkey(float f) {
 // grid_dep_wait() before it reads anything that kernel writes (or writes anything it reads).
 // grid_dep_wait() returns once every earlier grid of the stream has completed and its writes are
 // visible; in a kernel launched without the attribute it returns at once. grid_dep_launch() lets
-// the next such kernel begin launching once every block of this grid has called it or exited.
+// the next such kernel begin launching once every block of this grid has called it or exited. A
+// thread's call counts for its block: a kernel that takes tensor memory calls it once it has taken it (or holds all of an SM's
+// registers), else a block of the next kernel on the same SM could take the columns first and wait for this grid with them.
 B3_DEV void grid_dep_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 B3_DEV void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
 

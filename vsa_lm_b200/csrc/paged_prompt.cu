@@ -187,7 +187,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
     sm.err = 0;
   }
   meet_all();                                    // the barriers are there: loads may begin
-  grid_dep_launch();
   grid_dep_wait();
   bool bad = false;
   const int64_t s = p.c.len.rows(b, bad);
@@ -226,6 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
   if (warp == 17) {
     tc5::tmem_alloc(&sm.tbase, 512);
     tc5::tmem_relinquish();
+    grid_dep_launch();                           // here alone, for the whole CTA (common.cuh)
   }
   // every warp comes here once: the queries are in place, the TMEM is there
   auto all_ready = [&] {
@@ -599,7 +599,6 @@ __global__ void __launch_bounds__(kRecordThreads, 1) paged_prompt_record_kernel(
   meet_all();                                    // the barriers are there: loads may begin
   // Queries, keys, table and lengths come from kernels before the attention, but only this wait makes their writes visible here: read
   // before it, while the attention still runs, they saved 2 us and rested on an order that is promised nowhere
-  grid_dep_launch();
   grid_dep_wait();
   bool bad = false;
   const int64_t s = p.c.len.rows(b, bad);
@@ -609,6 +608,7 @@ __global__ void __launch_bounds__(kRecordThreads, 1) paged_prompt_record_kernel(
   if (warp == 17) {
     tc5::tmem_alloc(&sm.tbase, 512);
     tc5::tmem_relinquish();
+    grid_dep_launch();                           // here alone, for the whole CTA (common.cuh)
   }
   auto wait = [&](uint64_t* bar, int phase) {
     if (tc5::mbar_wait(bar, (uint32_t)phase & 1, kWaitIters)) return true;
