@@ -343,7 +343,7 @@ size_t bolt3_paged_attend_workspace(int B, int T, int H, int HKV, int HD, int64_
  * ones by the lowest row; where more than `keep` rows are that new, the same order decides among them. Of the dropped rows
  * below `keep`, the i-th (ascending) receives keys, values, weight and order of the i-th kept row at or above `keep`; what
  * stands at rows >= keep is left as it is. Here n (or lens[b] <= n) is the number of rows held; lens_out (optional, int32
- * [B]) becomes min(rows, keep), -1 for an idle sequence. Pages must not be shared between sequences. 0 <= recent <= keep,
+ * [B], no part of lens) becomes min(rows, keep), -1 for an idle sequence. Pages must not be shared between sequences. 0 <= recent <= keep,
  * keep >= 1. `workspace`: bolt3_paged_evict_workspace(...) bytes (none for most sizes), 16-byte aligned, used only within
  * the call. */
 typedef struct bolt3_paged_evict_args {

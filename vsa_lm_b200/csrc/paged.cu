@@ -593,6 +593,8 @@ extern "C" int bolt3_paged_evict(const bolt3_paged_evict_args* a, void* stream) 
   if (need > 0 && !a->workspace) return BOLT3_ERR_ARG;
   if (a->workspace_bytes < need) return BOLT3_ERR_CAPACITY;
   if (((uintptr_t)a->pages | (uintptr_t)a->workspace) & 15) return BOLT3_ERR_ALIGN;
+  // the first head of a sequence writes its new length where the others may not have read the old one yet
+  if (a->lens != nullptr && a->lens_out != nullptr && a->lens < a->lens_out + a->B && a->lens_out < a->lens + a->B) return BOLT3_ERR_ARG;
   p.a = *a;
   p.most = most_moves(a->n, a->keep);
   p.moves = reinterpret_cast<int2*>(a->workspace);
