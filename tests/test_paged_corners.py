@@ -1,0 +1,36 @@
+"""Corners of the paged cache's records and eviction: weights too small to hold, zeros of either sign. Tolerances as derived in
+test_paged.py."""
+import pytest
+import torch
+
+from test_paged import new_pages, put_rows, randn, ref_attend, ref_evict, same
+from vsa_lm_b200 import kernels as K
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("HD", [64, 128])
+@pytest.mark.parametrize("T", [1, 3, 40, 61, 150])
+def test_a_key_without_weight_has_a_record_of_zero(T, HD):
+    """Keys whose every weight is below 2^-150 (0 in fp32): their records stay as they were, to the bit, whatever the number of
+    query rows; and an eviction by such records keeps the lowest rows."""
+    B, H, HKV, page, n = 2, 8, 2, 32, 333
+    pages, table = new_pages(300, B, HKV, HD, page, n + T)
+    q = randn(301, B, T, H, HD, dtype=torch.bfloat16)
+    q[..., 0] = 40.0
+    heavy = 5
+    for b in range(B):
+        for h in range(HKV):
+            kv = randn(302 + 2 * b + h, 2, n + T, HD)
+            kv[0, :, 0] = -HD ** 0.5 * 2                  # every score about -80, and 80 at the heavy row: 2^-230 of its weight
+            kv[0, heavy, 0] = HD ** 0.5 * 2
+            put_rows(pages, table, b, h, kv.to(torch.bfloat16))
+    _, _, _, rec, _ = ref_attend(q, pages, table, [n] * B, HD ** -0.5, HKV)
+    light = rec < 2.0 ** -160
+    assert light[..., :heavy].all() and light[..., heavy + 1:].all() and (rec[..., heavy] > 0.99 * T * H // HKV).all()
+    gp, gt = pages.cuda(), table.cuda()
+    weight = torch.zeros(B, HKV, table.shape[1] * page, device="cuda")
+    K.paged_attend(q=q.cuda(), pages=gp, table=gt, n=n, weight=weight)
+    assert bool((weight.cpu()[light] == 0).all())
+    order = torch.arange(weight.shape[-1], dtype=torch.int32, device="cuda").expand_as(weight).contiguous()
+    K.paged_evict(pages=gp, table=gt, weight=weight, order=order, n=n + T, keep=100, recent=0)
+    assert bool((order[..., :100].cpu() == torch.arange(100)).all())

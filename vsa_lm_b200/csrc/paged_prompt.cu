@@ -121,11 +121,11 @@ B3_DEV void meet_all() {
   __syncwarp();
 }
 // 2^x of two numbers without the MUFU, relative error 2^-22: the nearest integer by adding 1.5 2^23, in whose low bits it then
-// stands, and a polynomial for the rest, in [-1/2, 1/2] (degree 5, its largest relative error the smallest: 2^-23.7). Below 2^-126:
-// 2^-126; a NaN stays one
+// stands, and a polynomial for the rest, in [-1/2, 1/2] (degree 5, its largest relative error the smallest: 2^-23.7). From -127
+// down, and so for a row past the last, 0, as by the MUFU: the exponent bits of 2^-127 are those of 0; a NaN stays one
 B3_DEV float2 ex2_fma(float2 x) {
-  asm("max.NaN.f32 %0, %0, %1;\n" : "+f"(x.x) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;\n" : "+f"(x.y) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;\n" : "+f"(x.x) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;\n" : "+f"(x.y) : "f"(-127.f));
   const uint64_t v = pair(x.x, x.y), r = add2(v, pair(12582912.f, 12582912.f));
   const uint64_t f = fma2(add2(r, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), v);
   uint64_t y = pair(0.00132764725f, 0.00132764725f);
