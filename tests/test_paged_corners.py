@@ -34,3 +34,22 @@ def test_a_key_without_weight_has_a_record_of_zero(T, HD):
     order = torch.arange(weight.shape[-1], dtype=torch.int32, device="cuda").expand_as(weight).contiguous()
     K.paged_evict(pages=gp, table=gt, weight=weight, order=order, n=n + T, keep=100, recent=0)
     assert bool((order[..., :100].cpu() == torch.arange(100)).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,keep", [(500, 100), (5000, 3000), (20000, 600)])
+def test_zeros_of_either_sign_are_equal_weights(n, keep):
+    """Ties go to the lowest row, the signs of zeros notwithstanding; what moves keeps its bits."""
+    B, HKV, HD, page = 2, 2, 64, 64
+    pages, table = new_pages(310, B, HKV, HD, page, n, poison=0.0)
+    pages.view(torch.int16).random_(-2 ** 15, 2 ** 15, generator=torch.Generator().manual_seed(311))
+    g = torch.Generator().manual_seed(312)
+    shape = (B, HKV, table.shape[1] * page)
+    weight = torch.where(torch.rand(shape, generator=g) < 0.5, -0.0, 0.0)
+    weight = torch.where(torch.rand(shape, generator=g) < 0.01, torch.rand(shape, generator=g), weight)
+    weight[1] = -weight[1]
+    order = torch.stack([torch.randperm(shape[-1], generator=g) for _ in range(B * HKV)]).view(shape).int()
+    gp, gw, go = pages.cuda(), weight.cuda(), order.cuda()
+    K.paged_evict(pages=gp, table=table.cuda(), weight=gw, order=go, n=n, keep=keep, recent=keep // 5)
+    ref_evict(pages, table, weight, order, [n] * B, keep, keep // 5)
+    assert same(gw.cpu(), weight) and torch.equal(go.cpu(), order) and same(gp.cpu(), pages)

@@ -336,8 +336,8 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) paged_evict_kernel(cons
   const int cached = min(n, kCached);
   uint32_t* s_key = s_dyn;
   int32_t* s_order = reinterpret_cast<int32_t*>(s_dyn + cached);
-  // NaN as +infinity; no key is 0
-  auto key_of = [&](float w) { return w != w ? 0xff800000u : fkey(w); };
+  // NaN as +infinity, -0 as 0 (the sum is +0); no key is 0
+  auto key_of = [&](float w) { return w != w ? 0xff800000u : fkey(w + 0.f); };
   __syncthreads();
 
   // positions and weights into shared memory, the newest position; every page that a row may leave or reach is in the pool
