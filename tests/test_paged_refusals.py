@@ -20,3 +20,16 @@ def _evict(**over):
 @pytest.mark.parametrize("at", [0, 4, 12, -4, -12])
 def test_an_eviction_does_not_overwrite_its_own_lengths(at):
     assert _evict(lens_out=5 * A + at) == ERR_ARG
+
+
+def _attend(**over):
+    """2 sequences of 8 tokens, 4 query heads of 64 on one KV head: queries of a wider projection of 384 values a token."""
+    a = dict(B=2, T=8, H=4, HKV=1, HD=64, q=A, q_sb=8 * 384, q_st=384, pages=2 * A, n_pages=64, page=16, table=3 * A, table_stride=8,
+             width=8, weight=4 * A, n=20, lens=None, y=5 * A, sm_scale=0.125, workspace=6 * A, workspace_bytes=A, status=None)
+    a.update(over)
+    return _lib.load().bolt3_paged_attend(ctypes.byref(_lib.PagedAttendArgs(**a)), None)
+
+
+@pytest.mark.parametrize("at", [0, 16, -16, 2 * 8 * 4 * 64 * 2 - 16, -(2 * 8 * 4 * 64 * 2 - 16), (15 * 384 + 256) * 2 - 16])
+def test_records_of_many_rows_need_their_queries_whole(at):
+    assert _attend(y=A + at) == ERR_ARG
