@@ -1,10 +1,12 @@
-"""Calls of the paged entry points that would give wrong results and are refused on the host, before anything is launched: the
-addresses here are never read."""
+"""Calls of the paged caches that would give wrong results, or have no effect, and are refused on the host, before anything is
+launched: the addresses here are never read."""
 import ctypes
 
 import pytest
 
-from vsa_lm_b200 import _lib
+from vsa_lm_b200 import Bolt3Decoder, _lib
+from vsa_lm_b200.model import Bolt3LM
+from vsa_lm_b200.workloads import MODEL_SHAPES
 
 ERR_ARG = 1
 A = 1 << 20                                               # addresses 1 MB apart
@@ -33,3 +35,14 @@ def _attend(**over):
 @pytest.mark.parametrize("at", [0, 16, -16, 2 * 8 * 4 * 64 * 2 - 16, -(2 * 8 * 4 * 64 * 2 - 16), (15 * 384 + 256) * 2 - 16])
 def test_records_of_many_rows_need_their_queries_whole(at):
     assert _attend(y=A + at) == ERR_ARG
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("page", [48, 32, 0])
+def test_a_page_size_goes_with_paged_caches(kind, page):
+    model = Bolt3LM(**dict(MODEL_SHAPES["tiny_lm"]))
+    for call in (lambda **kw: Bolt3Decoder(model, **kw), lambda **kw: Bolt3Decoder.blank_state(model, 1, "cpu", **kw),
+                 lambda **kw: Bolt3Decoder.state_bytes(model, **kw)):
+        with pytest.raises(ValueError, match="page size"):
+            call(kv_cache=kind, kv_page=page)
+    Bolt3Decoder(model, kv_cache=kind, kv_page=64)

@@ -1182,6 +1182,8 @@ def _check_kv_cache(kind: str, model=None, budget: int | None = None, recent: in
         check_budget(page, budget, recent)
     elif budget is not None or recent is not None:
         raise ValueError(f"a budget of rows goes with kv_cache='paged', got {kind!r}")
+    elif page != 64:                      # the default
+        raise ValueError(f"a page size goes with kv_cache='paged', got {kind!r}")
     if kind != "bf16" and model is not None:
         what = "8-bit" if kind == "int8" else "paged"
         for blk in model.blocks:
