@@ -319,7 +319,8 @@ int bolt3_paged_append(const bolt3_paged_append_args* a, void* stream);
  * weights over all T * G query rows of its head are added to its record, in a fixed order. A key or value that is not finite
  * spoils every query row that sees it, and, of the T newest tokens, also rows before it in the same call; rows behind a
  * sequence's length may hold anything. H a multiple of HKV, G = H / HKV <= 16, T * G <= 2^24; sm_scale > 0 and finite.
- * With `weight` and T * G > 16 y must not overlap what q spans: the queries are read again once y is written.
+ * y must not overlap what q spans, but may be q itself where that is laid out like y (not with `weight` and T * G > 16: the
+ * queries are read again once y is written).
  * `workspace`: device memory of bolt3_paged_attend_workspace(...) bytes (weigh: whether `weight` is given), 16-byte
  * aligned, used only within the call. */
 typedef struct bolt3_paged_attend_args {

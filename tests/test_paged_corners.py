@@ -1,5 +1,5 @@
-"""Corners of the paged cache's records and eviction: weights too small to hold, zeros of either sign. Tolerances as derived in
-test_paged.py."""
+"""Corners of the paged cache's records and eviction: weights too small to hold, zeros of either sign, outputs in the queries' place.
+Tolerances as derived in test_paged.py."""
 import pytest
 import torch
 
@@ -53,3 +53,23 @@ def test_zeros_of_either_sign_are_equal_weights(n, keep):
     K.paged_evict(pages=gp, table=table.cuda(), weight=gw, order=go, n=n, keep=keep, recent=keep // 5)
     ref_evict(pages, table, weight, order, [n] * B, keep, keep // 5)
     assert same(gw.cpu(), weight) and torch.equal(go.cpu(), order) and same(gp.cpu(), pages)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("HD", [64, 128])
+@pytest.mark.parametrize("B,T,H,HKV,n,weigh", [
+    (2, 1, 8, 2, 100, True),                              # a CTA per head
+    (1, 4, 16, 4, 5000, True),                            # runs of several warps, joined
+    (160, 1, 4, 1, 333, True),                            # whole heads by a warp
+    (2, 37, 8, 2, 100, False),                            # many rows
+    (1, 64, 8, 1, 9000, False),                           # and splits of the keys
+])
+def test_outputs_in_the_place_of_their_queries(HD, B, T, H, HKV, n, weigh):
+    pages, table = (x.cuda() for x in new_pages(320, B, HKV, HD, 32, n + T, poison=0.0))
+    pages.copy_(randn(321, *pages.shape, dtype=torch.bfloat16))
+    q = randn(322, B, T, H, HD, dtype=torch.bfloat16).cuda()
+    weight = [torch.zeros(B, HKV, table.shape[1] * 32, device="cuda") if weigh else None for _ in range(2)]
+    y = K.paged_attend(q=q, pages=pages, table=table, n=n, weight=weight[0])
+    K.paged_attend(q=q, pages=pages, table=table, n=n, weight=weight[1], y=q)
+    assert torch.equal(q.view(B, T, H * HD), y)
+    assert not weigh or torch.equal(*weight)

@@ -37,6 +37,15 @@ def test_records_of_many_rows_need_their_queries_whole(at):
     assert _attend(y=A + at) == ERR_ARG
 
 
+@pytest.mark.parametrize("weight", [None, 4 * A])
+@pytest.mark.parametrize("T", [1, 4, 8, 200])
+@pytest.mark.parametrize("at,stride", [(0, 384), (256, 384), (16, 256), (-16, 256), (512, 256), (-512, 256), (0, 0), (0, -256)])
+def test_outputs_are_not_written_over_queries_of_other_rows(T, weight, at, stride):
+    """Over queries that are not laid out like the outputs, or over some of them."""
+    sb = max(abs(stride) * T, 384)                        # of one token the token's stride says nothing
+    assert _attend(T=T, n=0, width=16, weight=weight, q=A, q_sb=sb if stride != 0 else 0, q_st=stride, y=A + at) == ERR_ARG
+
+
 @pytest.mark.parametrize("kind", ["bf16", "int8"])
 @pytest.mark.parametrize("page", [48, 32, 0])
 def test_a_page_size_goes_with_paged_caches(kind, page):

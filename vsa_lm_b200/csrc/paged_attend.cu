@@ -880,12 +880,16 @@ bool shape_ok(int B, int T, int H, int HKV, int HD) {
          T <= (1 << 24) / (H / HKV) && (int64_t)B * HKV <= 0x3fffffff;
 }
 
-// Whether the outputs stand where queries do: the records of many rows read the queries again once the outputs are written
-bool overlaps(const bolt3_paged_attend_args& a) {
+// Whether outputs would be written over queries that are still to be read. Outputs in the place of their own queries are not: a
+// query row's output is written by who has read it, after all of the row's keys, or by the join. But the records of many rows read
+// the queries again once the outputs are written
+bool overwrites(const bolt3_paged_attend_args& a) {
   const int64_t row = (int64_t)a.H * a.HD, sb = (a.B - 1) * a.q_sb, st = (a.T - 1) * a.q_st;
   const bf16* q = reinterpret_cast<const bf16*>(a.q);
   const bf16* y = reinterpret_cast<const bf16*>(a.y);
-  return y < q + (sb > 0 ? sb : 0) + (st > 0 ? st : 0) + row && q + (sb < 0 ? sb : 0) + (st < 0 ? st : 0) < y + (int64_t)a.B * a.T * row;
+  const bool apart = y >= q + (sb > 0 ? sb : 0) + (st > 0 ? st : 0) + row || q + (sb < 0 ? sb : 0) + (st < 0 ? st : 0) >= y + (int64_t)a.B * a.T * row;
+  const bool own = y == q && (a.T == 1 || a.q_st == row) && (a.B == 1 || a.q_sb == a.T * row);
+  return !apart && !(own && (a.weight == nullptr || !many_rows(a.T, a.H, a.HKV)));
 }
 
 }  // namespace
@@ -909,7 +913,7 @@ extern "C" int bolt3_paged_attend(const bolt3_paged_attend_args* a, void* stream
   if (!(a->sm_scale > 0.f && a->sm_scale <= 3.4e38f)) return BOLT3_ERR_ARG;
   const uintptr_t al = (uintptr_t)a->q | (uintptr_t)a->pages | (uintptr_t)a->y | (uintptr_t)a->workspace;
   if ((al & 15) || ((a->q_sb | a->q_st) & 7)) return BOLT3_ERR_ALIGN;
-  if (a->weight != nullptr && many_rows(a->T, a->H, a->HKV) && overlaps(*a)) return BOLT3_ERR_ARG;
+  if (overwrites(*a)) return BOLT3_ERR_ARG;
   const int64_t n = a->n + dmax;                                // no sequence holds more before the call
   if (bolt3_paged_attend_workspace(a->B, a->T, a->H, a->HKV, a->HD, n, a->weight != nullptr) >
       (a->workspace != nullptr ? a->workspace_bytes : 0))

@@ -864,8 +864,8 @@ def paged_attend(*, q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, n
     """Softmax attention of the T newest tokens, q = [B, T, H, HD] (or [B, T, H * HD]), over a paged cache that holds n
     rows before them and has them appended (bolt3_paged_attend): query t sees rows 0 .. n + t. With `lens` sequence b holds
     lens[b] rows before them (-1: idle, its outputs are 0), at most n. `weight` (fp32 [B, HKV, W * page]): the softmax weight
-    of every row, summed over the query rows of its head, is added to its record (with more than 16 of them y must not overlap
-    what q spans). Returns y, bf16 [B, T, H * HD]."""
+    of every row, summed over the query rows of its head, is added to its record. Returns y, bf16 [B, T, H * HD]:
+    given, it must not overlap what q spans, but may be a dense q itself (not with `weight` and more than 16 query rows)."""
     dev = _here()
     P, HKV, page, HD, B, W, stride, at, tat = _need_pages(pages, table, dev)
     T, H, q_sb, q_st, q_at = _tokens_heads(q, "q", B, HD, dev)
