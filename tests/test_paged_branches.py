@@ -22,6 +22,8 @@ EVICT = [
     (300, 1, 128, 32, 2100, 1030, 64, _lens(300, 2100, 900, 1031, -1), "random"),   # and moves listed in the workspace
     (148, 1, 128, 16, 2100, 1040, 64, None, "random"),               # listed in the workspace, moved by the head's own block
     (148, 1, 64, 64, 4200, 1030, 100, _lens(148, 4200, 1029, 2000), "few"),   # the same, blocks of 1024 threads
+    (149, 1, 64, 64, 4200, 1030, 100, _lens(149, 4200, 1029, 2000), "few"),   # one head more: blocks of 512
+    (75, 2, 64, 128, 10300, 10200, 900, _lens(75, 10300, 10201, 500), "random"),   # of 1024 again
     (147, 1, 64, 64, 2100, 1040, 64, _lens(147, 2100, 5, 1041), "random"),    # one head less: moved by a kernel of its own
 ]
 

@@ -514,11 +514,14 @@ int launch_select(const Evict& p, cudaStream_t s) {
 template <int HD>
 int launch_evict(const Evict& p, cudaStream_t s) {
   const int64_t heads = (int64_t)p.a.B * p.a.HKV;
-  // A thread per few rows (4 heads of 5128 rows: 1024 threads 14.7 us with the append, 512 15.7), in smaller blocks where the machine
-  // holds fewer of 512 threads than there are heads (two to an SM, by registers): 512 heads of 2176 rows 20 us, in blocks of 512 25;
-  // 288 heads 19.5, in blocks of 512 13.4
-  const int rc = p.a.n > 4096 ? launch_select<HD, 1024>(p, s)
-               : heads > 148 * 2 ? launch_select<HD, 256>(p, s) : launch_select<HD, 512>(p, s);
+  // Times with cold caches. A thread per few rows where an SM has a head at most (4 heads of 4224 rows: 1024 threads 16.4 us, 512 20.5, 256 28.7; 148 heads
+  // 18.4, 22.5, 30.7), and where shared memory holds two heads' rows on an SM at most (400 heads of 12000 rows, 3808 moves: 334, 446, 717).
+  // Else smaller blocks, of which an SM holds two of 512 threads by registers (400 heads of 4224 rows: 45.1, 39.4, 38.9; of 8320 53.2,
+  // 49.2, 49.2; 512 heads 69.6, 57.3, 79.8), or four of 256: where there are more heads than that holds of 512, up to 4096 rows (512 heads
+  // of 2176 rows: 49.1, 38.9, 34.8; 296 heads 28.7, 24.6, 28.7)
+  const bool many = heads > 148, full = p.a.n > 10240;
+  const int rc = p.a.n > 4096 && (!many || full) ? launch_select<HD, 1024>(p, s)
+               : p.a.n <= 4096 && heads > 148 * 2 ? launch_select<HD, 256>(p, s) : launch_select<HD, 512>(p, s);
   if (rc != BOLT3_OK) return rc;
   if (!p.split) return BOLT3_OK;
   const int64_t per = kThreads / 32 * 4 * (HD == 128 ? 1 : 2), want = (p.most + per - 1) / per, fit = (148 * 4 + heads - 1) / heads;
