@@ -835,7 +835,8 @@ Plan plan_of(int B, int T, int H, int HKV, int HD, int64_t n, bool weigh) {
   pl.tiles = (int)((rows + 255) / 256);
   // Splits of the keys, as many as fit the machine with the rows' tiles: of a few numbers the one with the shortest time, a block
   // taking 1.65 us, a join 3.3 and its sums, written and read, their bytes at 10 TB/s. 5 heads of 396 keys, 192 rows: 4 splits
-  // 9.9 us, 1 13.0; 2 of 1700 keys, 1200 rows: 7 splits 17.2, 3 or 14 20.2; 8 of 428 keys, 512 rows: 1 split 15.1, 4 14.3
+  // 9.9 us, 1 13.0; 2 of 1700 keys, 1200 rows: 7 splits 17.2, 3 or 14 20.2. An estimate: near its border it takes the slower side (8 of
+  // 428 keys, 512 rows: 6.60 for 1 split against 6.63 for 4, measured 15.1 and 14.3 us)
   pl.splits = 1;
   double best = (double)blocks * 1.65;
   for (int64_t room = min(148 / (heads * pl.tiles), blocks); room > 1; room = room * 3 / 4) {
